@@ -11,7 +11,7 @@ Kinds of cases (`run` is one pass of each):
   evict      of every request's rows the first, the latest and the weightiest go to new pages with their sums; the rows are
              handed back as values
 
-A value is held as c s: s the largest magnitude of its 32 neighbours along the head over 7, rounded to float16 (at most 65504),
+A value is held as c s: s the largest magnitude of its 32 neighbours along the head times 1/7 (in float), rounded to float16 (at most 65504),
 c = x / s rounded to the nearest whole number, at most 7 in size.  A page of one key head holds blocks of 8 rows: 8 rows of
 4-bit codes c + 8, then the scales.  `places` says where in a block a code and a scale are.
 
@@ -167,7 +167,7 @@ def quantized(x):
     """x [..., dim] as codes and scales."""
     groups = x.unflatten(-1, (-1, GROUP))
     top = groups.abs().amax(-1).float()
-    scales = (top / 7).clamp(max=65504.0).to(torch.float16)
+    scales = (top * (1 / 7)).clamp(max=65504.0).to(torch.float16)
     held = scales.double()[..., None]
     codes = torch.where(held > 0, (groups.double() / held).round().clamp(-7, 7), torch.zeros_like(held))
     return codes.flatten(-2), scales
@@ -401,7 +401,7 @@ def work(case):
 def nearest(x):
     """What 4 bits hold of x [..., dim], in 64 bits: the definition of the format, group by group."""
     x = x.double().unflatten(-1, (-1, GROUP))
-    step = (x.abs().max(-1, keepdim=True).values.float() / 7.0).to(torch.float16).double()
+    step = (x.abs().max(-1, keepdim=True).values.float() * (1.0 / 7.0)).to(torch.float16).double()
     step = torch.where(step.isinf(), torch.full_like(step, 65504.0), step)
     whole = torch.round(x / step).nan_to_num(0.0, 0.0, 0.0).clamp(-7.0, 7.0)
     return (whole * step).flatten(-2)
