@@ -1,0 +1,715 @@
+// Attention over a cache held in 4 bits (int4_cache.cuh): a few new tokens per request (one in a decode step), all query heads of a
+// key head at once, key ranges in parallel, the weights of the keys added up where that is asked for.
+// Specialised by HEAD_DIM (32, 64, 96, 128) and the queries' type (STORAGE_BF16).
+//
+// With codes n = c + 8, steps s and t the place of a key, of one query row q:
+//   score   scale log2(e) sum_g s_g(t) (sum_{d in g} q_d n_d - 8 sum_{d in g} q_d)          groups g of 32 dimensions
+//   output  sum_t p_t s_g(t) n_d(t) - 8 sum_t p_t s_g(t),     p = 2^(score - max), divided by sum_t p_t
+// The cache is read once, 9 D / 8 bytes a key for both planes, 3.6 times less than in bfloat16; at the rate of memory that is some 44 values a
+// clock and SM, so what has to be small here is the number of instructions per value:
+//   * A code is a float16 operand by one mask: the low half byte of a 16-bit half is the subnormal n 2^-24, the next one n 2^-20, which
+//     the matrix instructions take exactly; the two upper half bytes follow after one shift by 8.  Five integer instructions for
+//     8 values, none of them a conversion.  The factor 16 is taken out of the query (exactly) or of the finished output.
+//   * The offset 8 is never subtracted from a code: the score's accumulators start at -8 sum q, and the output's share is the
+//     product of the same probabilities with a constant operand, one matrix instruction per group and 16 keys.
+//   * A is the cache (16 keys by 16 dimensions of K; 16 dimensions by 16 keys of V), B the queries or probabilities, of which 8 columns are
+//     the least there is: a group of 3 or 4 query heads fills half of them, where it as A would fill a quarter.
+//   * Steps of K are applied to the score of a group (float), those of V to the probabilities (float16 pairs).
+// Operands other than codes are float16: of queries, normed by a power of two per row, exactly what bfloat16 holds (elements below 2^-24 of
+// the row's largest lose digits); of probabilities 11 bits.  Float queries take two float16 terms (22 bits) for both.
+// Scores, running maxima, sums and outputs are float.
+#include "int4_cache.cuh"
+#include "tma.cuh"
+
+#ifndef HEAD_DIM
+#define HEAD_DIM 128
+#endif
+#ifndef STORAGE_BF16
+#define STORAGE_BF16 1
+#endif
+
+namespace {
+constexpr int D = HEAD_DIM, NG = D / 32;
+static_assert(D % 32 == 0 && D >= 32 && D <= 128, "head sizes of whole groups up to 128");
+#if STORAGE_BF16
+typedef __nv_bfloat16 T;
+constexpr int TERMS = 1;
+#else
+typedef float T;
+constexpr int TERMS = 2;
+#endif
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int TK = 32;                                             // keys of a warp's tile: four blocks of 8
+constexpr int STAGES = 2;
+constexpr int BLOCK_BYTES = int4_block_bytes(D), TILE_BYTES = 2 * (TK / INT4_BLOCK) * BLOCK_BYTES;
+constexpr float LOG2E = 1.4426950408889634f;
+// Probabilities are held times 2^14, so that small ones keep their digits in float16, while every step of V that a warp has met is
+// below 2; from the first larger step on (values above 14) times 2^-1, so that no product with a step (up to 65504) overflows.
+constexpr float SMALL_SHIFT = 14.f, LARGE_SHIFT = -1.f;
+
+// Keys of one range, by the request's own length alone (so that a sum does not change with the neighbours): 16 ranges or fewer up
+// to 16384 keys, and ranges of 1024 beyond.
+__host__ __device__ inline int range_keys(int ctx) {
+    int keys = 128;
+    while (keys < 1024 && ctx > 16 * keys) keys *= 2;
+    return keys;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {        // of an 8 x 8 matrix of 16-bit elements spread over a warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two codes n, subnormals n 2^-24 (EXPONENT 15) or n 2^-20 (11), as (n - 8) 2^-9: exact, in one instruction.
+template <int EXPONENT> __device__ __forceinline__ uint32_t centred(uint32_t n) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&n), __float2half2_rn((float)(1 << EXPONENT)), __float2half2_rn(-8.f / 512.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float low_half(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x & 0xffff))); }
+__device__ __forceinline__ float high_half(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x >> 16))); }
+
+template <int N> struct Share { uint32_t w[(N + 3) / 4]; };         // N neighbouring bytes of shared memory, as wide as they are aligned
+template <int N> __device__ __forceinline__ Share<N> load_share(const unsigned char* p) {
+    Share<N> s;
+    if constexpr (N == 16) { const uint4 v = *reinterpret_cast<const uint4*>(p); s.w[0] = v.x; s.w[1] = v.y; s.w[2] = v.z; s.w[3] = v.w; }
+    else if constexpr (N == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); s.w[0] = v.x; s.w[1] = v.y; }
+    else if constexpr (N % 4 == 0) { for (int i = 0; i < N / 4; ++i) s.w[i] = reinterpret_cast<const uint32_t*>(p)[i]; }
+    else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        for (int i = 0; i < N / 2; i += 2) s.w[i / 2] = h[i] | (i + 1 < N / 2 ? (uint32_t)h[i + 1] << 16 : 0u);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+struct Args {
+    const T* q; T* out;
+    const unsigned char* k_cache; const unsigned char* v_cache;
+    const int* req_slot; const int* table; int width;
+    const int* q_start; const int* q_len; const int* ctx_len;
+    float* partial;      // [tile][kv head][row][split][D]
+    float* stats;        // [tile][kv head][row][split][2]: largest score (base 2, less the shift), sum
+    float* scores;       // [tile][kv head][longest][row_stride], base 2, or null
+    int max_queries, tiles, row_stride, n_splits, longest;
+    int hq, hkv, page_size, window, keep_first;
+    float scale, sink_all; const float* sink_heads;
+    int* error;
+};
+
+// What the rows of one (request, tile of 8 NT query rows, range of keys) see.
+struct Span { int req, n, ctx, group, row0, rows, first_pos, last_pos, ranges, lo, hi; };
+template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x, int split) {
+    s.req = x / a.tiles;
+    const int tile = x - s.req * a.tiles;
+    s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.group = a.hq / a.hkv; s.row0 = tile * ROWS;
+    s.rows = min(ROWS, s.n * s.group - s.row0);
+    if (s.n > a.max_queries || s.rows <= 0) return false;           // another kernel's request, or no such tile
+    if (s.ctx > a.longest) {                                        // more rows than the scratch was made for
+        if (threadIdx.x == 0) atomicExch(a.error, 6);
+        return false;
+    }
+    s.first_pos = s.ctx - s.n + s.row0 / s.group;
+    s.last_pos = s.ctx - s.n + (s.row0 + s.rows - 1) / s.group;
+    const int keys = range_keys(s.ctx);
+    s.ranges = s.ctx > 0 ? (s.ctx + keys - 1) / keys : 0;
+    s.lo = split * keys;
+    s.hi = min(s.lo + keys, s.last_pos + 1);
+    if (a.window > 0 && s.lo >= a.keep_first) s.lo = max(s.lo, s.first_pos - a.window + 1);
+    else if (a.window > 0 && s.first_pos - a.window + 1 >= s.hi) s.hi = min(s.hi, a.keep_first);
+    return true;
+}
+
+__device__ __forceinline__ bool in_sight(const Span& s, const Args& a, int key) {       // of some row of the tile
+    return key >= s.lo && key < s.hi && (a.window <= 0 || key >= s.first_pos - a.window + 1 || key < a.keep_first);
+}
+
+// NT: columns of 8 query rows.  Where there are two, or float queries, codes serve two matrix instructions, and the offset is
+// subtracted from them (and the subnormals made normal) by one instruction for two.  The matrix instructions align their
+// products by the operands' exponent fields, so that a sum over subnormals keeps some 2^-18 of its largest term only: far below the
+// rounding of a bfloat16 output, but not of a float one.
+template <int NT>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) attn_int4_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT;
+    constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
+    constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
+    constexpr int MERGE_STRIDE = D + 2;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint64_t full[WARPS * STAGES];
+    __shared__ int failed;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+    pdl_wait();
+    Span span;
+    if (!find_span<ROWS>(span, a, blockIdx.x, split)) return;
+    const size_t base_row = ((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride;
+    const bool direct = span.ranges <= 1;                           // nothing to merge: the finished rows go out
+    if (split > 0 && split >= span.ranges) return;                  // a range beyond the request's own length
+    if (span.lo >= span.hi) {                                       // behind the window, or no keys at all
+        if (direct) {
+            for (int e = tid; e < span.rows * D; e += THREADS) {
+                const int r = span.row0 + e / D;
+                a.out[((size_t)(a.q_start[span.req] + r / span.group) * a.hq + kvh * span.group + r % span.group) * D + e % D] = from_float<T>(0.f);
+            }
+        }
+        for (int r = tid; r < span.rows; r += THREADS) {
+            float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
+            st[0] = -INFINITY; st[1] = 0.f;
+        }
+        return;
+    }
+    const int* pages = a.table + (size_t)a.req_slot[span.req] * a.width;
+    if (tid == 0) {
+        failed = 0;
+        for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(full + i, 1);
+        mbar_init_fence();
+    }
+    __syncthreads();
+
+    const int base = span.lo & ~(TK - 1), n_tiles = (span.hi - base + TK - 1) / TK;
+    unsigned char* ring = smem + (size_t)warp * STAGES * TILE_BYTES;
+    uint64_t* bars = full + warp * STAGES;
+    // Tile t into stage `slot`: one copy per plane and run of blocks that lie in one page, by as many lanes.  Blocks behind the last key and
+    // pages that are not there are left out: what the stage holds in their place meets no probability.
+    const int page_blocks = a.page_size / INT4_BLOCK;
+    const int run = page_blocks % 4 == 0 ? 4 : page_blocks % 2 == 0 ? 2 : 1;
+    const auto fetch = [&](int t, int slot) {
+        const int b = (lane & 3) * run, pos = base + t * TK + b * INT4_BLOCK;
+        const bool is_v = lane >= 4;
+        const long long at = lane < 8 && b < 4 && pos < span.hi ? int4_block_at(pages, a.width, pos, a.page_size, a.hkv, kvh, D) : -1;
+        const unsigned copies = __popc(__ballot_sync(0xffffffffu, at >= 0));
+        if (lane == 0) mbar_expect_tx(bars + slot, copies * run * BLOCK_BYTES);
+        __syncwarp();
+        if (at >= 0) bulk_load(ring + (size_t)slot * TILE_BYTES + (is_v ? TILE_BYTES / 2 : 0) + b * BLOCK_BYTES, (is_v ? a.v_cache : a.k_cache) + at, run * BLOCK_BYTES, bars + slot);
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+        if (warp + WARPS * i < n_tiles) fetch(warp + WARPS * i, i);
+
+    // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
+    // after the shift, (2, 6), (3, 7) / 16.
+    uint32_t qf[NT][NG][2][TERMS][2];
+    float offset[NT][NG][2], unit[NT][2];
+    int reach[NT][2], behind[NT][2];                                // a column's last place in sight, and the first inside its window
+    const int tok0 = a.q_start[span.req];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        const bool there = r < span.rows;
+        const int row = span.row0 + (there ? r : 0);
+        const T* q = a.q + ((size_t)(tok0 + row / span.group) * a.hq + kvh * span.group + row % span.group) * D;
+        float x[NG][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+#if STORAGE_BF16
+            const uint4 v = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[j][2 * i] = __uint_as_float(w[i] << 16); x[j][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+#else
+            const float4 u = *reinterpret_cast<const float4*>(q + 32 * j + 8 * c), v = *reinterpret_cast<const float4*>(q + 32 * j + 8 * c + 4);
+            x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w; x[j][4] = v.x; x[j][5] = v.y; x[j][6] = v.z; x[j][7] = v.w;
+#endif
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!there) x[j][i] = 0.f;
+                top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
+            }
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int up = min(14 - ((int)(top >> 23) - 127), 120);     // the row times 2^up is below 2^15
+        const float factor = __uint_as_float((uint32_t)(up + 127) << 23);
+        float sum[NG];
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            sum[j] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float p[4] = {x[j][2 * k] * factor, x[j][2 * k + 4] * factor, x[j][2 * k + 1] * factor * SECOND, x[j][2 * k + 5] * factor * SECOND};
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t w = pack_f16(p[2 * h], p[2 * h + 1]);
+                        qf[nt][j][k][term][h] = w;
+                        const float lo = low_half(w), hi = high_half(w);
+                        if (OFFSET) sum[j] += (h ? 16.f : 1.f) * (lo + hi);
+                        p[2 * h] -= lo; p[2 * h + 1] -= hi;
+                    }
+            }
+            if constexpr (OFFSET) {
+                sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+                sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) offset[nt][j][h] = OFFSET ? -0x1p-21f * __shfl_sync(0xffffffffu, sum[j], 4 * (2 * c + h)) : 0.f;      // -8 2^-24 sum q
+        }
+        const float mine = a.scale * LOG2E * (OFFSET ? 0x1p24f : 0x1p9f) * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            unit[nt][h] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + h));
+            const int pos = span.ctx - span.n + (span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1)) / span.group;
+            reach[nt][h] = pos;
+            behind[nt][h] = a.window > 0 ? pos - a.window + 1 : 0;
+        }
+    }
+    const int sure_lo = a.window > 0 ? span.last_pos - a.window + 1 : 0;      // keys in [sure_lo, first_pos] are in sight of every row
+    float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < (OFFSET ? NG : 1); ++i) r_off[i][nt][0] = r_off[i][nt][1] = r_off[i][nt][2] = r_off[i][nt][3] = 0.f;
+        m_run[nt][0] = m_run[nt][1] = -INFINITY;
+        l_run[nt][0] = l_run[nt][1] = 0.f;
+    }
+    float shift = SMALL_SHIFT;
+    // alpha of column h into everything that is summed
+    const auto rescale = [&](int nt, float a0, float a1) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) { o[i][nt][0] *= a0; o[i][nt][1] *= a1; o[i][nt][2] *= a0; o[i][nt][3] *= a1; }
+        if constexpr (OFFSET) {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) { r_off[i][nt][0] *= a0; r_off[i][nt][1] *= a1; r_off[i][nt][2] *= a0; r_off[i][nt][3] *= a1; }
+        }
+        l_run[nt][0] *= a0; l_run[nt][1] *= a1;
+    };
+
+    for (int t = warp, it = 0; t < n_tiles; t += WARPS, ++it) {
+        const int slot = it % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + slot, (uint32_t)(it / STAGES) & 1))) {
+            if (lane == 0) { atomicExch(a.error, 3); failed = 1; }
+            for (int i = 0; i < STAGES; ++i)                        // another bounded chance for this warp's copies to land before the stages are given up
+                if (t + WARPS * i < n_tiles) mbar_wait(bars + (it + i) % STAGES, (uint32_t)((it + i) / STAGES) & 1);
+            break;
+        }
+        const unsigned char* ks = ring + (size_t)slot * TILE_BYTES;
+        const unsigned char* vs = ks + TILE_BYTES / 2;
+        const int k0 = base + t * TK;
+        const bool edge = k0 + TK > span.first_pos + 1 || k0 < sure_lo || k0 < span.lo;       // the same for the whole warp
+
+        float s[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                               // 16 keys: blocks 2 h and 2 h + 1
+            const unsigned char* b0 = ks + 2 * h * BLOCK_BYTES;
+            const unsigned char* b1 = b0 + BLOCK_BYTES;
+            const Share<4 * NG> w0 = load_share<4 * NG>(b0 + g * (D / 2) + c * 4 * NG), w1 = load_share<4 * NG>(b1 + g * (D / 2) + c * 4 * NG);
+            const Share<2 * NG> s0 = load_share<2 * NG>(b0 + 4 * D + g * 2 * NG), s1 = load_share<2 * NG>(b1 + 4 * D + g * 2 * NG);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                float acc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) { acc[nt][0] = acc[nt][2] = offset[nt][j][0]; acc[nt][1] = acc[nt][3] = offset[nt][j][1]; }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t x = k ? w0.w[j] >> 8 : w0.w[j], y = k ? w1.w[j] >> 8 : w1.w[j];
+                    uint32_t a0 = x & 0x000f000fu, a1 = y & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = y & 0x00f000f0u;
+                    if constexpr (!OFFSET) { a0 = centred<15>(a0); a1 = centred<15>(a1); a2 = centred<11>(a2); a3 = centred<11>(a3); }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
+                }
+                const float f0 = j & 1 ? high_half(s0.w[j / 2]) : low_half(s0.w[j / 2]), f1 = j & 1 ? high_half(s1.w[j / 2]) : low_half(s1.w[j / 2]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[h][nt][0] = j ? fmaf(f0, acc[nt][0], s[h][nt][0]) : f0 * acc[nt][0];
+                    s[h][nt][1] = j ? fmaf(f0, acc[nt][1], s[h][nt][1]) : f0 * acc[nt][1];
+                    s[h][nt][2] = j ? fmaf(f1, acc[nt][2], s[h][nt][2]) : f1 * acc[nt][2];
+                    s[h][nt][3] = j ? fmaf(f1, acc[nt][3], s[h][nt][3]) : f1 * acc[nt][3];
+                }
+            }
+        }
+        bool more = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = s[h][nt][e] * unit[nt][e & 1];
+                    if (edge) {
+                        const int key = k0 + 16 * h + g + 8 * (e >> 1);
+                        const bool seen = key <= reach[nt][e & 1] && (key >= behind[nt][e & 1] || key < a.keep_first) && key >= span.lo && key < span.hi;
+                        v = seen ? v : -INFINITY;
+                    }
+                    s[h][nt][e] = v;
+                    more |= v > m_run[nt][e & 1];
+                }
+        if (a.scores) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const int key = k0 + 16 * h + g + 8 * (e >> 1), col = nt * 8 + 2 * c;
+                        if (key < span.hi && col < span.rows)
+                            *reinterpret_cast<float2*>(a.scores + (((size_t)blockIdx.x * a.hkv + kvh) * a.longest + key) * a.row_stride + col) = make_float2(s[h][nt][e], s[h][nt][e + 1]);
+                    }
+        }
+        // The running maximum follows only when a score exceeds it (rarely, after the first tiles).
+        if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float alpha[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float m_new = fmaxf(m_run[nt][e], mx);
+                    alpha[e] = m_run[nt][e] == m_new ? 1.f : exp2_fast(m_run[nt][e] - m_new);
+                    m_run[nt][e] = m_new;
+                }
+                rescale(nt, alpha[0], alpha[1]);
+            }
+        }
+        // steps of V: those of two neighbouring keys side by side; a large one changes the probabilities' shift for good
+        Share<4 * NG> sv[4];
+        uint32_t any = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            sv[b] = load_share<4 * NG>(vs + b * BLOCK_BYTES + 4 * D + c * 4 * NG);
+            if (edge) {                                             // steps that belong to no key in sight of any row: whatever lies there
+                const int key = k0 + 8 * b + 2 * c;
+                const uint32_t keep = (in_sight(span, a, key) ? 0xffffu : 0u) | (in_sight(span, a, key + 1) ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int j = 0; j < NG; ++j) sv[b].w[j] &= keep;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j) any |= sv[b].w[j];
+        }
+        if (shift == SMALL_SHIFT && __any_sync(0xffffffffu, any & 0x40004000u)) {
+            shift = LARGE_SHIFT;
+            constexpr float down = 1.f / 32768.f;                   // 2^(LARGE_SHIFT - SMALL_SHIFT)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) rescale(nt, down, down);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float top = (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e]) - shift;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float p0 = exp2_fast(s[h][nt][e] - top), p1 = exp2_fast(s[h][nt][e + 2] - top);
+                    l_run[nt][e] += p0 + p1;
+                    if (edge) {                                     // a key out of sight gets -0, by which it is told from one of no weight
+                        if (s[h][nt][e] == -INFINITY) p0 = -0.f;
+                        if (s[h][nt][e + 2] == -INFINITY) p1 = -0.f;
+                    }
+                    s[h][nt][e] = p0; s[h][nt][e + 2] = p1;
+                }
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // probabilities as B: rows of the product above are keys, here columns: two 8 x 8 transpositions per 16 keys
+            uint32_t pt[NT][2];
+#if STORAGE_BF16
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                pt[nt][0] = transposed(pack_f16(s[h][nt][0], s[h][nt][1]));
+                pt[nt][1] = transposed(pack_f16(s[h][nt][2], s[h][nt][3]));
+            }
+#endif
+            const unsigned char* b0 = vs + 2 * h * BLOCK_BYTES;
+            const unsigned char* b1 = b0 + BLOCK_BYTES;
+            const int turned = (g ^ int4_value_turn<D>(c)) * 2 * NG;
+            const Share<2 * NG> u0 = load_share<2 * NG>(b0 + c * (D / 2) + turned), u1 = load_share<2 * NG>(b0 + (4 + c) * (D / 2) + turned);
+            const Share<2 * NG> u2 = load_share<2 * NG>(b1 + c * (D / 2) + turned), u3 = load_share<2 * NG>(b1 + (4 + c) * (D / 2) + turned);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                // B of this group: probability times step, of two keys a register
+                uint32_t pb[NT][TERMS][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#if STORAGE_BF16
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t v = mul_f16x2(pt[nt][b], sv[2 * h + b].w[j]);
+                        if (edge) v &= ~__vcmpeq2(pt[nt][b], 0x80008000u);      // out of sight: nothing, whatever the step there is
+                        pb[nt][0][b] = v;
+                    }
+#else
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        // before the transposition a lane has keys of row g: its step is half of the word of the pair of rows g / 2
+                        const uint32_t pair = __shfl_sync(0xffffffffu, sv[2 * h + b].w[j], g >> 1);
+                        const float step = g & 1 ? high_half(pair) : low_half(pair);
+                        float v0 = s[h][nt][2 * b] * step, v1 = s[h][nt][2 * b + 1] * step;
+                        if (edge) {
+                            if (__float_as_uint(s[h][nt][2 * b]) == 0x80000000u) v0 = 0.f;
+                            if (__float_as_uint(s[h][nt][2 * b + 1]) == 0x80000000u) v1 = 0.f;
+                        }
+                        const uint32_t hi = pack_f16(v0, v1);
+                        pb[nt][0][b] = transposed(hi);
+                        pb[nt][TERMS - 1][b] = transposed(pack_f16(v0 - low_half(hi), v1 - high_half(hi)));
+                    }
+#endif
+                }
+                const uint32_t r0 = __byte_perm(u0.w[j / 2], u1.w[j / 2], j & 1 ? 0x7632 : 0x5410);      // keys 2 c and 2 c + 1 of the first block
+                const uint32_t r1 = __byte_perm(u2.w[j / 2], u3.w[j / 2], j & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t x = k ? r0 >> 8 : r0, y = k ? r1 >> 8 : r1;
+                    uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    if constexpr (!OFFSET) { a0 = centred<15>(a0); a1 = centred<11>(a1); a2 = centred<15>(a2); a3 = centred<11>(a3); }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term) mma_f16(o[2 * j + k][nt], a0, a1, a2, a3, pb[nt][term][0], pb[nt][term][1]);
+                }
+                if constexpr (OFFSET) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int term = 0; term < TERMS; ++term)
+                            mma_f16(r_off[j][nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pb[nt][term][0], pb[nt][term][1]);
+                }
+            }
+        }
+        __syncwarp();                                               // every lane has read the stage
+        if (t + WARPS * STAGES < n_tiles) fetch(t + WARPS * STAGES, slot);
+    }
+    __syncthreads();                                                // every warp is done with its stages: they become the merge area
+    if (failed) return;                                             // the host reads the error flag
+    float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float l = l_run[nt][h];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            float* row = merge + ((size_t)warp * ROWS + nt * 8 + 2 * c + h) * MERGE_STRIDE;
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float off = OFFSET ? r_off[OFFSET ? j : 0][nt][h] : 0.f;
+                    constexpr float whole = OFFSET ? 0x1p24f : 0x1p9f;
+                    row[32 * j + 4 * g + 2 * k] = (o[2 * j + k][nt][h] - off) * whole;
+                    row[32 * j + 4 * g + 2 * k + 1] = (o[2 * j + k][nt][2 + h] * SECOND - off) * whole;
+                }
+            if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : m_run[nt][h] - shift; row[D + 1] = l; }
+        }
+    __syncthreads();
+    for (int e = tid; e < span.rows * D; e += THREADS) {
+        const int r = e / D, d = e - r * D;
+        float m = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, merge[((size_t)w * ROWS + r) * MERGE_STRIDE + D]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float* row = merge + ((size_t)w * ROWS + r) * MERGE_STRIDE;
+            const float wgt = row[D] == -INFINITY ? 0.f : exp2_fast(row[D] - m);
+            if (row[D] != -INFINITY) { num = fmaf(wgt, row[d], num); den = fmaf(wgt, row[D + 1], den); }
+            else if (!(row[D + 1] == 0.f)) den = NAN;               // scores that are not numbers have no largest
+        }
+        if (direct) {
+            const int row = span.row0 + r, head = kvh * span.group + row % span.group;
+            const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
+            float whole = den;
+            if (sink > -INFINITY) whole += exp2f(fmaf(sink, LOG2E, -m));       // one more term of the denominator, no value
+            a.out[((size_t)(tok0 + row / span.group) * a.hq + head) * D + d] = from_float<T>(den == 0.f ? 0.f : num / whole);
+        } else {
+            a.partial[((base_row + r) * a.n_splits + split) * D + d] = num;
+        }
+        if (d == 0) {
+            float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
+            st[0] = m; st[1] = den;
+        }
+    }
+}
+
+// Ranges of a row put together: a thread per output dimension, the ranges in their order.
+template <int ROWS>
+__global__ void __launch_bounds__(D) attn_int4_merge_kernel(const __grid_constant__ Args a) {
+    pdl_wait();
+    Span span;
+    if (!find_span<ROWS>(span, a, blockIdx.x, 0) || span.ranges <= 1) return;
+    const int r = blockIdx.z, kvh = blockIdx.y, d = threadIdx.x;
+    if (r >= span.rows) return;
+    const size_t base = (((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride + r) * a.n_splits;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + base;
+    float m = -INFINITY;
+    for (int i = 0; i < span.ranges; ++i) m = fmaxf(m, stats[i].x);
+    float num = 0.f, den = 0.f;
+    for (int i0 = 0; i0 < span.ranges; i0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i0 + i < span.ranges ? a.partial[(base + i0 + i) * D + d] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= span.ranges) continue;
+            const float2 st = stats[i0 + i];
+            if (st.x > -INFINITY) {
+                const float w = exp2_fast(st.x - m);
+                num = fmaf(w, v[i], num);
+                den = fmaf(w, st.y, den);
+            } else if (!(st.y == 0.f)) {
+                den = NAN;
+            }
+        }
+    }
+    const int row = span.row0 + r, head = kvh * span.group + row % span.group;
+    const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
+    float whole = den;
+    if (sink > -INFINITY) whole += exp2f(fmaf(sink, LOG2E, -m));
+    a.out[((size_t)(a.q_start[span.req] + row / span.group) * a.hq + head) * D + d] = from_float<T>(den == 0.f ? 0.f : num / whole);
+}
+
+// The weights of the keys: every key of a request gets the sum over the key head's query rows of 2^(score - max) / denominator added to
+// its number in `mass` [pages][hkv][page_size].  The rows in their order, so the sum does not change from run to run.
+constexpr int MASS_THREADS = 256, MASS_ROWS = 128;                  // rows whose denominators are at hand at a time
+template <int ROWS>
+__global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __grid_constant__ Args a, float* __restrict__ mass, int keys_per_block) {
+    __shared__ float lse[MASS_ROWS];
+    pdl_wait();
+    const int req = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
+    const int n = a.q_len[req], ctx = a.ctx_len[req], group = a.hq / a.hkv, rows = n * group;
+    if (n > a.max_queries || n <= 0 || ctx > a.longest) return;
+    const int keys = range_keys(ctx), ranges = (ctx + keys - 1) / keys;
+    const int lo = blockIdx.z * keys_per_block, hi = min(lo + keys_per_block, ctx);
+    if (lo >= hi) return;
+    const int* pages = a.table + (size_t)a.req_slot[req] * a.width;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};                              // keys_per_block is 4 MASS_THREADS at most
+    for (int row0 = 0; row0 < rows; row0 += MASS_ROWS) {
+        __syncthreads();
+        for (int r = tid; r < min(MASS_ROWS, rows - row0); r += MASS_THREADS) {
+            const int row = row0 + r, tile = row / ROWS;
+            const size_t base = ((((size_t)req * a.tiles + tile) * a.hkv + kvh) * a.row_stride + row - tile * ROWS) * a.n_splits;
+            const float2* stats = reinterpret_cast<const float2*>(a.stats) + base;
+            float m = -INFINITY, den = 0.f;
+            for (int i = 0; i < ranges; ++i) m = fmaxf(m, stats[i].x);
+            for (int i = 0; i < ranges; ++i) if (stats[i].x > -INFINITY) den = fmaf(exp2_fast(stats[i].x - m), stats[i].y, den);
+            const int head = kvh * group + row % group;
+            const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
+            if (sink > -INFINITY) den += exp2f(fmaf(sink, LOG2E, -m));
+            lse[r] = m + log2f(den);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = lo + i * MASS_THREADS + tid;
+            if (key >= hi) continue;
+            for (int r = 0; r < min(MASS_ROWS, rows - row0); ++r) {
+                const int row = row0 + r, tile = row / ROWS, pos = ctx - n + row / group;
+                if (key > pos || (a.window > 0 && pos - key >= a.window && key >= a.keep_first)) continue;
+                w[i] += exp2_fast(a.scores[((((size_t)req * a.tiles + tile) * a.hkv + kvh) * a.longest + key) * a.row_stride + row - tile * ROWS] - lse[r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int key = lo + i * MASS_THREADS + tid;
+        if (key >= hi || key / a.page_size >= a.width) continue;
+        const int page = pages[key / a.page_size];
+        if (page >= 0 && w[i] != 0.f) mass[((size_t)page * a.hkv + kvh) * a.page_size + key % a.page_size] += w[i];
+    }
+}
+
+// How many ranges of keys requests of up to `longest` rows have at most.
+int most_ranges(int longest) {
+    const int keys = range_keys(longest), few = longest < 16 * 128 ? (longest + 127) / 128 : 16, many = (longest + keys - 1) / keys;
+    return few > many ? (few > 1 ? few : 1) : many;
+}
+
+// What a launch has of everything: query rows of a tile (8, or 16 where requests bring more), tiles per request, rows that scratch is kept
+// for (even, so that pairs are aligned), ranges.
+struct Shape {
+    int rows, tiles, stride, splits;
+    long long units;                 // requests by tiles by key heads by rows
+    long long keys;
+    Shape(int n_req, int max_queries, int longest, int hq, int hkv) {
+        const int needed = max_queries * (hq / hkv);
+        rows = needed > 8 ? 16 : 8;
+        tiles = (needed + rows - 1) / rows;
+        stride = ((needed < rows ? needed : rows) + 1) & ~1;
+        splits = most_ranges(longest);
+        units = (long long)n_req * tiles * hkv * stride;
+        keys = longest;
+    }
+    long long partial() const { return splits > 1 ? units * splits * D : 0; }
+    long long stats() const { return units * splits * 2; }
+    long long scores() const { return units * keys; }
+};
+
+bool g_pdl = false;
+int* g_error = nullptr;
+
+template <int NT> int launch(const Args& a, int n_req, float* mass, cudaStream_t s) {
+    constexpr size_t RING = (size_t)WARPS * STAGES * TILE_BYTES, MERGE = sizeof(float) * WARPS * 8 * NT * (D + 2);
+    constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
+    static_assert(SMEM <= 48 * 1024, "no opt-in to more shared memory");
+    const dim3 grid((unsigned)(n_req * a.tiles), (unsigned)a.hkv, (unsigned)a.n_splits);
+    int status = launch_kernel(attn_int4_kernel<NT>, grid, dim3(THREADS), SMEM, s, g_pdl, a);
+    if (status) return status;
+    if (a.n_splits > 1) {
+        status = launch_kernel(attn_int4_merge_kernel<8 * NT>, dim3(grid.x, grid.y, (unsigned)a.row_stride), dim3(D), 0, s, true, a);
+        if (status) return status;
+    }
+    if (mass) {
+        const int per = 4 * MASS_THREADS;
+        status = launch_kernel(attn_int4_mass_kernel<8 * NT>, dim3((unsigned)n_req, (unsigned)a.hkv, (unsigned)((a.longest + per - 1) / per)), dim3(MASS_THREADS), 0, s, true, a, mass, per);
+    }
+    return status;
+}
+}  // namespace
+
+CISR_EXPORT void cisr_attn_int4_set_pdl(int on) { g_pdl = on != 0; }
+CISR_EXPORT int cisr_attn_int4_head_dim() { return D; }
+// `error_flag`: one zeroed int in device memory that the kernel sets when a wait on a copy ran out.
+CISR_EXPORT int cisr_attn_int4_init(int* error_flag) { g_error = error_flag; return 0; }
+
+// Floats of scratch that a call with these sizes takes (partial sums and statistics of the ranges, with `mass` also the scores).
+CISR_EXPORT long long cisr_attn_int4_scratch(int n_req, int max_queries, int longest, int hq, int hkv, int with_mass) {
+    const Shape s(n_req, max_queries, longest, hq, hkv);
+    return s.partial() + s.stats() + (with_mass ? s.scores() : 0);
+}
+
+// q, out [tokens][hq][D]; request r brings q_len[r] tokens from row q_start[r] on and has ctx_len[r] rows with them; those with more than
+// `max_queries` are left alone, and none may have more than `longest` rows (one that has sets the error flag).
+CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, const void* v_cache, const int* req_slot, const int* block_table, int width,
+                               const int* q_start, const int* q_len, const int* ctx_len, float* scratch, float* mass, int n_req, int max_queries, int longest,
+                               int hq, int hkv, int page_size, float scale, int window, int keep_first, float sink, const float* sink_heads, void* stream) {
+    if (n_req <= 0 || max_queries <= 0) return 0;
+    if (!g_error) return -13;
+    if (hkv <= 0 || hkv > 65535 || hq % hkv || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 7) return -2;      // rows are read by 16 bytes
+    const Shape shape(n_req, max_queries, longest, hq, hkv);
+    if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
+    Args a{};
+    a.q = (const T*)q; a.out = (T*)out; a.k_cache = (const unsigned char*)k_cache; a.v_cache = (const unsigned char*)v_cache;
+    a.req_slot = req_slot; a.table = block_table; a.width = width; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len;
+    a.partial = scratch; a.stats = scratch + shape.partial(); a.scores = mass ? a.stats + shape.stats() : nullptr;
+    a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits;
+    a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
+    a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
+    return shape.rows == 8 ? launch<1>(a, n_req, mass, (cudaStream_t)stream) : launch<2>(a, n_req, mass, (cudaStream_t)stream);
+}
+
+// Kernels that such a call launches.
+CISR_EXPORT int cisr_attn_int4_launches(int longest, int with_mass) { return 1 + (most_ranges(longest) > 1) + (with_mass != 0); }

@@ -1,0 +1,431 @@
+// Rows of a cache held in 4 bits (int4_cache.cuh): new keys and values brought in, rows handed back as values, and the rows
+// that attention has looked at least taken out.
+//
+// All of these move memory: a row of keys and values is 4 D bytes as bfloat16 and 9 D / 8 as held.  Head sizes 32, 64, 96 and 128.
+#include "int4_cache.cuh"
+
+namespace {
+constexpr int THREADS = 256;
+
+struct Place {                       // where a step's rows lie: token t belongs to request token_req[t] and has place positions[t] there;
+    const int* token_req;            // without lists, token t of row blockIdx.y of the grid is place t of that request
+    const int* positions;
+    const int* req_slot;
+    const int* table;
+    int width, page_size;
+};
+
+template <typename T> __device__ __forceinline__ void load4(const T* p, float* x, bool wide);
+template <> __device__ __forceinline__ void load4<float>(const float* p, float* x, bool wide) {
+    if (wide) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        for (int i = 0; i < 4; ++i) x[i] = p[i];
+    }
+}
+template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* x, bool wide) {
+    if (wide) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+    } else {
+        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const float* x);
+template <> __device__ __forceinline__ void store4<float>(float* p, const float* x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float* x) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// The step of a group from the bits of its largest magnitude (as whole numbers these order like the magnitudes, NaN above infinity).
+__device__ __forceinline__ __half step_of(uint32_t top) {
+    if (top >= 0x7f800000u) return __ushort_as_half((unsigned short)0x7e00u);
+    return __float2half_rn(fminf(__uint_as_float(top) * (1.f / 7.f), 65504.f));
+}
+// x / s to the nearest whole number, ties to even, within -7 .. 7; `inv` is 1 / s.  The product x inv is off by an ulp or two, which could
+// tip a quotient next to a half: the remainder x - t s is a float without rounding (t s has at most 15 digits and x lies within
+// a step of it) and says whether the next whole number is nearer.
+__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
+    float t = rintf(x * inv);
+    const float r = fmaf(-t, s, x), twice = 2.f * fabsf(r);
+    if (twice > s || (twice == s && ((int)t & 1))) t += copysignf(1.f, r);
+    t = s > 0.f ? fminf(fmaxf(t, -7.f), 7.f) : 0.f;
+    return (uint32_t)((int)t + 8);
+}
+
+template <int N> struct Word;
+template <> struct Word<2> { typedef unsigned short type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<16> { typedef uint4 type; };
+// `BYTES` neighbouring bytes (a lane's share of a row), as wide as they are aligned; 6 and 12 (head size 96) as their thirds.
+template <int BYTES> __device__ __forceinline__ void copy_share(void* to, const void* from) {
+    constexpr int PART = BYTES % 3 ? BYTES : BYTES / 3;
+    typedef typename Word<PART>::type W;
+    for (int i = 0; i < BYTES / PART; ++i) reinterpret_cast<W*>(to)[i] = reinterpret_cast<const W*>(from)[i];
+}
+
+// Keys: four lanes a row, lane c with the 8 neighbours 32 j + 8 c of every group j.  Values: eight lanes a row, lane g with the 4
+// neighbours 32 u + 4 g of every group u.  So a lane writes its codes of the row by one store, and a group's largest
+// magnitude is two or three shuffles away.  A warp does 8 rows of keys, or 4 of values.
+template <int D, typename T, bool VALUES>
+__device__ __forceinline__ void store_rows(const T* __restrict__ x, long long token_stride, long long head_stride, unsigned char* __restrict__ cache, float* __restrict__ mass, const Place& at,
+                                           int tokens, int hkv, bool wide, int unit) {
+    constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
+    const int lane = threadIdx.x % LANES;
+    const long long row = (long long)unit * (THREADS / LANES) + threadIdx.x / LANES;      // row = token * hkv + head
+    const bool inside = row < (long long)tokens * hkv;
+    const int token = inside ? (int)(row / hkv) : 0, head = inside ? (int)(row - (long long)token * hkv) : 0;
+    const int pos = inside ? at.positions[token] : -1;
+    const long long block = inside ? int4_block_at(at.table + (size_t)at.req_slot[at.token_req[token]] * at.width, at.width, pos, at.page_size, hkv, head, D) : -1;
+    const T* from = x + token * token_stride + head * head_stride;
+    float v[NG][PER];
+    uint32_t top[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+        top[j] = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            if (block >= 0) load4<T>(from + 32 * j + PER * lane + i, &v[j][i], wide);
+            else v[j][i] = v[j][i + 1] = v[j][i + 2] = v[j][i + 3] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) top[j] = max(top[j], __float_as_uint(v[j][i]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int o = 1; o < LANES; o *= 2) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+    if (block < 0) return;
+    alignas(16) __half step[NG];
+    union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+        step[j] = step_of(top[j]);
+        const float s = __half2float(step[j]), inv = 1.f / s;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) w |= code_of(v[j][i], s, inv) << (4 * i);
+        if (VALUES) code.half[j] = (unsigned short)w;
+        else code.word[j] = w;
+    }
+    const int r = pos % INT4_BLOCK;
+    unsigned char* to = cache + block;
+    if (VALUES) {
+        const int slot = int4_value_slot(r);
+        copy_share<2 * NG>(to + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG, &code);
+        if (lane < NG) {
+            __half mine = step[0];
+#pragma unroll
+            for (int j = 1; j < NG; ++j) if (lane == j) mine = step[j];
+            reinterpret_cast<__half*>(to + 4 * D)[((r >> 1) * NG + lane) * 2 + (r & 1)] = mine;
+        }
+    } else {
+        copy_share<4 * NG>(to + r * (D / 2) + lane * 4 * NG, &code);
+        if (lane == 0) {
+            copy_share<2 * NG>(to + 4 * D + r * 2 * NG, step);
+            if (mass) mass[block / int4_block_bytes(D) * INT4_BLOCK + r] = 0.f;
+        }
+    }
+}
+
+// One thread block row of the grid for the keys (blockIdx.y 0), one for the values.  us with 8192 tokens of 8 heads of 128: see int4_store.
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_token, long long k_head, long long v_token,
+                                                             long long v_head, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
+                                                             Place at, int tokens, int hkv, int wide) {
+    pdl_wait();
+    const long long rows = (long long)tokens * hkv;
+    const int key_units = (int)((rows + THREADS / 4 - 1) / (THREADS / 4));
+    if ((int)blockIdx.x < key_units) store_rows<D, T, false>(k, k_token, k_head, k_cache, mass, at, tokens, hkv, wide & 1, blockIdx.x);
+    else store_rows<D, T, true>(v, v_token, v_head, v_cache, mass, at, tokens, hkv, wide & 2, blockIdx.x - key_units);
+    pdl_trigger();
+}
+
+// Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
+// request's end, give zeros.
+template <int D, typename T, bool VALUES>
+__device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
+                                          const Place& at, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv, int unit) {
+    constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
+    const int lane = threadIdx.x % LANES;
+    const long long row = (long long)unit * (THREADS / LANES) + threadIdx.x / LANES;
+    if (row >= (long long)tokens * hkv) return;
+    int token, head, req, pos;
+    if (ends) {                      // neighbouring rows of a head lie side by side
+        head = (int)(row / tokens); token = (int)(row - (long long)head * tokens);
+        req = which ? which[blockIdx.y] : blockIdx.y; pos = token < ends[req] ? token : -1;
+    } else {
+        token = (int)(row / hkv); head = (int)(row - (long long)token * hkv);
+        req = at.token_req[token]; pos = at.positions[token];
+    }
+    const long long block = int4_block_at(at.table + (size_t)at.req_slot[req] * at.width, at.width, pos, at.page_size, hkv, head, D);
+    union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
+    float step[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) step[j] = 0.f;
+    const int r = pos & (INT4_BLOCK - 1);
+    if (block >= 0) {
+        const unsigned char* from = cache + block;
+        if (VALUES) {
+            const int slot = int4_value_slot(r);
+            copy_share<2 * NG>(&code, from + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) step[j] = __half2float(reinterpret_cast<const __half*>(from + 4 * D)[((r >> 1) * NG + j) * 2 + (r & 1)]);
+        } else {
+            copy_share<4 * NG>(&code, from + r * (D / 2) + lane * 4 * NG);
+            alignas(16) __half held[NG];
+            copy_share<2 * NG>(held, from + 4 * D + r * 2 * NG);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) step[j] = __half2float(held[j]);
+        }
+    }
+    T* to = out + (ends ? blockIdx.y * req_stride : 0) + token * token_stride + head * head_stride;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+        const uint32_t w = VALUES ? code.half[j] : code.word[j];
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = block >= 0 ? (float)((int)((w >> (4 * (i + e))) & 15) - 8) * step[j] : 0.f;
+            store4<T>(to + 32 * j + PER * lane + i, x);
+        }
+    }
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
+                                                            T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
+                                                            const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv) {
+    pdl_wait();
+    const long long rows = (long long)tokens * hkv;
+    const int key_units = (int)((rows + THREADS / 4 - 1) / (THREADS / 4));
+    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv, blockIdx.x);
+    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv, blockIdx.x - key_units);
+    pdl_trigger();
+}
+
+// ------------------------------------------------------------------ eviction
+// Of a request's `len` rows stay, per key head, the first `first`, the last `recent`, and of those between the `keep - first - recent` with
+// the largest sums, equal ones by the lowest place; NaN counts as the largest.  Two kernels: one finds the places and
+// lists them in order, the other moves the rows (and their sums) to the request's new pages.
+//
+// The choice is a search for the smallest sum that stays: the bits of a float, turned so that they order like the numbers, are found two at
+// a time, by counting how many sums reach each of three thresholds (16 passes over shared memory).
+constexpr int SELECT_THREADS = 1024, SELECT_CACHED = 48 * 1024;     // sums that fit shared memory; longer requests are read again in every pass
+
+__device__ __forceinline__ uint32_t ordered(float x) {
+    if (isnan(x)) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(x + 0.f);                    // -0 becomes 0
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(SELECT_THREADS) int4_select_kernel(const float* __restrict__ mass, const int* __restrict__ req_slot, const int* __restrict__ table,
+                                                                     int width, const int* __restrict__ ctx_len, int* __restrict__ kept, int hkv, int page_size,
+                                                                     int keep, int recent, int first, int cached) {
+    extern __shared__ uint32_t sums[];
+    __shared__ int count[2][3];
+    __shared__ int of_warp[2][32];
+    pdl_wait();
+    const int head = blockIdx.x, req = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int* pages = table + (size_t)req_slot[req] * width;
+    const int len = min(max(ctx_len[req], 0), (int)min((long long)width * page_size, 0x7fffffffll));
+    int* out = kept + ((size_t)req * hkv + head) * keep;
+    if (len <= keep) {
+        for (int i = tid; i < keep; i += SELECT_THREADS) out[i] = i < len ? i : -1;
+        return;
+    }
+    const int begin = first, n = len - recent - first, want = keep - recent - first;       // of n rows from `begin` on, `want` stay; want < n
+    const auto fetch = [&](int i) -> uint32_t {
+        const int pos = begin + i, page = pages[pos / page_size];
+        return page < 0 ? 0u : ordered(mass[((size_t)page * hkv + head) * page_size + pos % page_size]);
+    };
+    const bool in_shared = n <= cached;
+    if (in_shared) for (int i = tid; i < n; i += SELECT_THREADS) sums[i] = fetch(i);
+    if (tid < 6) (&count[0][0])[tid] = 0;
+    __syncthreads();
+    const auto at = [&](int i) -> uint32_t { return in_shared ? sums[i] : fetch(i); };
+    uint32_t floor_ = 0;                                            // the largest threshold that `want` sums or more reach
+    if (want > 0) {
+        for (int bit = 30; bit >= 0; bit -= 2) {
+            const int turn = (bit >> 1) & 1;
+            const uint32_t t1 = floor_ | 1u << bit, t2 = floor_ | 2u << bit, t3 = floor_ | 3u << bit;
+            int c1 = 0, c2 = 0, c3 = 0;
+            for (int i = tid; i < n; i += SELECT_THREADS) {
+                const uint32_t s = at(i);
+                c1 += s >= t1; c2 += s >= t2; c3 += s >= t3;
+            }
+            c1 = __reduce_add_sync(0xffffffffu, c1); c2 = __reduce_add_sync(0xffffffffu, c2); c3 = __reduce_add_sync(0xffffffffu, c3);
+            if (lane < 3) {
+                const int c = lane == 0 ? c1 : lane == 1 ? c2 : c3;
+                if (c) atomicAdd(&count[turn][lane], c);
+            }
+            __syncthreads();
+            floor_ |= (count[turn][2] >= want ? 3u : count[turn][1] >= want ? 2u : count[turn][0] >= want ? 1u : 0u) << bit;
+            if (tid < 3) count[turn ^ 1][tid] = 0;                  // last read before the barrier above, written again behind the next pass
+            __syncthreads();
+        }
+    }
+    // Places in order: a thread owns a run of neighbours (of odd length, so that runs start in different banks), counts those above the
+    // floor and those on it, and learns by a scan over the block how many lie before its run.
+    const int per = ((n + SELECT_THREADS - 1) / SELECT_THREADS) | 1, lo = min(n, tid * per), hi = min(n, lo + per);
+    int above = 0, equal = 0;
+    if (want > 0) {
+        for (int i = lo; i < hi; ++i) {
+            const uint32_t s = at(i);
+            above += s > floor_; equal += s == floor_;
+        }
+    }
+    int above_before = above, equal_before = equal;
+    for (int o = 1; o < 32; o *= 2) {
+        const int a = __shfl_up_sync(0xffffffffu, above_before, o), e = __shfl_up_sync(0xffffffffu, equal_before, o);
+        if (lane >= o) { above_before += a; equal_before += e; }
+    }
+    if (lane == 31) { of_warp[0][warp] = above_before; of_warp[1][warp] = equal_before; }
+    __syncthreads();
+    int a_sum = of_warp[0][lane], e_sum = of_warp[1][lane];
+    const int a_total = __reduce_add_sync(0xffffffffu, a_sum);
+    a_sum = lane < warp ? a_sum : 0; e_sum = lane < warp ? e_sum : 0;
+    above_before += __reduce_add_sync(0xffffffffu, a_sum) - above;
+    equal_before += __reduce_add_sync(0xffffffffu, e_sum) - equal;
+    const int spare = want - a_total;                               // of those on the floor, the first `spare` stay
+    if (want > 0) {
+        for (int i = lo; i < hi; ++i) {
+            const uint32_t s = at(i);
+            const bool stays = s > floor_ || (s == floor_ && equal_before < spare);
+            if (stays) out[first + above_before + min(equal_before, spare)] = begin + i;
+            above_before += s > floor_; equal_before += s == floor_;
+        }
+    }
+    for (int i = tid; i < first; i += SELECT_THREADS) out[i] = i;
+    for (int i = tid; i < recent; i += SELECT_THREADS) out[keep - recent + i] = len - recent + i;
+}
+
+// A warp moves the rows of one new block of 8: lane (r, c) a quarter of row r of the keys, of the row in slot r of the values, a step of
+// each, and (c = 0) the row's sum.
+template <int D>
+__global__ void __launch_bounds__(THREADS) int4_move_kernel(unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
+                                                            const int* __restrict__ req_slot, const int* __restrict__ table, int width,
+                                                            const int* __restrict__ to_table, int to_width, const int* __restrict__ kept, int hkv, int page_size, int keep) {
+    constexpr int NG = D / 32;
+    pdl_wait();
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = blockIdx.y, req = blockIdx.z;
+    const int first_row = (blockIdx.x * (THREADS / 32) + threadIdx.x / 32) * INT4_BLOCK;
+    if (first_row >= keep) return;
+    const long long to = int4_block_at(to_table + (size_t)req * to_width, to_width, first_row, page_size, hkv, head, D);
+    if (to < 0) return;
+    const int* pages = table + (size_t)req_slot[req] * width;
+    const int* places = kept + ((size_t)req * hkv + head) * keep;
+    const int slot_row = 2 * (r & 3) + (r >> 2);                    // the row in slot r of the values
+    const int key_pos = first_row + r < keep ? places[first_row + r] : -1;
+    const int value_pos = first_row + slot_row < keep ? places[first_row + slot_row] : -1;
+    const long long key_at = int4_block_at(pages, width, key_pos, page_size, hkv, head, D);
+    const long long value_at = int4_block_at(pages, width, value_pos, page_size, hkv, head, D);
+    if (key_at >= 0) {
+        const int from_r = key_pos % INT4_BLOCK;
+        copy_share<4 * NG>(k_cache + to + r * (D / 2) + c * 4 * NG, k_cache + key_at + from_r * (D / 2) + c * 4 * NG);
+        if (c < NG) *reinterpret_cast<__half*>(k_cache + to + 4 * D + (r * NG + c) * 2) = *reinterpret_cast<const __half*>(k_cache + key_at + 4 * D + (from_r * NG + c) * 2);
+        if (c == 0) {
+            const int logical = key_pos / page_size, to_logical = first_row / page_size;
+            mass[((size_t)to_table[(size_t)req * to_width + to_logical] * hkv + head) * page_size + first_row - to_logical * page_size + r] =
+                mass[((size_t)pages[logical] * hkv + head) * page_size + key_pos - logical * page_size];
+        }
+    }
+    if (value_at >= 0) {
+        const int from_r = value_pos % INT4_BLOCK, from_slot = int4_value_slot(from_r);
+        const int turned = int4_value_turn<D>(r) != int4_value_turn<D>(from_slot) ? 2 : 0;      // eighths exchanged four by four: quarters two by two
+        copy_share<4 * NG>(v_cache + to + r * (D / 2) + c * 4 * NG, v_cache + value_at + from_slot * (D / 2) + (c ^ turned) * 4 * NG);
+        if (c < NG)
+            *reinterpret_cast<__half*>(v_cache + to + 4 * D + (((slot_row >> 1) * NG + c) * 2 + (slot_row & 1)) * 2) =
+                *reinterpret_cast<const __half*>(v_cache + value_at + 4 * D + (((from_r >> 1) * NG + c) * 2 + (from_r & 1)) * 2);
+    }
+}
+
+bool g_pdl = false;
+
+template <typename F> int by_head_size(int dim, F f) {
+    switch (dim) {
+        case 32: return f(std::integral_constant<int, 32>());
+        case 64: return f(std::integral_constant<int, 64>());
+        case 96: return f(std::integral_constant<int, 96>());
+        case 128: return f(std::integral_constant<int, 128>());
+        default: return -2;
+    }
+}
+// Thread blocks for a launch over `rows` rows of keys (4 lanes each) and as many of values (8 lanes).
+long long units(long long rows) { return (rows + THREADS / 4 - 1) / (THREADS / 4) + (rows + THREADS / 8 - 1) / (THREADS / 8); }
+}  // namespace
+
+CISR_EXPORT void cisr_int4_rows_set_pdl(int on) { g_pdl = on != 0; }
+
+// k, v [tokens][hkv][dim] with strides in values; codes go to place positions[t] of request token_req[t], whose number in `mass` (if any) becomes 0.
+CISR_EXPORT int cisr_int4_store(const void* k, const void* v, int dtype, long long k_token, long long k_head, long long v_token, long long v_head, void* k_cache,
+                                void* v_cache, float* mass, const int* token_req, const int* positions, const int* req_slot, const int* block_table, int width, int page_size,
+                                int tokens, int hkv, int dim, void* stream) {
+    if (tokens <= 0) return 0;
+    if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || ((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
+    const long long blocks = units((long long)tokens * hkv);
+    if (blocks >= 1ll << 31) return -2;
+    const int per16 = dtype == CISR_F32 ? 4 : 8;
+    const int wide = (((uintptr_t)k & 15) == 0 && k_token % per16 == 0 && k_head % per16 == 0 ? 1 : 0) | (((uintptr_t)v & 15) == 0 && v_token % per16 == 0 && v_head % per16 == 0 ? 2 : 0);
+    const Place at{token_req, positions, req_slot, block_table, width, page_size};
+    return by_head_size(dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (dtype == CISR_F32)
+            return launch_kernel(int4_store_kernel<D, float>, dim3((unsigned)blocks), dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const float*)k, (const float*)v, k_token,
+                                 k_head, v_token, v_head, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, at, tokens, hkv, wide);
+        return launch_kernel(int4_store_kernel<D, __nv_bfloat16>, dim3((unsigned)blocks), dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const __nv_bfloat16*)k,
+                             (const __nv_bfloat16*)v, k_token, k_head, v_token, v_head, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, at, tokens, hkv, wide);
+    });
+}
+
+// The reverse: rows (token_req[t], positions[t]) into k, v [tokens][hkv][dim]; or, with `ends`, places 0 .. tokens - 1 of each of n_req
+// requests (request which[i], or i without a list) into [n_req][..] with the strides given; places from ends[request] on give zeros.
+CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k, void* v, int dtype, long long req_stride, long long token_stride, long long head_stride,
+                               const int* token_req, const int* positions, const int* req_slot, const int* block_table, int width, int page_size, const int* ends,
+                               const int* which, int n_req, int tokens, int hkv, int dim, void* stream) {
+    if (tokens <= 0 || n_req <= 0) return 0;
+    if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535) return -2;
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15 || token_stride % 4 || head_stride % 4 || req_stride % 4) return -2;
+    const long long blocks = units((long long)tokens * hkv);
+    if (blocks >= 1ll << 31) return -2;
+    const Place at{token_req, positions, req_slot, block_table, width, page_size};
+    const dim3 grid((unsigned)blocks, (unsigned)n_req);
+    return by_head_size(dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (dtype == CISR_F32)
+            return launch_kernel(int4_read_kernel<D, float>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
+                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv);
+        return launch_kernel(int4_read_kernel<D, __nv_bfloat16>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
+                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv);
+    });
+}
+
+// Places that stay into kept [n_req][hkv][keep] (-1 behind the last), their rows and sums to the pages of to_table [n_req][to_width].
+// `longest`: no request has more rows.
+CISR_EXPORT int cisr_int4_evict(void* k_cache, void* v_cache, float* mass, const int* req_slot, const int* block_table, int width, const int* ctx_len, int* kept,
+                                const int* to_table, int to_width, int n_req, int hkv, int dim, int page_size, int keep, int recent, int first, int longest, void* stream) {
+    if (n_req <= 0 || keep <= 0) return 0;
+    if (hkv <= 0 || hkv > 65535 || n_req > 65535 || page_size <= 0 || page_size % INT4_BLOCK || recent < 0 || first < 0 || recent > keep || first > keep - recent) return -2;
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
+    const int between = longest - recent - first;
+    const int cached = between < 0 ? 0 : between < SELECT_CACHED ? between : SELECT_CACHED;
+    const size_t smem = sizeof(uint32_t) * (size_t)(cached < SELECT_CACHED ? cached : SELECT_CACHED);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(int4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(uint32_t) * SELECT_CACHED));
+        if (e != cudaSuccess) return (int)e;
+    }
+    const cudaStream_t s = (cudaStream_t)stream;
+    const int status = launch_kernel(int4_select_kernel, dim3(hkv, n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)mass, req_slot, block_table, width, ctx_len, kept,
+                                     hkv, page_size, keep, recent, first, cached);
+    if (status) return status;
+    const dim3 grid((unsigned)((keep + INT4_BLOCK * (THREADS / 32) - 1) / (INT4_BLOCK * (THREADS / 32))), hkv, n_req);
+    return by_head_size(dim, [&](auto d) {
+        return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, req_slot, block_table,
+                             width, to_table, to_width, (const int*)kept, hkv, page_size, keep);
+    });
+}

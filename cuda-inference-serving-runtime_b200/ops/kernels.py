@@ -525,6 +525,224 @@ def attn_decode(q, out, k_cache, v_cache, req_slot, block_table, dec_req, n_dec,
                own=-(-(hq // hkv) // 16) + (1 if merge else 0))
 
 
+# ------------------------------------------------------------------ a cache held in 4 bits (csrc/int4_cache.cuh says how)
+INT4_GROUP = 32                  # values along a head that share a step
+INT4_BLOCK = 8                   # rows of a block; a page is whole blocks
+INT4_HEAD_DIMS = (32, 64, 96, 128)
+INT4_FEW = 16                    # new tokens of a request up to which attn_decode_int4 is the faster call (see attn_prefill_int4)
+_int4_rows_state = {}
+_attention_int4_libs = {}
+
+
+def int4_jobs(head_dim: int, dtype: torch.dtype):
+    """The build jobs of a 4-bit cache for this head size and type of queries."""
+    return [("int4_rows.cu", {}, ()), ("attention_int4.cu", {"HEAD_DIM": head_dim, "STORAGE_BF16": dtype_code(dtype)}, ())]
+
+
+def _int4_rows():
+    lib = _int4_rows_state.get("lib")
+    if lib is None:
+        lib = load_library("int4_rows.cu")
+        lib.cisr_int4_rows_set_pdl(int(_pdl_state["on"]))
+        _int4_rows_state["lib"] = lib
+    return lib
+
+
+def _attention_int4(head_dim: int, dtype: torch.dtype):
+    lib = _attention_int4_libs.get((head_dim, dtype))
+    if lib is None:
+        lib = load_library("attention_int4.cu", {"HEAD_DIM": head_dim, "STORAGE_BF16": dtype_code(dtype)})
+        assert lib.cisr_attn_int4_head_dim() == head_dim
+        _check(lib.cisr_attn_int4_init(_p(_error_flag())), "4-bit attention init", own=0)
+        lib.cisr_attn_int4_set_pdl(int(_pdl_state["on"]))
+        _attention_int4_libs[(head_dim, dtype)] = lib
+    return lib
+
+
+def int4_page_bytes(page_size: int, head_dim: int) -> int:
+    """Bytes of one page of one key head: `page_size` rows of keys, or of values."""
+    if page_size <= 0 or page_size % INT4_BLOCK:
+        raise KernelError(f"a page of a 4-bit cache holds a multiple of {INT4_BLOCK} rows, not {page_size}")
+    if head_dim not in INT4_HEAD_DIMS:
+        raise KernelError(f"a 4-bit cache takes head sizes {', '.join(map(str, INT4_HEAD_DIMS))}, not {head_dim}")
+    return page_size * 9 * head_dim // 16
+
+
+def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, hkv: Optional[int], dim: int) -> int:
+    """Checks a pair of 4-bit caches; the number of key heads."""
+    _need(k_cache, torch.uint8, "k_cache", 3); _need(v_cache, torch.uint8, "v_cache", 3)
+    if k_cache.shape != v_cache.shape or k_cache.shape[2] != int4_page_bytes(page_size, dim) or (hkv is not None and k_cache.shape[1] != hkv):
+        raise KernelError(f"{what}: a cache of {page_size} rows a page is [pages, kv_heads, {int4_page_bytes(page_size, dim)}] bytes at head size {dim}, "
+                          f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if _device is not None and k_cache.device.index != _device():
+        raise KernelError(f"{what}: the cache is on {k_cache.device}, the current device is cuda:{_device()}")
+    return k_cache.shape[1]
+
+
+def _int4_lists(what: str, device, table: torch.Tensor, count: int, **lists) -> None:
+    _need(table, torch.int32, "block_table", 2)
+    for name, t in lists.items():
+        _need(t, torch.int32, name, 1)
+        if t.device != device:
+            raise KernelError(f"{what}: {name} is on {t.device}, the cache on {device}")
+        if name != "req_slot" and t.numel() != count:
+            raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
+
+
+def _int4_mass(what: str, mass: torch.Tensor, k_cache: torch.Tensor, page_size: int) -> None:
+    _need(mass, torch.float32, "mass", 3)
+    if tuple(mass.shape) != (k_cache.shape[0], k_cache.shape[1], page_size) or mass.device != k_cache.device:
+        raise KernelError(f"{what}: mass must be [pages, kv_heads, page_size] on the cache's device")
+
+
+def _int4_rows_like(what: str, name: str, t: torch.Tensor, device) -> None:
+    if t.device != device or t.dim() != 3 or t.stride(2) != 1 or t.dtype not in _DTYPE_CODE:
+        raise KernelError(f"{what}: {name} must be float32 or bfloat16 [tokens, kv_heads, head_dim] with neighbouring values, on the cache's device")
+
+
+def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, token_req: torch.Tensor, positions: torch.Tensor,
+               req_slot: torch.Tensor, block_table: torch.Tensor, page_size: int, mass: Optional[torch.Tensor] = None) -> None:
+    """Bring new keys and values k, v [tokens, kv_heads, head_dim] (any strides between rows) into a 4-bit cache: token t becomes row
+    positions[t] of request token_req[t].  k_cache, v_cache: uint8 [pages, kv_heads, int4_page_bytes]; a row whose page
+    the table does not have is left out.  `mass` float [pages, kv_heads, page_size] (`attn_decode_int4`): the new rows' numbers become 0.
+
+    A value is held as c s: s the largest magnitude of its group of 32 neighbours over 7, in float16 (65504 at most: magnitudes beyond
+    458,528 are cut there), c the whole number nearest to x / s, so it is off by half of s and the rounding of s itself.  A
+    group that holds an infinity or a NaN becomes NaN."""
+    device = k_cache.device
+    _int4_rows_like("int4_store", "k", k, device); _int4_rows_like("int4_store", "v", v, device)
+    tokens, hkv, dim = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise KernelError("int4_store: k and v differ in shape or type")
+    _int4_cache("int4_store", k_cache, v_cache, page_size, hkv, dim)
+    _int4_lists("int4_store", device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
+    if mass is not None:
+        _int4_mass("int4_store", mass, k_cache, page_size)
+    _check(_int4_rows().cisr_int4_store(_p(k), _p(v), dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _p(k_cache), _p(v_cache),
+                                        _p(mass), _p(token_req), _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, tokens, hkv, dim,
+                                        _stream()), "int4_store")
+
+
+def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, token_req: torch.Tensor, positions: torch.Tensor,
+              req_slot: torch.Tensor, block_table: torch.Tensor, page_size: int) -> None:
+    """The reverse of `int4_store`: k_out, v_out [tokens, kv_heads, head_dim] become the values that rows positions[t] of requests
+    token_req[t] stand for (zeros where the table has no page)."""
+    _need(k_out, None, "k_out", 3); _need(v_out, k_out.dtype, "v_out", 3)
+    tokens, hkv, dim = k_out.shape
+    if v_out.shape != k_out.shape or k_out.device != k_cache.device:
+        raise KernelError("int4_read: k_out and v_out differ in shape, or lie elsewhere than the cache")
+    _int4_cache("int4_read", k_cache, v_cache, page_size, hkv, dim)
+    _int4_lists("int4_read", k_cache.device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
+    _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), 0, hkv * dim, dim, _p(token_req),
+                                       _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, 0, 0, 1, tokens, hkv, dim, _stream()), "int4_read")
+
+
+def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
+                ctx_len: torch.Tensor, page_size: int, requests: Optional[torch.Tensor] = None) -> None:
+    """Whole requests as values: k_out, v_out [requests, kv_heads, rows, head_dim] become rows 0 .. rows - 1 of every request (of those that
+    `requests` lists, where it is given), zeros from ctx_len[r] on."""
+    _need(k_out, None, "k_out", 4); _need(v_out, k_out.dtype, "v_out", 4)
+    n, hkv, rows, dim = k_out.shape
+    if v_out.shape != k_out.shape or k_out.device != k_cache.device:
+        raise KernelError("int4_expand: k_out and v_out differ in shape, or lie elsewhere than the cache")
+    _int4_cache("int4_expand", k_cache, v_cache, page_size, hkv, dim)
+    if requests is None:
+        _int4_lists("int4_expand", k_cache.device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+    else:
+        _int4_lists("int4_expand", k_cache.device, block_table, n, req_slot=req_slot, requests=requests)
+        _need(ctx_len, torch.int32, "ctx_len", 1)
+    _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), hkv * rows * dim, dim, rows * dim, 0, 0,
+                                       _p(req_slot), _p(block_table), block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()),
+           "int4_expand")
+
+
+def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
+                     q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_queries: int, longest: int, page_size: int, scale: float,
+                     window: Optional[int] = None, sink=None, keep_first: int = 0, mass: Optional[torch.Tensor] = None) -> None:
+    """Attention of a few new tokens per request (one in a decode step) over a 4-bit cache: q, out [tokens, heads, head_dim].
+    Request r brings q_len[r] tokens from row q_start[r] of q on and has ctx_len[r] rows in the cache, theirs included; requests that
+    bring none, or more than `max_queries`, are left alone.  `longest`: no request has more rows (a bound will do; one that has sets the
+    flag that `raise_if_kernel_gave_up` reads).  window, sink, keep_first: as for `attn_decode`.
+
+    `mass` float [pages, kv_heads, page_size]: every key's number grows by the weights that the query heads of its key head, and all of
+    the request's new tokens, have given it (a sink takes its part of them)."""
+    _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
+    tokens, hq, dim = q.shape
+    if out.shape != q.shape:
+        raise KernelError("attn_decode_int4: q and out differ in shape")
+    hkv = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
+    n = q_len.numel()
+    _int4_lists("attn_decode_int4", k_cache.device, block_table, n, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len)
+    if hq % hkv or max_queries < 1 or longest < 1 or req_slot.numel() < n or q.device != k_cache.device or out.device != k_cache.device:
+        raise KernelError("attn_decode_int4: heads, limits, lists or devices disagree")
+    if (window is not None and window < 1) or keep_first < 0:
+        raise KernelError("attn_decode_int4: a window has at least one key, and keep_first is not negative")
+    if mass is not None:
+        _int4_mass("attn_decode_int4", mass, k_cache, page_size)
+    lib = _attention_int4(dim, q.dtype)
+    scratch = torch.empty(lib.cisr_attn_int4_scratch(n, max_queries, longest, hq, hkv, mass is not None), dtype=torch.float32, device=k_cache.device)
+    _check(lib.cisr_attn_int4(_p(q), _p(out), _p(k_cache), _p(v_cache), _p(req_slot), _p(block_table), block_table.shape[1], _p(q_start), _p(q_len), _p(ctx_len),
+                              _p(scratch), _p(mass), n, max_queries, longest, hq, hkv, page_size, scale, window or 0, keep_first, *_sink(sink, hq), _stream()),
+           "attn_decode_int4", own=lib.cisr_attn_int4_launches(longest, mass is not None))
+
+
+def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
+                      tile_req: torch.Tensor, tile_q0: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, longest: int, page_size: int,
+                      scale: float, window: Optional[int] = None, sink=None, keep_first: int = 0, span: int = PREFILL_TILE,
+                      portions: Optional[tuple] = None) -> None:
+    """Attention of portions of prompts over a 4-bit cache: the requests' rows are written out as values once, and the prompt attention
+    of the queries' type runs over those, so codes are turned into operands once per key and not once per tile of queries.
+    Tiles of `span` queries as (request, first query): 64 as for `attn_prefill`, 128 or 256 (bfloat16, head sizes 64 and 128) as for
+    `attn_prefill_wide`.  `longest`: no request that is written out has more rows.  `portions` (requests, places): the requests
+    that are written out, and for every request of the step its place in that list (any number for the others); None: all, in order."""
+    _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
+    hq, dim = q.shape[1], q.shape[2]
+    hkv = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
+    n_all = q_len.numel()
+    if longest < 1 or hq % hkv or out.shape != q.shape or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.device != k_cache.device:
+        raise KernelError("attn_prefill_int4: heads, limits, shapes, devices or the span disagree")
+    requests, places = (None, None) if portions is None else portions
+    n = n_all if requests is None else requests.numel()
+    if places is None:
+        places = torch.arange(n, dtype=torch.int32, device=q.device)
+    _int4_lists("attn_prefill_int4", k_cache.device, block_table, n_all, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len, places=places)
+    rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
+    k, v = torch.empty((2, n, hkv, rows, dim), dtype=q.dtype, device=q.device)
+    int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
+    table = places.view(-1, 1) if requests is None else torch.arange(n, dtype=torch.int32, device=q.device).view(-1, 1)
+    if span == PREFILL_TILE:
+        attn_prefill(q, out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first)
+    else:
+        attn_prefill_wide(q, out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first,
+                          span=span)
+
+
+def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,
+               to_table: torch.Tensor, kept: torch.Tensor, page_size: int, longest: int, recent: int, first: int = 0) -> None:
+    """Cut every request down to `keep` rows by the weight that attention has given them: per key head stay its first `first` rows, its last
+    `recent`, and of those between the ones with the largest `mass` (of equal ones the lowest place; NaN counts as the largest), in
+    their order.  kept int32 [requests, kv_heads, keep] becomes the places that stay (-1 behind the last; a request of
+    `keep` rows or fewer keeps all), and the rows go, with their mass, to the pages that row r of to_table [requests, width] names
+    for request r.  Those must be no page that any request still reads (the request's own old pages among them): nothing is
+    moved in place, so shared pages stay as they are.  Rows of the new pages behind the last kept one are left as they were.
+    `longest`: no request has more rows (longer ones are right, but slower)."""
+    _need(kept, torch.int32, "kept", 3); _need(to_table, torch.int32, "to_table", 2)
+    n, hkv, keep = kept.shape
+    bytes_ = k_cache.shape[2] if k_cache.dim() == 3 else 0
+    dim = bytes_ * 16 // (9 * page_size) if page_size > 0 else 0
+    _int4_cache("int4_evict", k_cache, v_cache, page_size, hkv, dim)
+    _int4_lists("int4_evict", k_cache.device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+    _int4_mass("int4_evict", mass, k_cache, page_size)
+    if kept.device != k_cache.device or to_table.device != k_cache.device:
+        raise KernelError("int4_evict: kept and to_table must lie on the cache's device")
+    if req_slot.numel() < n or to_table.shape[0] != n or to_table.shape[1] * page_size < keep or longest < 1:
+        raise KernelError("int4_evict: req_slot and to_table need an entry per request, and to_table room for the rows that stay")
+    if recent < 0 or first < 0 or first + recent > keep:
+        raise KernelError(f"int4_evict: {first} first and {recent} recent rows do not fit {keep} that stay")
+    _check(_int4_rows().cisr_int4_evict(_p(k_cache), _p(v_cache), _p(mass), _p(req_slot), _p(block_table), block_table.shape[1], _p(ctx_len), _p(kept), _p(to_table),
+                                        to_table.shape[1], n, hkv, dim, page_size, keep, recent, first, longest, _stream()), "int4_evict", own=2)
+
+
 # ------------------------------------------------------------------ merge of the key ranges + output projection (decode steps)
 _merge_proj_state = {}
 
@@ -1940,6 +2158,10 @@ def set_pdl(on: bool) -> None:
         _ffn_rows_state["lib"].cisr_ffn_rows_set_pdl(int(on))
     if "lib" in _tcgen05_state:
         _tcgen05_state["lib"].cisr_gemm_tcgen05_set_pdl(int(on))
+    if "lib" in _int4_rows_state:
+        _int4_rows_state["lib"].cisr_int4_rows_set_pdl(int(on))
+    for lib in _attention_int4_libs.values():
+        lib.cisr_attn_int4_set_pdl(int(on))
     for (source, *_), lib in list(_attention_libs.items()):
         if source == "attention_mma.cu":
             lib.cisr_attn_set_pdl(int(on))
@@ -2298,7 +2520,8 @@ def gemm_tcgen05_rope(a: torch.Tensor, w: torch.Tensor, rope: dict) -> None:
 _GAVE_UP = {1: "a tcgen05 matrix product gave up waiting on a barrier",
             3: "an attention kernel gave up waiting on a tensor-map copy",
             4: "a weight-streaming product gave up waiting on a tensor-map copy",
-            5: "the tcgen05 attention gave up waiting on a barrier"}
+            5: "the tcgen05 attention gave up waiting on a barrier",
+            6: "an attention over a 4-bit cache met a request longer than the bound it was given"}
 
 
 def error_flag_tensor() -> Optional[torch.Tensor]:
@@ -2440,6 +2663,13 @@ _DESCRIBE = {
     "attn_decode": lambda q, out, k_cache, v_cache, req_slot, block_table, dec_req, n_dec, *rest, **kw:
         (int(n_dec), int(q.shape[1]), int(k_cache.shape[1]), int(q.shape[2]), bool(kw.get("merge", True)), k_cache.data_ptr() == v_cache.data_ptr(),
          int(rest[8] or 0)),
+    # (tokens, query heads, key heads, head width, longest) of attention; (tokens or requests, key heads, head width) of rows
+    "int4_store": lambda k, *a, **kw: tuple(int(n) for n in k.shape),
+    "int4_read": lambda k_cache, v_cache, k_out, *a, **kw: tuple(int(n) for n in k_out.shape),
+    "int4_expand": lambda k_cache, v_cache, k_out, *a, **kw: tuple(int(n) for n in k_out.shape),
+    "attn_decode_int4": lambda q, out, k_cache, v_cache, req_slot, block_table, q_start, q_len, ctx_len, max_queries, longest, *a, **kw:
+        (int(q.shape[0]), int(q.shape[1]), int(k_cache.shape[1]), int(q.shape[2]), int(longest)),
+    "int4_evict": lambda k_cache, v_cache, mass, req_slot, block_table, ctx_len, to_table, kept, *a, **kw: tuple(int(n) for n in kept.shape),
     "merge_out_proj": lambda partial, stats, n_splits, dec_req, q_start, n_dec, hq, dim, w, out, **kw:
         (int(n_dec), int(w.shape[0]), int(w.shape[1]), int(n_splits)),
     "sample": lambda logits, *rest, **kw: (int(logits.shape[0]), int(logits.shape[1])),
