@@ -38,22 +38,19 @@ constexpr int TERMS = 1;
 typedef float T;
 constexpr int TERMS = 2;
 #endif
-constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int TK = 32;                                             // keys of a warp's tile: four blocks of 8
-constexpr int STAGES = 2;
+constexpr int STAGES = 2;                                          // tiles that a warp has on the way
 constexpr int BLOCK_BYTES = int4_block_bytes(D), TILE_BYTES = 2 * (TK / INT4_BLOCK) * BLOCK_BYTES;
 constexpr float LOG2E = 1.4426950408889634f;
 // Probabilities are held times 2^14, so that small ones keep their digits in float16, while every step of V that a warp has met is
 // below 2; from the first larger step on (values above 14) times 2^-1, so that no product with a step (up to 65504) overflows.
 constexpr float SMALL_SHIFT = 14.f, LARGE_SHIFT = -1.f;
 
-// Keys of one range, by the request's own length alone (so that a sum does not change with the neighbours): 16 ranges or fewer up
-// to 16384 keys, and ranges of 1024 beyond.
-__host__ __device__ inline int range_keys(int ctx) {
-    int keys = 128;
-    while (keys < 1024 && ctx > 16 * keys) keys *= 2;
-    return keys;
-}
+constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
+
+// Warps of a thread block: eight where a warp's registers let two such blocks share an SM.
+template <int NT> constexpr int warps_of() { return NT == 1 && TERMS == 1 ? 8 : 4; }
+template <int NT> constexpr int blocks_of() { return NT == 1 ? (TERMS == 1 ? 2 : 3) : 2; }
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -99,24 +96,42 @@ __device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t b
                  ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
+// n / d for n below 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divider {
+    uint32_t d, m, shift;
+    __host__ __device__ Divider() : d(1), m(0), shift(0) {}
+    explicit Divider(uint32_t d_) : d(d_), shift(0) {
+        while ((1u << shift) < d) ++shift;                          // d >= 2
+        m = (uint32_t)((1ull << (31 + shift)) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)(__umulhi((uint32_t)n, m) >> (shift - 1)); }
+};
+
 struct Args {
     const T* q; T* out;
     const unsigned char* k_cache; const unsigned char* v_cache;
     const int* req_slot; const int* table; int width;
     const int* q_start; const int* q_len; const int* ctx_len;
-    float* partial;      // [tile][kv head][row][split][D]
-    float* stats;        // [tile][kv head][row][split][2]: largest score (base 2, less the shift), sum
+    float* partial;      // [tile][kv head][row][split][D], where the splits are not one cluster
+    float* stats;        // [tile][kv head][row][split or 1][2]: largest score (base 2, less the shift), sum
     float* scores;       // [tile][kv head][longest][row_stride], base 2, or null
-    int max_queries, tiles, row_stride, n_splits, longest;
+    float* mass;         // added to by this kernel itself, or null
+    int max_queries, tiles, row_stride, n_splits, cluster, longest;
     int hq, hkv, page_size, window, keep_first;
+    Divider by_page;
     float scale, sink_all; const float* sink_heads;
     int* error;
 };
 
-// What the rows of one (request, tile of 8 NT query rows, range of keys) see.
-struct Span { int req, n, ctx, group, row0, rows, first_pos, last_pos, ranges, lo, hi; };
-template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x, int split) {
-    s.req = x / a.tiles;
+// What the rows of one (request, tile of 8 NT query rows) see, as tiles of TK keys: those of the first keys that stay in sight behind a
+// window, then those from the first key inside the first row's window to the last row's own.
+struct Span {
+    int req, n, ctx, group, row0, rows, first_pos, last_pos;
+    int kept_tiles, window_base, tiles;
+    __device__ __forceinline__ int key(int t) const { return t < kept_tiles ? t * TK : window_base + (t - kept_tiles) * TK; }
+};
+template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x) {
+    s.req = a.tiles == 1 ? x : x / a.tiles;
     const int tile = x - s.req * a.tiles;
     s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.group = a.hq / a.hkv; s.row0 = tile * ROWS;
     s.rows = min(ROWS, s.n * s.group - s.row0);
@@ -127,76 +142,102 @@ template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Arg
     }
     s.first_pos = s.ctx - s.n + s.row0 / s.group;
     s.last_pos = s.ctx - s.n + (s.row0 + s.rows - 1) / s.group;
-    const int keys = range_keys(s.ctx);
-    s.ranges = s.ctx > 0 ? (s.ctx + keys - 1) / keys : 0;
-    s.lo = split * keys;
-    s.hi = min(s.lo + keys, s.last_pos + 1);
-    if (a.window > 0 && s.lo >= a.keep_first) s.lo = max(s.lo, s.first_pos - a.window + 1);
-    else if (a.window > 0 && s.first_pos - a.window + 1 >= s.hi) s.hi = min(s.hi, a.keep_first);
+    s.kept_tiles = 0; s.window_base = 0;
+    const int begin = s.first_pos - a.window + 1;
+    if (a.window > 0 && begin >= TK) {
+        s.kept_tiles = min((min(a.keep_first, begin) + TK - 1) / TK, begin / TK);
+        s.window_base = begin & ~(TK - 1);
+    }
+    s.tiles = s.last_pos < 0 ? 0 : s.kept_tiles + (s.last_pos - s.window_base) / TK + 1;
     return true;
 }
-
 __device__ __forceinline__ bool in_sight(const Span& s, const Args& a, int key) {       // of some row of the tile
-    return key >= s.lo && key < s.hi && (a.window <= 0 || key >= s.first_pos - a.window + 1 || key < a.keep_first);
+    return key <= s.last_pos && (a.window <= 0 || key >= s.first_pos - a.window + 1 || key < a.keep_first);
 }
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {      // of another thread block's shared memory
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A part of a row's keys joins the others: sums, largest score and denominator.  A part without a largest score has no keys in sight, or
+// scores that are not numbers, of which its denominator tells.
+struct Joined {
+    float m = -INFINITY, num = 0.f, den = 0.f;
+    __device__ __forceinline__ float weight(float part_m) const { return part_m == -INFINITY ? 0.f : exp2_fast(part_m - m); }
+    __device__ __forceinline__ void add(float part_m, float part_num, float part_den) {
+        if (part_m != -INFINITY) {
+            const float w = weight(part_m);
+            num = fmaf(w, part_num, num);
+            den = fmaf(w, part_den, den);
+        } else if (!(part_den == 0.f)) {
+            den = NAN;
+        }
+    }
+    // with the sink: one more term of the denominator, no value
+    __device__ __forceinline__ float whole(float sink) const { return sink > -INFINITY ? den + exp2f(fmaf(sink, LOG2E, -m)) : den; }
+};
 
 // NT: columns of 8 query rows.  Where there are two, or float queries, codes serve two matrix instructions, and the offset is
 // subtracted from them (and the subnormals made normal) by one instruction for two.  The matrix instructions align their
 // products by the operands' exponent fields, so that a sum over subnormals keeps some 2^-18 of its largest term only: far below the
 // rounding of a bfloat16 output, but not of a float one.
 template <int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) attn_int4_kernel(const __grid_constant__ Args a) {
-    constexpr int ROWS = 8 * NT;
+__global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int4_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT, WARPS = warps_of<NT>(), THREADS = 32 * WARPS;
     constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
     constexpr int MERGE_STRIDE = D + 2;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t full[WARPS * STAGES];
     __shared__ int failed;
+    __shared__ float others[MAX_CLUSTER][ROWS][2], lse[ROWS];       // a cluster's largest scores and denominators; the row's logarithm of its sum
+    __shared__ float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int kvh = blockIdx.y, split = blockIdx.z;
-    pdl_wait();
-    Span span;
-    if (!find_span<ROWS>(span, a, blockIdx.x, split)) return;
-    const size_t base_row = ((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride;
-    const bool direct = span.ranges <= 1;                           // nothing to merge: the finished rows go out
-    if (split > 0 && split >= span.ranges) return;                  // a range beyond the request's own length
-    if (span.lo >= span.hi) {                                       // behind the window, or no keys at all
-        if (direct) {
-            for (int e = tid; e < span.rows * D; e += THREADS) {
-                const int r = span.row0 + e / D;
-                a.out[((size_t)(a.q_start[span.req] + r / span.group) * a.hq + kvh * span.group + r % span.group) * D + e % D] = from_float<T>(0.f);
-            }
-        }
-        for (int r = tid; r < span.rows; r += THREADS) {
-            float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
-            st[0] = -INFINITY; st[1] = 0.f;
-        }
-        return;
-    }
-    const int* pages = a.table + (size_t)a.req_slot[span.req] * a.width;
     if (tid == 0) {
         failed = 0;
         for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(full + i, 1);
         mbar_init_fence();
     }
     __syncthreads();
+    pdl_wait();
+    Span span;
+    if (!find_span<ROWS>(span, a, blockIdx.x)) return;              // the same for a whole cluster
+    const size_t base_row = ((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride;
+    const int* pages = a.table + (size_t)a.req_slot[span.req] * a.width;
+    const int share = (span.tiles + a.n_splits - 1) / a.n_splits;   // tiles of a split: the request's own, so that a cluster ends together
+    const int t0 = split * share, n_tiles = max(0, min(share, span.tiles - t0));
 
-    const int base = span.lo & ~(TK - 1), n_tiles = (span.hi - base + TK - 1) / TK;
     unsigned char* ring = smem + (size_t)warp * STAGES * TILE_BYTES;
     uint64_t* bars = full + warp * STAGES;
     // Tile t into stage `slot`: one copy per plane and run of blocks that lie in one page, by as many lanes.  Blocks behind the last key and
     // pages that are not there are left out: what the stage holds in their place meets no probability.
     const int page_blocks = a.page_size / INT4_BLOCK;
     const int run = page_blocks % 4 == 0 ? 4 : page_blocks % 2 == 0 ? 2 : 1;
+    const int lane_block = (lane & 3) * run;
+    const bool copies_v = lane >= 4;
+    const unsigned char* plane = (copies_v ? a.v_cache : a.k_cache) + (size_t)kvh * page_blocks * BLOCK_BYTES;
+    unsigned char* landing = ring + (copies_v ? TILE_BYTES / 2 : 0) + lane_block * BLOCK_BYTES;
     const auto fetch = [&](int t, int slot) {
-        const int b = (lane & 3) * run, pos = base + t * TK + b * INT4_BLOCK;
-        const bool is_v = lane >= 4;
-        const long long at = lane < 8 && b < 4 && pos < span.hi ? int4_block_at(pages, a.width, pos, a.page_size, a.hkv, kvh, D) : -1;
-        const unsigned copies = __popc(__ballot_sync(0xffffffffu, at >= 0));
+        const int pos = span.key(t0 + t) + lane_block * INT4_BLOCK;
+        int page = -1, inside = 0;
+        if (lane < 8 && lane_block < 4 && pos <= span.last_pos) {
+            const int logical = a.by_page(pos);
+            inside = (pos - logical * a.page_size) / INT4_BLOCK;
+            if (logical < a.width) page = pages[logical];
+        }
+        const unsigned copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_expect_tx(bars + slot, copies * run * BLOCK_BYTES);
         __syncwarp();
-        if (at >= 0) bulk_load(ring + (size_t)slot * TILE_BYTES + (is_v ? TILE_BYTES / 2 : 0) + b * BLOCK_BYTES, (is_v ? a.v_cache : a.k_cache) + at, run * BLOCK_BYTES, bars + slot);
+        if (page >= 0) bulk_load(landing + (size_t)slot * TILE_BYTES, plane + ((size_t)page * a.hkv * page_blocks + inside) * BLOCK_BYTES, run * BLOCK_BYTES, bars + slot);
     };
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
@@ -271,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
             behind[nt][h] = a.window > 0 ? pos - a.window + 1 : 0;
         }
     }
-    const int sure_lo = a.window > 0 ? span.last_pos - a.window + 1 : 0;      // keys in [sure_lo, first_pos] are in sight of every row
+    const int sure_lo = a.window > 0 ? span.last_pos - a.window + 1 : 0;      // keys in [sure_lo, first_pos] are in sight of every row, kept first ones too
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -304,8 +345,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
         }
         const unsigned char* ks = ring + (size_t)slot * TILE_BYTES;
         const unsigned char* vs = ks + TILE_BYTES / 2;
-        const int k0 = base + t * TK;
-        const bool edge = k0 + TK > span.first_pos + 1 || k0 < sure_lo || k0 < span.lo;       // the same for the whole warp
+        const int k0 = span.key(t0 + t);
+        const bool edge = k0 + TK > span.first_pos + 1 || (k0 < sure_lo && k0 + TK > a.keep_first);       // the same for the whole warp
 
         float s[2][NT][4];
 #pragma unroll
@@ -349,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
                     float v = s[h][nt][e] * unit[nt][e & 1];
                     if (edge) {
                         const int key = k0 + 16 * h + g + 8 * (e >> 1);
-                        const bool seen = key <= reach[nt][e & 1] && (key >= behind[nt][e & 1] || key < a.keep_first) && key >= span.lo && key < span.hi;
+                        const bool seen = key <= reach[nt][e & 1] && (key >= behind[nt][e & 1] || key < a.keep_first);
                         v = seen ? v : -INFINITY;
                     }
                     s[h][nt][e] = v;
@@ -363,7 +404,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
                         const int key = k0 + 16 * h + g + 8 * (e >> 1), col = nt * 8 + 2 * c;
-                        if (key < span.hi && col < span.rows)
+                        if (key <= span.last_pos && col < span.rows)
                             *reinterpret_cast<float2*>(a.scores + (((size_t)blockIdx.x * a.hkv + kvh) * a.longest + key) * a.row_stride + col) = make_float2(s[h][nt][e], s[h][nt][e + 1]);
                     }
         }
@@ -493,7 +534,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
         if (t + WARPS * STAGES < n_tiles) fetch(t + WARPS * STAGES, slot);
     }
     __syncthreads();                                                // every warp is done with its stages: they become the merge area
-    if (failed) return;                                             // the host reads the error flag
     float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -516,73 +556,117 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? (TERMS == 1 ? 4 : 3) : 2) a
             if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : m_run[nt][h] - shift; row[D + 1] = l; }
         }
     __syncthreads();
+    // The warps' sums joined, in their order: into the first warp's place for the cluster, or to where they go.
+    const bool alone = a.n_splits == 1, clustered = a.cluster > 1;
+    const auto place = [&](int r) {                                 // of row r in q and out
+        const int row = span.row0 + r;
+        return ((size_t)(tok0 + row / span.group) * a.hq + kvh * span.group + row % span.group) * D;
+    };
+    const auto sink_of = [&](int r) { return a.sink_heads ? a.sink_heads[kvh * span.group + (span.row0 + r) % span.group] : a.sink_all; };
     for (int e = tid; e < span.rows * D; e += THREADS) {
         const int r = e / D, d = e - r * D;
-        float m = -INFINITY, num = 0.f, den = 0.f;
+        Joined j;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, merge[((size_t)w * ROWS + r) * MERGE_STRIDE + D]);
+        for (int w = 0; w < WARPS; ++w) j.m = fmaxf(j.m, merge[((size_t)w * ROWS + r) * MERGE_STRIDE + D]);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float* row = merge + ((size_t)w * ROWS + r) * MERGE_STRIDE;
-            const float wgt = row[D] == -INFINITY ? 0.f : exp2_fast(row[D] - m);
-            if (row[D] != -INFINITY) { num = fmaf(wgt, row[d], num); den = fmaf(wgt, row[D + 1], den); }
-            else if (!(row[D + 1] == 0.f)) den = NAN;               // scores that are not numbers have no largest
+            j.add(row[D], row[d], row[D + 1]);
         }
-        if (direct) {
-            const int row = span.row0 + r, head = kvh * span.group + row % span.group;
-            const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
-            float whole = den;
-            if (sink > -INFINITY) whole += exp2f(fmaf(sink, LOG2E, -m));       // one more term of the denominator, no value
-            a.out[((size_t)(tok0 + row / span.group) * a.hq + head) * D + d] = from_float<T>(den == 0.f ? 0.f : num / whole);
-        } else {
-            a.partial[((base_row + r) * a.n_splits + split) * D + d] = num;
+        if (clustered) {
+            sums[r * MERGE_STRIDE + d] = j.num;
+            if (d == 0) { sums[r * MERGE_STRIDE + D] = j.m; sums[r * MERGE_STRIDE + D + 1] = failed ? NAN : j.den; }
+            continue;
         }
+        if (alone) a.out[place(r) + d] = from_float<T>(j.den == 0.f ? 0.f : j.num / j.whole(sink_of(r)));
+        else a.partial[((base_row + r) * a.n_splits + split) * D + d] = j.num;
         if (d == 0) {
             float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
-            st[0] = m; st[1] = den;
+            st[0] = j.m; st[1] = j.den;
+            lse[r] = j.m + log2f(j.whole(sink_of(r)));
+        }
+    }
+    if (clustered) {
+        // A thread block finishes a slice of the output's dimensions of every row, from all the others' sums.
+        cluster_barrier();
+        const int rank = (int)cluster_rank(), parts = a.cluster;
+        for (int e = tid; e < 2 * span.rows * parts; e += THREADS) {
+            const int p = e / (2 * span.rows), i = e - p * 2 * span.rows;
+            others[p][i >> 1][i & 1] = load_cluster(sums + (i >> 1) * MERGE_STRIDE + D + (i & 1), (uint32_t)p);
+        }
+        __syncthreads();
+        const int cols = (D + parts - 1) / parts;
+        for (int e = tid; e < span.rows * cols; e += THREADS) {
+            const int r = e / cols, d = rank * cols + e - r * cols;
+            if (d >= D) continue;
+            float v[MAX_CLUSTER];
+#pragma unroll
+            for (int p = 0; p < MAX_CLUSTER; ++p) v[p] = p < parts ? load_cluster(sums + r * MERGE_STRIDE + d, (uint32_t)p) : 0.f;
+            Joined j;
+#pragma unroll
+            for (int p = 0; p < MAX_CLUSTER; ++p) if (p < parts) j.m = fmaxf(j.m, others[p][r][0]);
+#pragma unroll
+            for (int p = 0; p < MAX_CLUSTER; ++p) if (p < parts) j.add(others[p][r][0], v[p], others[p][r][1]);
+            a.out[place(r) + d] = from_float<T>(j.den == 0.f ? 0.f : j.num / j.whole(sink_of(r)));
+        }
+        if (tid < span.rows) {
+            Joined j;
+            for (int p = 0; p < parts; ++p) j.m = fmaxf(j.m, others[p][tid][0]);
+            for (int p = 0; p < parts; ++p) j.add(others[p][tid][0], 0.f, others[p][tid][1]);
+            lse[tid] = j.m + log2f(j.whole(sink_of(tid)));
+            if (rank == 0) {
+                float* st = a.stats + (base_row + tid) * 2;
+                st[0] = j.m; st[1] = j.den;
+            }
+        }
+        cluster_barrier();                                          // nobody leaves while its sums may be read
+    }
+    // The weights of this block's keys, from the scores that it has just written: the rows in their order.
+    if (a.mass) {
+        __syncthreads();
+        for (int i = tid; i < n_tiles * TK; i += THREADS) {
+            const int key = span.key(t0 + i / TK) + i % TK;
+            if (key > span.last_pos) continue;
+            const float* score = a.scores + (((size_t)blockIdx.x * a.hkv + kvh) * a.longest + key) * a.row_stride;
+            float w = 0.f;
+            for (int r = 0; r < span.rows; ++r) w += exp2_fast(score[r] - lse[r]);
+            const int logical = a.by_page(key), page = logical < a.width ? pages[logical] : -1;
+            if (page >= 0 && w != 0.f) a.mass[((size_t)page * a.hkv + kvh) * a.page_size + key - logical * a.page_size] += w;
         }
     }
 }
 
-// Ranges of a row put together: a thread per output dimension, the ranges in their order.
+// Splits of a row put together where they are no cluster: a thread per output dimension, the splits in their order.
 template <int ROWS>
 __global__ void __launch_bounds__(D) attn_int4_merge_kernel(const __grid_constant__ Args a) {
     pdl_wait();
     Span span;
-    if (!find_span<ROWS>(span, a, blockIdx.x, 0) || span.ranges <= 1) return;
+    if (!find_span<ROWS>(span, a, blockIdx.x)) return;
     const int r = blockIdx.z, kvh = blockIdx.y, d = threadIdx.x;
     if (r >= span.rows) return;
     const size_t base = (((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride + r) * a.n_splits;
     const float2* stats = reinterpret_cast<const float2*>(a.stats) + base;
-    float m = -INFINITY;
-    for (int i = 0; i < span.ranges; ++i) m = fmaxf(m, stats[i].x);
-    float num = 0.f, den = 0.f;
-    for (int i0 = 0; i0 < span.ranges; i0 += 8) {
+    Joined j;
+    for (int i = 0; i < a.n_splits; ++i) j.m = fmaxf(j.m, stats[i].x);
+    for (int i0 = 0; i0 < a.n_splits; i0 += 8) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i0 + i < span.ranges ? a.partial[(base + i0 + i) * D + d] : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] = i0 + i < a.n_splits ? a.partial[(base + i0 + i) * D + d] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i0 + i >= span.ranges) continue;
-            const float2 st = stats[i0 + i];
-            if (st.x > -INFINITY) {
-                const float w = exp2_fast(st.x - m);
-                num = fmaf(w, v[i], num);
-                den = fmaf(w, st.y, den);
-            } else if (!(st.y == 0.f)) {
-                den = NAN;
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < a.n_splits) {
+                const float2 st = stats[i0 + i];
+                j.add(st.x, v[i], st.y);
             }
-        }
     }
     const int row = span.row0 + r, head = kvh * span.group + row % span.group;
-    const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
-    float whole = den;
-    if (sink > -INFINITY) whole += exp2f(fmaf(sink, LOG2E, -m));
-    a.out[((size_t)(a.q_start[span.req] + row / span.group) * a.hq + head) * D + d] = from_float<T>(den == 0.f ? 0.f : num / whole);
+    const float whole = j.whole(a.sink_heads ? a.sink_heads[head] : a.sink_all);
+    a.out[((size_t)(a.q_start[span.req] + row / span.group) * a.hq + head) * D + d] = from_float<T>(j.den == 0.f ? 0.f : j.num / whole);
 }
 
-// The weights of the keys: every key of a request gets the sum over the key head's query rows of 2^(score - max) / denominator added to
-// its number in `mass` [pages][hkv][page_size].  The rows in their order, so the sum does not change from run to run.
+// The weights of the keys where several tiles of rows, or splits that are no cluster, share them: every key of a request gets the sum over the
+// key head's query rows of 2^(score - max) / denominator added to its number in `mass` [pages][hkv][page_size].  The rows in their order,
+// so the sum does not change from run to run.
 constexpr int MASS_THREADS = 256, MASS_ROWS = 128;                  // rows whose denominators are at hand at a time
 template <int ROWS>
 __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __grid_constant__ Args a, float* __restrict__ mass, int keys_per_block) {
@@ -591,7 +675,7 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
     const int req = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
     const int n = a.q_len[req], ctx = a.ctx_len[req], group = a.hq / a.hkv, rows = n * group;
     if (n > a.max_queries || n <= 0 || ctx > a.longest) return;
-    const int keys = range_keys(ctx), ranges = (ctx + keys - 1) / keys;
+    const int parts = a.cluster > 1 ? 1 : a.n_splits;
     const int lo = blockIdx.z * keys_per_block, hi = min(lo + keys_per_block, ctx);
     if (lo >= hi) return;
     const int* pages = a.table + (size_t)a.req_slot[req] * a.width;
@@ -600,15 +684,13 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
         __syncthreads();
         for (int r = tid; r < min(MASS_ROWS, rows - row0); r += MASS_THREADS) {
             const int row = row0 + r, tile = row / ROWS;
-            const size_t base = ((((size_t)req * a.tiles + tile) * a.hkv + kvh) * a.row_stride + row - tile * ROWS) * a.n_splits;
+            const size_t base = ((((size_t)req * a.tiles + tile) * a.hkv + kvh) * a.row_stride + row - tile * ROWS) * parts;
             const float2* stats = reinterpret_cast<const float2*>(a.stats) + base;
-            float m = -INFINITY, den = 0.f;
-            for (int i = 0; i < ranges; ++i) m = fmaxf(m, stats[i].x);
-            for (int i = 0; i < ranges; ++i) if (stats[i].x > -INFINITY) den = fmaf(exp2_fast(stats[i].x - m), stats[i].y, den);
+            Joined j;
+            for (int i = 0; i < parts; ++i) j.m = fmaxf(j.m, stats[i].x);
+            for (int i = 0; i < parts; ++i) j.add(stats[i].x, 0.f, stats[i].y);
             const int head = kvh * group + row % group;
-            const float sink = a.sink_heads ? a.sink_heads[head] : a.sink_all;
-            if (sink > -INFINITY) den += exp2f(fmaf(sink, LOG2E, -m));
-            lse[r] = m + log2f(den);
+            lse[r] = j.m + log2f(j.whole(a.sink_heads ? a.sink_heads[head] : a.sink_all));
         }
         __syncthreads();
 #pragma unroll
@@ -625,53 +707,74 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int key = lo + i * MASS_THREADS + tid;
-        if (key >= hi || key / a.page_size >= a.width) continue;
-        const int page = pages[key / a.page_size];
+        if (key >= hi || a.by_page(key) >= a.width) continue;
+        const int page = pages[a.by_page(key)];
         if (page >= 0 && w[i] != 0.f) mass[((size_t)page * a.hkv + kvh) * a.page_size + key % a.page_size] += w[i];
     }
 }
 
-// How many ranges of keys requests of up to `longest` rows have at most.
-int most_ranges(int longest) {
-    const int keys = range_keys(longest), few = longest < 16 * 128 ? (longest + 127) / 128 : 16, many = (longest + keys - 1) / keys;
-    return few > many ? (few > 1 ? few : 1) : many;
+bool g_pdl = false;
+int* g_error = nullptr;
+
+int sm_count() {                                                    // of the current device
+    static int known[64] = {};
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 1;
+    if (device < 64 && known[device]) return known[device];
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return 1;
+    if (device < 64) known[device] = n;
+    return n;
 }
 
 // What a launch has of everything: query rows of a tile (8, or 16 where requests bring more), tiles per request, rows that scratch is kept
-// for (even, so that pairs are aligned), ranges.
+// for (even, so that pairs are aligned), splits of a request's keys and whether they are one cluster.
 struct Shape {
-    int rows, tiles, stride, splits;
+    int rows, tiles, stride, splits, cluster;
     long long units;                 // requests by tiles by key heads by rows
     long long keys;
-    Shape(int n_req, int max_queries, int longest, int hq, int hkv) {
+    Shape(int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
         const int needed = max_queries * (hq / hkv);
         rows = needed > 8 ? 16 : 8;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
-        splits = most_ranges(longest);
-        units = (long long)n_req * tiles * hkv * stride;
+        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>(), blocks = rows == 8 ? blocks_of<1>() : blocks_of<2>();
+        const long long pairs = (long long)n_req * tiles * hkv, room = (long long)sm_count() * blocks;
+        long long reach = longest;
+        if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
+        const int most = (int)((reach + (long long)TK * warps - 1) / (TK * warps));      // a tile for every warp
+        const long long want = (2 * room + pairs - 1) / pairs;                          // two rounds of thread blocks
+        splits = (int)(want < most ? want : most);
+        if (splits > MAX_CLUSTER) splits = pairs * MAX_CLUSTER >= room / 2 ? MAX_CLUSTER : splits < 64 ? splits : 64;
+        if (splits < 1) splits = 1;
+        cluster = splits <= MAX_CLUSTER ? splits : 1;
+        units = pairs * stride;
         keys = longest;
     }
-    long long partial() const { return splits > 1 ? units * splits * D : 0; }
-    long long stats() const { return units * splits * 2; }
+    bool merged_by_kernel() const { return splits > 1 && cluster == 1; }
+    long long partial() const { return merged_by_kernel() ? units * splits * D : 0; }
+    long long stats() const { return units * (merged_by_kernel() ? splits : 1) * 2; }
     long long scores() const { return units * keys; }
+    bool mass_by_kernel() const { return merged_by_kernel() || tiles > 1; }
+    int launches(bool mass) const { return 1 + merged_by_kernel() + (mass && mass_by_kernel()); }
 };
 
-bool g_pdl = false;
-int* g_error = nullptr;
-
-template <int NT> int launch(const Args& a, int n_req, float* mass, cudaStream_t s) {
+template <int NT> int launch(Args a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
+    constexpr int WARPS = warps_of<NT>();
     constexpr size_t RING = (size_t)WARPS * STAGES * TILE_BYTES, MERGE = sizeof(float) * WARPS * 8 * NT * (D + 2);
     constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
-    static_assert(SMEM <= 48 * 1024, "no opt-in to more shared memory");
+    if constexpr (SMEM > 48 * 1024 - 8192) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+        if (e != cudaSuccess) return (int)e;
+    }
     const dim3 grid((unsigned)(n_req * a.tiles), (unsigned)a.hkv, (unsigned)a.n_splits);
-    int status = launch_kernel(attn_int4_kernel<NT>, grid, dim3(THREADS), SMEM, s, g_pdl, a);
+    a.mass = shape.mass_by_kernel() ? nullptr : mass;
+    int status = launch_kernel_cluster(attn_int4_kernel<NT>, grid, dim3(32 * WARPS), SMEM, s, g_pdl, a.cluster, a);
     if (status) return status;
-    if (a.n_splits > 1) {
+    if (shape.merged_by_kernel()) {
         status = launch_kernel(attn_int4_merge_kernel<8 * NT>, dim3(grid.x, grid.y, (unsigned)a.row_stride), dim3(D), 0, s, true, a);
         if (status) return status;
     }
-    if (mass) {
+    if (mass && shape.mass_by_kernel()) {
         const int per = 4 * MASS_THREADS;
         status = launch_kernel(attn_int4_mass_kernel<8 * NT>, dim3((unsigned)n_req, (unsigned)a.hkv, (unsigned)((a.longest + per - 1) / per)), dim3(MASS_THREADS), 0, s, true, a, mass, per);
     }
@@ -685,9 +788,11 @@ CISR_EXPORT int cisr_attn_int4_head_dim() { return D; }
 CISR_EXPORT int cisr_attn_int4_init(int* error_flag) { g_error = error_flag; return 0; }
 
 // Floats of scratch that a call with these sizes takes (partial sums and statistics of the ranges, with `mass` also the scores).
-CISR_EXPORT long long cisr_attn_int4_scratch(int n_req, int max_queries, int longest, int hq, int hkv, int with_mass) {
-    const Shape s(n_req, max_queries, longest, hq, hkv);
-    return s.partial() + s.stats() + (with_mass ? s.scores() : 0);
+// The kernels that it launches: a million million times their number is added.
+CISR_EXPORT long long cisr_attn_int4_scratch(int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first, int with_mass) {
+    if (n_req <= 0 || max_queries <= 0 || hkv <= 0 || longest <= 0) return 0;
+    const Shape s(n_req, max_queries, longest, hq, hkv, window, keep_first);
+    return s.partial() + s.stats() + (with_mass ? s.scores() : 0) + 1000000000000ll * s.launches(with_mass != 0);
 }
 
 // q, out [tokens][hq][D]; request r brings q_len[r] tokens from row q_start[r] on and has ctx_len[r] rows with them; those with more than
@@ -699,17 +804,15 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
     if (!g_error) return -13;
     if (hkv <= 0 || hkv > 65535 || hq % hkv || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 7) return -2;      // rows are read by 16 bytes
-    const Shape shape(n_req, max_queries, longest, hq, hkv);
+    const Shape shape(n_req, max_queries, longest, hq, hkv, window, keep_first);
     if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
     Args a{};
     a.q = (const T*)q; a.out = (T*)out; a.k_cache = (const unsigned char*)k_cache; a.v_cache = (const unsigned char*)v_cache;
     a.req_slot = req_slot; a.table = block_table; a.width = width; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len;
     a.partial = scratch; a.stats = scratch + shape.partial(); a.scores = mass ? a.stats + shape.stats() : nullptr;
-    a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits;
+    a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
+    a.by_page = Divider((uint32_t)page_size);
     a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
     a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
-    return shape.rows == 8 ? launch<1>(a, n_req, mass, (cudaStream_t)stream) : launch<2>(a, n_req, mass, (cudaStream_t)stream);
+    return shape.rows == 8 ? launch<1>(a, shape, n_req, mass, (cudaStream_t)stream) : launch<2>(a, shape, n_req, mass, (cudaStream_t)stream);
 }
-
-// Kernels that such a call launches.
-CISR_EXPORT int cisr_attn_int4_launches(int longest, int with_mass) { return 1 + (most_ranges(longest) > 1) + (with_mass != 0); }

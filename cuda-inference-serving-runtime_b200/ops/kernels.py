@@ -532,6 +532,7 @@ INT4_HEAD_DIMS = (32, 64, 96, 128)
 INT4_FEW = 16                    # new tokens of a request up to which attn_decode_int4 is the faster call (see attn_prefill_int4)
 _int4_rows_state = {}
 _attention_int4_libs = {}
+_attention_int4_calls = {}       # by the sizes of a call: the function, the floats of scratch it takes, the kernels it launches
 
 
 def int4_jobs(head_dim: int, dtype: torch.dtype):
@@ -568,35 +569,41 @@ def int4_page_bytes(page_size: int, head_dim: int) -> int:
     return page_size * 9 * head_dim // 16
 
 
-def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, hkv: Optional[int], dim: int) -> int:
-    """Checks a pair of 4-bit caches; the number of key heads."""
+def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, hkv: Optional[int], dim: int) -> tuple:
+    """Checks a pair of 4-bit caches; the number of key heads and the device's index."""
     _need(k_cache, torch.uint8, "k_cache", 3); _need(v_cache, torch.uint8, "v_cache", 3)
-    if k_cache.shape != v_cache.shape or k_cache.shape[2] != int4_page_bytes(page_size, dim) or (hkv is not None and k_cache.shape[1] != hkv):
+    pages, heads, bytes_ = k_cache.shape
+    if v_cache.shape != k_cache.shape or bytes_ != page_size * 9 * dim // 16 or page_size % INT4_BLOCK or dim not in INT4_HEAD_DIMS or (hkv is not None and heads != hkv):
         raise KernelError(f"{what}: a cache of {page_size} rows a page is [pages, kv_heads, {int4_page_bytes(page_size, dim)}] bytes at head size {dim}, "
                           f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if _device is not None and k_cache.device.index != _device():
-        raise KernelError(f"{what}: the cache is on {k_cache.device}, the current device is cuda:{_device()}")
-    return k_cache.shape[1]
+    device = k_cache.get_device()
+    if v_cache.get_device() != device or (_device is not None and device != _device()):
+        raise KernelError(f"{what}: the cache is on {k_cache.device} and {v_cache.device}, the current device is another")
+    return heads, device
 
 
-def _int4_lists(what: str, device, table: torch.Tensor, count: int, **lists) -> None:
-    _need(table, torch.int32, "block_table", 2)
+def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, **lists) -> None:
+    """Checks int32 lists of `count` entries each (`req_slot`: any number) and the block table, all on the cache's device."""
+    if not (table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.get_device() == device):
+        _need(table, torch.int32, "block_table", 2)
+        raise KernelError(f"{what}: block_table is on {table.device}, the cache on cuda:{device}")
     for name, t in lists.items():
+        if t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.get_device() == device and (t.numel() == count or name == "req_slot"):
+            continue
         _need(t, torch.int32, name, 1)
-        if t.device != device:
-            raise KernelError(f"{what}: {name} is on {t.device}, the cache on {device}")
-        if name != "req_slot" and t.numel() != count:
-            raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
+        if t.get_device() != device:
+            raise KernelError(f"{what}: {name} is on {t.device}, the cache on cuda:{device}")
+        raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
 
 
 def _int4_mass(what: str, mass: torch.Tensor, k_cache: torch.Tensor, page_size: int) -> None:
     _need(mass, torch.float32, "mass", 3)
-    if tuple(mass.shape) != (k_cache.shape[0], k_cache.shape[1], page_size) or mass.device != k_cache.device:
+    if mass.shape[2] != page_size or mass.shape[:2] != k_cache.shape[:2] or mass.get_device() != k_cache.get_device():
         raise KernelError(f"{what}: mass must be [pages, kv_heads, page_size] on the cache's device")
 
 
-def _int4_rows_like(what: str, name: str, t: torch.Tensor, device) -> None:
-    if t.device != device or t.dim() != 3 or t.stride(2) != 1 or t.dtype not in _DTYPE_CODE:
+def _int4_rows_like(what: str, name: str, t: torch.Tensor, device: int) -> None:
+    if t.get_device() != device or t.dim() != 3 or t.stride(2) != 1 or t.dtype not in _DTYPE_CODE:
         raise KernelError(f"{what}: {name} must be float32 or bfloat16 [tokens, kv_heads, head_dim] with neighbouring values, on the cache's device")
 
 
@@ -609,7 +616,7 @@ def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     A value is held as c s: s the largest magnitude of its group of 32 neighbours over 7, in float16 (65504 at most: magnitudes beyond
     458,528 are cut there), c the whole number nearest to x / s, so it is off by half of s and the rounding of s itself.  A
     group that holds an infinity or a NaN becomes NaN."""
-    device = k_cache.device
+    device = k_cache.get_device()
     _int4_rows_like("int4_store", "k", k, device); _int4_rows_like("int4_store", "v", v, device)
     tokens, hkv, dim = k.shape
     if v.shape != k.shape or v.dtype != k.dtype:
@@ -629,10 +636,10 @@ def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor,
     token_req[t] stand for (zeros where the table has no page)."""
     _need(k_out, None, "k_out", 3); _need(v_out, k_out.dtype, "v_out", 3)
     tokens, hkv, dim = k_out.shape
-    if v_out.shape != k_out.shape or k_out.device != k_cache.device:
+    _, device = _int4_cache("int4_read", k_cache, v_cache, page_size, hkv, dim)
+    if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_read: k_out and v_out differ in shape, or lie elsewhere than the cache")
-    _int4_cache("int4_read", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_read", k_cache.device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
+    _int4_lists("int4_read", device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
     _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), 0, hkv * dim, dim, _p(token_req),
                                        _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, 0, 0, 1, tokens, hkv, dim, _stream()), "int4_read")
 
@@ -643,13 +650,13 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
     `requests` lists, where it is given), zeros from ctx_len[r] on."""
     _need(k_out, None, "k_out", 4); _need(v_out, k_out.dtype, "v_out", 4)
     n, hkv, rows, dim = k_out.shape
-    if v_out.shape != k_out.shape or k_out.device != k_cache.device:
+    _, device = _int4_cache("int4_expand", k_cache, v_cache, page_size, hkv, dim)
+    if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_expand: k_out and v_out differ in shape, or lie elsewhere than the cache")
-    _int4_cache("int4_expand", k_cache, v_cache, page_size, hkv, dim)
     if requests is None:
-        _int4_lists("int4_expand", k_cache.device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+        _int4_lists("int4_expand", device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
     else:
-        _int4_lists("int4_expand", k_cache.device, block_table, n, req_slot=req_slot, requests=requests)
+        _int4_lists("int4_expand", device, block_table, n, req_slot=req_slot, requests=requests)
         _need(ctx_len, torch.int32, "ctx_len", 1)
     _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), hkv * rows * dim, dim, rows * dim, 0, 0,
                                        _p(req_slot), _p(block_table), block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()),
@@ -668,22 +675,27 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     the request's new tokens, have given it (a sink takes its part of them)."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     tokens, hq, dim = q.shape
-    if out.shape != q.shape:
-        raise KernelError("attn_decode_int4: q and out differ in shape")
-    hkv = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
+    hkv, device = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
     n = q_len.numel()
-    _int4_lists("attn_decode_int4", k_cache.device, block_table, n, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len)
-    if hq % hkv or max_queries < 1 or longest < 1 or req_slot.numel() < n or q.device != k_cache.device or out.device != k_cache.device:
-        raise KernelError("attn_decode_int4: heads, limits, lists or devices disagree")
+    _int4_lists("attn_decode_int4", device, block_table, n, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len)
+    if out.shape != q.shape or hq % hkv or max_queries < 1 or longest < 1 or req_slot.numel() < n or q.get_device() != device or out.get_device() != device:
+        raise KernelError("attn_decode_int4: shapes, heads, limits, lists or devices disagree")
     if (window is not None and window < 1) or keep_first < 0:
         raise KernelError("attn_decode_int4: a window has at least one key, and keep_first is not negative")
     if mass is not None:
         _int4_mass("attn_decode_int4", mass, k_cache, page_size)
-    lib = _attention_int4(dim, q.dtype)
-    scratch = torch.empty(lib.cisr_attn_int4_scratch(n, max_queries, longest, hq, hkv, mass is not None), dtype=torch.float32, device=k_cache.device)
-    _check(lib.cisr_attn_int4(_p(q), _p(out), _p(k_cache), _p(v_cache), _p(req_slot), _p(block_table), block_table.shape[1], _p(q_start), _p(q_len), _p(ctx_len),
-                              _p(scratch), _p(mass), n, max_queries, longest, hq, hkv, page_size, scale, window or 0, keep_first, *_sink(sink, hq), _stream()),
-           "attn_decode_int4", own=lib.cisr_attn_int4_launches(longest, mass is not None))
+    key = (device, dim, q.dtype, n, max_queries, longest, hq, hkv, window, keep_first, mass is None)
+    call = _attention_int4_calls.get(key)
+    if call is None:
+        if len(_attention_int4_calls) >= 4096:
+            _attention_int4_calls.clear()
+        lib = _attention_int4(dim, q.dtype)
+        launches, floats = divmod(lib.cisr_attn_int4_scratch(n, max_queries, longest, hq, hkv, window or 0, keep_first, mass is not None), 10 ** 12)
+        call = _attention_int4_calls[key] = (lib.cisr_attn_int4, floats, launches)
+    scratch = torch.empty(call[1], dtype=torch.float32, device=q.device)
+    _check(call[0](q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+                   q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), scratch.data_ptr(), _p(mass), n, max_queries, longest, hq, hkv, page_size, scale,
+                   window or 0, keep_first, *_sink(sink, hq), _stream()), "attn_decode_int4", own=call[2])
 
 
 def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
@@ -697,15 +709,15 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     that are written out, and for every request of the step its place in that list (any number for the others); None: all, in order."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     hq, dim = q.shape[1], q.shape[2]
-    hkv = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
+    hkv, device = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
     n_all = q_len.numel()
-    if longest < 1 or hq % hkv or out.shape != q.shape or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.device != k_cache.device:
+    if longest < 1 or hq % hkv or out.shape != q.shape or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.get_device() != device:
         raise KernelError("attn_prefill_int4: heads, limits, shapes, devices or the span disagree")
     requests, places = (None, None) if portions is None else portions
     n = n_all if requests is None else requests.numel()
     if places is None:
         places = torch.arange(n, dtype=torch.int32, device=q.device)
-    _int4_lists("attn_prefill_int4", k_cache.device, block_table, n_all, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len, places=places)
+    _int4_lists("attn_prefill_int4", device, block_table, n_all, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len, places=places)
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     k, v = torch.empty((2, n, hkv, rows, dim), dtype=q.dtype, device=q.device)
     int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
@@ -730,10 +742,10 @@ def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor,
     n, hkv, keep = kept.shape
     bytes_ = k_cache.shape[2] if k_cache.dim() == 3 else 0
     dim = bytes_ * 16 // (9 * page_size) if page_size > 0 else 0
-    _int4_cache("int4_evict", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_evict", k_cache.device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+    _, device = _int4_cache("int4_evict", k_cache, v_cache, page_size, hkv, dim)
+    _int4_lists("int4_evict", device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
     _int4_mass("int4_evict", mass, k_cache, page_size)
-    if kept.device != k_cache.device or to_table.device != k_cache.device:
+    if kept.get_device() != device or to_table.get_device() != device:
         raise KernelError("int4_evict: kept and to_table must lie on the cache's device")
     if req_slot.numel() < n or to_table.shape[0] != n or to_table.shape[1] * page_size < keep or longest < 1:
         raise KernelError("int4_evict: req_slot and to_table need an entry per request, and to_table room for the rows that stay")

@@ -334,18 +334,24 @@ def test_no_keys_no_tokens_and_requests_left_alone():
     assert not out[0].any() and (out[1:5] == 7).all() and (out[5] != 7).any()       # no keys: zeros; four tokens are more than three
 
 
-def test_a_request_does_not_depend_on_its_neighbours():
-    hq, hkv, dim = 32, 8, 128
-    lens = [5000, 17, 1200, 20000]
-    cache = Cache(lens, hkv, dim, 16)
-    q = queries(4, hq, dim, torch.bfloat16)
-    whole = cache.attend(q, [1] * 4)
-    for r in range(4):
-        out = torch.empty_like(q[:1])
-        kernels.attn_decode_int4(q[r:r + 1], out, cache.k_cache, cache.v_cache, cache.slots[r:], cache.table, i32([0]), i32([1]), cache.ctx[r:r + 1].clone(), 1, lens[r], 16,
-                                 dim ** -0.5)
-        assert torch.equal(out[0], whole[r])
-    check(cache, q, whole, [1] * 4)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_few_and_many_requests(n, dtype):
+    """Keys in one part, in a cluster of parts, in parts that a kernel of their own puts together: whatever the sizes choose."""
+    hq, hkv, dim = 4, 1, 64
+    for longest in (20, 600, 5000, 30000):
+        lens = [max(1, longest - 37 * i * i) for i in range(n)]
+        if sum(lens) > 400000:
+            continue
+        cache = Cache(lens, hkv, dim, 64)
+        q = queries(n, hq, dim, dtype)
+        mass = torch.zeros((cache.pages, hkv, 64), device="cuda")
+        got = cache.attend(q, [1] * n, mass=mass)
+        check(cache, q, got, [1] * n)
+        assert torch.equal(cache.attend(q, [1] * n), got)
+        for r in range(n):
+            total = float(sum(mass[p].double().sum() for p in cache.table[r].tolist() if p >= 0))
+            assert abs(total - hq) < hq * 1e-3                   # every query head's weights are one in all
 
 
 def test_a_request_longer_than_the_bound_is_reported():
@@ -579,7 +585,7 @@ def test_captured_replayed_and_on_two_streams():
         turn(cache, q, plain_out, plain_mass)
         assert torch.equal(out, plain_out) and torch.equal(mass, plain_mass)
         expected = torch.empty_like(q)
-        kernels.attn_decode_int4(other_q, expected, other.k_cache, other.v_cache, other.slots, other.table, starts, ones, other.ctx, 1, 700, page, dim ** -0.5)
+        kernels.attn_decode_int4(other_q, expected, other.k_cache, other.v_cache, other.slots, other.table, starts, ones, other.ctx, 1, 1024, page, dim ** -0.5)
         assert torch.equal(expected, other_out)
     kernels.raise_if_kernel_gave_up()
 
