@@ -10,8 +10,9 @@
 //   * A code is a float16 operand by one mask: the low half byte of a 16-bit half is the subnormal n 2^-24, the next one n 2^-20, which
 //     the matrix instructions take exactly; the two upper half bytes follow after one shift by 8.  Five integer instructions for
 //     8 values, none of them a conversion.  The factor 16 is taken out of the query (exactly) or of the finished output.
-//   * The offset 8 is never subtracted from a code: the score's accumulators start at -8 sum q, and the output's share is the
-//     product of the same probabilities with a constant operand, one matrix instruction per group and 16 keys.
+//   * The offset 8 is never subtracted from a code: a score's share, -8 sum_g s_g sum q, is the product of a key's steps with the queries'
+//     sums (two float16 terms), the output's share the product of the probabilities with a constant operand: one matrix instruction per
+//     16 keys, and one per group of them.
 //   * A is the cache (16 keys by 16 dimensions of K; 16 dimensions by 16 keys of V), B the queries or probabilities, of which 8 columns are
 //     the least there is: a group of 3 or 4 query heads fills half of them, where it as A would fill a quarter.
 //   * Steps of K are applied to the score of a group (float), those of V to the probabilities (float16 pairs).
@@ -56,6 +57,15 @@ __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.f
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same without sums from before, and with 8 of K.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16_8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {        // of an 8 x 8 matrix of 16-bit elements spread over a warp
     uint32_t y;
@@ -124,11 +134,16 @@ struct Args {
 };
 
 // What the rows of one (request, tile of 8 NT query rows) see, as tiles of TK keys: those of the first keys that stay in sight behind a
-// window, then those from the first key inside the first row's window to the last row's own.
+// window, then those from the first key inside the first row's window to the last row's own.  They are walked from the `lead`th on, the
+// others last: then the tiles that some row does not see whole are the last ones, and the first `plain` need no masks.
 struct Span {
     int req, n, ctx, group, row0, rows, first_pos, last_pos;
-    int kept_tiles, window_base, tiles;
-    __device__ __forceinline__ int key(int t) const { return t < kept_tiles ? t * TK : window_base + (t - kept_tiles) * TK; }
+    int kept_tiles, window_base, tiles, lead, plain;
+    __device__ __forceinline__ int key(int t) const {
+        t += lead;
+        t -= t >= tiles ? tiles : 0;
+        return t < kept_tiles ? t * TK : window_base + (t - kept_tiles) * TK;
+    }
 };
 template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x) {
     s.req = a.tiles == 1 ? x : x / a.tiles;
@@ -149,10 +164,14 @@ template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Arg
         s.window_base = begin & ~(TK - 1);
     }
     s.tiles = s.last_pos < 0 ? 0 : s.kept_tiles + (s.last_pos - s.window_base) / TK + 1;
+    s.lead = a.window > 0 && s.last_pos >= a.window ? min(s.tiles, s.kept_tiles + 2) : 0;      // the rows' windows begin within 16 keys
+    s.plain = min(s.tiles - s.lead, max(0, s.first_pos + 1 < s.window_base ? 0 : (s.first_pos + 1 - s.window_base) / TK + s.kept_tiles - s.lead));
     return true;
 }
-__device__ __forceinline__ bool in_sight(const Span& s, const Args& a, int key) {       // of some row of the tile
-    return key <= s.last_pos && (a.window <= 0 || key >= s.first_pos - a.window + 1 || key < a.keep_first);
+// Of a pair of steps those of keys that some row of the tile sees: what lies in the others' place does not matter.
+__device__ __forceinline__ uint32_t in_sight(const Span& s, const Args& a, int key) {
+    const auto seen = [&](int k) { return k <= s.last_pos && (a.window <= 0 || k >= s.first_pos - a.window + 1 || k < a.keep_first); };
+    return (seen(key) ? 0xffffu : 0u) | (seen(key + 1) ? 0xffff0000u : 0u);
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -199,6 +218,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     __shared__ uint64_t full[WARPS * STAGES];
     __shared__ int failed;
     __shared__ float others[MAX_CLUSTER][ROWS][2], lse[ROWS];       // a cluster's largest scores and denominators; the row's logarithm of its sum
+    __shared__ float weight[WARPS][ROWS];                           // of a warp's sums among the block's
     __shared__ float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int kvh = blockIdx.y, split = blockIdx.z;
@@ -246,8 +266,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
     // after the shift, (2, 6), (3, 7) / 16.
     uint32_t qf[NT][NG][2][TERMS][2];
-    float offset[NT][NG][2], unit[NT][2];
-    int reach[NT][2], behind[NT][2];                                // a column's last place in sight, and the first inside its window
+    uint32_t qs[NT];                                                // -8 2^-24 sum q of two groups, the first float16 term (c below 2) or the second
+    float unit[NT][2];                                              // of a column's sums, in the softmax's exponent (base 2); positive
     const int tok0 = a.q_start[span.req];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -277,11 +297,10 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int up = min(14 - ((int)(top >> 23) - 127), 120);     // the row times 2^up is below 2^15
-        const float factor = __uint_as_float((uint32_t)(up + 127) << 23);
-        float sum[NG];
+        const float factor = copysignf(__uint_as_float((uint32_t)(up + 127) << 23), a.scale);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-            sum[j] = 0.f;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 float p[4] = {x[j][2 * k] * factor, x[j][2 * k + 4] * factor, x[j][2 * k + 1] * factor * SECOND, x[j][2 * k + 5] * factor * SECOND};
@@ -300,19 +319,16 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
                 sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) offset[nt][j][h] = OFFSET ? -0x1p-21f * __shfl_sync(0xffffffffu, sum[j], 4 * (2 * c + h)) : 0.f;      // -8 2^-24 sum q
         }
-        const float mine = a.scale * LOG2E * (OFFSET ? 0x1p24f : 0x1p9f) * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            unit[nt][h] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + h));
-            const int pos = span.ctx - span.n + (span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1)) / span.group;
-            reach[nt][h] = pos;
-            behind[nt][h] = a.window > 0 ? pos - a.window + 1 : 0;
+        if constexpr (OFFSET) {
+            const float s0 = -0x1p-21f * (c & 1 ? sum[2] : sum[0]), s1 = -0x1p-21f * (c & 1 ? sum[3] : sum[1]);
+            qs[nt] = pack_f16(s0, s1);
+            if (c >= 2) qs[nt] = pack_f16(s0 - low_half(qs[nt]), s1 - high_half(qs[nt]));
         }
+        const float mine = fmaxf(fabsf(a.scale) * LOG2E * (OFFSET ? 0x1p24f : 0x1p9f) * __uint_as_float((uint32_t)(127 - up) << 23), 0x1p-126f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) unit[nt][h] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + h));
     }
-    const int sure_lo = a.window > 0 ? span.last_pos - a.window + 1 : 0;      // keys in [sure_lo, first_pos] are in sight of every row, kept first ones too
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -335,19 +351,10 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         l_run[nt][0] *= a0; l_run[nt][1] *= a1;
     };
 
-    for (int t = warp, it = 0; t < n_tiles; t += WARPS, ++it) {
-        const int slot = it % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(bars + slot, (uint32_t)(it / STAGES) & 1))) {
-            if (lane == 0) { atomicExch(a.error, 3); failed = 1; }
-            for (int i = 0; i < STAGES; ++i)                        // another bounded chance for this warp's copies to land before the stages are given up
-                if (t + WARPS * i < n_tiles) mbar_wait(bars + (it + i) % STAGES, (uint32_t)((it + i) / STAGES) & 1);
-            break;
-        }
-        const unsigned char* ks = ring + (size_t)slot * TILE_BYTES;
-        const unsigned char* vs = ks + TILE_BYTES / 2;
-        const int k0 = span.key(t0 + t);
-        const bool edge = k0 + TK > span.first_pos + 1 || (k0 < sure_lo && k0 + TK > a.keep_first);       // the same for the whole warp
-
+    float* scores = a.scores ? a.scores + ((size_t)blockIdx.x * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
+    // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.
+    const auto work = [&](auto is_edge, const unsigned char* ks, const unsigned char* vs, int k0) {
+        constexpr bool EDGE = decltype(is_edge)::value;
         float s[2][NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                               // 16 keys: blocks 2 h and 2 h + 1
@@ -355,11 +362,14 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             const Share<4 * NG> w0 = load_share<4 * NG>(b0 + g * (D / 2) + c * 4 * NG), w1 = load_share<4 * NG>(b1 + g * (D / 2) + c * 4 * NG);
             const Share<2 * NG> s0 = load_share<2 * NG>(b0 + 4 * D + g * 2 * NG), s1 = load_share<2 * NG>(b1 + 4 * D + g * 2 * NG);
+            if constexpr (OFFSET) {
+                const uint32_t a0 = c & 1 ? (NG > 2 ? s0.w[(NG - 1) / 2] : 0u) : s0.w[0], a1 = c & 1 ? (NG > 2 ? s1.w[(NG - 1) / 2] : 0u) : s1.w[0];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_f16_8_new(s[h][nt], a0, a1, qs[nt]);
+            }
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 float acc[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) { acc[nt][0] = acc[nt][2] = offset[nt][j][0]; acc[nt][1] = acc[nt][3] = offset[nt][j][1]; }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t x = k ? w0.w[j] >> 8 : w0.w[j], y = k ? w1.w[j] >> 8 : w1.w[j];
@@ -368,16 +378,16 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int term = 0; term < TERMS; ++term) mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
+                        for (int term = 0; term < TERMS; ++term) {
+                            if (k || term) mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
+                            else mma_f16_new(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
+                        }
                 }
                 const float f0 = j & 1 ? high_half(s0.w[j / 2]) : low_half(s0.w[j / 2]), f1 = j & 1 ? high_half(s1.w[j / 2]) : low_half(s1.w[j / 2]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    s[h][nt][0] = j ? fmaf(f0, acc[nt][0], s[h][nt][0]) : f0 * acc[nt][0];
-                    s[h][nt][1] = j ? fmaf(f0, acc[nt][1], s[h][nt][1]) : f0 * acc[nt][1];
-                    s[h][nt][2] = j ? fmaf(f1, acc[nt][2], s[h][nt][2]) : f1 * acc[nt][2];
-                    s[h][nt][3] = j ? fmaf(f1, acc[nt][3], s[h][nt][3]) : f1 * acc[nt][3];
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[h][nt][e] = OFFSET || j ? fmaf(e < 2 ? f0 : f1, acc[nt][e], s[h][nt][e]) : (e < 2 ? f0 : f1) * acc[nt][e];
             }
         }
         bool more = false;
@@ -387,16 +397,14 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float v = s[h][nt][e] * unit[nt][e & 1];
-                    if (edge) {
-                        const int key = k0 + 16 * h + g + 8 * (e >> 1);
-                        const bool seen = key <= reach[nt][e & 1] && (key >= behind[nt][e & 1] || key < a.keep_first);
-                        v = seen ? v : -INFINITY;
+                    if constexpr (EDGE) {
+                        const int key = k0 + 16 * h + g + 8 * (e >> 1), pos = span.ctx - span.n + (span.row0 + min(nt * 8 + 2 * c + (e & 1), span.rows - 1)) / span.group;
+                        const bool seen = key <= pos && (a.window <= 0 || pos - key < a.window || key < a.keep_first);
+                        if (!seen) s[h][nt][e] = -INFINITY;
                     }
-                    s[h][nt][e] = v;
-                    more |= v > m_run[nt][e & 1];
+                    more |= s[h][nt][e] > m_run[nt][e & 1];
                 }
-        if (a.scores) {
+        if (scores) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     for (int e = 0; e < 4; e += 2) {
                         const int key = k0 + 16 * h + g + 8 * (e >> 1), col = nt * 8 + 2 * c;
                         if (key <= span.last_pos && col < span.rows)
-                            *reinterpret_cast<float2*>(a.scores + (((size_t)blockIdx.x * a.hkv + kvh) * a.longest + key) * a.row_stride + col) = make_float2(s[h][nt][e], s[h][nt][e + 1]);
+                            *reinterpret_cast<float2*>(scores + (size_t)key * a.row_stride + col) = make_float2(s[h][nt][e] * unit[nt][0], s[h][nt][e + 1] * unit[nt][1]);
                     }
         }
         // The running maximum follows only when a score exceeds it (rarely, after the first tiles).
@@ -420,26 +428,20 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float m_new = fmaxf(m_run[nt][e], mx);
-                    alpha[e] = m_run[nt][e] == m_new ? 1.f : exp2_fast(m_run[nt][e] - m_new);
+                    alpha[e] = m_run[nt][e] == m_new ? 1.f : exp2_fast((m_run[nt][e] - m_new) * unit[nt][e]);
                     m_run[nt][e] = m_new;
                 }
                 rescale(nt, alpha[0], alpha[1]);
             }
         }
-        // steps of V: those of two neighbouring keys side by side; a large one changes the probabilities' shift for good
-        Share<4 * NG> sv[4];
+        // a large step of V changes the probabilities' shift for good
         uint32_t any = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            sv[b] = load_share<4 * NG>(vs + b * BLOCK_BYTES + 4 * D + c * 4 * NG);
-            if (edge) {                                             // steps that belong to no key in sight of any row: whatever lies there
-                const int key = k0 + 8 * b + 2 * c;
-                const uint32_t keep = (in_sight(span, a, key) ? 0xffffu : 0u) | (in_sight(span, a, key + 1) ? 0xffff0000u : 0u);
-#pragma unroll
-                for (int j = 0; j < NG; ++j) sv[b].w[j] &= keep;
-            }
-#pragma unroll
-            for (int j = 0; j < NG; ++j) any |= sv[b].w[j];
+        for (int i = lane; i < 16 * NG; i += 32) {
+            const int b = i / (4 * NG), w = i - b * 4 * NG;
+            uint32_t two = *reinterpret_cast<const uint32_t*>(vs + b * BLOCK_BYTES + 4 * D + 4 * w);
+            if constexpr (EDGE) two &= in_sight(span, a, k0 + 8 * b + 2 * (w / NG));
+            any |= two;
         }
         if (shift == SMALL_SHIFT && __any_sync(0xffffffffu, any & 0x40004000u)) {
             shift = LARGE_SHIFT;
@@ -451,12 +453,12 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float top = (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e]) - shift;
+                const float top = shift - (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e] * unit[nt][e]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float p0 = exp2_fast(s[h][nt][e] - top), p1 = exp2_fast(s[h][nt][e + 2] - top);
+                    float p0 = exp2_fast(fmaf(s[h][nt][e], unit[nt][e], top)), p1 = exp2_fast(fmaf(s[h][nt][e + 2], unit[nt][e], top));
                     l_run[nt][e] += p0 + p1;
-                    if (edge) {                                     // a key out of sight gets -0, by which it is told from one of no weight
+                    if constexpr (EDGE) {                                     // a key out of sight gets -0, by which it is told from one of no weight
                         if (s[h][nt][e] == -INFINITY) p0 = -0.f;
                         if (s[h][nt][e + 2] == -INFINITY) p1 = -0.f;
                     }
@@ -476,6 +478,16 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 #endif
             const unsigned char* b0 = vs + 2 * h * BLOCK_BYTES;
             const unsigned char* b1 = b0 + BLOCK_BYTES;
+            Share<4 * NG> sv[2];                                    // the steps of two neighbouring keys side by side
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                sv[b] = load_share<4 * NG>(vs + (2 * h + b) * BLOCK_BYTES + 4 * D + c * 4 * NG);
+                if constexpr (EDGE) {
+                    const uint32_t keep = in_sight(span, a, k0 + 16 * h + 8 * b + 2 * c);
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) sv[b].w[j] &= keep;
+                }
+            }
             const int turned = (g ^ int4_value_turn<D>(c)) * 2 * NG;
             const Share<2 * NG> u0 = load_share<2 * NG>(b0 + c * (D / 2) + turned), u1 = load_share<2 * NG>(b0 + (4 + c) * (D / 2) + turned);
             const Share<2 * NG> u2 = load_share<2 * NG>(b1 + c * (D / 2) + turned), u3 = load_share<2 * NG>(b1 + (4 + c) * (D / 2) + turned);
@@ -488,18 +500,18 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 #if STORAGE_BF16
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        uint32_t v = mul_f16x2(pt[nt][b], sv[2 * h + b].w[j]);
-                        if (edge) v &= ~__vcmpeq2(pt[nt][b], 0x80008000u);      // out of sight: nothing, whatever the step there is
+                        uint32_t v = mul_f16x2(pt[nt][b], sv[b].w[j]);
+                        if constexpr (EDGE) v &= ~__vcmpeq2(pt[nt][b], 0x80008000u);      // out of sight: nothing, whatever the step there is
                         pb[nt][0][b] = v;
                     }
 #else
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         // before the transposition a lane has keys of row g: its step is half of the word of the pair of rows g / 2
-                        const uint32_t pair = __shfl_sync(0xffffffffu, sv[2 * h + b].w[j], g >> 1);
+                        const uint32_t pair = __shfl_sync(0xffffffffu, sv[b].w[j], g >> 1);
                         const float step = g & 1 ? high_half(pair) : low_half(pair);
                         float v0 = s[h][nt][2 * b] * step, v1 = s[h][nt][2 * b + 1] * step;
-                        if (edge) {
+                        if constexpr (EDGE) {
                             if (__float_as_uint(s[h][nt][2 * b]) == 0x80000000u) v0 = 0.f;
                             if (__float_as_uint(s[h][nt][2 * b + 1]) == 0x80000000u) v1 = 0.f;
                         }
@@ -530,9 +542,27 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 }
             }
         }
+    };
+
+    // The it-th tile of this warp; false where its copies never came.
+    const auto step = [&](auto is_edge, int t, int it) {
+        const int slot = it % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + slot, (uint32_t)(it / STAGES) & 1))) {
+            if (lane == 0) { atomicExch(a.error, 3); failed = 1; }
+            for (int i = 0; i < STAGES; ++i)                        // another bounded chance for this warp's copies to land before the stages are given up
+                if (t + WARPS * i < n_tiles) mbar_wait(bars + (it + i) % STAGES, (uint32_t)((it + i) / STAGES) & 1);
+            return false;
+        }
+        const unsigned char* ks = ring + (size_t)slot * TILE_BYTES;
+        work(is_edge, ks, ks + TILE_BYTES / 2, span.key(t0 + t));
         __syncwarp();                                               // every lane has read the stage
         if (t + WARPS * STAGES < n_tiles) fetch(t + WARPS * STAGES, slot);
-    }
+        return true;
+    };
+    int t = warp, it = 0;
+    bool came = true;
+    for (const int plain = min(n_tiles, span.plain - t0); came && t < plain; t += WARPS, ++it) came = step(std::false_type(), t, it);
+    for (; came && t < n_tiles; t += WARPS, ++it) came = step(std::true_type(), t, it);
     __syncthreads();                                                // every warp is done with its stages: they become the merge area
     float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
 #pragma unroll
@@ -553,7 +583,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     row[32 * j + 4 * g + 2 * k] = (o[2 * j + k][nt][h] - off) * whole;
                     row[32 * j + 4 * g + 2 * k + 1] = (o[2 * j + k][nt][2 + h] * SECOND - off) * whole;
                 }
-            if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : m_run[nt][h] - shift; row[D + 1] = l; }
+            if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : fmaf(m_run[nt][h], unit[nt][h], -shift); row[D + 1] = l; }
         }
     __syncthreads();
     // The warps' sums joined, in their order: into the first warp's place for the cluster, or to where they go.
@@ -563,27 +593,38 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         return ((size_t)(tok0 + row / span.group) * a.hq + kvh * span.group + row % span.group) * D;
     };
     const auto sink_of = [&](int r) { return a.sink_heads ? a.sink_heads[kvh * span.group + (span.row0 + r) % span.group] : a.sink_all; };
-    for (int e = tid; e < span.rows * D; e += THREADS) {
-        const int r = e / D, d = e - r * D;
+    if (tid < WARPS * ROWS) {
+        const int w = tid / ROWS, r = tid - w * ROWS;
         Joined j;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) j.m = fmaxf(j.m, merge[((size_t)w * ROWS + r) * MERGE_STRIDE + D]);
+        for (int i = 0; i < WARPS; ++i) j.m = fmaxf(j.m, merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D]);
+        weight[w][r] = j.weight(merge[((size_t)w * ROWS + r) * MERGE_STRIDE + D]);
+        if (w == 0) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float* row = merge + ((size_t)w * ROWS + r) * MERGE_STRIDE;
-            j.add(row[D], row[d], row[D + 1]);
+            for (int i = 0; i < WARPS; ++i) j.add(merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D], 0.f, merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D + 1]);
+            if (failed) j.den = NAN;
+            sums[r * MERGE_STRIDE + D] = j.m; sums[r * MERGE_STRIDE + D + 1] = j.den;
+            if (!clustered && r < span.rows) {
+                float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
+                st[0] = j.m; st[1] = j.den;
+                lse[r] = j.m + log2f(j.whole(sink_of(r)));
+            }
         }
+    }
+    __syncthreads();
+    for (int e = tid; e < span.rows * D; e += THREADS) {
+        const int r = e / D, d = e - r * D;
+        float num = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) num = fmaf(weight[w][r], merge[((size_t)w * ROWS + r) * MERGE_STRIDE + d], num);
         if (clustered) {
-            sums[r * MERGE_STRIDE + d] = j.num;
-            if (d == 0) { sums[r * MERGE_STRIDE + D] = j.m; sums[r * MERGE_STRIDE + D + 1] = failed ? NAN : j.den; }
-            continue;
-        }
-        if (alone) a.out[place(r) + d] = from_float<T>(j.den == 0.f ? 0.f : j.num / j.whole(sink_of(r)));
-        else a.partial[((base_row + r) * a.n_splits + split) * D + d] = j.num;
-        if (d == 0) {
-            float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
-            st[0] = j.m; st[1] = j.den;
-            lse[r] = j.m + log2f(j.whole(sink_of(r)));
+            sums[r * MERGE_STRIDE + d] = num;
+        } else if (alone) {
+            Joined j;
+            j.m = sums[r * MERGE_STRIDE + D]; j.den = sums[r * MERGE_STRIDE + D + 1];
+            a.out[place(r) + d] = from_float<T>(j.den == 0.f ? 0.f : num / j.whole(sink_of(r)));
+        } else {
+            a.partial[((base_row + r) * a.n_splits + split) * D + d] = num;
         }
     }
     if (clustered) {
@@ -802,7 +843,7 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
                                int hq, int hkv, int page_size, float scale, int window, int keep_first, float sink, const float* sink_heads, void* stream) {
     if (n_req <= 0 || max_queries <= 0) return 0;
     if (!g_error) return -13;
-    if (hkv <= 0 || hkv > 65535 || hq % hkv || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
+    if (hkv <= 0 || hkv > 65535 || hq % hkv || !isfinite(scale) || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 7) return -2;      // rows are read by 16 bytes
     const Shape shape(n_req, max_queries, longest, hq, hkv, window, keep_first);
     if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
