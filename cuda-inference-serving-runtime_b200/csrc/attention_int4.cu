@@ -20,7 +20,6 @@
 // the row's largest lose digits); of probabilities 11 bits.  Float queries take two float16 terms (22 bits) for both.
 // Scores, running maxima, sums and outputs are float.
 #include "int4_cache.cuh"
-#include "tma.cuh"
 
 #ifndef HEAD_DIM
 #define HEAD_DIM 128
@@ -43,9 +42,11 @@ constexpr int TK = 32;                                             // keys of a 
 constexpr int STAGES = 2;                                          // tiles that a warp has on the way
 constexpr int BLOCK_BYTES = int4_block_bytes(D), TILE_BYTES = 2 * (TK / INT4_BLOCK) * BLOCK_BYTES;
 constexpr float LOG2E = 1.4426950408889634f;
-// Probabilities are held times 2^14, so that small ones keep their digits in float16, while every step of V that a warp has met is
-// below 2; from the first larger step on (values above 14) times 2^-1, so that no product with a step (up to 65504) overflows.
-constexpr float SMALL_SHIFT = 14.f, LARGE_SHIFT = -1.f;
+// The running maximum follows a score only where that is 2^SLACK times its weight above it, which after a warp's first tile is rare (each time
+// costs 50 multiplications a lane).  Probabilities are held times 2^10, so that small ones keep their digits in float16, while every
+// step of V that a warp has met is below 2; from the first larger step on (values above 14) times 2^-5, so that no product with a
+// step (up to 65504) overflows.
+constexpr float SLACK = 4.f, SMALL_SHIFT = 10.f, LARGE_SHIFT = -5.f;
 
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 
@@ -101,9 +102,8 @@ template <int N> __device__ __forceinline__ Share<N> load_share(const unsigned c
     return s;
 }
 
-__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {      // zeros where it is not there
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
 // n / d for n below 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
@@ -178,7 +178,7 @@ __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("m
 __device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {      // of another thread block's shared memory
     uint32_t at;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
@@ -215,19 +215,11 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
     constexpr int MERGE_STRIDE = D + 2;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint64_t full[WARPS * STAGES];
-    __shared__ int failed;
     __shared__ float others[MAX_CLUSTER][ROWS][2], lse[ROWS];       // a cluster's largest scores and denominators; the row's logarithm of its sum
     __shared__ float weight[WARPS][ROWS];                           // of a warp's sums among the block's
     __shared__ float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int kvh = blockIdx.y, split = blockIdx.z;
-    if (tid == 0) {
-        failed = 0;
-        for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(full + i, 1);
-        mbar_init_fence();
-    }
-    __syncthreads();
     pdl_wait();
     Span span;
     if (!find_span<ROWS>(span, a, blockIdx.x)) return;              // the same for a whole cluster
@@ -237,31 +229,38 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     const int t0 = split * share, n_tiles = max(0, min(share, span.tiles - t0));
 
     unsigned char* ring = smem + (size_t)warp * STAGES * TILE_BYTES;
-    uint64_t* bars = full + warp * STAGES;
-    // Tile t into stage `slot`: one copy per plane and run of blocks that lie in one page, by as many lanes.  Blocks behind the last key and
-    // pages that are not there are left out: what the stage holds in their place meets no probability.
-    const int page_blocks = a.page_size / INT4_BLOCK;
-    const int run = page_blocks % 4 == 0 ? 4 : page_blocks % 2 == 0 ? 2 : 1;
-    const int lane_block = (lane & 3) * run;
-    const bool copies_v = lane >= 4;
-    const unsigned char* plane = (copies_v ? a.v_cache : a.k_cache) + (size_t)kvh * page_blocks * BLOCK_BYTES;
-    unsigned char* landing = ring + (copies_v ? TILE_BYTES / 2 : 0) + lane_block * BLOCK_BYTES;
-    const auto fetch = [&](int t, int slot) {
-        const int pos = span.key(t0 + t) + lane_block * INT4_BLOCK;
-        int page = -1, inside = 0;
-        if (lane < 8 && lane_block < 4 && pos <= span.last_pos) {
-            const int logical = a.by_page(pos);
-            inside = (pos - logical * a.page_size) / INT4_BLOCK;
-            if (logical < a.width) page = pages[logical];
-        }
-        const unsigned copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        if (lane == 0) mbar_expect_tx(bars + slot, copies * run * BLOCK_BYTES);
-        __syncwarp();
-        if (page >= 0) bulk_load(landing + (size_t)slot * TILE_BYTES, plane + ((size_t)page * a.hkv * page_blocks + inside) * BLOCK_BYTES, run * BLOCK_BYTES, bars + slot);
+    // A tile into a stage: eight lanes a block, 16 bytes a lane at a time, the same of keys and values.  (A bulk copy per page took less
+    // address arithmetic but a loop of some 15 instructions for each of its four.)  Its page is looked up one tile ahead.  Blocks behind
+    // the last key and pages that are not there become zeros.
+    constexpr int CHUNKS = BLOCK_BYTES / 16;
+    const uint32_t page_chunks = (uint32_t)(a.hkv * (a.page_size / INT4_BLOCK) * CHUNKS);
+    const size_t lane_bytes = (size_t)kvh * (a.page_size / INT4_BLOCK) * BLOCK_BYTES + (lane & 7) * 16;
+    const unsigned char* k_plane = a.k_cache + lane_bytes;
+    const unsigned char* v_plane = a.v_cache + lane_bytes;
+    const uint32_t landing = (uint32_t)__cvta_generic_to_shared(ring) + (lane >> 3) * BLOCK_BYTES + (lane & 7) * 16;
+    int page = -1, inside = 0;
+    const auto look_up = [&](int t) {
+        const int pos = span.key(t0 + t) + (lane >> 3) * INT4_BLOCK, logical = a.by_page(pos);
+        inside = (pos - logical * a.page_size) / INT4_BLOCK * CHUNKS;
+        page = t < n_tiles && pos <= span.last_pos && logical < a.width ? pages[logical] : -1;
     };
+    const auto fetch = [&](int t, int slot) {
+        if (t < n_tiles) {
+            const size_t at = page < 0 ? 0 : ((size_t)page * page_chunks + inside) * 16;
+            const uint32_t to = landing + slot * TILE_BYTES;
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i)
-        if (warp + WARPS * i < n_tiles) fetch(warp + WARPS * i, i);
+            for (int i = 0; i < CHUNKS; i += 8)
+                if (i + 8 <= CHUNKS || i + (lane & 7) < CHUNKS) {
+                    copy16(to + i * 16, k_plane + at + i * 16, page >= 0);
+                    copy16(to + TILE_BYTES / 2 + i * 16, v_plane + at + i * 16, page >= 0);
+                }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        look_up(t + WARPS);
+    };
+    look_up(warp);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i);
 
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
     // after the shift, (2, 6), (3, 7) / 16.
@@ -330,16 +329,20 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         for (int h = 0; h < 2; ++h) unit[nt][h] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + h));
     }
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
+    float limit[NT][2];                                             // scores above it move the maximum
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < (OFFSET ? NG : 1); ++i) r_off[i][nt][0] = r_off[i][nt][1] = r_off[i][nt][2] = r_off[i][nt][3] = 0.f;
-        m_run[nt][0] = m_run[nt][1] = -INFINITY;
+        m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
         l_run[nt][0] = l_run[nt][1] = 0.f;
     }
     float shift = SMALL_SHIFT;
+    uint32_t eights[4];                                             // the constant operand, kept in registers: as an immediate it was loaded again for every product
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, 0x00080008;" : "=r"(eights[i]));
     // alpha of column h into everything that is summed
     const auto rescale = [&](int nt, float a0, float a1) {
 #pragma unroll
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                         const bool seen = key <= pos && (a.window <= 0 || pos - key < a.window || key < a.keep_first);
                         if (!seen) s[h][nt][e] = -INFINITY;
                     }
-                    more |= s[h][nt][e] > m_run[nt][e & 1];
+                    more |= s[h][nt][e] > limit[nt][e & 1];
                 }
         if (scores) {
 #pragma unroll
@@ -416,7 +419,6 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                             *reinterpret_cast<float2*>(scores + (size_t)key * a.row_stride + col) = make_float2(s[h][nt][e] * unit[nt][0], s[h][nt][e + 1] * unit[nt][1]);
                     }
         }
-        // The running maximum follows only when a score exceeds it (rarely, after the first tiles).
         if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -430,6 +432,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     const float m_new = fmaxf(m_run[nt][e], mx);
                     alpha[e] = m_run[nt][e] == m_new ? 1.f : exp2_fast((m_run[nt][e] - m_new) * unit[nt][e]);
                     m_run[nt][e] = m_new;
+                    limit[nt][e] = m_new + SLACK / unit[nt][e];
                 }
                 rescale(nt, alpha[0], alpha[1]);
             }
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         }
         if (shift == SMALL_SHIFT && __any_sync(0xffffffffu, any & 0x40004000u)) {
             shift = LARGE_SHIFT;
-            constexpr float down = 1.f / 32768.f;                   // 2^(LARGE_SHIFT - SMALL_SHIFT)
+            constexpr float down = 0x1p-15f;                        // 2^(LARGE_SHIFT - SMALL_SHIFT)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) rescale(nt, down, down);
         }
@@ -538,31 +541,24 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int term = 0; term < TERMS; ++term)
-                            mma_f16(r_off[j][nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pb[nt][term][0], pb[nt][term][1]);
+                            mma_f16(r_off[j][nt], eights[0], eights[1], eights[2], eights[3], pb[nt][term][0], pb[nt][term][1]);
                 }
             }
         }
     };
 
-    // The it-th tile of this warp; false where its copies never came.
-    const auto step = [&](auto is_edge, int t, int it) {
-        const int slot = it % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(bars + slot, (uint32_t)(it / STAGES) & 1))) {
-            if (lane == 0) { atomicExch(a.error, 3); failed = 1; }
-            for (int i = 0; i < STAGES; ++i)                        // another bounded chance for this warp's copies to land before the stages are given up
-                if (t + WARPS * i < n_tiles) mbar_wait(bars + (it + i) % STAGES, (uint32_t)((it + i) / STAGES) & 1);
-            return false;
-        }
-        const unsigned char* ks = ring + (size_t)slot * TILE_BYTES;
+    const auto step = [&](auto is_edge, int t, int slot) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const unsigned char* ks = ring + slot * TILE_BYTES;
         work(is_edge, ks, ks + TILE_BYTES / 2, span.key(t0 + t));
         __syncwarp();                                               // every lane has read the stage
-        if (t + WARPS * STAGES < n_tiles) fetch(t + WARPS * STAGES, slot);
-        return true;
+        fetch(t + WARPS * STAGES, slot);
     };
-    int t = warp, it = 0;
-    bool came = true;
-    for (const int plain = min(n_tiles, span.plain - t0); came && t < plain; t += WARPS, ++it) came = step(std::false_type(), t, it);
-    for (; came && t < n_tiles; t += WARPS, ++it) came = step(std::true_type(), t, it);
+    int t = warp, slot = 0;
+    for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::false_type(), t, slot);
+    for (; t < n_tiles; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::true_type(), t, slot);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                                // every warp is done with its stages: they become the merge area
     float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
 #pragma unroll
@@ -602,7 +598,6 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         if (w == 0) {
 #pragma unroll
             for (int i = 0; i < WARPS; ++i) j.add(merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D], 0.f, merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D + 1]);
-            if (failed) j.den = NAN;
             sums[r * MERGE_STRIDE + D] = j.m; sums[r * MERGE_STRIDE + D + 1] = j.den;
             if (!clustered && r < span.rows) {
                 float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
@@ -825,7 +820,7 @@ template <int NT> int launch(Args a, const Shape& shape, int n_req, float* mass,
 
 CISR_EXPORT void cisr_attn_int4_set_pdl(int on) { g_pdl = on != 0; }
 CISR_EXPORT int cisr_attn_int4_head_dim() { return D; }
-// `error_flag`: one zeroed int in device memory that the kernel sets when a wait on a copy ran out.
+// `error_flag`: one zeroed int in device memory that the kernels set when a request is longer than they were told.
 CISR_EXPORT int cisr_attn_int4_init(int* error_flag) { g_error = error_flag; return 0; }
 
 // Floats of scratch that a call with these sizes takes (partial sums and statistics of the ranges, with `mass` also the scores).
