@@ -43,11 +43,10 @@ constexpr int STAGES = 2;                                          // tiles that
 constexpr int BLOCK_BYTES = int4_block_bytes(D), TILE_BYTES = 2 * (TK / INT4_BLOCK) * BLOCK_BYTES;
 constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum follows a score only where that is 2^SLACK times its weight above it, which after a warp's first tile is rare (each time
-// costs 50 multiplications a lane).  Probabilities are held times 2^10, so that small ones keep their digits in float16, while every
-// step of V that a warp has met is below 2; from the first larger step on (values above 14) times 2^-5, so that no product with a
-// step (up to 65504) overflows.
-constexpr float SLACK = 4.f, SMALL_SHIFT = 10.f, LARGE_SHIFT = -5.f;
-
+// costs 50 multiplications a lane).  Probabilities are held times 2^5 (for float queries, whose second terms are 2^-11 of the first, 2^9): with
+// steps of V below 128 (8; values below 896 or 56) no product of the two overflows a float16, and small ones keep their digits.  A warp whose sums come out not finite does its keys
+// again with probabilities times 2^-5, where no step can overflow.  (Looking at every step instead took 8 instructions per 16 keys.)
+constexpr float SLACK = 4.f, USUAL_SHIFT = TERMS == 1 ? 5.f : 9.f, LARGE_SHIFT = -5.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 
 // Warps of a thread block: eight where a warp's registers let two such blocks share an SM.
@@ -108,13 +107,15 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
 
 // n / d for n below 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
 struct Divider {
-    uint32_t d, m, shift;
-    __host__ __device__ Divider() : d(1), m(0), shift(0) {}
-    explicit Divider(uint32_t d_) : d(d_), shift(0) {
-        while ((1u << shift) < d) ++shift;                          // d >= 2
+    uint32_t m, shift;               // m 0: divided by one
+    __host__ __device__ Divider() : m(0), shift(0) {}
+    explicit Divider(uint32_t d) : m(0), shift(0) {
+        if (d < 2) return;
+        while ((1u << shift) < d) ++shift;
         m = (uint32_t)((1ull << (31 + shift)) / d + 1);
+        --shift;
     }
-    __device__ __forceinline__ int operator()(int n) const { return (int)(__umulhi((uint32_t)n, m) >> (shift - 1)); }
+    __device__ __forceinline__ int operator()(int n) const { return m ? (int)(__umulhi((uint32_t)n, m) >> shift) : n; }
 };
 
 struct Args {
@@ -128,7 +129,8 @@ struct Args {
     float* mass;         // added to by this kernel itself, or null
     int max_queries, tiles, row_stride, n_splits, cluster, longest;
     int hq, hkv, page_size, window, keep_first;
-    Divider by_page;
+    Divider by_page, by_group, by_tiles;
+    int group;
     float scale, sink_all; const float* sink_heads;
     int* error;
 };
@@ -146,17 +148,17 @@ struct Span {
     }
 };
 template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x) {
-    s.req = a.tiles == 1 ? x : x / a.tiles;
+    s.req = a.by_tiles(x);
     const int tile = x - s.req * a.tiles;
-    s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.group = a.hq / a.hkv; s.row0 = tile * ROWS;
+    s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.group = a.group; s.row0 = tile * ROWS;
     s.rows = min(ROWS, s.n * s.group - s.row0);
     if (s.n > a.max_queries || s.rows <= 0) return false;           // another kernel's request, or no such tile
     if (s.ctx > a.longest) {                                        // more rows than the scratch was made for
         if (threadIdx.x == 0) atomicExch(a.error, 6);
         return false;
     }
-    s.first_pos = s.ctx - s.n + s.row0 / s.group;
-    s.last_pos = s.ctx - s.n + (s.row0 + s.rows - 1) / s.group;
+    s.first_pos = s.ctx - s.n + a.by_group(s.row0);
+    s.last_pos = s.ctx - s.n + a.by_group(s.row0 + s.rows - 1);
     s.kept_tiles = 0; s.window_base = 0;
     const int begin = s.first_pos - a.window + 1;
     if (a.window > 0 && begin >= TK) {
@@ -168,12 +170,6 @@ template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Arg
     s.plain = min(s.tiles - s.lead, max(0, s.first_pos + 1 < s.window_base ? 0 : (s.first_pos + 1 - s.window_base) / TK + s.kept_tiles - s.lead));
     return true;
 }
-// Of a pair of steps those of keys that some row of the tile sees: what lies in the others' place does not matter.
-__device__ __forceinline__ uint32_t in_sight(const Span& s, const Args& a, int key) {
-    const auto seen = [&](int k) { return k <= s.last_pos && (a.window <= 0 || k >= s.first_pos - a.window + 1 || k < a.keep_first); };
-    return (seen(key) ? 0xffffu : 0u) | (seen(key + 1) ? 0xffff0000u : 0u);
-}
-
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {      // of another thread block's shared memory
     uint32_t at;
@@ -258,9 +254,12 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         asm volatile("cp.async.commit_group;" ::: "memory");
         look_up(t + WARPS);
     };
-    look_up(warp);
+    const auto begin = [&] {
+        look_up(warp);
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i);
+        for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i);
+    };
+    begin();
 
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
     // after the shift, (2, 6), (3, 7) / 16.
@@ -273,7 +272,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         const int r = nt * 8 + g;
         const bool there = r < span.rows;
         const int row = span.row0 + (there ? r : 0);
-        const T* q = a.q + ((size_t)(tok0 + row / span.group) * a.hq + kvh * span.group + row % span.group) * D;
+        const int token = a.by_group(row);
+        const T* q = a.q + ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D;
         float x[NG][8];
         uint32_t top = 0;
 #pragma unroll
@@ -330,16 +330,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     }
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
     float limit[NT][2];                                             // scores above it move the maximum
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < (OFFSET ? NG : 1); ++i) r_off[i][nt][0] = r_off[i][nt][1] = r_off[i][nt][2] = r_off[i][nt][3] = 0.f;
-        m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
-        l_run[nt][0] = l_run[nt][1] = 0.f;
-    }
-    float shift = SMALL_SHIFT;
+    int own_pos[NT][2];                                             // a column's place, for tiles with masks
+    float shift = USUAL_SHIFT;
     uint32_t eights[4];                                             // the constant operand, kept in registers: as an immediate it was loaded again for every product
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, 0x00080008;" : "=r"(eights[i]));
@@ -401,7 +393,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (EDGE) {
-                        const int key = k0 + 16 * h + g + 8 * (e >> 1), pos = span.ctx - span.n + (span.row0 + min(nt * 8 + 2 * c + (e & 1), span.rows - 1)) / span.group;
+                        const int key = k0 + 16 * h + g + 8 * (e >> 1), pos = own_pos[nt][e & 1];
                         const bool seen = key <= pos && (a.window <= 0 || pos - key < a.window || key < a.keep_first);
                         if (!seen) s[h][nt][e] = -INFINITY;
                     }
@@ -437,21 +429,6 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 rescale(nt, alpha[0], alpha[1]);
             }
         }
-        // a large step of V changes the probabilities' shift for good
-        uint32_t any = 0;
-#pragma unroll
-        for (int i = lane; i < 16 * NG; i += 32) {
-            const int b = i / (4 * NG), w = i - b * 4 * NG;
-            uint32_t two = *reinterpret_cast<const uint32_t*>(vs + b * BLOCK_BYTES + 4 * D + 4 * w);
-            if constexpr (EDGE) two &= in_sight(span, a, k0 + 8 * b + 2 * (w / NG));
-            any |= two;
-        }
-        if (shift == SMALL_SHIFT && __any_sync(0xffffffffu, any & 0x40004000u)) {
-            shift = LARGE_SHIFT;
-            constexpr float down = 0x1p-15f;                        // 2^(LARGE_SHIFT - SMALL_SHIFT)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) rescale(nt, down, down);
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -483,14 +460,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             Share<4 * NG> sv[2];                                    // the steps of two neighbouring keys side by side
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                sv[b] = load_share<4 * NG>(vs + (2 * h + b) * BLOCK_BYTES + 4 * D + c * 4 * NG);
-                if constexpr (EDGE) {
-                    const uint32_t keep = in_sight(span, a, k0 + 16 * h + 8 * b + 2 * c);
-#pragma unroll
-                    for (int j = 0; j < NG; ++j) sv[b].w[j] &= keep;
-                }
-            }
+            for (int b = 0; b < 2; ++b) sv[b] = load_share<4 * NG>(vs + (2 * h + b) * BLOCK_BYTES + 4 * D + c * 4 * NG);
             const int turned = (g ^ int4_value_turn<D>(c)) * 2 * NG;
             const Share<2 * NG> u0 = load_share<2 * NG>(b0 + c * (D / 2) + turned), u1 = load_share<2 * NG>(b0 + (4 + c) * (D / 2) + turned);
             const Share<2 * NG> u2 = load_share<2 * NG>(b1 + c * (D / 2) + turned), u3 = load_share<2 * NG>(b1 + (4 + c) * (D / 2) + turned);
@@ -555,9 +525,32 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         __syncwarp();                                               // every lane has read the stage
         fetch(t + WARPS * STAGES, slot);
     };
-    int t = warp, slot = 0;
-    for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::false_type(), t, slot);
-    for (; t < n_tiles; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::true_type(), t, slot);
+    for (;;) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < (OFFSET ? NG : 1); ++i) r_off[i][nt][0] = r_off[i][nt][1] = r_off[i][nt][2] = r_off[i][nt][3] = 0.f;
+            m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
+            l_run[nt][0] = l_run[nt][1] = 0.f;
+        }
+        int t = warp, slot = 0;
+        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::false_type(), t, slot);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
+        for (; t < n_tiles; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::true_type(), t, slot);
+        float all = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) all += (o[i][nt][0] + o[i][nt][1] + o[i][nt][2] + o[i][nt][3]) * 0.f;
+        if (shift == LARGE_SHIFT || !__any_sync(0xffffffffu, all != 0.f)) break;
+        shift = LARGE_SHIFT;
+        begin();
+    }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                                // every warp is done with its stages: they become the merge area
     float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
@@ -585,8 +578,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     // The warps' sums joined, in their order: into the first warp's place for the cluster, or to where they go.
     const bool alone = a.n_splits == 1, clustered = a.cluster > 1;
     const auto place = [&](int r) {                                 // of row r in q and out
-        const int row = span.row0 + r;
-        return ((size_t)(tok0 + row / span.group) * a.hq + kvh * span.group + row % span.group) * D;
+        const int row = span.row0 + r, token = a.by_group(row);
+        return ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D;
     };
     const auto sink_of = [&](int r) { return a.sink_heads ? a.sink_heads[kvh * span.group + (span.row0 + r) % span.group] : a.sink_all; };
     if (tid < WARPS * ROWS) {
@@ -778,7 +771,7 @@ struct Shape {
         long long reach = longest;
         if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
         const int most = (int)((reach + (long long)TK * warps - 1) / (TK * warps));      // a tile for every warp
-        const long long want = (2 * room + pairs - 1) / pairs;                          // two rounds of thread blocks
+        const long long want = (room + pairs - 1) / pairs;                              // thread blocks for every place
         splits = (int)(want < most ? want : most);
         if (splits > MAX_CLUSTER) splits = pairs * MAX_CLUSTER >= room / 2 ? MAX_CLUSTER : splits < 64 ? splits : 64;
         if (splits < 1) splits = 1;
@@ -842,12 +835,13 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 7) return -2;      // rows are read by 16 bytes
     const Shape shape(n_req, max_queries, longest, hq, hkv, window, keep_first);
     if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
+    const int group = hq / hkv;
     Args a{};
     a.q = (const T*)q; a.out = (T*)out; a.k_cache = (const unsigned char*)k_cache; a.v_cache = (const unsigned char*)v_cache;
     a.req_slot = req_slot; a.table = block_table; a.width = width; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len;
     a.partial = scratch; a.stats = scratch + shape.partial(); a.scores = mass ? a.stats + shape.stats() : nullptr;
     a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
-    a.by_page = Divider((uint32_t)page_size);
+    a.by_page = Divider((uint32_t)page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.group = group;
     a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
     a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
     return shape.rows == 8 ? launch<1>(a, shape, n_req, mass, (cudaStream_t)stream) : launch<2>(a, shape, n_req, mass, (cudaStream_t)stream);
