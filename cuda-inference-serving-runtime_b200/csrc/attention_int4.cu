@@ -209,11 +209,11 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     constexpr int ROWS = 8 * NT, WARPS = warps_of<NT>(), THREADS = 32 * WARPS;
     constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
-    constexpr int MERGE_STRIDE = D + 2;
+    constexpr int MERGE_STRIDE = D + 4;                  // rows of whole 16 bytes
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float others[MAX_CLUSTER][ROWS][2], lse[ROWS];       // a cluster's largest scores and denominators; the row's logarithm of its sum
     __shared__ float weight[WARPS][ROWS];                           // of a warp's sums among the block's
-    __shared__ float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
+    __shared__ __align__(16) float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int kvh = blockIdx.y, split = blockIdx.z;
     pdl_wait();
@@ -262,71 +262,93 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     begin();
 
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
-    // after the shift, (2, 6), (3, 7) / 16.
-    uint32_t qf[NT][NG][2][TERMS][2];
-    uint32_t qs[NT];                                                // -8 2^-24 sum q of two groups, the first float16 term (c below 2) or the second
-    float unit[NT][2];                                              // of a column's sums, in the softmax's exponent (base 2); positive
+    // after the shift, (2, 6), (3, 7) / 16.  All warps need the same: each makes some groups' operands and they exchange them.
+    constexpr int TURNS = (NT * NG + WARPS - 1) / WARPS;
+    __shared__ uint4 operand[NT * NG][TERMS][32];
+    __shared__ uint32_t largest[ROWS];
+    __shared__ float group_sum[ROWS][4];
     const int tok0 = a.q_start[span.req];
+    if (tid < ROWS) {
+        largest[tid] = 0;
+        for (int j = NG; j < 4; ++j) group_sum[tid][j] = 0.f;
+    }
+    __syncthreads();
+    float x[TURNS][8];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int r = nt * 8 + g;
+    for (int turn = 0; turn < TURNS; ++turn) {
+        const int i = warp + turn * WARPS, nt = i / NG, j = i - nt * NG, r = nt * 8 + g;
+        if (i >= NT * NG) continue;
         const bool there = r < span.rows;
-        const int row = span.row0 + (there ? r : 0);
-        const int token = a.by_group(row);
-        const T* q = a.q + ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D;
-        float x[NG][8];
+        const int row = span.row0 + (there ? r : 0), token = a.by_group(row);
+        const T* q = a.q + ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D + 32 * j + 8 * c;
+#if STORAGE_BF16
+        const uint4 v = *reinterpret_cast<const uint4*>(q);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[turn][2 * e] = __uint_as_float(w[e] << 16); x[turn][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+#else
+        const float4 u = *reinterpret_cast<const float4*>(q), v = *reinterpret_cast<const float4*>(q + 4);
+        x[turn][0] = u.x; x[turn][1] = u.y; x[turn][2] = u.z; x[turn][3] = u.w; x[turn][4] = v.x; x[turn][5] = v.y; x[turn][6] = v.z; x[turn][7] = v.w;
+#endif
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-#if STORAGE_BF16
-            const uint4 v = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * c);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { x[j][2 * i] = __uint_as_float(w[i] << 16); x[j][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-#else
-            const float4 u = *reinterpret_cast<const float4*>(q + 32 * j + 8 * c), v = *reinterpret_cast<const float4*>(q + 32 * j + 8 * c + 4);
-            x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w; x[j][4] = v.x; x[j][5] = v.y; x[j][6] = v.z; x[j][7] = v.w;
-#endif
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (!there) x[j][i] = 0.f;
-                top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
-            }
+        for (int e = 0; e < 8; ++e) {
+            if (!there) x[turn][e] = 0.f;
+            top = max(top, __float_as_uint(x[turn][e]) & 0x7fffffffu);
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int up = min(14 - ((int)(top >> 23) - 127), 120);     // the row times 2^up is below 2^15
-        const float factor = copysignf(__uint_as_float((uint32_t)(up + 127) << 23), a.scale);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c == 0) atomicMax(&largest[r], top);
+    }
+    __syncthreads();
+    const auto exponent = [&](int r) { return min(14 - ((int)(largest[r] >> 23) - 127), 120); };       // the row times 2 to it is below 2^15
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
+    for (int turn = 0; turn < TURNS; ++turn) {
+        const int i = warp + turn * WARPS, nt = i / NG, j = i - nt * NG, r = nt * 8 + g;
+        if (i >= NT * NG) continue;
+        const float factor = copysignf(__uint_as_float((uint32_t)(exponent(r) + 127) << 23), a.scale);
+        float sum = 0.f;
+        uint32_t w[TERMS][4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float p[4] = {x[j][2 * k] * factor, x[j][2 * k + 4] * factor, x[j][2 * k + 1] * factor * SECOND, x[j][2 * k + 5] * factor * SECOND};
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int term = 0; term < TERMS; ++term)
+            for (int h = 0; h < 2; ++h) {
+                float p0 = x[turn][2 * k + h] * factor * (h ? SECOND : 1.f), p1 = x[turn][2 * k + h + 4] * factor * (h ? SECOND : 1.f);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t w = pack_f16(p[2 * h], p[2 * h + 1]);
-                        qf[nt][j][k][term][h] = w;
-                        const float lo = low_half(w), hi = high_half(w);
-                        if (OFFSET) sum[j] += (h ? 16.f : 1.f) * (lo + hi);
-                        p[2 * h] -= lo; p[2 * h + 1] -= hi;
-                    }
+                for (int term = 0; term < TERMS; ++term) {
+                    w[term][2 * k + h] = pack_f16(p0, p1);
+                    const float lo = low_half(w[term][2 * k + h]), hi = high_half(w[term][2 * k + h]);
+                    sum += (h ? 1.f / SECOND : 1.f) * (lo + hi);
+                    p0 -= lo; p1 -= hi;
+                }
             }
-            if constexpr (OFFSET) {
-                sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-                sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) operand[i][term][lane] = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (c == 0) group_sum[r][j] = sum;
+    }
+    __syncthreads();
+    uint32_t qf[NT][NG][2][TERMS][2];
+    uint32_t qs[NT];                                                // -8 2^-24 sum q of two groups, the first float16 term (c below 2) or the second
+    float unit[NT][2];                                              // of a column's sums, in the softmax's exponent (base 2); positive
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+                const uint4 w = operand[nt * NG + j][term][lane];
+                qf[nt][j][0][term][0] = w.x; qf[nt][j][0][term][1] = w.y; qf[nt][j][1][term][0] = w.z; qf[nt][j][1][term][1] = w.w;
             }
-        }
         if constexpr (OFFSET) {
-            const float s0 = -0x1p-21f * (c & 1 ? sum[2] : sum[0]), s1 = -0x1p-21f * (c & 1 ? sum[3] : sum[1]);
+            const float s0 = -0x1p-21f * group_sum[nt * 8 + g][2 * (c & 1)], s1 = -0x1p-21f * group_sum[nt * 8 + g][2 * (c & 1) + 1];
             qs[nt] = pack_f16(s0, s1);
             if (c >= 2) qs[nt] = pack_f16(s0 - low_half(qs[nt]), s1 - high_half(qs[nt]));
         }
-        const float mine = fmaxf(fabsf(a.scale) * LOG2E * (OFFSET ? 0x1p24f : 0x1p9f) * __uint_as_float((uint32_t)(127 - up) << 23), 0x1p-126f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) unit[nt][h] = __shfl_sync(0xffffffffu, mine, 4 * (2 * c + h));
+        for (int h = 0; h < 2; ++h)
+            unit[nt][h] = fmaxf(fabsf(a.scale) * LOG2E * (OFFSET ? 0x1p24f : 0x1p9f) * __uint_as_float((uint32_t)(127 - exponent(nt * 8 + 2 * c + h)) << 23), 0x1p-126f);
     }
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
     float limit[NT][2];                                             // scores above it move the maximum
@@ -542,11 +564,14 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 #pragma unroll
             for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
         for (; t < n_tiles; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::true_type(), t, slot);
-        float all = 0.f;
+        float all = 0.f;                                            // an overflow is in the sums of the constant operand too
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) all += (o[i][nt][0] + o[i][nt][1] + o[i][nt][2] + o[i][nt][3]) * 0.f;
+            for (int i = 0; i < (OFFSET ? NG : D / 16); ++i) {
+                const float* v = OFFSET ? r_off[OFFSET ? i : 0][nt] : o[i][nt];
+                all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
+            }
         if (shift == LARGE_SHIFT || !__any_sync(0xffffffffu, all != 0.f)) break;
         shift = LARGE_SHIFT;
         begin();
@@ -564,14 +589,13 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             float* row = merge + ((size_t)warp * ROWS + nt * 8 + 2 * c + h) * MERGE_STRIDE;
 #pragma unroll
-            for (int j = 0; j < NG; ++j)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float off = OFFSET ? r_off[OFFSET ? j : 0][nt][h] : 0.f;
-                    constexpr float whole = OFFSET ? 0x1p24f : 0x1p9f;
-                    row[32 * j + 4 * g + 2 * k] = (o[2 * j + k][nt][h] - off) * whole;
-                    row[32 * j + 4 * g + 2 * k + 1] = (o[2 * j + k][nt][2 + h] * SECOND - off) * whole;
-                }
+            for (int j = 0; j < NG; ++j) {
+                const float off = OFFSET ? r_off[OFFSET ? j : 0][nt][h] : 0.f;
+                constexpr float whole = OFFSET ? 0x1p24f : 0x1p9f;
+                *reinterpret_cast<float4*>(row + 32 * j + 4 * g) =
+                    make_float4((o[2 * j][nt][h] - off) * whole, (o[2 * j][nt][2 + h] * SECOND - off) * whole, (o[2 * j + 1][nt][h] - off) * whole,
+                                (o[2 * j + 1][nt][2 + h] * SECOND - off) * whole);
+            }
             if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : fmaf(m_run[nt][h], unit[nt][h], -shift); row[D + 1] = l; }
         }
     __syncthreads();
@@ -600,19 +624,26 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         }
     }
     __syncthreads();
-    for (int e = tid; e < span.rows * D; e += THREADS) {
-        const int r = e / D, d = e - r * D;
-        float num = 0.f;
+    for (int e = tid; e < span.rows * (D / 4); e += THREADS) {
+        const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
+        float num[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) num = fmaf(weight[w][r], merge[((size_t)w * ROWS + r) * MERGE_STRIDE + d], num);
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(merge + ((size_t)w * ROWS + r) * MERGE_STRIDE + d);
+            const float part = weight[w][r];
+            num[0] = fmaf(part, v.x, num[0]); num[1] = fmaf(part, v.y, num[1]); num[2] = fmaf(part, v.z, num[2]); num[3] = fmaf(part, v.w, num[3]);
+        }
         if (clustered) {
-            sums[r * MERGE_STRIDE + d] = num;
+            *reinterpret_cast<float4*>(sums + r * MERGE_STRIDE + d) = make_float4(num[0], num[1], num[2], num[3]);
         } else if (alone) {
             Joined j;
             j.m = sums[r * MERGE_STRIDE + D]; j.den = sums[r * MERGE_STRIDE + D + 1];
-            a.out[place(r) + d] = from_float<T>(j.den == 0.f ? 0.f : num / j.whole(sink_of(r)));
+            const float whole = j.whole(sink_of(r));
+            T* to = a.out + place(r) + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = from_float<T>(j.den == 0.f ? 0.f : num[i] / whole);
         } else {
-            a.partial[((base_row + r) * a.n_splits + split) * D + d] = num;
+            *reinterpret_cast<float4*>(a.partial + ((base_row + r) * a.n_splits + split) * D + d) = make_float4(num[0], num[1], num[2], num[3]);
         }
     }
     if (clustered) {
@@ -789,9 +820,9 @@ struct Shape {
 
 template <int NT> int launch(Args a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
     constexpr int WARPS = warps_of<NT>();
-    constexpr size_t RING = (size_t)WARPS * STAGES * TILE_BYTES, MERGE = sizeof(float) * WARPS * 8 * NT * (D + 2);
+    constexpr size_t RING = (size_t)WARPS * STAGES * TILE_BYTES, MERGE = sizeof(float) * WARPS * 8 * NT * (D + 4);
     constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
-    if constexpr (SMEM > 48 * 1024 - 8192) {
+    if constexpr (SMEM > 48 * 1024 - 20480) {
         const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
         if (e != cudaSuccess) return (int)e;
     }
@@ -832,7 +863,7 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
     if (n_req <= 0 || max_queries <= 0) return 0;
     if (!g_error) return -13;
     if (hkv <= 0 || hkv > 65535 || hq % hkv || !isfinite(scale) || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
-    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 7) return -2;      // rows are read by 16 bytes
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 15) return -2;      // rows are read by 16 bytes
     const Shape shape(n_req, max_queries, longest, hq, hkv, window, keep_first);
     if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
     const int group = hq / hkv;
