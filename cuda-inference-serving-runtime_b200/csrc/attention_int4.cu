@@ -48,6 +48,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // again with probabilities times 2^-5, where no step can overflow.  (Looking at every step instead took 8 instructions per 16 keys.)
 constexpr float SLACK = 4.f, USUAL_SHIFT = TERMS == 1 ? 5.f : 9.f, LARGE_SHIFT = -5.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
+constexpr int MAX_RANKED = 128;                                    // requests that are put in order of length, a thread each
 
 // Warps of a thread block: eight where a warp's registers let two such blocks share an SM.
 template <int NT> constexpr int warps_of() { return NT == 1 && TERMS == 1 ? 8 : 4; }
@@ -129,8 +130,8 @@ struct Args {
     float* mass;         // added to by this kernel itself, or null
     int max_queries, tiles, row_stride, n_splits, cluster, longest;
     int hq, hkv, page_size, window, keep_first;
-    Divider by_page, by_group, by_tiles;
-    int group;
+    Divider by_page, by_group, by_tiles, by_heads;
+    int group, n_req, ranked;
     float scale, sink_all; const float* sink_heads;
     int* error;
 };
@@ -215,11 +216,29 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     __shared__ float weight[WARPS][ROWS];                           // of a warp's sums among the block's
     __shared__ __align__(16) float sums[ROWS * MERGE_STRIDE];                     // this block's, for its cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    // The key heads of a request's tile of rows are neighbours in the order of thread blocks (a page's heads lie side by side), and where
+    // not all blocks run at once the longest requests come first, so that the last blocks to end are short ones: 64 requests of 4000 to
+    // 8000 rows 111 us in the order of requests.
+    const int split = blockIdx.z, id = blockIdx.x + gridDim.x * blockIdx.y;
+    int unit_of = a.by_heads(id);
+    const int kvh = id - unit_of * a.hkv;
     pdl_wait();
+    if (a.ranked) {
+        __shared__ int lens[MAX_RANKED], chosen;
+        for (int i = tid; i < a.n_req; i += THREADS) lens[i] = a.ctx_len[i];
+        __syncthreads();
+        const int rank = a.by_tiles(unit_of);
+        if (tid < a.n_req) {
+            int before = 0;
+            for (int i = 0; i < a.n_req; ++i) before += lens[i] > lens[tid] || (lens[i] == lens[tid] && i < tid);
+            if (before == rank) chosen = tid;
+        }
+        __syncthreads();
+        unit_of += (chosen - rank) * a.tiles;
+    }
     Span span;
-    if (!find_span<ROWS>(span, a, blockIdx.x)) return;              // the same for a whole cluster
-    const size_t base_row = ((size_t)blockIdx.x * a.hkv + kvh) * a.row_stride;
+    if (!find_span<ROWS>(span, a, unit_of)) return;                 // the same for a whole cluster
+    const size_t base_row = ((size_t)unit_of * a.hkv + kvh) * a.row_stride;
     const int* pages = a.table + (size_t)a.req_slot[span.req] * a.width;
     const int share = (span.tiles + a.n_splits - 1) / a.n_splits;   // tiles of a split: the request's own, so that a cluster ends together
     const int t0 = split * share, n_tiles = max(0, min(share, span.tiles - t0));
@@ -368,7 +387,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         l_run[nt][0] *= a0; l_run[nt][1] *= a1;
     };
 
-    float* scores = a.scores ? a.scores + ((size_t)blockIdx.x * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
+    float* scores = a.scores ? a.scores + ((size_t)unit_of * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
     // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.
     const auto work = [&](auto is_edge, const unsigned char* ks, const unsigned char* vs, int k0) {
         constexpr bool EDGE = decltype(is_edge)::value;
@@ -687,7 +706,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         for (int i = tid; i < n_tiles * TK; i += THREADS) {
             const int key = span.key(t0 + i / TK) + i % TK;
             if (key > span.last_pos) continue;
-            const float* score = a.scores + (((size_t)blockIdx.x * a.hkv + kvh) * a.longest + key) * a.row_stride;
+            const float* score = a.scores + (((size_t)unit_of * a.hkv + kvh) * a.longest + key) * a.row_stride;
             float w = 0.f;
             for (int r = 0; r < span.rows; ++r) w += exp2_fast(score[r] - lse[r]);
             const int logical = a.by_page(key), page = logical < a.width ? pages[logical] : -1;
@@ -790,6 +809,7 @@ int sm_count() {                                                    // of the cu
 // for (even, so that pairs are aligned), splits of a request's keys and whether they are one cluster.
 struct Shape {
     int rows, tiles, stride, splits, cluster;
+    bool ranked;
     long long units;                 // requests by tiles by key heads by rows
     long long keys;
     Shape(int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
@@ -801,12 +821,24 @@ struct Shape {
         const long long pairs = (long long)n_req * tiles * hkv, room = (long long)sm_count() * blocks;
         long long reach = longest;
         if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
+        // A block takes as long as its warps' tiles and some five more for its start and end (fitted to the times of 1 to 3 splits); blocks beyond
+        // those that run at once come in rounds, of which the last is not even.  The count of splits with the least of it; up to a cluster's size,
+        // where that leaves no SM idle, else more, which another kernel joins.
+        const double tiles_of_warp = (double)reach / (TK * warps);
         const int most = (int)((reach + (long long)TK * warps - 1) / (TK * warps));      // a tile for every warp
-        const long long want = (room + pairs - 1) / pairs;                              // thread blocks for every place
-        splits = (int)(want < most ? want : most);
-        if (splits > MAX_CLUSTER) splits = pairs * MAX_CLUSTER >= room / 2 ? MAX_CLUSTER : splits < 64 ? splits : 64;
-        if (splits < 1) splits = 1;
+        splits = 1;
+        double best = 0;
+        for (int s = 1; s <= (most < MAX_CLUSTER ? most : MAX_CLUSTER); ++s) {
+            const double rounds = (double)pairs * s / room, time = (rounds > 1 ? rounds + 0.4 : 1) * (5 + tiles_of_warp / s);
+            if (s == 1 || time < best) { best = time; splits = s; }
+        }
+        if (splits == MAX_CLUSTER && pairs * MAX_CLUSTER < room / 2) {
+            const long long want = (room + pairs - 1) / pairs;
+            splits = (int)(want < most ? want : most);
+            if (splits > 64) splits = 64;
+        }
         cluster = splits <= MAX_CLUSTER ? splits : 1;
+        ranked = n_req > 1 && n_req <= MAX_RANKED && pairs * splits > room;
         units = pairs * stride;
         keys = longest;
     }
@@ -872,7 +904,8 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
     a.req_slot = req_slot; a.table = block_table; a.width = width; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len;
     a.partial = scratch; a.stats = scratch + shape.partial(); a.scores = mass ? a.stats + shape.stats() : nullptr;
     a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
-    a.by_page = Divider((uint32_t)page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.group = group;
+    a.by_page = Divider((uint32_t)page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.by_heads = Divider((uint32_t)hkv);
+    a.group = group; a.n_req = n_req; a.ranked = shape.ranked;
     a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
     a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
     return shape.rows == 8 ? launch<1>(a, shape, n_req, mass, (cudaStream_t)stream) : launch<2>(a, shape, n_req, mass, (cudaStream_t)stream);
