@@ -19,6 +19,8 @@
 // Operands other than codes are float16: of queries, normed by a power of two per row, exactly what bfloat16 holds (elements below 2^-24 of
 // the row's largest lose digits); of probabilities 11 bits.  Float queries take two float16 terms (22 bits) for both.
 // Scores, running maxima, sums and outputs are float.
+#include <climits>
+
 #include "int4_cache.cuh"
 
 #ifndef HEAD_DIM
@@ -703,14 +705,33 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     // The weights of this block's keys, from the scores that it has just written: the rows in their order.
     if (a.mass) {
         __syncthreads();
-        for (int i = tid; i < n_tiles * TK; i += THREADS) {
-            const int key = span.key(t0 + i / TK) + i % TK;
-            if (key > span.last_pos) continue;
-            const float* score = a.scores + (((size_t)unit_of * a.hkv + kvh) * a.longest + key) * a.row_stride;
-            float w = 0.f;
-            for (int r = 0; r < span.rows; ++r) w += exp2_fast(score[r] - lse[r]);
-            const int logical = a.by_page(key), page = logical < a.width ? pages[logical] : -1;
-            if (page >= 0 && w != 0.f) a.mass[((size_t)page * a.hkv + kvh) * a.page_size + key - logical * a.page_size] += w;
+        constexpr int AT_ONCE = 4;                                  // keys of a thread on their way together
+        for (int i0 = tid; i0 < n_tiles * TK; i0 += AT_ONCE * THREADS) {
+            float* to[AT_ONCE];
+            float w[AT_ONCE], old[AT_ONCE];
+            const float* score[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int i = i0 + u * THREADS, key = i < n_tiles * TK ? span.key(t0 + i / TK) + i % TK : INT_MAX;
+                const bool there = key <= span.last_pos;
+                const int logical = there ? a.by_page(key) : 0, at = there && logical < a.width ? pages[logical] : -1;
+                to[u] = at < 0 ? nullptr : a.mass + ((size_t)at * a.hkv + kvh) * a.page_size + key - logical * a.page_size;
+                score[u] = scores + (there ? (size_t)key * a.row_stride : 0);
+                old[u] = to[u] ? *to[u] : 0.f;
+                w[u] = 0.f;
+            }
+            for (int r = 0; r < span.rows; r += 2) {
+                const float first = lse[r], second = lse[r + 1 < span.rows ? r + 1 : r];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    if (!to[u]) continue;
+                    const float2 v = *reinterpret_cast<const float2*>(score[u] + r);
+                    w[u] += exp2_fast(v.x - first);
+                    if (r + 1 < span.rows) w[u] += exp2_fast(v.y - second);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) if (to[u] && w[u] != 0.f) *to[u] = old[u] + w[u];
         }
     }
 }
