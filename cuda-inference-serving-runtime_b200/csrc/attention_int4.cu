@@ -133,7 +133,7 @@ struct Args {
     int max_queries, tiles, row_stride, n_splits, cluster, longest;
     int hq, hkv, page_size, window, keep_first;
     Divider by_page, by_group, by_tiles, by_heads;
-    int group, n_req, ranked;
+    int group, n_req, ranked, rank_threads;       // rank_threads: a power of two of n_req or more
     float scale, sink_all; const float* sink_heads;
     int* error;
 };
@@ -142,7 +142,7 @@ struct Args {
 // window, then those from the first key inside the first row's window to the last row's own.  They are walked from the `lead`th on, the
 // others last: then the tiles that some row does not see whole are the last ones, and the first `plain` need no masks.
 struct Span {
-    int req, n, ctx, group, row0, rows, first_pos, last_pos;
+    int req, n, ctx, slot, tok0, group, row0, rows, first_pos, last_pos;
     int kept_tiles, window_base, tiles, lead, plain;
     __device__ __forceinline__ int key(int t) const {
         t += lead;
@@ -153,7 +153,8 @@ struct Span {
 template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x) {
     s.req = a.by_tiles(x);
     const int tile = x - s.req * a.tiles;
-    s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.group = a.group; s.row0 = tile * ROWS;
+    s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.slot = a.req_slot[s.req]; s.tok0 = a.q_start[s.req];      // one trip to memory
+    s.group = a.group; s.row0 = tile * ROWS;
     s.rows = min(ROWS, s.n * s.group - s.row0);
     if (s.n > a.max_queries || s.rows <= 0) return false;           // another kernel's request, or no such tile
     if (s.ctx > a.longest) {                                        // more rows than the scratch was made for
@@ -226,22 +227,26 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     const int kvh = id - unit_of * a.hkv;
     pdl_wait();
     if (a.ranked) {
-        __shared__ int lens[MAX_RANKED], chosen;
-        for (int i = tid; i < a.n_req; i += THREADS) lens[i] = a.ctx_len[i];
+        __shared__ int lens[MAX_RANKED], before[MAX_RANKED], chosen;
+        for (int i = tid; i < a.n_req; i += THREADS) { lens[i] = a.ctx_len[i]; before[i] = 0; }
         __syncthreads();
-        const int rank = a.by_tiles(unit_of);
-        if (tid < a.n_req) {
-            int before = 0;
-            for (int i = 0; i < a.n_req; ++i) before += lens[i] > lens[tid] || (lens[i] == lens[tid] && i < tid);
-            if (before == rank) chosen = tid;
+        const int rank = a.by_tiles(unit_of), threads_each = THREADS / a.rank_threads, i = tid & (a.rank_threads - 1);
+        if (i < a.n_req) {                                          // how many come before request i, counted by several threads
+            const int mine = lens[i];
+            int n = 0;
+            for (int j = tid / a.rank_threads; j < a.n_req; j += threads_each) n += lens[j] > mine || (lens[j] == mine && j < i);
+            if (n) atomicAdd(&before[i], n);
         }
+        __syncthreads();
+        if (tid < a.n_req && before[tid] == rank) chosen = tid;
         __syncthreads();
         unit_of += (chosen - rank) * a.tiles;
     }
     Span span;
     if (!find_span<ROWS>(span, a, unit_of)) return;                 // the same for a whole cluster
     const size_t base_row = ((size_t)unit_of * a.hkv + kvh) * a.row_stride;
-    const int* pages = a.table + (size_t)a.req_slot[span.req] * a.width;
+    const int* pages = a.table + (size_t)span.slot * a.width;
+    const int tok0 = span.tok0;
     const int share = (span.tiles + a.n_splits - 1) / a.n_splits;   // tiles of a split: the request's own, so that a cluster ends together
     const int t0 = split * share, n_tiles = max(0, min(share, span.tiles - t0));
 
@@ -255,62 +260,69 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     const unsigned char* k_plane = a.k_cache + lane_bytes;
     const unsigned char* v_plane = a.v_cache + lane_bytes;
     const uint32_t landing = (uint32_t)__cvta_generic_to_shared(ring) + (lane >> 3) * BLOCK_BYTES + (lane & 7) * 16;
-    int page = -1, inside = 0;
+    struct Found { int page, inside; };
     const auto look_up = [&](int t) {
         const int pos = span.key(t0 + t) + (lane >> 3) * INT4_BLOCK, logical = a.by_page(pos);
-        inside = (pos - logical * a.page_size) / INT4_BLOCK * CHUNKS;
-        page = t < n_tiles && pos <= span.last_pos && logical < a.width ? pages[logical] : -1;
+        return Found{t < n_tiles && pos <= span.last_pos && logical < a.width ? pages[logical] : -1, (pos - logical * a.page_size) / INT4_BLOCK * CHUNKS};
     };
-    const auto fetch = [&](int t, int slot) {
+    const auto fetch = [&](int t, int slot, Found found) {
         if (t < n_tiles) {
-            const size_t at = page < 0 ? 0 : ((size_t)page * page_chunks + inside) * 16;
+            const bool there = found.page >= 0;
+            const size_t at = there ? ((size_t)found.page * page_chunks + found.inside) * 16 : 0;
             const uint32_t to = landing + slot * TILE_BYTES;
 #pragma unroll
             for (int i = 0; i < CHUNKS; i += 8)
                 if (i + 8 <= CHUNKS || i + (lane & 7) < CHUNKS) {
-                    copy16(to + i * 16, k_plane + at + i * 16, page >= 0);
-                    copy16(to + TILE_BYTES / 2 + i * 16, v_plane + at + i * 16, page >= 0);
+                    copy16(to + i * 16, k_plane + at + i * 16, there);
+                    copy16(to + TILE_BYTES / 2 + i * 16, v_plane + at + i * 16, there);
                 }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        look_up(t + WARPS);
     };
-    const auto begin = [&] {
-        look_up(warp);
+    Found next;
+    const auto begin = [&] {                                        // all look-ups on their way at once
+        Found first[STAGES];
 #pragma unroll
-        for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i);
+        for (int i = 0; i < STAGES; ++i) first[i] = look_up(warp + WARPS * i);
+        next = look_up(warp + WARPS * STAGES);
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i, first[i]);
     };
-    begin();
 
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
     // after the shift, (2, 6), (3, 7) / 16.  All warps need the same: each makes some groups' operands and they exchange them.
     constexpr int TURNS = (NT * NG + WARPS - 1) / WARPS;
     __shared__ uint4 operand[NT * NG][TERMS][32];
-    __shared__ uint32_t largest[ROWS];
-    __shared__ float group_sum[ROWS][4];
-    const int tok0 = a.q_start[span.req];
-    if (tid < ROWS) {
-        largest[tid] = 0;
-        for (int j = NG; j < 4; ++j) group_sum[tid][j] = 0.f;
+    __shared__ uint32_t largest[ROWS][NG];
+    __shared__ float group_sum[ROWS][NG];
+    uint4 raw[TURNS][TERMS];                                        // asked for before the first tiles' look-ups are waited for
+#pragma unroll
+    for (int turn = 0; turn < TURNS; ++turn) {
+        const int i = min(warp + turn * WARPS, NT * NG - 1), nt = i / NG, j = i - nt * NG, r = nt * 8 + g;
+        const int row = span.row0 + (r < span.rows ? r : 0), token = a.by_group(row);
+        const T* q = a.q + ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D + 32 * j + 8 * c;
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) raw[turn][i] = reinterpret_cast<const uint4*>(q)[i];
     }
-    __syncthreads();
+    begin();
     float x[TURNS][8];
 #pragma unroll
     for (int turn = 0; turn < TURNS; ++turn) {
         const int i = warp + turn * WARPS, nt = i / NG, j = i - nt * NG, r = nt * 8 + g;
         if (i >= NT * NG) continue;
         const bool there = r < span.rows;
-        const int row = span.row0 + (there ? r : 0), token = a.by_group(row);
-        const T* q = a.q + ((size_t)(tok0 + token) * a.hq + kvh * span.group + row - token * span.group) * D + 32 * j + 8 * c;
-#if STORAGE_BF16
-        const uint4 v = *reinterpret_cast<const uint4*>(q);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { x[turn][2 * e] = __uint_as_float(w[e] << 16); x[turn][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+        for (int i = 0; i < TERMS; ++i) {
+            const uint32_t w[4] = {raw[turn][i].x, raw[turn][i].y, raw[turn][i].z, raw[turn][i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#if STORAGE_BF16
+                x[turn][2 * e] = __uint_as_float(w[e] << 16); x[turn][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
 #else
-        const float4 u = *reinterpret_cast<const float4*>(q), v = *reinterpret_cast<const float4*>(q + 4);
-        x[turn][0] = u.x; x[turn][1] = u.y; x[turn][2] = u.z; x[turn][3] = u.w; x[turn][4] = v.x; x[turn][5] = v.y; x[turn][6] = v.z; x[turn][7] = v.w;
+                x[turn][4 * i + e] = __uint_as_float(w[e]);
 #endif
+            }
+        }
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -319,10 +331,15 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (c == 0) atomicMax(&largest[r], top);
+        if (c == 0) largest[r][j] = top;
     }
     __syncthreads();
-    const auto exponent = [&](int r) { return min(14 - ((int)(largest[r] >> 23) - 127), 120); };       // the row times 2 to it is below 2^15
+    const auto exponent = [&](int r) {                              // the row times 2 to it is below 2^15
+        uint32_t top = largest[r][0];
+#pragma unroll
+        for (int j = 1; j < NG; ++j) top = max(top, largest[r][j]);
+        return min(14 - ((int)(top >> 23) - 127), 120);
+    };
 #pragma unroll
     for (int turn = 0; turn < TURNS; ++turn) {
         const int i = warp + turn * WARPS, nt = i / NG, j = i - nt * NG, r = nt * 8 + g;
@@ -363,7 +380,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 qf[nt][j][0][term][0] = w.x; qf[nt][j][0][term][1] = w.y; qf[nt][j][1][term][0] = w.z; qf[nt][j][1][term][1] = w.w;
             }
         if constexpr (OFFSET) {
-            const float s0 = -0x1p-21f * group_sum[nt * 8 + g][2 * (c & 1)], s1 = -0x1p-21f * group_sum[nt * 8 + g][2 * (c & 1) + 1];
+            const int j0 = 2 * (c & 1);
+            const float s0 = j0 < NG ? -0x1p-21f * group_sum[nt * 8 + g][j0 < NG ? j0 : 0] : 0.f, s1 = j0 + 1 < NG ? -0x1p-21f * group_sum[nt * 8 + g][j0 + 1 < NG ? j0 + 1 : 0] : 0.f;
             qs[nt] = pack_f16(s0, s1);
             if (c >= 2) qs[nt] = pack_f16(s0 - low_half(qs[nt]), s1 - high_half(qs[nt]));
         }
@@ -566,7 +584,8 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         const unsigned char* ks = ring + slot * TILE_BYTES;
         work(is_edge, ks, ks + TILE_BYTES / 2, span.key(t0 + t));
         __syncwarp();                                               // every lane has read the stage
-        fetch(t + WARPS * STAGES, slot);
+        fetch(t + WARPS * STAGES, slot, next);
+        next = look_up(t + WARPS * (STAGES + 1));
     };
     for (;;) {
 #pragma unroll
@@ -816,6 +835,11 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
 bool g_pdl = false;
 int* g_error = nullptr;
 
+template <int NT> constexpr size_t dynamic_smem() {
+    constexpr size_t ring = (size_t)warps_of<NT>() * STAGES * TILE_BYTES, merge = sizeof(float) * warps_of<NT>() * 8 * NT * (D + 4);
+    return ring > merge ? ring : merge;
+}
+
 int sm_count() {                                                    // of the current device
     static int known[64] = {};
     int device = 0, n = 0;
@@ -824,6 +848,35 @@ int sm_count() {                                                    // of the cu
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return 1;
     if (device < 64) known[device] = n;
     return n;
+}
+
+// Thread blocks of the kernel that run at once on the current device in clusters of `size`: a cluster lies in one part of the chip, whose
+// last places it may not fill (48 clusters of 6 took two rounds where 296 blocks have places).
+template <int NT> int places(int size) {
+    static int known[64][MAX_CLUSTER + 1] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return size;
+    if (!known[device][size]) {
+        constexpr size_t SMEM = dynamic_smem<NT>();
+        int n = 0;
+        if (cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) != cudaSuccess) return size;
+        if (size == 1) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_int4_kernel<NT>, 32 * warps_of<NT>(), SMEM) != cudaSuccess) n = 0;
+            n *= sm_count();
+        } else {
+            cudaLaunchConfig_t config = {};
+            config.gridDim = dim3(1, 1, size); config.blockDim = dim3(32 * warps_of<NT>()); config.dynamicSmemBytes = SMEM;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = (unsigned)size;
+            config.attrs = attr; config.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, attn_int4_kernel<NT>, &config) != cudaSuccess) n = 0;
+            n *= size;
+        }
+        cudaGetLastError();
+        known[device][size] = n > 0 ? n : size;
+    }
+    return known[device][size];
 }
 
 // What a launch has of everything: query rows of a tile (8, or 16 where requests bring more), tiles per request, rows that scratch is kept
@@ -838,8 +891,9 @@ struct Shape {
         rows = needed > 8 ? 16 : 8;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
-        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>(), blocks = rows == 8 ? blocks_of<1>() : blocks_of<2>();
-        const long long pairs = (long long)n_req * tiles * hkv, room = (long long)sm_count() * blocks;
+        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>();
+        const auto room_of = [&](int size) { return rows == 8 ? places<1>(size) : places<2>(size); };
+        const long long pairs = (long long)n_req * tiles * hkv, room = room_of(1);
         long long reach = longest;
         if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
         // A block takes as long as its warps' tiles and some five more for its start and end (fitted to the times of 1 to 3 splits); blocks beyond
@@ -850,7 +904,7 @@ struct Shape {
         splits = 1;
         double best = 0;
         for (int s = 1; s <= (most < MAX_CLUSTER ? most : MAX_CLUSTER); ++s) {
-            const double rounds = (double)pairs * s / room, time = (rounds > 1 ? rounds + 0.4 : 1) * (5 + tiles_of_warp / s);
+            const double rounds = (double)pairs * s / room_of(s), time = (rounds > 1 ? rounds + 0.4 : 1) * (5 + tiles_of_warp / s);
             if (s == 1 || time < best) { best = time; splits = s; }
         }
         if (splits == MAX_CLUSTER && pairs * MAX_CLUSTER < room / 2) {
@@ -873,8 +927,7 @@ struct Shape {
 
 template <int NT> int launch(Args a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
     constexpr int WARPS = warps_of<NT>();
-    constexpr size_t RING = (size_t)WARPS * STAGES * TILE_BYTES, MERGE = sizeof(float) * WARPS * 8 * NT * (D + 4);
-    constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
+    constexpr size_t SMEM = dynamic_smem<NT>();
     if constexpr (SMEM > 48 * 1024 - 20480) {
         const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
         if (e != cudaSuccess) return (int)e;
@@ -927,6 +980,8 @@ CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, co
     a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
     a.by_page = Divider((uint32_t)page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.by_heads = Divider((uint32_t)hkv);
     a.group = group; a.n_req = n_req; a.ranked = shape.ranked;
+    a.rank_threads = 1;
+    while (a.rank_threads < n_req && a.rank_threads < MAX_RANKED) a.rank_threads *= 2;
     a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
     a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
     return shape.rows == 8 ? launch<1>(a, shape, n_req, mass, (cudaStream_t)stream) : launch<2>(a, shape, n_req, mass, (cudaStream_t)stream);
