@@ -40,9 +40,10 @@ constexpr int TERMS = 1;
 typedef float T;
 constexpr int TERMS = 2;
 #endif
-constexpr int TK = 32;                                             // keys of a warp's tile: four blocks of 8
-constexpr int STAGES = 2;                                          // tiles that a warp has on the way
-constexpr int BLOCK_BYTES = int4_block_bytes(D), TILE_BYTES = 2 * (TK / INT4_BLOCK) * BLOCK_BYTES;
+// Keys of a warp's tile.  A warp has one tile in shared memory, its keys and its values apart: the next tile's keys are on their way while this
+// one's values are worked on, and the other way round.
+template <int NT> constexpr int tile_keys() { return NT == 1 ? 64 : 32; }
+constexpr int BLOCK_BYTES = int4_block_bytes(D);
 constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum follows a score only where that is 2^SLACK times its weight above it, which after a warp's first tile is rare (each time
 // costs 50 multiplications a lane).  Probabilities are held times 2^5 (for float queries, whose second terms are 2^-11 of the first, 2^9): with
@@ -141,7 +142,7 @@ struct Args {
 // What the rows of one (request, tile of 8 NT query rows) see, as tiles of TK keys: those of the first keys that stay in sight behind a
 // window, then those from the first key inside the first row's window to the last row's own.  They are walked from the `lead`th on, the
 // others last: then the tiles that some row does not see whole are the last ones, and the first `plain` need no masks.
-struct Span {
+template <int TK> struct Span {
     int req, n, ctx, slot, tok0, group, row0, rows, first_pos, last_pos;
     int kept_tiles, window_base, tiles, lead, plain;
     __device__ __forceinline__ int key(int t) const {
@@ -150,7 +151,7 @@ struct Span {
         return t < kept_tiles ? t * TK : window_base + (t - kept_tiles) * TK;
     }
 };
-template <int ROWS> __device__ __forceinline__ bool find_span(Span& s, const Args& a, int x) {
+template <int ROWS, int TK> __device__ __forceinline__ bool find_span(Span<TK>& s, const Args& a, int x) {
     s.req = a.by_tiles(x);
     const int tile = x - s.req * a.tiles;
     s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.slot = a.req_slot[s.req]; s.tok0 = a.q_start[s.req];      // one trip to memory
@@ -214,6 +215,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
     constexpr int MERGE_STRIDE = D + 4;                  // rows of whole 16 bytes
+    constexpr int TK = tile_keys<NT>(), HALVES = TK / 16, PLANE_BYTES = TK / INT4_BLOCK * BLOCK_BYTES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float others[MAX_CLUSTER][ROWS][2], lse[ROWS];       // a cluster's largest scores and denominators; the row's logarithm of its sum
     __shared__ float weight[WARPS][ROWS];                           // of a warp's sums among the block's
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         __syncthreads();
         unit_of += (chosen - rank) * a.tiles;
     }
-    Span span;
+    Span<TK> span;
     if (!find_span<ROWS>(span, a, unit_of)) return;                 // the same for a whole cluster
     const size_t base_row = ((size_t)unit_of * a.hkv + kvh) * a.row_stride;
     const int* pages = a.table + (size_t)span.slot * a.width;
@@ -250,43 +252,35 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
     const int share = (span.tiles + a.n_splits - 1) / a.n_splits;   // tiles of a split: the request's own, so that a cluster ends together
     const int t0 = split * share, n_tiles = max(0, min(share, span.tiles - t0));
 
-    unsigned char* ring = smem + (size_t)warp * STAGES * TILE_BYTES;
-    // A tile into a stage: eight lanes a block, 16 bytes a lane at a time, the same of keys and values.  (A bulk copy per page took less
-    // address arithmetic but a loop of some 15 instructions for each of its four.)  Its page is looked up one tile ahead.  Blocks behind
-    // the last key and pages that are not there become zeros.
-    constexpr int CHUNKS = BLOCK_BYTES / 16;
+    unsigned char* ks = smem + (size_t)warp * 2 * PLANE_BYTES;
+    unsigned char* vs = ks + PLANE_BYTES;
+    // A tile's keys or values: 16 bytes a lane at a time, some lanes a block.  (A bulk copy per page took less address arithmetic but a loop
+    // of some 15 instructions for each copy.)  Its page is looked up one tile ahead.  Blocks behind the last key and pages that are
+    // not there become zeros.
+    constexpr int CHUNKS = BLOCK_BYTES / 16, LANES = 32 / (TK / INT4_BLOCK);
     const uint32_t page_chunks = (uint32_t)(a.hkv * (a.page_size / INT4_BLOCK) * CHUNKS);
-    const size_t lane_bytes = (size_t)kvh * (a.page_size / INT4_BLOCK) * BLOCK_BYTES + (lane & 7) * 16;
-    const unsigned char* k_plane = a.k_cache + lane_bytes;
-    const unsigned char* v_plane = a.v_cache + lane_bytes;
-    const uint32_t landing = (uint32_t)__cvta_generic_to_shared(ring) + (lane >> 3) * BLOCK_BYTES + (lane & 7) * 16;
-    struct Found { int page, inside; };
-    const auto look_up = [&](int t) {
-        const int pos = span.key(t0 + t) + (lane >> 3) * INT4_BLOCK, logical = a.by_page(pos);
-        return Found{t < n_tiles && pos <= span.last_pos && logical < a.width ? pages[logical] : -1, (pos - logical * a.page_size) / INT4_BLOCK * CHUNKS};
+    const size_t lane_bytes = (size_t)kvh * (a.page_size / INT4_BLOCK) * BLOCK_BYTES + (lane % LANES) * 16;
+    const uint32_t landing = (uint32_t)__cvta_generic_to_shared(ks) + (lane / LANES) * BLOCK_BYTES + (lane % LANES) * 16;
+    const auto look_up = [&](int t) {                               // the block's place in a plane, in 16 bytes, or all ones
+        const int pos = span.key(t0 + t) + (lane / LANES) * INT4_BLOCK, logical = a.by_page(pos);
+        const int page = t < n_tiles && pos <= span.last_pos && logical < a.width ? pages[logical] : -1;
+        return page < 0 ? ~0u : page * page_chunks + (pos - logical * a.page_size) / INT4_BLOCK * CHUNKS;
     };
-    const auto fetch = [&](int t, int slot, Found found) {
-        if (t < n_tiles) {
-            const bool there = found.page >= 0;
-            const size_t at = there ? ((size_t)found.page * page_chunks + found.inside) * 16 : 0;
-            const uint32_t to = landing + slot * TILE_BYTES;
+    const auto fetch = [&](const unsigned char* plane, uint32_t to, uint32_t found, bool any) {
+        if (any) {
+            const bool there = found != ~0u;
+            const unsigned char* from = plane + lane_bytes + (there ? (size_t)found * 16 : 0);
 #pragma unroll
-            for (int i = 0; i < CHUNKS; i += 8)
-                if (i + 8 <= CHUNKS || i + (lane & 7) < CHUNKS) {
-                    copy16(to + i * 16, k_plane + at + i * 16, there);
-                    copy16(to + TILE_BYTES / 2 + i * 16, v_plane + at + i * 16, there);
-                }
+            for (int i = 0; i < CHUNKS; i += LANES)
+                if (i + LANES <= CHUNKS || i + lane % LANES < CHUNKS) copy16(to + i * 16, from + i * 16, there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    Found next;
-    const auto begin = [&] {                                        // all look-ups on their way at once
-        Found first[STAGES];
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i) first[i] = look_up(warp + WARPS * i);
-        next = look_up(warp + WARPS * STAGES);
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i) fetch(warp + WARPS * i, i, first[i]);
+    uint32_t here, next;                                            // of this tile, of the next one
+    const auto begin = [&] {
+        here = look_up(warp); next = look_up(warp + WARPS);         // on their way at once
+        fetch(a.k_cache, landing, here, warp < n_tiles);
+        fetch(a.v_cache, landing + PLANE_BYTES, here, warp < n_tiles);
     };
 
     // Queries as B: lane (g, c) has dimensions 32 j + 8 c + 0 .. 7 of row g, in the order of the half bytes: pairs (0, 4), (1, 5) / 16 and,
@@ -409,11 +403,14 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 
     float* scores = a.scores ? a.scores + ((size_t)unit_of * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
     // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.
-    const auto work = [&](auto is_edge, const unsigned char* ks, const unsigned char* vs, int k0) {
+    const auto step = [&](auto is_edge, int t) {
         constexpr bool EDGE = decltype(is_edge)::value;
-        float s[2][NT][4];
+        const int k0 = span.key(t0 + t);
+        float s[HALVES][NT][4];
+        asm volatile("cp.async.wait_group 1;" ::: "memory");        // the keys
+        __syncwarp();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                               // 16 keys: blocks 2 h and 2 h + 1
+        for (int h = 0; h < HALVES; ++h) {                          // 16 keys: blocks 2 h and 2 h + 1
             const unsigned char* b0 = ks + 2 * h * BLOCK_BYTES;
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             const Share<4 * NG> w0 = load_share<4 * NG>(b0 + g * (D / 2) + c * 4 * NG), w1 = load_share<4 * NG>(b1 + g * (D / 2) + c * 4 * NG);
@@ -446,11 +443,14 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     for (int e = 0; e < 4; ++e) s[h][nt][e] = OFFSET || j ? fmaf(e < 2 ? f0 : f1, acc[nt][e], s[h][nt][e]) : (e < 2 ? f0 : f1) * acc[nt][e];
             }
         }
+        __syncwarp();                                               // every lane has read the keys
+        const bool again = t + WARPS < n_tiles;
+        fetch(a.k_cache, landing, next, again);
         bool more = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (EDGE) {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 }
         if (scores) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -478,7 +478,9 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 float alpha[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float mx = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                    float mx = s[0][nt][e];
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) mx = fmaxf(mx, fmaxf(s[h][nt][e], s[h][nt][e + 2]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             for (int e = 0; e < 2; ++e) {
                 const float top = shift - (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e] * unit[nt][e]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < HALVES; ++h) {
                     float p0 = exp2_fast(fmaf(s[h][nt][e], unit[nt][e], top)), p1 = exp2_fast(fmaf(s[h][nt][e + 2], unit[nt][e], top));
                     l_run[nt][e] += p0 + p1;
                     if constexpr (EDGE) {                                     // a key out of sight gets -0, by which it is told from one of no weight
@@ -506,8 +508,10 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                     s[h][nt][e] = p0; s[h][nt][e + 2] = p1;
                 }
             }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");        // the values
+        __syncwarp();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HALVES; ++h) {
             // probabilities as B: rows of the product above are keys, here columns: two 8 x 8 transpositions per 16 keys
             uint32_t pt[NT][2];
 #if STORAGE_BF16
@@ -576,17 +580,12 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 }
             }
         }
+        __syncwarp();                                               // every lane has read the values
+        here = next;
+        fetch(a.v_cache, landing + PLANE_BYTES, here, again);
+        next = look_up(t + 2 * WARPS);
     };
 
-    const auto step = [&](auto is_edge, int t, int slot) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        __syncwarp();
-        const unsigned char* ks = ring + slot * TILE_BYTES;
-        work(is_edge, ks, ks + TILE_BYTES / 2, span.key(t0 + t));
-        __syncwarp();                                               // every lane has read the stage
-        fetch(t + WARPS * STAGES, slot, next);
-        next = look_up(t + WARPS * (STAGES + 1));
-    };
     for (;;) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -597,13 +596,13 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
             l_run[nt][0] = l_run[nt][1] = 0.f;
         }
-        int t = warp, slot = 0;
-        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::false_type(), t, slot);
+        int t = warp;
+        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), t);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
-        for (; t < n_tiles; t += WARPS, slot = slot + 1 == STAGES ? 0 : slot + 1) step(std::true_type(), t, slot);
+        for (; t < n_tiles; t += WARPS) step(std::true_type(), t);
         float all = 0.f;                                            // an overflow is in the sums of the constant operand too
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -617,7 +616,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         begin();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();                                                // every warp is done with its stages: they become the merge area
+    __syncthreads();                                                // every warp is done with its tiles: their place becomes the merge area
     float* merge = reinterpret_cast<float*>(smem);                  // [warp][ROWS][D + 2]: sums, largest score, denominator
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -759,7 +758,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
 template <int ROWS>
 __global__ void __launch_bounds__(D) attn_int4_merge_kernel(const __grid_constant__ Args a) {
     pdl_wait();
-    Span span;
+    Span<32> span;                                                  // (of its tiles nothing is used here)
     if (!find_span<ROWS>(span, a, blockIdx.x)) return;
     const int r = blockIdx.z, kvh = blockIdx.y, d = threadIdx.x;
     if (r >= span.rows) return;
@@ -836,7 +835,7 @@ bool g_pdl = false;
 int* g_error = nullptr;
 
 template <int NT> constexpr size_t dynamic_smem() {
-    constexpr size_t ring = (size_t)warps_of<NT>() * STAGES * TILE_BYTES, merge = sizeof(float) * warps_of<NT>() * 8 * NT * (D + 4);
+    constexpr size_t ring = (size_t)warps_of<NT>() * 2 * (tile_keys<NT>() / INT4_BLOCK) * BLOCK_BYTES, merge = sizeof(float) * warps_of<NT>() * 8 * NT * (D + 4);
     return ring > merge ? ring : merge;
 }
 
@@ -891,7 +890,7 @@ struct Shape {
         rows = needed > 8 ? 16 : 8;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
-        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>();
+        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>(), TK = rows == 8 ? tile_keys<1>() : tile_keys<2>();
         const auto room_of = [&](int size) { return rows == 8 ? places<1>(size) : places<2>(size); };
         const long long pairs = (long long)n_req * tiles * hkv, room = room_of(1);
         long long reach = longest;
