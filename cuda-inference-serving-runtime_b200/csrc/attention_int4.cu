@@ -109,19 +109,6 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-// n / d for n below 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
-struct Divider {
-    uint32_t m, shift;               // m 0: divided by one
-    __host__ __device__ Divider() : m(0), shift(0) {}
-    explicit Divider(uint32_t d) : m(0), shift(0) {
-        if (d < 2) return;
-        while ((1u << shift) < d) ++shift;
-        m = (uint32_t)((1ull << (31 + shift)) / d + 1);
-        --shift;
-    }
-    __device__ __forceinline__ int operator()(int n) const { return m ? (int)(__umulhi((uint32_t)n, m) >> shift) : n; }
-};
-
 struct Args {
     const T* q; T* out;
     const unsigned char* k_cache; const unsigned char* v_cache;

@@ -26,12 +26,26 @@ __host__ __device__ constexpr int int4_block_bytes(int dim) { return 9 * dim / 2
 __device__ __forceinline__ int int4_value_slot(int r) { return (r >> 1) + 4 * (r & 1); }          // where a block keeps row r of the values
 template <int D> __device__ __forceinline__ int int4_value_turn(int slot) { return D == 128 ? ((slot >> 1) & 1) << 2 : 0; }
 
-// Byte offset of the block that holds place `pos` of a sequence, from the start of the cache, or -1 where there is no page.
-__device__ __forceinline__ long long int4_block_at(const int* __restrict__ table, int width, int pos, int page_size, int hkv, int head, int dim) {
-    const int logical = pos / page_size;
-    if (pos < 0 || logical >= width) return -1;
-    const int page = table[logical];
+// n / d for n below 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divider {
+    uint32_t m, shift;               // m 0: divided by one
+    __host__ __device__ Divider() : m(0), shift(0) {}
+    explicit Divider(uint32_t d) : m(0), shift(0) {
+        if (d < 2) return;
+        while ((1u << shift) < d) ++shift;
+        m = (uint32_t)((1ull << (31 + shift)) / d + 1);
+        --shift;
+    }
+    __device__ __forceinline__ int operator()(int n) const { return m ? (int)(__umulhi((uint32_t)n, m) >> shift) : n; }
+};
+
+// Where the block of place `pos` of a sequence is, in blocks from the start of the cache, or -1 where there is no page.  `by_page` divides by
+// the page size, `page_blocks` is the page size over 8.
+struct Pages { const int* table; int width, page_blocks, hkv; Divider by_page; };
+__device__ __forceinline__ long long int4_block_at(const Pages& p, int slot, int pos, int head) {
+    const int logical = p.by_page(max(pos, 0));
+    const int page = pos >= 0 && logical < p.width ? p.table[(size_t)slot * p.width + logical] : -1;
     if (page < 0) return -1;
-    return (((long long)page * hkv + head) * (page_size / INT4_BLOCK) + (pos - logical * page_size) / INT4_BLOCK) * int4_block_bytes(dim);
+    return (long long)((size_t)page * p.hkv + head) * p.page_blocks + ((pos / INT4_BLOCK) - logical * p.page_blocks);
 }
 }  // namespace

@@ -2,45 +2,65 @@
 // that attention has looked at least taken out.
 //
 // All of these move memory: a row of keys and values is 4 D bytes as bfloat16 and 9 D / 8 as held.  Head sizes 32, 64, 96 and 128.
+#include <type_traits>
+
 #include "int4_cache.cuh"
 
 namespace {
 constexpr int THREADS = 256;
 
-struct Place {                       // where a step's rows lie: token t belongs to request token_req[t] and has place positions[t] there;
-    const int* token_req;            // without lists, token t of row blockIdx.y of the grid is place t of that request
-    const int* positions;
-    const int* req_slot;
-    const int* table;
-    int width, page_size;
-};
+// Where a step's rows lie: token t is place positions[t] of request token_req[t].
+struct Place { const int* token_req; const int* positions; const int* req_slot; Pages pages; Divider by_heads; };
 
-template <typename T> __device__ __forceinline__ void load4(const T* p, float* x, bool wide);
-template <> __device__ __forceinline__ void load4<float>(const float* p, float* x, bool wide) {
-    if (wide) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-        for (int i = 0; i < 4; ++i) x[i] = p[i];
+__device__ __forceinline__ float widened(const float* x, int i) { return x[i]; }
+__device__ __forceinline__ float widened(const uint32_t* x, int i) { return __uint_as_float(i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16); }
+// N neighbours as they are stored: bfloat16 two to a word.
+template <int N> __device__ __forceinline__ void load_raw(const float* p, float* x, bool wide) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if (wide) {
+            const float4 v = *reinterpret_cast<const float4*>(p + i);
+            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+        } else {
+            for (int e = 0; e < 4; ++e) x[i + e] = p[i + e];
+        }
     }
 }
-template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, float* x, bool wide) {
-    if (wide) {
+template <int N> __device__ __forceinline__ void load_raw(const __nv_bfloat16* p, uint32_t* x, bool wide) {
+    if (wide && N == 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        x[0] = v.x; x[1] = v.y; x[N / 2 - 2] = v.z; x[N / 2 - 1] = v.w;
+    } else if (wide) {
         const uint2 v = *reinterpret_cast<const uint2*>(p);
-        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+        x[0] = v.x; x[1] = v.y;
     } else {
-        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) x[i / 2] = h[i] | (uint32_t)h[i + 1] << 16;
     }
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, const float* x);
-template <> __device__ __forceinline__ void store4<float>(float* p, const float* x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float* x) {
+// The largest magnitude's bits, as a float's: as whole numbers they order like the magnitudes, NaN above infinity.
+template <int N> __device__ __forceinline__ uint32_t largest(const float* x) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    return top;
+}
+template <int N> __device__ __forceinline__ uint32_t largest(const uint32_t* x) {
+    uint32_t two = 0;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) two = __vmaxu2(two, x[i] & 0x7fff7fffu);
+    return max(two << 16, two & 0xffff0000u);
+}
+template <typename T> struct Raw { typedef float type; static constexpr int PER = 1; };
+template <> struct Raw<__nv_bfloat16> { typedef uint32_t type; static constexpr int PER = 2; };
+
+__device__ __forceinline__ void store4(float* p, const float* x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// The step of a group from the bits of its largest magnitude (as whole numbers these order like the magnitudes, NaN above infinity).
 __device__ __forceinline__ __half step_of(uint32_t top) {
     if (top >= 0x7f800000u) return __ushort_as_half((unsigned short)0x7e00u);
     return __float2half_rn(fminf(__uint_as_float(top) * (1.f / 7.f), 65504.f));
@@ -54,6 +74,26 @@ __device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
     if (twice > s || (twice == s && ((int)t & 1))) t += copysignf(1.f, r);
     t = s > 0.f ? fminf(fmaxf(t, -7.f), 7.f) : 0.f;
     return (uint32_t)((int)t + 8);
+}
+// N codes of a group, lowest half byte first.  A bfloat16 over a float16 is a half or at least 2^-12 away from one, so that rounding the
+// product to 2^-18 (48 is added: floats there are 2^-18 apart) puts it on the half or leaves it on its side; then 1.5 2^23 - 40 makes
+// it the whole number c + 8 in a float's low digits, and the digits above, the same for all, are taken off the sum of N at once.
+template <int N, typename R> __device__ __forceinline__ uint32_t codes_of(const R* x, float s, uint32_t top) {
+    const float inv = s > 0.f ? 1.f / s : 0.f;
+    uint32_t w = 0;
+    if (sizeof(R) == 4 && std::is_same<R, uint32_t>::value && __uint_as_float(top) * inv < 7.49f) {
+        constexpr float whole = 12582912.f - 40.f;
+        uint32_t above = 0;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) {
+            w = w * 16 + __float_as_uint((widened(x, i) * inv + 48.f) + whole);
+            above = above * 16 + 0x4b400000u;
+        }
+        return w - above;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w |= code_of(widened(x, i), s, inv) << (4 * i);
+    return w;
 }
 
 template <int N> struct Word;
@@ -76,44 +116,34 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
                                            int tokens, int hkv, bool wide, int unit) {
     constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
     const int lane = threadIdx.x % LANES;
-    const long long row = (long long)unit * (THREADS / LANES) + threadIdx.x / LANES;      // row = token * hkv + head
-    const bool inside = row < (long long)tokens * hkv;
-    const int token = inside ? (int)(row / hkv) : 0, head = inside ? (int)(row - (long long)token * hkv) : 0;
-    const int pos = inside ? at.positions[token] : -1;
-    const long long block = inside ? int4_block_at(at.table + (size_t)at.req_slot[at.token_req[token]] * at.width, at.width, pos, at.page_size, hkv, head, D) : -1;
+    const int row = unit * (THREADS / LANES) + threadIdx.x / LANES;      // token * hkv + head
+    const bool inside = row < tokens * hkv;
+    const int token = at.by_heads(inside ? row : 0), head = inside ? row - token * hkv : 0;
+    const int pos = at.positions[token];
+    const long long block = inside ? int4_block_at(at.pages, at.req_slot[at.token_req[token]], pos, head) : -1;
     const T* from = x + token * token_stride + head * head_stride;
-    float v[NG][PER];
+    typename Raw<T>::type v[NG][PER / Raw<T>::PER];
     uint32_t top[NG];
 #pragma unroll
+    for (int j = 0; j < NG; ++j) load_raw<PER>(from + 32 * j + PER * lane, v[j], wide);       // (of a row without a page it is not used)
+#pragma unroll
     for (int j = 0; j < NG; ++j) {
-        top[j] = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            if (block >= 0) load4<T>(from + 32 * j + PER * lane + i, &v[j][i], wide);
-            else v[j][i] = v[j][i + 1] = v[j][i + 2] = v[j][i + 3] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) top[j] = max(top[j], __float_as_uint(v[j][i]) & 0x7fffffffu);
-    }
-#pragma unroll
-    for (int j = 0; j < NG; ++j)
+        top[j] = largest<PER>(v[j]);
 #pragma unroll
         for (int o = 1; o < LANES; o *= 2) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+    }
     if (block < 0) return;
     alignas(16) __half step[NG];
     union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
         step[j] = step_of(top[j]);
-        const float s = __half2float(step[j]), inv = 1.f / s;
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) w |= code_of(v[j][i], s, inv) << (4 * i);
+        const uint32_t w = codes_of<PER>(v[j], __half2float(step[j]), top[j]);
         if (VALUES) code.half[j] = (unsigned short)w;
         else code.word[j] = w;
     }
     const int r = pos % INT4_BLOCK;
-    unsigned char* to = cache + block;
+    unsigned char* to = cache + block * int4_block_bytes(D);
     if (VALUES) {
         const int slot = int4_value_slot(r);
         copy_share<2 * NG>(to + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG, &code);
@@ -127,7 +157,7 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
         copy_share<4 * NG>(to + r * (D / 2) + lane * 4 * NG, &code);
         if (lane == 0) {
             copy_share<2 * NG>(to + 4 * D + r * 2 * NG, step);
-            if (mass) mass[block / int4_block_bytes(D) * INT4_BLOCK + r] = 0.f;
+            if (mass) mass[block * INT4_BLOCK + r] = 0.f;
         }
     }
 }
@@ -149,32 +179,34 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 // request's end, give zeros.
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
-                                          const Place& at, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv, int unit) {
+                                          const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv, int unit) {
     constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
     const int lane = threadIdx.x % LANES;
-    const long long row = (long long)unit * (THREADS / LANES) + threadIdx.x / LANES;
-    if (row >= (long long)tokens * hkv) return;
+    const int row = unit * (THREADS / LANES) + threadIdx.x / LANES;
+    if (row >= tokens * hkv) return;
     int token, head, req, pos;
     if (ends) {                      // neighbouring rows of a head lie side by side
-        head = (int)(row / tokens); token = (int)(row - (long long)head * tokens);
+        head = by_tokens(row); token = row - head * tokens;
         req = which ? which[blockIdx.y] : blockIdx.y; pos = token < ends[req] ? token : -1;
     } else {
-        token = (int)(row / hkv); head = (int)(row - (long long)token * hkv);
+        token = at.by_heads(row); head = row - token * hkv;
         req = at.token_req[token]; pos = at.positions[token];
     }
-    const long long block = int4_block_at(at.table + (size_t)at.req_slot[req] * at.width, at.width, pos, at.page_size, hkv, head, D);
+    const long long block = int4_block_at(at.pages, at.req_slot[req], pos, head);
     union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
     float step[NG];
 #pragma unroll
-    for (int j = 0; j < NG; ++j) step[j] = 0.f;
+    for (int j = 0; j < NG; ++j) { step[j] = 0.f; code.word[j] = 0; }
     const int r = pos & (INT4_BLOCK - 1);
     if (block >= 0) {
-        const unsigned char* from = cache + block;
+        const unsigned char* from = cache + block * int4_block_bytes(D);
         if (VALUES) {
             const int slot = int4_value_slot(r);
             copy_share<2 * NG>(&code, from + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG);
+            alignas(16) uint32_t held[NG];                          // of two rows, side by side
+            copy_share<4 * NG>(held, from + 4 * D + (r >> 1) * 4 * NG);
 #pragma unroll
-            for (int j = 0; j < NG; ++j) step[j] = __half2float(reinterpret_cast<const __half*>(from + 4 * D)[((r >> 1) * NG + j) * 2 + (r & 1)]);
+            for (int j = 0; j < NG; ++j) step[j] = __half2float(__ushort_as_half((unsigned short)(r & 1 ? held[j] >> 16 : held[j] & 0xffff)));
         } else {
             copy_share<4 * NG>(&code, from + r * (D / 2) + lane * 4 * NG);
             alignas(16) __half held[NG];
@@ -189,10 +221,10 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
         const uint32_t w = VALUES ? code.half[j] : code.word[j];
 #pragma unroll
         for (int i = 0; i < PER; i += 4) {
-            float x[4];
+            float x[4];              // 2^23 + n as a float, less 2^23 + 8; the step of a row that is not there is 0
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = block >= 0 ? (float)((int)((w >> (4 * (i + e))) & 15) - 8) * step[j] : 0.f;
-            store4<T>(to + 32 * j + PER * lane + i, x);
+            for (int e = 0; e < 4; ++e) x[e] = (__uint_as_float(0x4b000000u | ((w >> (4 * (i + e))) & 15)) - 8388616.f) * step[j];
+            store4(to + 32 * j + PER * lane + i, x);
         }
     }
 }
@@ -200,12 +232,12 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
 template <int D, typename T>
 __global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
                                                             T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
-                                                            const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv) {
+                                                            Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv) {
     pdl_wait();
     const long long rows = (long long)tokens * hkv;
     const int key_units = (int)((rows + THREADS / 4 - 1) / (THREADS / 4));
-    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv, blockIdx.x);
-    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv, blockIdx.x - key_units);
+    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x);
+    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x - key_units);
     pdl_trigger();
 }
 
@@ -214,9 +246,11 @@ __global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char*
 // the largest sums, equal ones by the lowest place; NaN counts as the largest.  Two kernels: one finds the places and
 // lists them in order, the other moves the rows (and their sums) to the request's new pages.
 //
-// The choice is a search for the smallest sum that stays: the bits of a float, turned so that they order like the numbers, are found two at
-// a time, by counting how many sums reach each of three thresholds (16 passes over shared memory).
-constexpr int SELECT_THREADS = 1024, SELECT_CACHED = 48 * 1024;     // sums that fit shared memory; longer requests are read again in every pass
+// The choice is a search for the smallest sum that stays: the bits of a float, turned so that they order like the numbers, are found eleven,
+// eleven and ten at a time, by counting how many of the sums that begin with the bits found so far have which bits next.
+constexpr int SELECT_THREADS = 1024, SELECT_BITS = 11;              // two counts a thread
+constexpr int SELECT_CACHED = 48 * 1024;                            // sums that fit shared memory; those of longer requests are read again in every pass
+static_assert(2 * SELECT_THREADS == 1 << SELECT_BITS, "a thread has two counts");
 
 __device__ __forceinline__ uint32_t ordered(float x) {
     if (isnan(x)) return 0xffffffffu;
@@ -224,50 +258,61 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS) int4_select_kernel(const float* __restrict__ mass, const int* __restrict__ req_slot, const int* __restrict__ table,
-                                                                     int width, const int* __restrict__ ctx_len, int* __restrict__ kept, int hkv, int page_size,
-                                                                     int keep, int recent, int first, int cached) {
+__global__ void __launch_bounds__(SELECT_THREADS) int4_select_kernel(const float* __restrict__ mass, const int* __restrict__ req_slot, Pages pages,
+                                                                     const int* __restrict__ ctx_len, int* __restrict__ kept, int keep, int recent, int first, int cached) {
     extern __shared__ uint32_t sums[];
-    __shared__ int count[2][3];
+    __shared__ int count[1 << SELECT_BITS], found[2];               // by the next bits; the ones found, and how many are above them
     __shared__ int of_warp[2][32];
     pdl_wait();
     const int head = blockIdx.x, req = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int* pages = table + (size_t)req_slot[req] * width;
-    const int len = min(max(ctx_len[req], 0), (int)min((long long)width * page_size, 0x7fffffffll));
-    int* out = kept + ((size_t)req * hkv + head) * keep;
+    const int* table = pages.table + (size_t)req_slot[req] * pages.width;
+    const int page_size = pages.page_blocks * INT4_BLOCK;
+    const int len = min(max(ctx_len[req], 0), (int)min((long long)pages.width * page_size, 0x7fffffffll));
+    int* out = kept + ((size_t)req * pages.hkv + head) * keep;
     if (len <= keep) {
         for (int i = tid; i < keep; i += SELECT_THREADS) out[i] = i < len ? i : -1;
         return;
     }
     const int begin = first, n = len - recent - first, want = keep - recent - first;       // of n rows from `begin` on, `want` stay; want < n
     const auto fetch = [&](int i) -> uint32_t {
-        const int pos = begin + i, page = pages[pos / page_size];
-        return page < 0 ? 0u : ordered(mass[((size_t)page * hkv + head) * page_size + pos % page_size]);
+        const int pos = begin + i, logical = pages.by_page(pos), page = table[logical];
+        return page < 0 ? 0u : ordered(mass[((size_t)page * pages.hkv + head) * page_size + pos - logical * page_size]);
     };
     const bool in_shared = n <= cached;
     if (in_shared) for (int i = tid; i < n; i += SELECT_THREADS) sums[i] = fetch(i);
-    if (tid < 6) (&count[0][0])[tid] = 0;
     __syncthreads();
     const auto at = [&](int i) -> uint32_t { return in_shared ? sums[i] : fetch(i); };
-    uint32_t floor_ = 0;                                            // the largest threshold that `want` sums or more reach
+    uint32_t floor_ = 0;                                            // the smallest sum that stays
     if (want > 0) {
-        for (int bit = 30; bit >= 0; bit -= 2) {
-            const int turn = (bit >> 1) & 1;
-            const uint32_t t1 = floor_ | 1u << bit, t2 = floor_ | 2u << bit, t3 = floor_ | 3u << bit;
-            int c1 = 0, c2 = 0, c3 = 0;
+        int need = want;                                            // of those that begin with the bits found
+        for (int shift = 32 - SELECT_BITS, bits = SELECT_BITS; ;) {
+            for (int i = tid; i < 1 << SELECT_BITS; i += SELECT_THREADS) count[i] = 0;
+            __syncthreads();
+            const uint32_t known = shift + bits >= 32 ? 0u : ~0u << (shift + bits);
             for (int i = tid; i < n; i += SELECT_THREADS) {
                 const uint32_t s = at(i);
-                c1 += s >= t1; c2 += s >= t2; c3 += s >= t3;
-            }
-            c1 = __reduce_add_sync(0xffffffffu, c1); c2 = __reduce_add_sync(0xffffffffu, c2); c3 = __reduce_add_sync(0xffffffffu, c3);
-            if (lane < 3) {
-                const int c = lane == 0 ? c1 : lane == 1 ? c2 : c3;
-                if (c) atomicAdd(&count[turn][lane], c);
+                if ((s & known) == floor_) atomicAdd(&count[(s >> shift) & ((1u << bits) - 1)], 1);
             }
             __syncthreads();
-            floor_ |= (count[turn][2] >= want ? 3u : count[turn][1] >= want ? 2u : count[turn][0] >= want ? 1u : 0u) << bit;
-            if (tid < 3) count[turn ^ 1][tid] = 0;                  // last read before the barrier above, written again behind the next pass
+            // from the largest down: a thread has two neighbours, and learns how many lie above them
+            const int hi = (1 << SELECT_BITS) - 1 - 2 * tid, c0 = count[hi], c1 = count[hi - 1];
+            int above = c0 + c1;
+            for (int o = 1; o < 32; o *= 2) {
+                const int a = __shfl_up_sync(0xffffffffu, above, o);
+                if (lane >= o) above += a;
+            }
+            if (lane == 31) of_warp[0][warp] = above;
             __syncthreads();
+            int before = lane < warp ? of_warp[0][lane] : 0;
+            above += __reduce_add_sync(0xffffffffu, before) - c0 - c1;
+            if (above < need && above + c0 >= need) { found[0] = hi; found[1] = above; }
+            else if (above + c0 < need && above + c0 + c1 >= need) { found[0] = hi - 1; found[1] = above + c0; }
+            __syncthreads();
+            floor_ |= (uint32_t)found[0] << shift;
+            need -= found[1];
+            if (shift == 0) break;
+            bits = shift < SELECT_BITS ? shift : SELECT_BITS;
+            shift -= bits;
         }
     }
     // Places in order: a thread owns a run of neighbours (of odd length, so that runs start in different banks), counts those above the
@@ -305,47 +350,72 @@ __global__ void __launch_bounds__(SELECT_THREADS) int4_select_kernel(const float
     for (int i = tid; i < recent; i += SELECT_THREADS) out[keep - recent + i] = len - recent + i;
 }
 
-// A warp moves the rows of one new block of 8: lane (r, c) a quarter of row r of the keys, of the row in slot r of the values, a step of
-// each, and (c = 0) the row's sum.
+// A warp moves the rows of MOVE_BLOCKS new blocks of 8, all of them on their way at once: lane (r, c) a quarter of row r of the keys, of the row
+// in slot r of the values, a step of each, and (c = 0) the row's sum.
+constexpr int MOVE_BLOCKS = 4;
 template <int D>
 __global__ void __launch_bounds__(THREADS) int4_move_kernel(unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
-                                                            const int* __restrict__ req_slot, const int* __restrict__ table, int width,
-                                                            const int* __restrict__ to_table, int to_width, const int* __restrict__ kept, int hkv, int page_size, int keep) {
+                                                            const int* __restrict__ req_slot, Pages pages, Pages to_pages, const int* __restrict__ kept, int keep) {
     constexpr int NG = D / 32;
     pdl_wait();
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = blockIdx.y, req = blockIdx.z;
-    const int first_row = (blockIdx.x * (THREADS / 32) + threadIdx.x / 32) * INT4_BLOCK;
-    if (first_row >= keep) return;
-    const long long to = int4_block_at(to_table + (size_t)req * to_width, to_width, first_row, page_size, hkv, head, D);
-    if (to < 0) return;
-    const int* pages = table + (size_t)req_slot[req] * width;
-    const int* places = kept + ((size_t)req * hkv + head) * keep;
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = blockIdx.y, req = blockIdx.z, slot = req_slot[req];
+    const int* places = kept + ((size_t)req * pages.hkv + head) * keep;
     const int slot_row = 2 * (r & 3) + (r >> 2);                    // the row in slot r of the values
-    const int key_pos = first_row + r < keep ? places[first_row + r] : -1;
-    const int value_pos = first_row + slot_row < keep ? places[first_row + slot_row] : -1;
-    const long long key_at = int4_block_at(pages, width, key_pos, page_size, hkv, head, D);
-    const long long value_at = int4_block_at(pages, width, value_pos, page_size, hkv, head, D);
-    if (key_at >= 0) {
-        const int from_r = key_pos % INT4_BLOCK;
-        copy_share<4 * NG>(k_cache + to + r * (D / 2) + c * 4 * NG, k_cache + key_at + from_r * (D / 2) + c * 4 * NG);
-        if (c < NG) *reinterpret_cast<__half*>(k_cache + to + 4 * D + (r * NG + c) * 2) = *reinterpret_cast<const __half*>(k_cache + key_at + 4 * D + (from_r * NG + c) * 2);
-        if (c == 0) {
-            const int logical = key_pos / page_size, to_logical = first_row / page_size;
-            mass[((size_t)to_table[(size_t)req * to_width + to_logical] * hkv + head) * page_size + first_row - to_logical * page_size + r] =
-                mass[((size_t)pages[logical] * hkv + head) * page_size + key_pos - logical * page_size];
+    const int warp_row = (blockIdx.x * (THREADS / 32) + threadIdx.x / 32) * MOVE_BLOCKS * INT4_BLOCK;
+    long long to[MOVE_BLOCKS], key_at[MOVE_BLOCKS], value_at[MOVE_BLOCKS];
+    int key_pos[MOVE_BLOCKS], value_pos[MOVE_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < MOVE_BLOCKS; ++b) {
+        const int row = warp_row + b * INT4_BLOCK;
+        key_pos[b] = row + r < keep ? places[row + r] : -1;
+        value_pos[b] = row + slot_row < keep ? places[row + slot_row] : -1;
+        to[b] = row < keep ? int4_block_at(to_pages, req, row, head) : -1;
+    }
+#pragma unroll
+    for (int b = 0; b < MOVE_BLOCKS; ++b) {
+        key_at[b] = to[b] < 0 ? -1 : int4_block_at(pages, slot, key_pos[b], head);
+        value_at[b] = to[b] < 0 ? -1 : int4_block_at(pages, slot, value_pos[b], head);
+    }
+    struct alignas(16) Part { uint32_t w[NG]; };
+    Part k[MOVE_BLOCKS], v[MOVE_BLOCKS];
+    __half k_step[MOVE_BLOCKS], v_step[MOVE_BLOCKS];
+    float sum[MOVE_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < MOVE_BLOCKS; ++b) {
+        if (key_at[b] >= 0) {
+            const unsigned char* from = k_cache + key_at[b] * int4_block_bytes(D);
+            const int from_r = key_pos[b] % INT4_BLOCK;
+            copy_share<4 * NG>(&k[b], from + from_r * (D / 2) + c * 4 * NG);
+            if (c < NG) k_step[b] = reinterpret_cast<const __half*>(from + 4 * D)[from_r * NG + c];
+            if (c == 0) sum[b] = mass[key_at[b] * INT4_BLOCK + from_r];
+        }
+        if (value_at[b] >= 0) {
+            const unsigned char* from = v_cache + value_at[b] * int4_block_bytes(D);
+            const int from_r = value_pos[b] % INT4_BLOCK, from_slot = int4_value_slot(from_r);
+            const int turned = int4_value_turn<D>(r) != int4_value_turn<D>(from_slot) ? 2 : 0;      // eighths exchanged four by four: quarters two by two
+            copy_share<4 * NG>(&v[b], from + from_slot * (D / 2) + (c ^ turned) * 4 * NG);
+            if (c < NG) v_step[b] = reinterpret_cast<const __half*>(from + 4 * D)[((from_r >> 1) * NG + c) * 2 + (from_r & 1)];
         }
     }
-    if (value_at >= 0) {
-        const int from_r = value_pos % INT4_BLOCK, from_slot = int4_value_slot(from_r);
-        const int turned = int4_value_turn<D>(r) != int4_value_turn<D>(from_slot) ? 2 : 0;      // eighths exchanged four by four: quarters two by two
-        copy_share<4 * NG>(v_cache + to + r * (D / 2) + c * 4 * NG, v_cache + value_at + from_slot * (D / 2) + (c ^ turned) * 4 * NG);
-        if (c < NG)
-            *reinterpret_cast<__half*>(v_cache + to + 4 * D + (((slot_row >> 1) * NG + c) * 2 + (slot_row & 1)) * 2) =
-                *reinterpret_cast<const __half*>(v_cache + value_at + 4 * D + (((from_r >> 1) * NG + c) * 2 + (from_r & 1)) * 2);
+#pragma unroll
+    for (int b = 0; b < MOVE_BLOCKS; ++b) {
+        if (key_at[b] >= 0) {
+            unsigned char* dest = k_cache + to[b] * int4_block_bytes(D);
+            copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &k[b]);
+            if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[r * NG + c] = k_step[b];
+            if (c == 0) mass[to[b] * INT4_BLOCK + r] = sum[b];
+        }
+        if (value_at[b] >= 0) {
+            unsigned char* dest = v_cache + to[b] * int4_block_bytes(D);
+            copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &v[b]);
+            if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[((slot_row >> 1) * NG + c) * 2 + (slot_row & 1)] = v_step[b];
+        }
     }
 }
 
 bool g_pdl = false;
+
+Pages pages_of(const int* table, int width, int page_size, int hkv) { return Pages{table, width, page_size / INT4_BLOCK, hkv, Divider((uint32_t)page_size)}; }
 
 template <typename F> int by_head_size(int dim, F f) {
     switch (dim) {
@@ -368,11 +438,11 @@ CISR_EXPORT int cisr_int4_store(const void* k, const void* v, int dtype, long lo
                                 int tokens, int hkv, int dim, void* stream) {
     if (tokens <= 0) return 0;
     if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || ((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
+    if ((long long)tokens * hkv >= 1ll << 30) return -2;
     const long long blocks = units((long long)tokens * hkv);
-    if (blocks >= 1ll << 31) return -2;
     const int per16 = dtype == CISR_F32 ? 4 : 8;
     const int wide = (((uintptr_t)k & 15) == 0 && k_token % per16 == 0 && k_head % per16 == 0 ? 1 : 0) | (((uintptr_t)v & 15) == 0 && v_token % per16 == 0 && v_head % per16 == 0 ? 2 : 0);
-    const Place at{token_req, positions, req_slot, block_table, width, page_size};
+    const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
     return by_head_size(dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         if (dtype == CISR_F32)
@@ -391,17 +461,17 @@ CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k
     if (tokens <= 0 || n_req <= 0) return 0;
     if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535) return -2;
     if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15 || token_stride % 4 || head_stride % 4 || req_stride % 4) return -2;
+    if ((long long)tokens * hkv >= 1ll << 30) return -2;
     const long long blocks = units((long long)tokens * hkv);
-    if (blocks >= 1ll << 31) return -2;
-    const Place at{token_req, positions, req_slot, block_table, width, page_size};
+    const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
     const dim3 grid((unsigned)blocks, (unsigned)n_req);
     return by_head_size(dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         if (dtype == CISR_F32)
             return launch_kernel(int4_read_kernel<D, float>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
-                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv);
+                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, tokens, hkv);
         return launch_kernel(int4_read_kernel<D, __nv_bfloat16>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
-                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, ends, which, tokens, hkv);
+                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, tokens, hkv);
     });
 }
 
@@ -412,6 +482,7 @@ CISR_EXPORT int cisr_int4_evict(void* k_cache, void* v_cache, float* mass, const
     if (n_req <= 0 || keep <= 0) return 0;
     if (hkv <= 0 || hkv > 65535 || n_req > 65535 || page_size <= 0 || page_size % INT4_BLOCK || recent < 0 || first < 0 || recent > keep || first > keep - recent) return -2;
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
+    const Pages pages = pages_of(block_table, width, page_size, hkv);
     const int between = longest - recent - first;
     const int cached = between < 0 ? 0 : between < SELECT_CACHED ? between : SELECT_CACHED;
     const size_t smem = sizeof(uint32_t) * (size_t)(cached < SELECT_CACHED ? cached : SELECT_CACHED);
@@ -420,12 +491,13 @@ CISR_EXPORT int cisr_int4_evict(void* k_cache, void* v_cache, float* mass, const
         if (e != cudaSuccess) return (int)e;
     }
     const cudaStream_t s = (cudaStream_t)stream;
-    const int status = launch_kernel(int4_select_kernel, dim3(hkv, n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)mass, req_slot, block_table, width, ctx_len, kept,
-                                     hkv, page_size, keep, recent, first, cached);
+    const int status = launch_kernel(int4_select_kernel, dim3(hkv, n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)mass, req_slot, pages, ctx_len, kept, keep,
+                                     recent, first, cached);
     if (status) return status;
-    const dim3 grid((unsigned)((keep + INT4_BLOCK * (THREADS / 32) - 1) / (INT4_BLOCK * (THREADS / 32))), hkv, n_req);
+    constexpr int rows = MOVE_BLOCKS * INT4_BLOCK * (THREADS / 32);
+    const dim3 grid((unsigned)((keep + rows - 1) / rows), hkv, n_req);
     return by_head_size(dim, [&](auto d) {
-        return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, req_slot, block_table,
-                             width, to_table, to_width, (const int*)kept, hkv, page_size, keep);
+        return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, req_slot, pages,
+                             pages_of(to_table, to_width, page_size, hkv), (const int*)kept, keep);
     });
 }
