@@ -55,10 +55,18 @@ template <int N> __device__ __forceinline__ uint32_t largest(const uint32_t* x) 
 template <typename T> struct Raw { typedef float type; static constexpr int PER = 1; };
 template <> struct Raw<__nv_bfloat16> { typedef uint32_t type; static constexpr int PER = 2; };
 
-__device__ __forceinline__ void store4(float* p, const float* x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+__device__ __forceinline__ void store8(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ __half step_of(uint32_t top) {
@@ -108,24 +116,42 @@ template <int BYTES> __device__ __forceinline__ void copy_share(void* to, const 
     for (int i = 0; i < BYTES / PART; ++i) reinterpret_cast<W*>(to)[i] = reinterpret_cast<const W*>(from)[i];
 }
 
-// Keys: four lanes a row, lane c with the 8 neighbours 32 j + 8 c of every group j.  Values: eight lanes a row, lane g with the 4
-// neighbours 32 u + 4 g of every group u.  So a lane writes its codes of the row by one store, and a group's largest
-// magnitude is two or three shuffles away.  A warp does 8 rows of keys, or 4 of values.
+// Four lanes a row, lane c with the 8 neighbours 32 j + 8 c of every group j: its codes are a quarter of the row, written by one store, and a
+// group's largest magnitude is two shuffles away.  (With eight lanes a row of values the arithmetic on places was half of the work.)
+constexpr int LANES = 4, PER = 8;
+// A quarter row of keys as it is kept is a word per group; of values first the low halves of those words, then the high ones.
+template <int NG> __device__ __forceinline__ void to_value_order(uint32_t* w) {
+    uint32_t t[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) t[j] = w[j];
+    unsigned short h[2 * NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) { h[j] = (unsigned short)t[j]; h[NG + j] = (unsigned short)(t[j] >> 16); }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+}
+template <int NG> __device__ __forceinline__ void from_value_order(uint32_t* w) {
+    unsigned short h[2 * NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) { h[2 * j] = (unsigned short)w[j]; h[2 * j + 1] = (unsigned short)(w[j] >> 16); }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) w[j] = h[j] | (uint32_t)h[NG + j] << 16;
+}
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long token_stride, long long head_stride, unsigned char* __restrict__ cache, float* __restrict__ mass, const Place& at,
                                            int tokens, int hkv, bool wide, int unit) {
-    constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
+    constexpr int NG = D / 32;
     const int lane = threadIdx.x % LANES;
     const int row = unit * (THREADS / LANES) + threadIdx.x / LANES;      // token * hkv + head
     const bool inside = row < tokens * hkv;
     const int token = at.by_heads(inside ? row : 0), head = inside ? row - token * hkv : 0;
-    const int pos = at.positions[token];
-    const long long block = inside ? int4_block_at(at.pages, at.req_slot[at.token_req[token]], pos, head) : -1;
     const T* from = x + token * token_stride + head * head_stride;
     typename Raw<T>::type v[NG][PER / Raw<T>::PER];
     uint32_t top[NG];
 #pragma unroll
-    for (int j = 0; j < NG; ++j) load_raw<PER>(from + 32 * j + PER * lane, v[j], wide);       // (of a row without a page it is not used)
+    for (int j = 0; j < NG; ++j) load_raw<PER>(from + 32 * j + PER * lane, v[j], wide);       // before the row's page is waited for
+    const int pos = at.positions[token];
+    const long long block = inside ? int4_block_at(at.pages, at.req_slot[at.token_req[token]], pos, head) : -1;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
         top[j] = largest<PER>(v[j]);
@@ -134,19 +160,18 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
     }
     if (block < 0) return;
     alignas(16) __half step[NG];
-    union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
+    alignas(16) uint32_t code[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
         step[j] = step_of(top[j]);
-        const uint32_t w = codes_of<PER>(v[j], __half2float(step[j]), top[j]);
-        if (VALUES) code.half[j] = (unsigned short)w;
-        else code.word[j] = w;
+        code[j] = codes_of<PER>(v[j], __half2float(step[j]), top[j]);
     }
     const int r = pos % INT4_BLOCK;
     unsigned char* to = cache + block * int4_block_bytes(D);
     if (VALUES) {
         const int slot = int4_value_slot(r);
-        copy_share<2 * NG>(to + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG, &code);
+        to_value_order<NG>(code);
+        copy_share<4 * NG>(to + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot) / 2) * 4 * NG, code);
         if (lane < NG) {
             __half mine = step[0];
 #pragma unroll
@@ -154,7 +179,7 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
             reinterpret_cast<__half*>(to + 4 * D)[((r >> 1) * NG + lane) * 2 + (r & 1)] = mine;
         }
     } else {
-        copy_share<4 * NG>(to + r * (D / 2) + lane * 4 * NG, &code);
+        copy_share<4 * NG>(to + r * (D / 2) + lane * 4 * NG, code);
         if (lane == 0) {
             copy_share<2 * NG>(to + 4 * D + r * 2 * NG, step);
             if (mass) mass[block * INT4_BLOCK + r] = 0.f;
@@ -169,7 +194,7 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
                                                              Place at, int tokens, int hkv, int wide) {
     pdl_wait();
     const long long rows = (long long)tokens * hkv;
-    const int key_units = (int)((rows + THREADS / 4 - 1) / (THREADS / 4));
+    const int key_units = (int)((rows + THREADS / LANES - 1) / (THREADS / LANES));
     if ((int)blockIdx.x < key_units) store_rows<D, T, false>(k, k_token, k_head, k_cache, mass, at, tokens, hkv, wide & 1, blockIdx.x);
     else store_rows<D, T, true>(v, v_token, v_head, v_cache, mass, at, tokens, hkv, wide & 2, blockIdx.x - key_units);
     pdl_trigger();
@@ -177,54 +202,61 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
 // request's end, give zeros.
+constexpr int READ_ROWS = 4;         // of a thread, on their way together
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
                                           const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv, int unit) {
-    constexpr int NG = D / 32, LANES = VALUES ? 8 : 4, PER = VALUES ? 4 : 8;
+    constexpr int NG = D / 32;
     const int lane = threadIdx.x % LANES;
-    const int row = unit * (THREADS / LANES) + threadIdx.x / LANES;
-    if (row >= tokens * hkv) return;
-    int token, head, req, pos;
-    if (ends) {                      // neighbouring rows of a head lie side by side
-        head = by_tokens(row); token = row - head * tokens;
-        req = which ? which[blockIdx.y] : blockIdx.y; pos = token < ends[req] ? token : -1;
-    } else {
-        token = at.by_heads(row); head = row - token * hkv;
-        req = at.token_req[token]; pos = at.positions[token];
-    }
-    const long long block = int4_block_at(at.pages, at.req_slot[req], pos, head);
-    union alignas(16) { uint32_t word[NG]; unsigned short half[NG]; } code;
-    float step[NG];
+    const int first = unit * READ_ROWS * (THREADS / LANES) + threadIdx.x / LANES;
+    int token[READ_ROWS], head[READ_ROWS], pos[READ_ROWS], slot[READ_ROWS];
 #pragma unroll
-    for (int j = 0; j < NG; ++j) { step[j] = 0.f; code.word[j] = 0; }
-    const int r = pos & (INT4_BLOCK - 1);
-    if (block >= 0) {
-        const unsigned char* from = cache + block * int4_block_bytes(D);
-        if (VALUES) {
-            const int slot = int4_value_slot(r);
-            copy_share<2 * NG>(&code, from + slot * (D / 2) + (lane ^ int4_value_turn<D>(slot)) * 2 * NG);
-            alignas(16) uint32_t held[NG];                          // of two rows, side by side
-            copy_share<4 * NG>(held, from + 4 * D + (r >> 1) * 4 * NG);
-#pragma unroll
-            for (int j = 0; j < NG; ++j) step[j] = __half2float(__ushort_as_half((unsigned short)(r & 1 ? held[j] >> 16 : held[j] & 0xffff)));
+    for (int i = 0; i < READ_ROWS; ++i) {
+        const int row = first + i * (THREADS / LANES);
+        token[i] = -1;
+        if (row >= tokens * hkv) continue;
+        if (ends) {                  // neighbouring rows of a head lie side by side
+            head[i] = by_tokens(row); token[i] = row - head[i] * tokens;
+            const int req = which ? which[blockIdx.y] : blockIdx.y;
+            slot[i] = at.req_slot[req]; pos[i] = token[i] < ends[req] ? token[i] : -1;
         } else {
-            copy_share<4 * NG>(&code, from + r * (D / 2) + lane * 4 * NG);
-            alignas(16) __half held[NG];
-            copy_share<2 * NG>(held, from + 4 * D + r * 2 * NG);
-#pragma unroll
-            for (int j = 0; j < NG; ++j) step[j] = __half2float(held[j]);
+            token[i] = at.by_heads(row); head[i] = row - token[i] * hkv;
+            slot[i] = at.req_slot[at.token_req[token[i]]]; pos[i] = at.positions[token[i]];
         }
     }
-    T* to = out + (ends ? blockIdx.y * req_stride : 0) + token * token_stride + head * head_stride;
+    long long block[READ_ROWS];
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-        const uint32_t w = VALUES ? code.half[j] : code.word[j];
+    for (int i = 0; i < READ_ROWS; ++i) block[i] = token[i] < 0 ? -1 : int4_block_at(at.pages, slot[i], pos[i], head[i]);
+    struct alignas(16) Part { uint32_t w[NG]; };
+    Part code[READ_ROWS], held[READ_ROWS];                          // held: steps, of keys the row's (the first half), of values two rows' side by side
 #pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            float x[4];              // 2^23 + n as a float, less 2^23 + 8; the step of a row that is not there is 0
+    for (int i = 0; i < READ_ROWS; ++i) {
+        if (block[i] < 0) continue;
+        const unsigned char* from = cache + block[i] * int4_block_bytes(D);
+        const int r = pos[i] & (INT4_BLOCK - 1);
+        if (VALUES) {
+            const int at_slot = int4_value_slot(r);
+            copy_share<4 * NG>(&code[i], from + at_slot * (D / 2) + (lane ^ int4_value_turn<D>(at_slot) / 2) * 4 * NG);
+            copy_share<4 * NG>(&held[i], from + 4 * D + (r >> 1) * 4 * NG);
+        } else {
+            copy_share<4 * NG>(&code[i], from + r * (D / 2) + lane * 4 * NG);
+            copy_share<2 * NG>(&held[i], from + 4 * D + r * 2 * NG);
+        }
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (__uint_as_float(0x4b000000u | ((w >> (4 * (i + e))) & 15)) - 8388616.f) * step[j];
-            store4(to + 32 * j + PER * lane + i, x);
+    for (int i = 0; i < READ_ROWS; ++i) {
+        if (token[i] < 0) continue;
+        T* to = out + (ends ? blockIdx.y * req_stride : 0) + token[i] * token_stride + head[i] * head_stride;
+        if (VALUES) from_value_order<NG>(code[i].w);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            const uint32_t two = VALUES ? held[i].w[j] : held[i].w[j / 2];
+            const float step = __half2float(__ushort_as_half((unsigned short)((VALUES ? pos[i] & 1 : j & 1) ? two >> 16 : two & 0xffff)));
+            float x[PER];            // 2^23 + n as a float, less 2^23 + 8
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                x[e] = block[i] < 0 ? 0.f : (__uint_as_float(0x4b000000u | ((code[i].w[j] >> (4 * e)) & 15)) - 8388616.f) * step;
+            store8(to + 32 * j + PER * lane, x);
         }
     }
 }
@@ -235,7 +267,8 @@ __global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char*
                                                             Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv) {
     pdl_wait();
     const long long rows = (long long)tokens * hkv;
-    const int key_units = (int)((rows + THREADS / 4 - 1) / (THREADS / 4));
+    constexpr int EACH = READ_ROWS * (THREADS / LANES);
+    const int key_units = (int)((rows + EACH - 1) / EACH);
     if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x);
     else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x - key_units);
     pdl_trigger();
@@ -258,7 +291,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS) int4_select_kernel(const float* __restrict__ mass, const int* __restrict__ req_slot, Pages pages,
+__global__ void __launch_bounds__(SELECT_THREADS, 2) int4_select_kernel(const float* __restrict__ mass, const int* __restrict__ req_slot, Pages pages,
                                                                      const int* __restrict__ ctx_len, int* __restrict__ kept, int keep, int recent, int first, int cached) {
     extern __shared__ uint32_t sums[];
     __shared__ int count[1 << SELECT_BITS], found[2];               // by the next bits; the ones found, and how many are above them
@@ -426,8 +459,8 @@ template <typename F> int by_head_size(int dim, F f) {
         default: return -2;
     }
 }
-// Thread blocks for a launch over `rows` rows of keys (4 lanes each) and as many of values (8 lanes).
-long long units(long long rows) { return (rows + THREADS / 4 - 1) / (THREADS / 4) + (rows + THREADS / 8 - 1) / (THREADS / 8); }
+// Thread blocks for a launch over `rows` rows of keys and as many of values, `each` a block.
+long long units(long long rows, int each) { return 2 * ((rows + each - 1) / each); }
 }  // namespace
 
 CISR_EXPORT void cisr_int4_rows_set_pdl(int on) { g_pdl = on != 0; }
@@ -439,7 +472,7 @@ CISR_EXPORT int cisr_int4_store(const void* k, const void* v, int dtype, long lo
     if (tokens <= 0) return 0;
     if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || ((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
     if ((long long)tokens * hkv >= 1ll << 30) return -2;
-    const long long blocks = units((long long)tokens * hkv);
+    const long long blocks = units((long long)tokens * hkv, THREADS / LANES);
     const int per16 = dtype == CISR_F32 ? 4 : 8;
     const int wide = (((uintptr_t)k & 15) == 0 && k_token % per16 == 0 && k_head % per16 == 0 ? 1 : 0) | (((uintptr_t)v & 15) == 0 && v_token % per16 == 0 && v_head % per16 == 0 ? 2 : 0);
     const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
@@ -460,9 +493,9 @@ CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k
                                const int* which, int n_req, int tokens, int hkv, int dim, void* stream) {
     if (tokens <= 0 || n_req <= 0) return 0;
     if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535) return -2;
-    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15 || token_stride % 4 || head_stride % 4 || req_stride % 4) return -2;
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15 || token_stride % 8 || head_stride % 8 || req_stride % 8) return -2;
     if ((long long)tokens * hkv >= 1ll << 30) return -2;
-    const long long blocks = units((long long)tokens * hkv);
+    const long long blocks = units((long long)tokens * hkv, READ_ROWS * (THREADS / LANES));
     const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
     const dim3 grid((unsigned)blocks, (unsigned)n_req);
     return by_head_size(dim, [&](auto d) {

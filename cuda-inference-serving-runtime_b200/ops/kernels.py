@@ -529,6 +529,7 @@ def attn_decode(q, out, k_cache, v_cache, req_slot, block_table, dec_req, n_dec,
 INT4_GROUP = 32                  # values along a head that share a step
 INT4_BLOCK = 8                   # rows of a block; a page is whole blocks
 INT4_HEAD_DIMS = (32, 64, 96, 128)
+INT4_MAX_BYTES = 1 << 36         # of a plane: places in it are counted in 16 bytes, as 32-bit numbers
 INT4_FEW = 16                    # new tokens of a request up to which attn_decode_int4 is the faster call (see attn_prefill_int4)
 _int4_rows_state = {}
 _attention_int4_libs = {}
@@ -571,24 +572,27 @@ def int4_page_bytes(page_size: int, head_dim: int) -> int:
 
 def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, hkv: Optional[int], dim: int) -> tuple:
     """Checks a pair of 4-bit caches; the number of key heads and the device's index."""
+    shape, device = k_cache.shape, k_cache.get_device()
+    if (len(shape) == 3 and v_cache.shape == shape and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and device >= 0 and v_cache.get_device() == device
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[2] == page_size * 9 * dim // 16 and not page_size % INT4_BLOCK and dim in INT4_HEAD_DIMS
+            and (hkv is None or shape[1] == hkv) and (_device is None or device == _device()) and shape[0] * shape[1] * shape[2] < INT4_MAX_BYTES):
+        return shape[1], device
     _need(k_cache, torch.uint8, "k_cache", 3); _need(v_cache, torch.uint8, "v_cache", 3)
-    pages, heads, bytes_ = k_cache.shape
-    if v_cache.shape != k_cache.shape or bytes_ != page_size * 9 * dim // 16 or page_size % INT4_BLOCK or dim not in INT4_HEAD_DIMS or (hkv is not None and heads != hkv):
-        raise KernelError(f"{what}: a cache of {page_size} rows a page is [pages, kv_heads, {int4_page_bytes(page_size, dim)}] bytes at head size {dim}, "
-                          f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    device = k_cache.get_device()
-    if v_cache.get_device() != device or (_device is not None and device != _device()):
+    if k_cache.numel() >= INT4_MAX_BYTES:
+        raise KernelError(f"{what}: a plane of a 4-bit cache has less than {INT4_MAX_BYTES >> 30} GB")
+    if device != v_cache.get_device() or (_device is not None and device != _device()):
         raise KernelError(f"{what}: the cache is on {k_cache.device} and {v_cache.device}, the current device is another")
-    return heads, device
+    raise KernelError(f"{what}: a cache of {page_size} rows a page is [pages, kv_heads, {int4_page_bytes(page_size, dim)}] bytes at head size {dim}, "
+                      f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
 
 
-def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, **lists) -> None:
+def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, names: tuple, lists: tuple) -> None:
     """Checks int32 lists of `count` entries each (`req_slot`: any number) and the block table, all on the cache's device."""
-    if not (table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.get_device() == device):
+    if not (table.dtype is torch.int32 and table.dim() == 2 and table.is_contiguous() and table.get_device() == device):
         _need(table, torch.int32, "block_table", 2)
         raise KernelError(f"{what}: block_table is on {table.device}, the cache on cuda:{device}")
-    for name, t in lists.items():
-        if t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.get_device() == device and (t.numel() == count or name == "req_slot"):
+    for name, t in zip(names, lists):
+        if t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous() and t.get_device() == device and (t.shape[0] == count or name == "req_slot"):
             continue
         _need(t, torch.int32, name, 1)
         if t.get_device() != device:
@@ -596,15 +600,13 @@ def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, **lists
         raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
 
 
+_ROW_LISTS, _REQUEST_LISTS = ("token_req", "positions", "req_slot"), ("req_slot", "q_start", "q_len", "ctx_len")
+
+
 def _int4_mass(what: str, mass: torch.Tensor, k_cache: torch.Tensor, page_size: int) -> None:
     _need(mass, torch.float32, "mass", 3)
     if mass.shape[2] != page_size or mass.shape[:2] != k_cache.shape[:2] or mass.get_device() != k_cache.get_device():
         raise KernelError(f"{what}: mass must be [pages, kv_heads, page_size] on the cache's device")
-
-
-def _int4_rows_like(what: str, name: str, t: torch.Tensor, device: int) -> None:
-    if t.get_device() != device or t.dim() != 3 or t.stride(2) != 1 or t.dtype not in _DTYPE_CODE:
-        raise KernelError(f"{what}: {name} must be float32 or bfloat16 [tokens, kv_heads, head_dim] with neighbouring values, on the cache's device")
 
 
 def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, token_req: torch.Tensor, positions: torch.Tensor,
@@ -617,17 +619,19 @@ def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     458,528 are cut there), c the whole number nearest to x / s, so it is off by half of s and the rounding of s itself.  A
     group that holds an infinity or a NaN becomes NaN."""
     device = k_cache.get_device()
-    _int4_rows_like("int4_store", "k", k, device); _int4_rows_like("int4_store", "v", v, device)
-    tokens, hkv, dim = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise KernelError("int4_store: k and v differ in shape or type")
+    shape = k.shape
+    if not (len(shape) == 3 and v.shape == shape and k.dtype is v.dtype and k.dtype in _DTYPE_CODE and k.stride(2) == v.stride(2) == 1
+            and k.get_device() == v.get_device() == device):
+        raise KernelError("int4_store: k and v must be alike, float32 or bfloat16 [tokens, kv_heads, head_dim] with neighbouring values, on the cache's device")
+    tokens, hkv, dim = shape
     _int4_cache("int4_store", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_store", device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
+    _int4_lists("int4_store", device, block_table, tokens, _ROW_LISTS, (token_req, positions, req_slot))
     if mass is not None:
         _int4_mass("int4_store", mass, k_cache, page_size)
-    _check(_int4_rows().cisr_int4_store(_p(k), _p(v), dtype_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _p(k_cache), _p(v_cache),
-                                        _p(mass), _p(token_req), _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, tokens, hkv, dim,
-                                        _stream()), "int4_store")
+    (k_token, k_head, _), (v_token, v_head, _) = k.stride(), v.stride()
+    _check(_int4_rows().cisr_int4_store(k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], k_token, k_head, v_token, v_head, k_cache.data_ptr(), v_cache.data_ptr(), _p(mass),
+                                        token_req.data_ptr(), positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, tokens, hkv,
+                                        dim, _stream()), "int4_store")
 
 
 def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, token_req: torch.Tensor, positions: torch.Tensor,
@@ -639,7 +643,7 @@ def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor,
     _, device = _int4_cache("int4_read", k_cache, v_cache, page_size, hkv, dim)
     if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_read: k_out and v_out differ in shape, or lie elsewhere than the cache")
-    _int4_lists("int4_read", device, block_table, tokens, token_req=token_req, positions=positions, req_slot=req_slot)
+    _int4_lists("int4_read", device, block_table, tokens, _ROW_LISTS, (token_req, positions, req_slot))
     _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), 0, hkv * dim, dim, _p(token_req),
                                        _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, 0, 0, 1, tokens, hkv, dim, _stream()), "int4_read")
 
@@ -654,9 +658,9 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
     if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_expand: k_out and v_out differ in shape, or lie elsewhere than the cache")
     if requests is None:
-        _int4_lists("int4_expand", device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "ctx_len"), (req_slot, ctx_len))
     else:
-        _int4_lists("int4_expand", device, block_table, n, req_slot=req_slot, requests=requests)
+        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "requests"), (req_slot, requests))
         _need(ctx_len, torch.int32, "ctx_len", 1)
     _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), hkv * rows * dim, dim, rows * dim, 0, 0,
                                        _p(req_slot), _p(block_table), block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()),
@@ -677,7 +681,7 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     tokens, hq, dim = q.shape
     hkv, device = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
     n = q_len.numel()
-    _int4_lists("attn_decode_int4", device, block_table, n, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len)
+    _int4_lists("attn_decode_int4", device, block_table, n, _REQUEST_LISTS, (req_slot, q_start, q_len, ctx_len))
     if out.shape != q.shape or hq % hkv or max_queries < 1 or longest < 1 or req_slot.numel() < n or q.get_device() != device or out.get_device() != device:
         raise KernelError("attn_decode_int4: shapes, heads, limits, lists or devices disagree")
     if (window is not None and window < 1) or keep_first < 0:
@@ -717,7 +721,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     n = n_all if requests is None else requests.numel()
     if places is None:
         places = torch.arange(n, dtype=torch.int32, device=q.device)
-    _int4_lists("attn_prefill_int4", device, block_table, n_all, req_slot=req_slot, q_start=q_start, q_len=q_len, ctx_len=ctx_len, places=places)
+    _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS + ("places",), (req_slot, q_start, q_len, ctx_len, places))
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     k, v = torch.empty((2, n, hkv, rows, dim), dtype=q.dtype, device=q.device)
     int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
@@ -743,7 +747,7 @@ def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor,
     bytes_ = k_cache.shape[2] if k_cache.dim() == 3 else 0
     dim = bytes_ * 16 // (9 * page_size) if page_size > 0 else 0
     _, device = _int4_cache("int4_evict", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_evict", device, block_table, n, req_slot=req_slot, ctx_len=ctx_len)
+    _int4_lists("int4_evict", device, block_table, n, ("req_slot", "ctx_len"), (req_slot, ctx_len))
     _int4_mass("int4_evict", mass, k_cache, page_size)
     if kept.get_device() != device or to_table.get_device() != device:
         raise KernelError("int4_evict: kept and to_table must lie on the cache's device")
