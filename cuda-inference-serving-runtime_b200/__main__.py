@@ -7,7 +7,7 @@ where it has them: --dtype, --execution, --checkpoint, --prompt, --tokens,
 requests[key, status, generated, text, ttft_ms]).  Differences: --device accepts only
 cuda (there is no CPU path); --dtype has no float16; without --checkpoint the model is
 a named shape with seeded random weights (--config, --seed) instead of one fixed toy;
---temperature, --max-active and --reserve are added; several EOS ids are accepted.
+--temperature, --max-active, --reserve, --cache and --keep are added; several EOS ids are accepted.
 """
 from __future__ import annotations
 
@@ -44,6 +44,8 @@ def build_parser() -> argparse.ArgumentParser:
     parser.add_argument("--token-budget", type=int, default=32)
     parser.add_argument("--prefill-chunk", type=int, default=8)
     parser.add_argument("--max-active", type=int, default=8)
+    parser.add_argument("--cache", choices=["int4"], help="int4: keys and values held in 4 bits (default: in the compute dtype)")
+    parser.add_argument("--keep", type=int, help="with --cache int4: cut a request down to this many rows, those that attention has looked at most")
     return parser
 
 
@@ -66,7 +68,7 @@ def main(argv=None) -> int:
         prompt = [int(t) for t in args.tokens.split(",")]
     engine = Engine.for_model(model, pages=args.pages, page_size=args.page_size, max_active=args.max_active,
                               token_budget=args.token_budget, prefill_chunk=args.prefill_chunk, policy=args.policy,
-                              reserve=args.reserve, graph=args.execution == "graph")
+                              reserve=args.reserve, graph=args.execution == "graph", cache=args.cache, keep=args.keep)
     inputs = json.loads(args.requests.read_text()) if args.requests else [
         {"key": "request-0", "prompt": prompt, "max_new_tokens": args.max_new_tokens}]
     for item in inputs:

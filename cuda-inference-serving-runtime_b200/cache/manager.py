@@ -22,6 +22,11 @@ Parity: runtime/cache.py:9-118 (create, fork, copy-on-write of a shared partial 
 atomic failure, release, invariants, report).  Unlike the reference (one allocator per
 layer, runtime/model.py:66-67) there is one allocator per group, and lengths are
 committed by the caller after the step is enqueued (runtime/execution.py:125-126).
+
+Pages may hold keys and values in 4 bits (`CacheUse.held`).  With `weigh` every key has a number beside it, the weight that
+attention has given it so far, and a request can be cut down to its weightiest rows (`plan_cut`, `finish_cut`): its rows
+are then fewer than the tokens it has seen (`length` and `seen`), and they lie on pages of their own again, so a page that
+another request shares is never written.
 """
 from __future__ import annotations
 
@@ -32,6 +37,7 @@ import numpy as np
 import torch
 
 from ..config.spec import CacheUse
+from ..ops.kernels import int4_page_bytes
 from .pages import OutOfPages, PagePool
 
 
@@ -46,6 +52,8 @@ class PagedBinding:
     window: Optional[int]
     keep_first: int = 0          # the sequence's first keys that stay (and stay in sight) behind the window
     state: Optional[torch.Tensor] = None     # the entry's own side state [slots, ...], where its mixer asked for one
+    held: str = ""                           # "int4": k and v are uint8 [pages, kv_heads, bytes of a page]
+    mass: Optional[torch.Tensor] = None      # float [pages, kv_heads, page_size], where keys are weighed
 
 
 @dataclass
@@ -57,24 +65,31 @@ class StateBinding:
 @dataclass
 class _Request:
     slot: int
-    length: int = 0
+    length: int = 0              # rows in the cache
+    seen: int = 0                # tokens so far: the next one's position
     tables: Dict[int, List[int]] = field(default_factory=dict)   # group index -> logical page -> physical page or -1
     first_live: Dict[int, int] = field(default_factory=dict)     # group index -> first logical page still held
 
 
 class PageGroup:
     def __init__(self, index: int, use: CacheUse, entries: List[int], n_pages: int, page_size: int, max_slots: int,
-                 width: int, dtype: torch.dtype, device):
+                 width: int, dtype: torch.dtype, device, weigh: bool = False):
         self.index, self.use, self.entries = index, use, entries
         self.page_size, self.width = page_size, width
         self.pool = PagePool(n_pages)
         self.entry_slot = {e: i for i, e in enumerate(entries)}
-        self.storage = None
+        self.storage = self.mass = None
         self.device_table = None
         if device is not None:
             # [entries, key|value, pages, kv_heads, page_size, head_dim]; one plane where a row serves as both
-            self.storage = torch.zeros((len(entries), use.planes, n_pages, use.kv_heads, page_size, use.head_dim), dtype=dtype,
-                                       device=device)
+            if use.held == "int4":
+                self.storage = torch.zeros((len(entries), use.planes, n_pages, use.kv_heads, int4_page_bytes(page_size, use.head_dim)), dtype=torch.uint8,
+                                           device=device)
+            else:
+                self.storage = torch.zeros((len(entries), use.planes, n_pages, use.kv_heads, page_size, use.head_dim), dtype=dtype,
+                                           device=device)
+            if weigh:
+                self.mass = torch.zeros((len(entries), n_pages, use.kv_heads, page_size), dtype=torch.float32, device=device)
             self.planes = [(s[0], s[use.planes - 1]) for s in self.storage]      # each entry's keys and values
             self.device_table = torch.full((max_slots + 1, width), -1, dtype=torch.int32, device=device)   # last row: the null slot
         self.host_table = np.full((max_slots, width), -1, dtype=np.int32)
@@ -86,7 +101,7 @@ class PageGroup:
         self.updates.append((slot * self.width + logical, page))
 
     def page_bytes(self) -> int:
-        return self.use.kv_heads * self.page_size * self.use.head_dim * self.storage.element_size()
+        return self.storage[0, 0, 0].numel() * self.storage.element_size()
 
 
 class StateGroup:
@@ -108,16 +123,21 @@ class CacheManager:
     group.  `side_states[i]`, where given, is a `CacheUse("state", ...)` that run entry i holds besides
     its pages (or besides the pages it reads); places behind the last run entry are states that belong to no
     entry (`side_state` gives them).  With `device=None` only the host bookkeeping exists
-    (tests of the allocator).
+    (tests of the allocator).  `weigh`: every page group keeps a number per key (`PagedBinding.mass`) beside pages in 4 bits.
     """
 
     def __init__(self, uses: Sequence, n_pages: int, page_size: int, max_slots: int, max_positions: int,
-                 dtype: torch.dtype = torch.float32, device=None, side_states: Optional[Sequence] = None):
+                 dtype: torch.dtype = torch.float32, device=None, side_states: Optional[Sequence] = None, weigh: bool = False):
         if n_pages <= 0 or page_size <= 0 or max_slots <= 0:
             raise ValueError("cache dimensions must be positive")
         self.page_size, self.max_slots, self.max_positions = page_size, max_slots, max_positions
         self.width = -(-max_positions // page_size)
-        self.device, self.dtype = device, dtype
+        self.device, self.dtype, self.weigh = device, dtype, weigh
+        for use in uses:
+            if not isinstance(use, int) and use.kind == "pages" and use.held not in ("", "int4"):
+                raise ValueError(f"unknown form of a cache {use.held!r}")
+            if weigh and not isinstance(use, int) and use.kind == "pages" and (use.held != "int4" or use.window is not None):
+                raise ValueError("keys are weighed, and requests cut by their weights, in caches held in 4 bits without a window")
         self.page_groups: List[PageGroup] = []
         self.state_groups: List[StateGroup] = []
         self.entry_group: Dict[int, Tuple[str, int]] = {}   # run entry -> ("pages"|"state", group index)
@@ -133,7 +153,7 @@ class CacheManager:
         for key, entries in by_key.items():
             use = uses[entries[0]]
             if use.kind == "pages":
-                group = PageGroup(len(self.page_groups), use, entries, n_pages, page_size, max_slots, self.width, dtype, device)
+                group = PageGroup(len(self.page_groups), use, entries, n_pages, page_size, max_slots, self.width, dtype, device, weigh)
                 self.page_groups.append(group)
                 for e in entries:
                     self.entry_group[e] = ("pages", group.index)
@@ -189,7 +209,7 @@ class CacheManager:
         if not self.free_slots:
             raise OutOfPages(f"all {self.max_slots} request slots are in use")
         slot = self.free_slots.pop()
-        req = _Request(slot, src.length)
+        req = _Request(slot, src.length, src.seen)
         for g in self.page_groups:
             table = list(src.tables[g.index])
             req.tables[g.index] = table
@@ -206,6 +226,10 @@ class CacheManager:
 
     def length(self, key) -> int:
         return self.requests[key].length
+
+    def seen(self, key) -> int:
+        """Tokens the request has brought so far (its rows, unless it was cut)."""
+        return self.requests[key].seen
 
     def slot(self, key) -> int:
         return self.requests[key].slot
@@ -236,7 +260,7 @@ class CacheManager:
         """
         for key, n_tokens in portions:
             req = self.requests[key]
-            if n_tokens < 0 or req.length + n_tokens > self.max_positions:
+            if n_tokens < 0 or req.seen + n_tokens > self.max_positions:
                 raise ValueError(f"sequence {key!r} would exceed the context limit of {self.max_positions}")
         for g in self.page_groups:
             need = sum(self._plan(self.requests[key], g, n)[0] for key, n in portions)
@@ -264,6 +288,7 @@ class CacheManager:
         """The step that wrote `n_tokens` more tokens is enqueued: advance the length, give back passed pages."""
         req = self.requests[key]
         req.length += n_tokens
+        req.seen += n_tokens
         for g in self.page_groups:
             if g.use.window is None:
                 continue
@@ -277,6 +302,32 @@ class CacheManager:
                     table[logical] = -1
                     g.set_entry(req.slot, logical, -1)
             req.first_live[g.index] = max(req.first_live[g.index], min(dead, len(table)))
+
+    def plan_free(self, n_requests: int, rows: int) -> bool:
+        """Whether every group has the free pages for so many requests of so many rows."""
+        return all(n_requests * -(-rows // self.page_size) <= g.pool.n_free for g in self.page_groups)
+
+    def plan_cut(self, keys: Sequence, rows: int) -> Optional[List[List[List[int]]]]:
+        """Fresh pages for `rows` rows of every request, [group][request][pages], or None (and nothing taken) where some group has
+        too few.  The caller moves the rows that stay there and calls `finish_cut`."""
+        if not self.plan_free(len(keys), rows):
+            return None
+        n = -(-rows // self.page_size)
+        return [[g.pool.allocate(n) for _ in keys] for g in self.page_groups]
+
+    def finish_cut(self, keys: Sequence, rows: int, pages: List[List[List[int]]]) -> None:
+        """The rows that stay are on their way to `pages`: the requests have `rows` rows there now, and their old pages go back (steps
+        that use them again follow on the same stream)."""
+        for g, of_request in zip(self.page_groups, pages):
+            for key, fresh in zip(keys, of_request):
+                req = self.requests[key]
+                for logical, page in enumerate(req.tables[g.index]):
+                    if page >= 0:
+                        g.pool.release(page)
+                    g.set_entry(req.slot, logical, fresh[logical] if logical < len(fresh) else -1)
+                req.tables[g.index] = list(fresh)
+        for key in keys:
+            self.requests[key].length = rows
 
     def release(self, key) -> None:
         """The request is over: every page it holds goes back (to be used again), its slot too.
@@ -319,7 +370,8 @@ class CacheManager:
             g = self.page_groups[gi]
             k, v = g.planes[g.entry_slot[source]]
             return PagedBinding(k, v, g.device_table, g.page_size,
-                                write=reads_from is None, window=g.use.window, keep_first=g.use.keep_first, state=self.side_state(entry))
+                                write=reads_from is None, window=g.use.window, keep_first=g.use.keep_first, state=self.side_state(entry),
+                                held=g.use.held, mass=None if g.mass is None else g.mass[g.entry_slot[source]])
         g = self.state_groups[gi]
         return StateBinding(g.states[g.entry_slot[source]])
 

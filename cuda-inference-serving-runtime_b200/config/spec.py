@@ -67,6 +67,7 @@ class CacheUse:
     `window` None keeps every key, an integer keeps the last `window` of them, and with it `keep_first` also the
     sequence's first `keep_first` keys (their pages are never given back while the request lives).  `planes` 2: a key
     plane and a value plane; 1: one plane of rows that serve as both (a latent from which keys and values are derived).
+    `held` "": pages in the compute dtype; "int4": 4 bits a value (uint8 pages of `ops.kernels.int4_page_bytes` per key head).
     kind "state": a fixed-size tensor per request of `state_shape`/`state_dtype`.
     kind "none": nothing.
     """
@@ -78,10 +79,11 @@ class CacheUse:
     state_dtype: str = "float32"
     planes: int = 2
     keep_first: int = 0
+    held: str = ""
 
     def group_key(self) -> tuple:
         return (self.kind, self.kv_heads, self.head_dim, self.window, self.state_shape, self.state_dtype, self.planes,
-                self.keep_first if self.window is not None else 0)
+                self.keep_first if self.window is not None else 0, self.held)
 
 
 @dataclass(frozen=True)

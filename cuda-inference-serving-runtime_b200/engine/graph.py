@@ -164,8 +164,9 @@ class DecodeGraph:
         start, size = self.offsets[name]
         return self.dev[start:start + size]
 
-    def fill(self, slots, tokens, positions, temperature, seed, counter, updates) -> None:
-        """Write one step's contents into the pinned buffer (rows beyond the live ones become padding)."""
+    def fill(self, slots, tokens, positions, temperature, seed, counter, updates, rows_before=None) -> None:
+        """Write one step's contents into the pinned buffer (rows beyond the live ones become padding).  `rows_before`: the requests' rows
+        in the cache, where those are not their positions (requests that were cut)."""
         n, rows = len(slots), self.rows
         null = self.stepper.cache.null_slot
         if self.sent is not None:
@@ -173,7 +174,7 @@ class DecodeGraph:
         self.h("token_ids")[:n] = tokens; self.h("token_ids")[n:] = 0
         self.h("positions")[:n] = positions; self.h("positions")[n:] = 0
         self.h("req_slot")[:n] = slots; self.h("req_slot")[n:] = null
-        self.h("ctx_len")[:n] = np.asarray(positions) + 1; self.h("ctx_len")[n:] = 0
+        self.h("ctx_len")[:n] = np.asarray(positions if rows_before is None else rows_before) + 1; self.h("ctx_len")[n:] = 0
         self.h("live")[:n] = 1; self.h("live")[n:] = 0
         self.h("temperature").view(np.float32)[:n] = temperature; self.h("temperature")[n:] = 0
         self.h("seed").view(np.int64)[:n] = seed

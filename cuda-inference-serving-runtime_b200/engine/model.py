@@ -137,9 +137,28 @@ class Model:
         own = self.embedding.side_state()
         return states if own is None else states + [own]
 
-    def make_cache(self, n_pages: int, page_size: int = 16, max_slots: int = 64) -> CacheManager:
-        return CacheManager(self.cache_uses(), n_pages, page_size, max_slots, self.spec.max_positions,
-                            dtype=self.dtype, device=self.device, side_states=self.side_states())
+    def make_cache(self, n_pages: int, page_size: int = 16, max_slots: int = 64, held: Optional[str] = None, weigh: bool = False) -> CacheManager:
+        """`held` "int4": pages in 4 bits, for models whose paged mixers all take them.  `weigh`: with it, a number per key for the weight that
+        attention has given it."""
+        uses = self.cache_uses()
+        if held not in (None, "int4"):
+            raise ValueError(f"a cache is held in the compute dtype (None) or in \"int4\", not {held!r}")
+        if weigh and held is None:
+            raise ValueError("keys are weighed in caches held in 4 bits")
+        if held:
+            jobs = []
+            for entry, use in zip(self.spec.run, uses):
+                mixer = self.layers[entry.layer].mixer
+                if mixer.cache_use().kind == "pages":
+                    if not mixer.takes_int4():
+                        raise ValueError(f"{mixer.spec.kind} keeps its keys and values in the compute dtype only: no cache in 4 bits for this model")
+                    jobs += mixer.int4_jobs()
+            if page_size % 8:
+                raise ValueError(f"a page of a cache in 4 bits holds a multiple of 8 rows, not {page_size}")
+            uses = [use if isinstance(use, int) or use.kind != "pages" else replace(use, held=held) for use in uses]
+            kernel_build.compile_many(list({repr(j): j for j in jobs}.values()))
+        return CacheManager(uses, n_pages, page_size, max_slots, self.spec.max_positions,
+                            dtype=self.dtype, device=self.device, side_states=self.side_states(), weigh=weigh)
 
     # ---------------------------------------------------------------- forward
     def step_beginners(self) -> list:

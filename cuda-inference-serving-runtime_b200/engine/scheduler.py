@@ -81,7 +81,7 @@ class Engine:
 
     def __init__(self, stepper, choose: Callable, vocab_size: int, max_positions: int, max_active: int = 8,
                  token_budget: int = 32, prefill_chunk: int = 8, policy: str = "chunked", reserve: str = "full",
-                 lookahead: bool = False):
+                 lookahead: bool = False, keep=None):
         if min(max_active, token_budget, prefill_chunk) <= 0:
             raise ValueError("invalid scheduler limits")
         if policy not in POLICIES:
@@ -93,6 +93,7 @@ class Engine:
         self.max_active = 1 if policy == "serial" else max_active
         self.token_budget, self.prefill_chunk, self.policy, self.reserve = token_budget, prefill_chunk, policy, reserve
         self.lookahead = lookahead
+        self.keep = keep           # a `Keep` of the stepper's: requests are cut down to its rows
         self.waiting: deque = deque()
         self.active: List[Request] = []
         self.requests = {}
@@ -104,14 +105,16 @@ class Engine:
 
     @classmethod
     def for_model(cls, model, pages: int = 128, page_size: int = 16, max_active: int = 8, token_budget: int = 32,
-                  prefill_chunk: int = 8, policy: str = "chunked", reserve: str = "full", graph: bool = False) -> "Engine":
+                  prefill_chunk: int = 8, policy: str = "chunked", reserve: str = "full", graph: bool = False, cache: Optional[str] = None,
+                  keep=None) -> "Engine":
+        """`cache` "int4": keys and values in 4 bits; `keep`, with it: a number of rows (or a `Keep`) that requests are cut down to."""
         from ..sampling import DeviceSampler
         from .step import Stepper
 
-        stepper = Stepper(model, n_pages=pages, page_size=page_size, max_slots=max(max_active, 1), graph=graph)
+        stepper = Stepper(model, n_pages=pages, page_size=page_size, max_slots=max(max_active, 1), graph=graph, cache=cache, keep=keep)
         sampler = DeviceSampler(stepper)
         return cls(stepper, sampler, model.spec.vocab_size, model.spec.max_positions, max_active, token_budget,
-                   prefill_chunk, policy, reserve, lookahead=graph)
+                   prefill_chunk, policy, reserve, lookahead=graph, keep=stepper.keep)
 
     # ---------------------------------------------------------------- page arithmetic
     @property
@@ -122,7 +125,8 @@ class Engine:
         return [g.pool for g in self.stepper.cache.page_groups]
 
     def _pool_pages(self) -> int:
-        return min((pool.n_pages for pool in self._pools()), default=1 << 30)
+        """Pages for requests: of requests that are cut, a cut's fresh pages stay free."""
+        return min((pool.n_pages for pool in self._pools()), default=1 << 30) - (self._pages_for(self.keep.rows) if self.keep else 0)
 
     def _free_pages(self) -> int:
         return min((pool.n_free for pool in self._pools()), default=1 << 30)
@@ -135,7 +139,10 @@ class Engine:
 
     def _life_pages(self, r: Request) -> int:
         """Pages of a request's whole life.  The last token chosen is never fed back, so it needs no place in the cache
-        (runtime/engine.py:46-47)."""
+        (runtime/engine.py:46-47).  A request that is cut has at most the rows that call for a cut, and a portion more."""
+        if self.keep is not None:
+            most = self.keep.rows + self.keep.slack + max(1, min(self.prefill_chunk, self.token_budget)) - 1
+            return self._pages_for(min(r.life_tokens(), most))
         return self._pages_for(r.life_tokens())
 
     # ---------------------------------------------------------------- requests
@@ -194,10 +201,10 @@ class Engine:
     def _entry_price(self, r: Request) -> int:
         """Pages a request must find to be admitted: its whole life under "full" (then it can never lack one later,
         runtime/engine.py:65-76), what it holds tokens for now under "lazy"."""
-        return self._life_pages(r) if self.reserve == "full" else self._pages_for(len(r.tokens()))
+        return self._life_pages(r) if self.reserve == "full" else min(self._life_pages(r), self._pages_for(len(r.tokens())))
 
     def _admit(self) -> None:
-        budget = self._pool_pages() - sum(self.reserved.values()) if self.reserve == "full" else self._free_pages()
+        budget = self._pool_pages() - sum(self.reserved.values()) if self.reserve == "full" else self._free_pages() - (self._pages_for(self.keep.rows) if self.keep else 0)
         now = time.perf_counter()
         # every waiting request is looked at, so a large one does not hold up smaller ones behind it
         for r in [w for w in self.waiting if w.submitted_at <= now]:

@@ -11,6 +11,7 @@ logits for every row; here a request brings any number of tokens and names the r
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -47,6 +48,9 @@ def run_page_copies(cache: CacheManager, device) -> None:
             pairs = torch.tensor(copies, dtype=torch.int32, device=device)
             page_bytes = g.page_bytes()
             kernels.page_copy(g.storage, pairs, g.storage.shape[0] * g.storage.shape[1], g.pool.n_pages * page_bytes, page_bytes)
+            if g.mass is not None:
+                mass_bytes = g.mass[0, 0].numel() * 4
+                kernels.page_copy(g.mass, pairs, g.mass.shape[0], g.pool.n_pages * mass_bytes, mass_bytes)
 
 
 def prepare_step(cache: CacheManager, ring: PinnedRing, device, entries: Sequence[StepEntry], vocab_size: int,
@@ -65,8 +69,8 @@ def prepare_step(cache: CacheManager, ring: PinnedRing, device, entries: Sequenc
     total = 0
     for r, e in enumerate(entries):
         n = len(e.tokens)
-        start = cache.length(e.key)
-        slots.append(cache.slot(e.key)); q_start.append(total); q_len.append(n); ctx_len.append(start + n)
+        start = cache.seen(e.key)
+        slots.append(cache.slot(e.key)); q_start.append(total); q_len.append(n); ctx_len.append(cache.length(e.key) + n)
         token_ids.extend(int(t) for t in e.tokens)
         positions.extend(range(start, start + n))
         token_req.extend([r] * n)
@@ -114,16 +118,43 @@ class StagedTokens:
         return self.pinned[:self.n].tolist()
 
 
+@dataclass(frozen=True)
+class Keep:
+    """How far a request's cache may grow, and what stays when it is cut: as soon as it has `rows` + `slack` rows, the first `first`,
+    the latest `recent`, and of those between the ones that attention has given most weight so far, `rows` in all, per key head."""
+    rows: int
+    recent: int
+    first: int
+    slack: int
+
+    def __post_init__(self):
+        if min(self.rows, self.slack) < 1 or min(self.recent, self.first) < 0 or self.recent + self.first > self.rows:
+            raise ValueError(f"a cache cannot be cut to {self.rows} rows, {self.recent} of them the latest and {self.first} the first, every {self.slack} rows")
+
+    @classmethod
+    def of(cls, rows, page_size: int) -> "Keep":
+        """From a number of rows: half of them the latest, four the first, cut whenever an eighth more (whole pages) has come."""
+        if isinstance(rows, cls):
+            return rows
+        return cls(rows, rows // 2, min(4, rows // 4), -(-max(1, rows // 8) // page_size) * page_size)
+
+
 class Stepper:
-    """`graph=True` replays steps made only of single new tokens from captured CUDA graphs (see engine/graph.py);
+    """`cache` "int4": keys and values are held in 4 bits (models whose mixers all take that).  `keep` (a number of rows, or a `Keep`), with it:
+    requests are cut down to the rows that attention has looked at most.
+
+    `graph=True` replays steps made only of single new tokens from captured CUDA graphs (see engine/graph.py);
     it is ignored when a mixer of the model reads the step through host values."""
 
-    def __init__(self, model: Model, n_pages: int, page_size: int = 16, max_slots: int = 64, graph: bool = False):
+    def __init__(self, model: Model, n_pages: int, page_size: int = 16, max_slots: int = 64, graph: bool = False, cache: Optional[str] = None,
+                 keep=None):
         if not model.loaded:
             raise RuntimeError("the model has no weights yet")
         self.model = model
         self.max_slots = max_slots
-        self.cache: CacheManager = model.make_cache(n_pages, page_size, max_slots)
+        self.keep = None if keep is None else Keep.of(keep, page_size)
+        self.cache: CacheManager = model.make_cache(n_pages, page_size, max_slots, held=cache, weigh=self.keep is not None)
+        self.held = cache
         self.ring = PinnedRing()
         self.planners = model.planners()
         self.last_context: Optional[StepContext] = None
@@ -161,14 +192,37 @@ class Stepper:
         if self.graphs is not None and entries and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries):
             return self._graph_step(entries, extra)
         ctx, extras, graph = prepare_step(self.cache, self.ring, self.model.device, entries, self.model.spec.vocab_size,
-                                          extra, shape_graphs=self.graphs, planners=self.planners)
+                                          extra, shape_graphs=None if self.held else self.graphs, planners=self.planners)
         if graph is not None:
             logits = graph.run(ctx, ctx.update_views)
         else:
             logits = self.model.forward(ctx, self.cache)
         commit_step(self.cache, entries)
         self.last_context, self.last_extras, self.last_tokens = ctx, extras, None
+        self._cut([e.key for e in entries])
         return logits
+
+    def _cut(self, keys) -> None:
+        """Cut the requests that have grown far enough (`Keep`), together if the free pages allow it, else one by one; one that finds no
+        pages waits for a later step."""
+        keep = self.keep
+        keys = [] if keep is None else [k for k in keys if self.cache.length(k) >= keep.rows + keep.slack]
+        if not keys:
+            return
+        self._ahead = None           # a graph's own buffers hold the lengths from before
+        for some in [keys] if self.cache.plan_free(len(keys), keep.rows) else [[k] for k in keys]:
+            pages = self.cache.plan_cut(some, keep.rows)
+            if pages is None:
+                continue
+            device = self.model.device
+            lens = [self.cache.length(k) for k in some]
+            meta = torch.tensor([[self.cache.slot(k) for k in some], lens], dtype=torch.int32, device=device)
+            for g, of_request in zip(self.cache.page_groups, pages):
+                to = torch.tensor(of_request, dtype=torch.int32, device=device)
+                kept = torch.empty((len(some), g.use.kv_heads, keep.rows), dtype=torch.int32, device=device)
+                for (k, v), mass in zip(g.planes, g.mass):
+                    kernels.int4_evict(k, v, mass, meta[0], g.device_table, meta[1], to, kept, g.page_size, max(lens), keep.recent, keep.first)
+            self.cache.finish_cut(some, keep.rows, pages)
 
     def _flush_tables(self, limit: int):
         """Pending block-table changes per group; those beyond `limit` entries are applied at once."""
@@ -189,12 +243,12 @@ class Stepper:
         cache.reserve([(e.key, 1) for e in entries])
         n = len(entries)
         slots = [cache.slot(e.key) for e in entries]
-        positions = [cache.length(e.key) for e in entries]
-        graph, fresh = self.graphs.get(n, max(positions) + 1)
+        positions, rows = [cache.seen(e.key) for e in entries], [cache.length(e.key) for e in entries]
+        graph, fresh = self.graphs.get(n, max(rows) + 1)
         updates = self._flush_tables(graph.n_updates)
         extra = extra or {}
         graph.fill(slots, [int(e.tokens[0]) for e in entries], positions, extra.get("temperature", 0.0),
-                   extra.get("seed", 0), extra.get("counter", 0), updates)
+                   extra.get("seed", 0), extra.get("counter", 0), updates, rows)
         graph.upload()
         if fresh:
             graph.capture(warm_up=self.graphs.first_of_its_rows(graph))
@@ -205,6 +259,7 @@ class Stepper:
         self.last_tokens = graph.tokens[:n].clone()       # a later replay overwrites the graph's own buffer
         self._last_graph = None
         self._ahead = (graph, [e.key for e in entries])
+        self._cut([e.key for e in entries])
         return graph.logits[:n]
 
     def decode_ahead(self, steps: int, history: bool = True) -> Optional[torch.Tensor]:
@@ -221,7 +276,9 @@ class Stepper:
         graph, keys = self._ahead
         cache = self.cache
         longest = max(cache.length(k) for k in keys)
-        steps = min(steps, graph.ctx_bucket - longest, self.model.spec.max_positions - longest)
+        steps = min(steps, graph.ctx_bucket - longest, self.model.spec.max_positions - max(cache.seen(k) for k in keys))
+        if self.keep is not None:            # up to the next cut
+            steps = min(steps, max(0, self.keep.rows + self.keep.slack - longest))
         device = self.model.device
         if steps <= 0:
             return torch.empty((0, len(keys)), dtype=torch.int32, device=device) if history else 0
@@ -237,6 +294,7 @@ class Stepper:
                 kept[i].copy_(graph.tokens, non_blocking=True)
         for k in keys:
             cache.commit(k, steps)
+        self._cut(keys)
         if kept is None:
             self.last_tokens = graph.tokens[:len(keys)]
             self._last_graph = graph

@@ -7,7 +7,7 @@ by construction).  q_proj, k_proj and v_proj are stacked into one matrix at load
 """
 from __future__ import annotations
 
-from typing import Dict, Optional
+from typing import Dict, NamedTuple, Optional
 
 import numpy as np
 import torch
@@ -69,6 +69,12 @@ class GQAAttention(Mixer):
     def cache_use(self) -> CacheUse:
         return CacheUse("pages", kv_heads=self.hkv, head_dim=self.dim, window=self.window)
 
+    def takes_int4(self) -> bool:
+        return self.dim in kernels.INT4_HEAD_DIMS
+
+    def int4_jobs(self) -> list:
+        return kernels.int4_jobs(self.dim, self.dtype)
+
     # ---------------------------------------------------------------- the launch plan of a step
     def plan_key(self):
         return ATTENTION_PLAN_KEY
@@ -86,13 +92,16 @@ class GQAAttention(Mixer):
         device = ctx.device
         rot = self.position.rotation(ctx)
         q = torch.empty((tokens, hq, dim), dtype=self.dtype, device=device)
+        # where the new keys and values go: straight into the cache, or, where that is held in 4 bits, into a page of this step first
+        to = staged_rows(ctx, hkv, dim, self.dtype) if cache.held else StepRows(cache.k, cache.v, ctx.positions, ctx.token_req, ctx.req_slot, cache.block_table,
+                                                                               cache.page_size)
         turn = (dim, rot.rot_half, rot.interleaved) if rot else (dim, 0, False)
         if cache.write and kernels.skinny_ok(tokens, self.qkv, turn):
             # few tokens: one launch computes (the norm,) the projection, the rotation and the cache write
             rope = dict(cos=rot.cos if rot else None, sin=rot.sin if rot else None, rot_half=rot.rot_half if rot else 0,
-                        interleaved=rot.interleaved if rot else False, q_out=q, k_cache=cache.k, v_cache=cache.v,
-                        positions=ctx.positions, token_req=ctx.token_req, req_slot=ctx.req_slot,
-                        block_table=cache.block_table, page_size=cache.page_size, hq=hq, hkv=hkv, dim=dim)
+                        interleaved=rot.interleaved if rot else False, q_out=q, k_cache=to.k, v_cache=to.v,
+                        positions=to.positions, token_req=to.token_req, req_slot=to.req_slot,
+                        block_table=to.block_table, page_size=to.page_size, hq=hq, hkv=hkv, dim=dim)
             if norm_fusable(h, tokens, self.qkv, turn):
                 x_out = h.new_stream_buffer()
                 kernels.skinny_gemm(self.qkv, tokens, x=h.x, delta=h.delta, norm_w=h.weight, eps=h.eps, x_out=x_out,
@@ -104,8 +113,8 @@ class GQAAttention(Mixer):
               and kernels.tcgen05_ok(as_tensor(h) if isinstance(h, torch.Tensor) else h.materialize_once(), self.qkv, fused=True)):
             # many tokens: rotation and cache write are the epilogue of the tcgen05 product
             kernels.gemm_tcgen05_rope(h if isinstance(h, torch.Tensor) else h.materialize_once(), self.qkv, dict(
-                cos=rot.cos, sin=rot.sin, q_out=q, k_cache=cache.k, v_cache=cache.v, positions=ctx.positions,
-                token_req=ctx.token_req, req_slot=ctx.req_slot, block_table=cache.block_table, page_size=cache.page_size,
+                cos=rot.cos, sin=rot.sin, q_out=q, k_cache=to.k, v_cache=to.v, positions=to.positions,
+                token_req=to.token_req, req_slot=to.req_slot, block_table=to.block_table, page_size=to.page_size,
                 hq=hq, hkv=hkv, dim=dim))
         else:
             h = h if isinstance(h, torch.Tensor) else h.materialize_once()
@@ -117,8 +126,14 @@ class GQAAttention(Mixer):
                 k_col = v_col = -1
             kernels.rope_store(proj, k_col, v_col, rot.cos if rot else None, rot.sin if rot else None,
                                rot.rot_half if rot else 0, rot.interleaved if rot else False, q,
-                               cache.k if cache.write else None, cache.v if cache.write else None,
-                               ctx.token_req, ctx.positions, ctx.req_slot, cache.block_table, cache.page_size, hq, hkv, dim)
+                               to.k if cache.write else None, to.v if cache.write else None,
+                               to.token_req, to.positions, to.req_slot, to.block_table, to.page_size, hq, hkv, dim)
+        if cache.held:
+            if cache.write:
+                kernels.int4_store(to.k[0].transpose(0, 1), to.v[0].transpose(0, 1), cache.k, cache.v, ctx.token_req, token_rows(ctx, cache), ctx.req_slot,
+                                   cache.block_table, cache.page_size, mass=cache.mass)
+            out = int4_attention(ctx.plan_for(self), q, cache, ctx, hq, self.scale, self.window)
+            return linear_to_stream(out.view(tokens, hq * dim), self.o, h0)
         out = torch.empty((tokens, hq, dim), dtype=self.dtype, device=device)
         plan = ctx.plan_for(self)
         if plan.info["n_tiles"] and kernels.attn_prefill_wide_ok(q, cache.k, cache.page_size):
@@ -151,6 +166,78 @@ class GQAAttention(Mixer):
                 projected = torch.empty((tokens, self.hidden), dtype=torch.float32, device=device)
                 return kernels.merge_out_proj(partial, stats, n_splits, plan["dec_req"], ctx.q_start, n_decode, hq, dim, self.o, projected)
         return linear_to_stream(out.view(tokens, hq * dim), self.o, h0)
+
+
+class StepRows(NamedTuple):
+    """Where the new keys and values of a step go: pages, and every token's place in them."""
+    k: Optional[torch.Tensor]
+    v: Optional[torch.Tensor]
+    positions: torch.Tensor
+    token_req: torch.Tensor
+    req_slot: torch.Tensor
+    block_table: torch.Tensor
+    page_size: int
+
+
+def staged_rows(ctx, hkv: int, dim: int, dtype: torch.dtype) -> StepRows:
+    """One page per plane that holds a step's new keys and values [1, kv_heads, tokens, head_dim], token t in row t: what the products'
+    epilogues write into where the cache itself is held in another form."""
+    tokens, device = ctx.n_tokens, ctx.device
+    k, v = torch.empty((2, 1, hkv, tokens, dim), dtype=dtype, device=device)
+    places = ctx.shared.get("staged")
+    if places is None:
+        zeros = torch.zeros(tokens, dtype=torch.int32, device=device)
+        places = ctx.shared["staged"] = (torch.arange(tokens, dtype=torch.int32, device=device), zeros, zeros[:1], zeros[:1].view(1, 1))
+    return StepRows(k, v, *places, tokens)
+
+
+def token_rows(ctx, cache) -> torch.Tensor:
+    """Every token's row in its request's cache: its position, or, of requests that are cut down, the place behind the rows that they
+    have.  Padding rows of a captured step get a negative one."""
+    if cache.mass is None:
+        return ctx.positions
+    rows = ctx.shared.get("token_rows")
+    if rows is None:
+        behind = (ctx.ctx_len - ctx.q_len - ctx.q_start)[ctx.token_req.long()]
+        rows = ctx.shared["token_rows"] = behind + torch.arange(ctx.n_tokens, dtype=torch.int32, device=ctx.device)
+    return rows
+
+
+def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, window) -> torch.Tensor:
+    """Attention of a step's queries over pages held in 4 bits: portions of more than a few tokens by the prompt kernels over the rows written
+    out as values, all others straight over the pages.  Where keys are weighed, what counts are the latest tokens of every
+    portion, a few at most: those run over the pages, too."""
+    out = torch.empty_like(q)
+    few = kernels.INT4_FEW
+    lens, ends = ctx.host.q_len, ctx.host.ctx_len
+    most = max(lens)
+    by_portions = most > few
+    if by_portions:
+        step = ctx.shared.get("int4_portions")
+        if step is None:                     # once per step: which requests bring portions, and the place of each among them
+            which = [r for r, n in enumerate(lens) if n > 1]
+            places = [which.index(r) if n > 1 else 0 for r, n in enumerate(lens)]
+            lists = torch.tensor(which + places, dtype=torch.int32, device=ctx.device)
+            step = ctx.shared["int4_portions"] = (lists[:len(which)], lists[len(which):], max(ends[r] for r in which))
+        if q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS:
+            (tile_req, tile_q0), span = wide_tiles(plan, ctx, hq, window)
+        else:
+            tile_req, tile_q0, span = plan["tile_req"], plan["tile_q0"], kernels.PREFILL_TILE
+        kernels.attn_prefill_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, tile_req, tile_q0, ctx.q_start, ctx.q_len, ctx.ctx_len, step[2],
+                                  cache.page_size, scale, window, span=span, portions=step[:2])
+        if cache.mass is None and not plan.info["n_decode"]:
+            return out
+    q_start, q_len, queries = ctx.q_start, ctx.q_len, 1 if by_portions else most
+    if by_portions and cache.mass is not None:
+        latest = ctx.shared.get("int4_latest")
+        if latest is None:
+            n = ctx.q_len.clamp(max=few)
+            latest = ctx.shared["int4_latest"] = (ctx.q_start + ctx.q_len - n, n)
+        (q_start, q_len), queries = latest, few
+    longest = max(max(c for n, c in zip(lens, ends) if n <= queries or cache.mass is not None), ctx.host.ctx_bound or 0)
+    kernels.attn_decode_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, q_start, q_len, ctx.ctx_len, queries, longest, cache.page_size, scale, window,
+                             mass=cache.mass)
+    return out
 
 
 def decode_ranges(longest_context: int) -> int:

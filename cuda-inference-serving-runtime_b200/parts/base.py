@@ -167,6 +167,13 @@ class Mixer(Part):
     def cache_use(self) -> CacheUse:
         return CacheUse("none")
 
+    def takes_int4(self) -> bool:
+        """Whether `forward` also runs on pages held in 4 bits (`PagedBinding.held`); `int4_jobs`: the libraries it needs then."""
+        return False
+
+    def int4_jobs(self) -> list:
+        return []
+
     def forward(self, h: torch.Tensor, ctx, cache) -> torch.Tensor:
         """h [tokens, hidden] in the compute dtype -> float [tokens, hidden] to add to the residual stream (a part that
         took a `PendingNorm` may instead add its output to `h.stream.x` itself and return None)."""
