@@ -25,8 +25,7 @@ committed by the caller after the step is enqueued (runtime/execution.py:125-126
 
 Pages may hold keys and values in 4 bits (`CacheUse.held`).  With `weigh` every key has a number beside it, the weight that
 attention has given it so far, and a request can be cut down to its weightiest rows (`plan_cut`, `finish_cut`): its rows
-are then fewer than the tokens it has seen (`length` and `seen`), and they lie on pages of their own again, so a page that
-another request shares is never written.
+are then fewer than the tokens it has seen (`length` and `seen`).  No page is shared then: a fork copies them.
 """
 from __future__ import annotations
 
@@ -202,21 +201,29 @@ class CacheManager:
         return slot
 
     def fork(self, source, target) -> int:
-        """`target` starts as a copy of `source`, sharing its pages (copied only when written)."""
+        """`target` starts as a copy of `source`, sharing its pages (copied only when written).  Where keys are weighed every request has
+        pages of its own, since their numbers are written in every step: the copies are queued in `group.copies`."""
         if target in self.requests:
             raise ValueError(f"duplicate sequence {target!r}")
         src = self.requests[source]
         if not self.free_slots:
             raise OutOfPages(f"all {self.max_slots} request slots are in use")
+        for g in self.page_groups:
+            if self.weigh and len(src.tables[g.index]) > g.pool.n_free:
+                raise OutOfPages(f"insufficient KV pages for a copy: {len(src.tables[g.index])} wanted, {g.pool.n_free} free (group {g.index})")
         slot = self.free_slots.pop()
         req = _Request(slot, src.length, src.seen)
         for g in self.page_groups:
             table = list(src.tables[g.index])
+            if self.weigh:
+                table = g.pool.allocate(len(table))
+                g.copies += zip(src.tables[g.index], table)
             req.tables[g.index] = table
             req.first_live[g.index] = src.first_live[g.index]
             for logical, page in enumerate(table):
                 if page >= 0:
-                    g.pool.retain(page)
+                    if not self.weigh:
+                        g.pool.retain(page)
                     g.set_entry(slot, logical, page)
         for g in self.state_groups:
             if g.storage is not None:

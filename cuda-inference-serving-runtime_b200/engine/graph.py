@@ -85,16 +85,19 @@ def _align(n: int) -> int:
 
 
 def keep_states(cache) -> list:
-    """Copies of the per-request state tensors (a recurrent mixer's), taken before a warm-up run outside a graph.  Such a run
-    writes the same keys and values into the pages as the replay after it, which is harmless, but it advances a state that the
-    replay advances again: the state is put back after the warm-up (`put_states_back`)."""
-    return [None if g.storage is None else g.storage.clone() for g in cache.state_groups]
+    """Copies of the per-request state tensors (a recurrent mixer's) and of the keys' weights, taken before a warm-up run outside a graph.
+    Such a run writes the same keys and values into the pages as the replay after it, which is harmless, but it advances a state, or adds
+    to a key's weight, as the replay does again: they are put back after the warm-up (`put_states_back`)."""
+    return [t.clone() for t in _advanced(cache)]
+
+
+def _advanced(cache) -> list:
+    return [t for t in [g.storage for g in cache.state_groups] + [g.mass for g in cache.page_groups] if t is not None]
 
 
 def put_states_back(cache, kept: list) -> None:
-    for g, saved in zip(cache.state_groups, kept):
-        if saved is not None:
-            g.storage.copy_(saved)
+    for tensor, saved in zip(_advanced(cache), kept):
+        tensor.copy_(saved)
 
 
 class DecodeGraph:

@@ -179,6 +179,8 @@ class Stepper:
 
     def fork(self, source, target) -> None:
         self.cache.fork(source, target)
+        if self.cache.weigh:             # before a page of the source goes back
+            run_page_copies(self.cache, self.model.device)
 
     @staticmethod
     def check_kernels() -> None:

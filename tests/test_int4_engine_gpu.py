@@ -147,6 +147,32 @@ def test_a_forked_request_goes_its_own_way():
     assert torch.allclose(again.step([StepEntry("c", [9], [0])]), other, atol=1e-3) and not torch.allclose(one, other, atol=1e-2)
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_fork_of_a_request_that_is_cut(graph):
+    """Source and copy run side by side with the same tokens, and are cut: each has its own numbers beside its keys, and they stay the same."""
+    from cisr_b200 import StepEntry
+    from cisr_b200.engine.step import Keep
+    from cisr_b200.ops import kernels
+
+    model = model_of("bfloat16")
+    mixer = model.layers[0].mixer
+    stepper = stepper_of(model, graph=graph, keep=Keep(rows=24, recent=8, first=2, slack=8))
+    stepper.create("a")
+    stepper.step([StepEntry("a", tokens_of(21))])
+    stepper.fork("a", "b")
+    group = stepper.cache.page_groups[0]
+    for i, t in enumerate(tokens_of(40, 3)):
+        logits = stepper.step([StepEntry(k, [t], [0]) for k in ("a", "b")])
+        assert torch.equal(logits[0], logits[1])
+        stepper.cache.check()
+        n = stepper.cache.length("a")
+        one, other = (torch.cat([group.mass[:, p] for p in stepper.cache.requests[k].tables[0]], -1)[..., :n] for k in ("a", "b"))
+        assert torch.equal(one, other) and n < 32
+        if i < 10:           # not cut yet: every query head has given one in all for each of the portion's latest tokens and each token since
+            given = mixer.hq // mixer.hkv * (min(21, kernels.INT4_FEW) + i + 1)
+            assert ((one.double().sum(-1) - given).abs() < 1e-3 * given).all()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("graph", [False, True])
 def test_requests_that_are_cut(dtype, graph):
