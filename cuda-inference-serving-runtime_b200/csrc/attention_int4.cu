@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
         constexpr int AT_ONCE = 4;                                  // keys of a thread on their way together
         for (int i0 = tid; i0 < n_tiles * TK; i0 += AT_ONCE * THREADS) {
             float* to[AT_ONCE];
-            float w[AT_ONCE], old[AT_ONCE];
+            float w[AT_ONCE];
             const float* score[AT_ONCE];
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
@@ -722,7 +722,6 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 const int logical = there ? a.by_page(key) : 0, at = there && logical < a.width ? pages[logical] : -1;
                 to[u] = at < 0 ? nullptr : a.mass + ((size_t)at * a.hkv + kvh) * a.page_size + key - logical * a.page_size;
                 score[u] = scores + (there ? (size_t)key * a.row_stride : 0);
-                old[u] = to[u] ? *to[u] : 0.f;
                 w[u] = 0.f;
             }
             for (int r = 0; r < span.rows; r += 2) {
@@ -736,7 +735,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
                 }
             }
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) if (to[u] && w[u] != 0.f) *to[u] = old[u] + w[u];
+            for (int u = 0; u < AT_ONCE; ++u) if (to[u] && w[u] != 0.f) atomicAdd(to[u], w[u]);      // (requests may share a page)
         }
     }
 }
@@ -814,7 +813,7 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
         const int key = lo + i * MASS_THREADS + tid;
         if (key >= hi || a.by_page(key) >= a.width) continue;
         const int page = pages[a.by_page(key)];
-        if (page >= 0 && w[i] != 0.f) mass[((size_t)page * a.hkv + kvh) * a.page_size + key % a.page_size] += w[i];
+        if (page >= 0 && w[i] != 0.f) atomicAdd(mass + ((size_t)page * a.hkv + kvh) * a.page_size + key % a.page_size, w[i]);
     }
 }
 

@@ -36,6 +36,12 @@
 // With -DSOFTCAP=1 a score becomes cap tanh(score / cap) before the softmax (`softcap`; ignored otherwise): each thread
 // bends its scores as it takes them from tensor memory.
 //
+// With -DHALF_OPERANDS=1 all operands are float16 instead of bfloat16, for keys and values that were written out of a cache in 4 bits
+// (three binary digits times eleven: bfloat16 would cut six of them).  Rows of queries come times a power of two, and a key head's keys and its
+// values, too, so that each has its largest magnitude below 2^15; `q_factor` [tokens][hq] and `kv_factor` [request][kv head][2]
+// are what takes those out again, of the scores' scale and of the finished rows.  P is held times 2^6, which keeps it below 2^14 and
+// loses no key of more than 2^-31 of a row's largest weight.
+//
 // Every wait on an mbarrier is bounded; a role whose wait ran out raises the CTA's abort flag and the device flag
 // (5), the other roles leave at their next wait, tensor memory is freed, and the host reports the failure.
 //
@@ -53,9 +59,30 @@
 #error "the tcgen05 attention takes head sizes 64 and 128"
 #endif
 
+#ifndef HALF_OPERANDS
+#define HALF_OPERANDS 0
+#endif
+#if HALF_OPERANDS && SOFTCAP
+#error "float16 operands have no bent scores"
+#endif
+#if HALF_OPERANDS
+#include <cuda_fp16.h>
+#endif
+
 namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int D = HEAD_DIM;
+constexpr float P_SHIFT = HALF_OPERANDS ? 6.f : 0.f;         // P is held times 2 to it
+// two operands; and the instruction descriptor's bits for their types
+__device__ __forceinline__ uint32_t pack_operands(float a, float b) {
+#if HALF_OPERANDS
+    const __half2 pair = __floats2half2_rn(a, b);
+#else
+    const __nv_bfloat162 pair = __floats2bfloat162_rn(a, b);
+#endif
+    return *reinterpret_cast<const uint32_t*>(&pair);
+}
+constexpr uint32_t typed(uint32_t idesc) { return HALF_OPERANDS ? idesc & ~((1u << 7) | (1u << 10)) : idesc; }
 constexpr int NSUB = D / 64;                  // 64-column sub-tiles of Q, K and V rows
 constexpr int BN = 128;                       // keys per tile
 constexpr int SUB_BYTES = 128 * 128;          // one 128-row x 64-column sub-tile (queries)
@@ -114,7 +141,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                             const int* __restrict__ tile_req, const int* __restrict__ tile_q0, int span,
                             const int* __restrict__ q_start, const int* __restrict__ q_len,
                             const int* __restrict__ ctx_len, int hq, int hkv, int page_size, float scale, float softcap, int window,
-                            int keep_first, float sink_all, const float* __restrict__ sink_heads, int* __restrict__ error) {
+                            int keep_first, float sink_all, const float* __restrict__ sink_heads, int* __restrict__ error,
+                            const float* __restrict__ q_factor, const float* __restrict__ kv_factor) {
     CISR_TRACE_SCOPE(TRACE_ATTN_PREFILL);
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -261,8 +289,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     } else if (warp < FIRST_SOFTMAX_WARP) {
         // ------------------------------------------------------------ products
         // The whole warp walks the tiles and looks at the barriers; one lane issues.
-        constexpr uint32_t idesc_s = umma_idesc(BN);
-        constexpr uint32_t idesc_o = umma_idesc(D) | UMMA_B_MN_MAJOR;
+        constexpr uint32_t idesc_s = typed(umma_idesc(BN));
+        constexpr uint32_t idesc_o = typed(umma_idesc(D)) | UMMA_B_MN_MAJOR;
         const bool clean_last = tile_k0(n_tiles - 1) + BN > k_end;
         // descriptor addresses count 16 bytes; every tile lies below 256 KB, so the sums stay inside the field
         const uint64_t desc_q0 = umma_desc(Qs), desc_q1 = umma_desc(Qs1), desc_k0 = umma_desc(Kring), desc_v0 = umma_desc_mn_major(Vring, KV_SUB);
@@ -343,7 +371,14 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const uint32_t tmem_own = tmem_base + TMEM_O + lane_base + (uint32_t)(stream * D);     // this thread's row of its accumulator
         const uint32_t s_addr = tmem_base + lane_base + (uint32_t)(stream * BN);
         const uint32_t p_addr = OWN_P ? tmem_base + TMEM_P + lane_base + (uint32_t)(stream * 64) : s_addr;
-        const float scale2 = SOFTCAP ? 1.f : scale * LOG2E;        // bent scores come in base-2 units
+        float scale2 = SOFTCAP ? 1.f : scale * LOG2E;              // bent scores come in base-2 units
+        float v_factor = 1.f;
+        if (HALF_OPERANDS) {
+            const int mine = (shared ? 0 : stream * BM) + row;
+            const float* of_head = kv_factor + ((size_t)req_slot[req] * hkv + kvh) * 2;
+            scale2 *= (mine < rows ? q_factor[(size_t)(tok0 + mine) * hq + head] : 0.f) * of_head[0];
+            v_factor = of_head[1];
+        }
         // bent scores lie in (-cap, cap): where 2^(cap log2 e) is far from a float's range they need no running max, and
         // every exponential is taken against 0
         const bool bounded = SOFTCAP && softcap * LOG2E <= 60.f;
@@ -450,9 +485,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 }
             }
             const float m_ref = m_used == -INFINITY ? 0.f : m_used;
-            const uint64_t scale_pair = pack2(scale2, scale2), minus_m = pack2(-m_ref, -m_ref);
+            const uint64_t scale_pair = pack2(scale2, scale2), minus_m = pack2(P_SHIFT - m_ref, P_SHIFT - m_ref);
             uint64_t sums[2] = {0, 0};
-            // P = 2^(s - m) of 32 columns, rounded to bfloat16 for the product; the sum keeps the unrounded values
+            // P = 2^(s - m) of 32 columns, rounded to an operand's type for the product; the sum keeps the unrounded values
             auto powers = [&](int c0, uint32_t* v) {
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
@@ -461,8 +496,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     p0 = fast_exp2(p0);                             // -inf (masked) gives 0
                     p1 = fast_exp2(p1);
                     sums[(c >> 1) & 1] = add2(sums[(c >> 1) & 1], pack2(p0, p1));
-                    __nv_bfloat162 pair = __floats2bfloat162_rn(p0, p1);
-                    v[c >> 1] = *reinterpret_cast<uint32_t*>(&pair);
+                    v[c >> 1] = pack_operands(p0, p1);
                 }
                 tmem_store16_nowait(p_addr + (c0 >> 1), v);
             };
@@ -507,9 +541,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             const int mine = stream * BM + row;
             if (all_ok) {
                 float total = l;
-                if (total > 0.f && sink > -INFINITY) total += exp2f(sink * LOG2E - m_used);   // the sink: one more term of the denominator, no value
+                if (total > 0.f && sink > -INFINITY) total += exp2f(sink * LOG2E - m_used + P_SHIFT);   // the sink: one more term of the denominator, no value
                 const bool some = m_used != -INFINITY;             // a key in sight (NaN and infinite scores pass through)
-                const float inv = fabsf(m_used) < INFINITY ? 1.f / total : NAN;
+                const float inv = fabsf(m_used) < INFINITY ? v_factor / total : NAN;
                 bf16* dst = out + ((size_t)(tok0 + mine) * hq + head) * D;
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
@@ -543,8 +577,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 const float m0 = exchange[row], m1 = exchange[BM + row], m = fmaxf(m0, m1);
                 const float w0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m), w1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m);
                 float total = exchange[2 * BM + row] * w0 + exchange[3 * BM + row] * w1;
-                if (total > 0.f && sink > -INFINITY) total += exp2f(sink * LOG2E - m);
-                const float inv = total > 0.f ? 1.f / total : 0.f;
+                if (total > 0.f && sink > -INFINITY) total += exp2f(sink * LOG2E - m + P_SHIFT);
+                const float inv = total > 0.f ? v_factor / total : 0.f;
                 const float f0 = w0 * inv, f1 = w1 * inv;
                 const uint32_t tmem_o = tmem_base + TMEM_O + lane_base;
                 bf16* dst = out + ((size_t)(tok0 + row) * hq + head) * D;
@@ -610,13 +644,15 @@ CISR_EXPORT int cisr_attn_tcgen05_ok(int page_size) {
     return page_size > 0 && page_size % 8 == 0 && (BN % page_size == 0 || page_size % BN == 0);
 }
 
-// Attention of portions: q, out [n_tokens, hq, D]; tiles of `span` (128 or 256) queries given as (request, first query) pairs.
+// Attention of portions: q, out [n_tokens, hq, D] (out always bfloat16; q_factor and kv_factor with float16 operands, else null); tiles of `span` (128 or 256) queries given as (request, first query) pairs.
 CISR_EXPORT int cisr_attn_prefill_tcgen05(const void* q, void* out, int n_tokens, const void* k_cache, const void* v_cache,
                                           int n_pages, const int* req_slot, const int* block_table, int table_width,
                                           const int* tile_req, const int* tile_q0, int n_tiles, int span, const int* q_start,
                                           const int* q_len, const int* ctx_len, int hq, int hkv, int page_size, float scale, float softcap,
-                                          int window, int keep_first, float sink, const float* sink_heads, void* stream) {
+                                          int window, int keep_first, float sink, const float* sink_heads, const float* q_factor, const float* kv_factor,
+                                          void* stream) {
     if (n_tiles <= 0) return 0;
+    if (HALF_OPERANDS != (q_factor && kv_factor)) return -2;
     if (!g_encode || !g_error) return -13;
     if (hq % hkv || (span != BM && span != 2 * BM) || !cisr_attn_tcgen05_ok(page_size) || (SOFTCAP ? !(softcap > 0.f) : softcap != 0.f)) return -2;
     const long long cache_rows = (long long)n_pages * hkv * page_size;
@@ -637,5 +673,5 @@ CISR_EXPORT int cisr_attn_prefill_tcgen05(const void* q, void* out, int n_tokens
     }
     return launch_kernel(attn_prefill_tcgen05_kernel, dim3((unsigned)n_tiles * hq), dim3(THREADS), smem, (cudaStream_t)stream, g_pdl, map_q,
                          map_k, map_v, (bf16*)out, (int)cache_rows, req_slot, block_table, table_width, tile_req, tile_q0, span,
-                         q_start, q_len, ctx_len, hq, hkv, page_size, scale, softcap, window, keep_first, sink, sink_heads, g_error);
+                         q_start, q_len, ctx_len, hq, hkv, page_size, scale, softcap, window, keep_first, sink, sink_heads, g_error, q_factor, kv_factor);
 }

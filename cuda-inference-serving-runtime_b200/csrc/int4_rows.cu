@@ -68,6 +68,15 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* x) {
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
+__device__ __forceinline__ void store8(__half* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 two = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 __device__ __forceinline__ __half step_of(uint32_t top) {
     if (top >= 0x7f800000u) return __ushort_as_half((unsigned short)0x7e00u);
@@ -187,7 +196,7 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
     }
 }
 
-// One thread block row of the grid for the keys (blockIdx.y 0), one for the values.  us with 8192 tokens of 8 heads of 128: see int4_store.
+// One thread block row of the grid for the keys (blockIdx.y 0), one for the values.
 template <int D, typename T>
 __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_token, long long k_head, long long v_token,
                                                              long long v_head, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
@@ -201,11 +210,12 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 }
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
-// request's end, give zeros.
+// request's end, give zeros.  float16 (three binary digits times eleven, rounded to eleven): divided by the key head's factor (int4_prompt_kernel).
 constexpr int READ_ROWS = 4;         // of a thread, on their way together
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
-                                          const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv, int unit) {
+                                          const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
+                                          int tokens, int hkv, int unit) {
     constexpr int NG = D / 32;
     const int lane = threadIdx.x % LANES;
     const int first = unit * READ_ROWS * (THREADS / LANES) + threadIdx.x / LANES;
@@ -248,10 +258,12 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
         if (token[i] < 0) continue;
         T* to = out + (ends ? blockIdx.y * req_stride : 0) + token[i] * token_stride + head[i] * head_stride;
         if (VALUES) from_value_order<NG>(code[i].w);
+        float inverse = 1.f;
+        if constexpr (std::is_same<T, __half>::value) inverse = 1.f / factors[((size_t)blockIdx.y * hkv + head[i]) * 2 + VALUES];
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
             const uint32_t two = VALUES ? held[i].w[j] : held[i].w[j / 2];
-            const float step = __half2float(__ushort_as_half((unsigned short)((VALUES ? pos[i] & 1 : j & 1) ? two >> 16 : two & 0xffff)));
+            const float step = __half2float(__ushort_as_half((unsigned short)((VALUES ? pos[i] & 1 : j & 1) ? two >> 16 : two & 0xffff))) * inverse;
             float x[PER];            // 2^23 + n as a float, less 2^23 + 8
 #pragma unroll
             for (int e = 0; e < PER; ++e)
@@ -264,14 +276,78 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
 template <int D, typename T>
 __global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
                                                             T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
-                                                            Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, int tokens, int hkv) {
+                                                            Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
+                                                            int tokens, int hkv) {
     pdl_wait();
     const long long rows = (long long)tokens * hkv;
     constexpr int EACH = READ_ROWS * (THREADS / LANES);
     const int key_units = (int)((rows + EACH - 1) / EACH);
-    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x);
-    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, tokens, hkv, blockIdx.x - key_units);
+    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x);
+    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x - key_units);
     pdl_trigger();
+}
+
+// What a prompt's attention with float16 operands needs before its rows are written out: a power of two for each request's key head, keys and
+// values apart, which brings the largest of them to 2^14 .. 2^15 (a thread block reads all its steps, 1/9 of what is held); and the
+// queries [rows][D] as float16, each row times a power of two to the same end, which is taken back by its factor.  NaN is left out of a largest
+// one, and stays NaN.
+constexpr int PROMPT_THREADS = 512;
+template <int D>
+__global__ void __launch_bounds__(PROMPT_THREADS) int4_prompt_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
+                                                                     const int* __restrict__ req_slot, Pages pages, const int* __restrict__ ends, const int* __restrict__ which,
+                                                                     float* __restrict__ factors, int n_req, const uint4* __restrict__ q, uint4* __restrict__ q_half,
+                                                                     float* __restrict__ q_factor, long long q_rows) {
+    constexpr int NG = D / 32, PARTS = D / 8;                       // threads that share a row of queries
+    __shared__ uint32_t of_warp[PROMPT_THREADS / 32];
+    pdl_wait();
+    const int heads = n_req * pages.hkv, tid = threadIdx.x;
+    if ((int)blockIdx.x < 2 * heads) {
+        const bool values = (int)blockIdx.x >= heads;
+        const int unit = blockIdx.x - (values ? heads : 0), i = unit / pages.hkv, head = unit - i * pages.hkv;
+        const int req = which ? which[i] : i, slot = req_slot[req], end = ends[req];
+        const unsigned char* cache = values ? v_cache : k_cache;
+        uint32_t top = 0;
+        for (int c = tid; c < (end + INT4_BLOCK - 1) / INT4_BLOCK * NG; c += PROMPT_THREADS) {      // eight steps each
+            const int row0 = c / NG * INT4_BLOCK, part = c % NG;
+            const long long block = int4_block_at(pages, slot, row0, head);
+            if (block < 0) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(cache + block * int4_block_bytes(D) + 4 * D + 16 * part);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = 8 * part + e, row = row0 + (values ? at / (2 * NG) * 2 + (at & 1) : at / NG);
+                const uint32_t s = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffff;
+                if (row < end && s < 0x7c00u) top = max(top, s);
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (tid % 32 == 0) of_warp[tid / 32] = top;
+        __syncthreads();
+        if (tid < 32) {
+            top = __reduce_max_sync(0xffffffffu, tid < PROMPT_THREADS / 32 ? of_warp[tid] : 0u);
+            const float most = 7.f * __half2float(__ushort_as_half((unsigned short)top));           // 2^-22 .. 2^19
+            const int exponent = top ? (int)(__float_as_uint(most) >> 23) - 127 - 14 : 0;
+            if (tid == 0) factors[((size_t)i * pages.hkv + head) * 2 + values] = __uint_as_float((uint32_t)(exponent + 127) << 23);
+        }
+        return;
+    }
+    const long long at = (long long)(blockIdx.x - 2 * heads) * PROMPT_THREADS + tid, row = at / PARTS;
+    const bool there = row < q_rows;
+    const uint4 v = there ? q[at] : make_uint4(0, 0, 0, 0);
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t top = largest<8>(x);
+#pragma unroll
+    for (int o = 1; o < PARTS; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int exponent = min(14 - ((int)(top >> 23) - 127), 120);
+    const float up = __uint_as_float((uint32_t)(exponent + 127) << 23);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 two = __floats2half2_rn(widened(x, 2 * i) * up, widened(x, 2 * i + 1) * up);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    if (there) q_half[at] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (there && at % PARTS == 0) q_factor[row] = __uint_as_float((uint32_t)(127 - exponent) << 23);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -502,10 +578,34 @@ CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k
         constexpr int D = decltype(d)::value;
         if (dtype == CISR_F32)
             return launch_kernel(int4_read_kernel<D, float>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
-                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, tokens, hkv);
+                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, (const float*)nullptr, tokens, hkv);
         return launch_kernel(int4_read_kernel<D, __nv_bfloat16>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
-                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, tokens, hkv);
+                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, (const float*)nullptr, tokens, hkv);
     });
+}
+
+// For a prompt's attention with float16 operands (head sizes 64 and 128): places 0 .. rows - 1 of n_req requests (request which[i], or i without a list) into
+// k, v float16 [n_req][hkv][rows][dim] over `factors` [n_req][hkv][2], and queries bfloat16 [q_rows][dim] into q_half over q_factor [q_rows].
+CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void* k, void* v, float* factors, const void* q, void* q_half, float* q_factor, long long q_rows,
+                                 const int* req_slot, const int* block_table, int width, int page_size, const int* ends, const int* which, int n_req, int rows, int hkv, int dim,
+                                 void* stream) {
+    if (rows <= 0 || n_req <= 0) return 0;
+    if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535 || (long long)rows * hkv >= 1ll << 30) return -2;
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_half) & 15) return -2;
+    const Pages pages = pages_of(block_table, width, page_size, hkv);
+    const Place at{nullptr, nullptr, req_slot, pages, Divider((uint32_t)hkv)};
+    const dim3 grid((unsigned)units((long long)rows * hkv, READ_ROWS * (THREADS / LANES)), (unsigned)n_req);
+    const auto run = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        const long long blocks = 2ll * n_req * hkv + (q_rows * (D / 8) + PROMPT_THREADS - 1) / PROMPT_THREADS;
+        if (blocks >= 1ll << 31) return -2;
+        const int status = launch_kernel(int4_prompt_kernel<D>, dim3((unsigned)blocks), dim3(PROMPT_THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
+                                         (const unsigned char*)v_cache, req_slot, pages, ends, which, factors, n_req, (const uint4*)q, (uint4*)q_half, q_factor, q_rows);
+        if (status) return status;
+        return launch_kernel(int4_read_kernel<D, __half>, grid, dim3(THREADS), 0, (cudaStream_t)stream, true, (const unsigned char*)k_cache, (const unsigned char*)v_cache, (__half*)k,
+                             (__half*)v, (long long)hkv * rows * D, (long long)D, (long long)rows * D, at, Divider((uint32_t)rows), ends, which, (const float*)factors, rows, hkv);
+    };
+    return dim == 64 ? run(std::integral_constant<int, 64>()) : dim == 128 ? run(std::integral_constant<int, 128>()) : -2;
 }
 
 // Places that stay into kept [n_req][hkv][keep] (-1 behind the last), their rows and sums to the pages of to_table [n_req][to_width].
@@ -519,7 +619,7 @@ CISR_EXPORT int cisr_int4_evict(void* k_cache, void* v_cache, float* mass, const
     const int between = longest - recent - first;
     const int cached = between < 0 ? 0 : between < SELECT_CACHED ? between : SELECT_CACHED;
     const size_t smem = sizeof(uint32_t) * (size_t)(cached < SELECT_CACHED ? cached : SELECT_CACHED);
-    if (smem > 48 * 1024) {
+    if (smem > 32 * 1024) {          // with the counts more than the 48 KB that need no leave
         const cudaError_t e = cudaFuncSetAttribute(int4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(uint32_t) * SELECT_CACHED));
         if (e != cudaSuccess) return (int)e;
     }

@@ -393,16 +393,17 @@ def _attention_float(head_dim: int, softcap: bool = False):
 _attention_tcgen05_libs = {}
 
 
-def _attention_tcgen05(head_dim: int, softcap: bool = False):
-    lib = _attention_tcgen05_libs.get((head_dim, softcap))
+def _attention_tcgen05(head_dim: int, softcap: bool = False, half: bool = False):
+    """`half`: with float16 operands and a power of two to each row of queries and each key head (a cache in 4 bits)."""
+    lib = _attention_tcgen05_libs.get((head_dim, softcap, half))
     if lib is None:
-        lib = load_library("attention_tcgen05.cu", {"HEAD_DIM": head_dim, **({"SOFTCAP": 1} if softcap else {})})
+        lib = load_library("attention_tcgen05.cu", {"HEAD_DIM": head_dim, **({"SOFTCAP": 1} if softcap else {}), **({"HALF_OPERANDS": 1} if half else {})})
         for name in ("cisr_attn_prefill_tcgen05", "cisr_attn_tcgen05_init", "cisr_attn_tcgen05_ok", "cisr_attn_tcgen05_tile"):
             getattr(lib, name).restype = ctypes.c_int
         assert lib.cisr_attn_tcgen05_tile() == WIDE_TILE
         _check(lib.cisr_attn_tcgen05_init(_p(_error_flag())), "tcgen05 attention init", own=0)
         lib.cisr_attn_tcgen05_set_pdl(int(_pdl_state["on"]))
-        _attention_tcgen05_libs[(head_dim, softcap)] = lib
+        _attention_tcgen05_libs[(head_dim, softcap, half)] = lib
     return lib
 
 
@@ -444,7 +445,7 @@ def attn_prefill_wide(q, out, k_cache, v_cache, req_slot, block_table, wide_req,
     _check(lib.cisr_attn_prefill_tcgen05(_p(q), _p(out), q.shape[0], _p(k_cache), _p(v_cache), k_cache.shape[0], _p(req_slot),
                                          _p(block_table), block_table.shape[1], _p(wide_req), _p(wide_q0), wide_req.numel(),
                                          span, _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, page_size, scale,
-                                         _softcap(softcap), int(window or 0), int(keep_first or 0), *_sink(sink, hq), _stream()), "attn_prefill_wide")
+                                         _softcap(softcap), int(window or 0), int(keep_first or 0), *_sink(sink, hq), 0, 0, _stream()), "attn_prefill_wide")
 
 
 PREFILL_TILE = 64
@@ -538,7 +539,9 @@ _attention_int4_calls = {}       # by the sizes of a call: the function, the flo
 
 def int4_jobs(head_dim: int, dtype: torch.dtype):
     """The build jobs of a 4-bit cache for this head size and type of queries."""
-    return [("int4_rows.cu", {}, ()), ("attention_int4.cu", {"HEAD_DIM": head_dim, "STORAGE_BF16": dtype_code(dtype)}, ())]
+    half = dtype == torch.bfloat16 and head_dim in TCGEN05_HEAD_DIMS
+    return ([("int4_rows.cu", {}, ()), ("attention_int4.cu", {"HEAD_DIM": head_dim, "STORAGE_BF16": dtype_code(dtype)}, ())]
+            + ([("attention_tcgen05.cu", {"HEAD_DIM": head_dim, "HALF_OPERANDS": 1}, ())] if half else attention_tcgen05_jobs(head_dim, torch.float32)))
 
 
 def _int4_rows():
@@ -613,7 +616,7 @@ def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
                req_slot: torch.Tensor, block_table: torch.Tensor, page_size: int, mass: Optional[torch.Tensor] = None) -> None:
     """Bring new keys and values k, v [tokens, kv_heads, head_dim] (any strides between rows) into a 4-bit cache: token t becomes row
     positions[t] of request token_req[t].  k_cache, v_cache: uint8 [pages, kv_heads, int4_page_bytes]; a row whose page
-    the table does not have is left out.  `mass` float [pages, kv_heads, page_size] (`attn_decode_int4`): the new rows' numbers become 0.
+    the table does not have is left out, and no two tokens of a call may go to the same place.  `mass` float [pages, kv_heads, page_size] (`attn_decode_int4`): the new rows' numbers become 0.
 
     A value is held as c s: s the largest magnitude of its group of 32 neighbours over 7, in float16 (65504 at most: magnitudes beyond
     458,528 are cut there), c the whole number nearest to x / s, so it is off by half of s and the rounding of s itself.  A
@@ -661,7 +664,9 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
         _int4_lists("int4_expand", device, block_table, n, ("req_slot", "ctx_len"), (req_slot, ctx_len))
     else:
         _int4_lists("int4_expand", device, block_table, n, ("req_slot", "requests"), (req_slot, requests))
-        _need(ctx_len, torch.int32, "ctx_len", 1)
+        _int4_lists("int4_expand", device, block_table, req_slot.numel(), ("ctx_len",), (ctx_len,))
+    if requests is None and req_slot.numel() < n:
+        raise KernelError(f"int4_expand: req_slot has {req_slot.numel()} entries for {n} requests")
     _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), hkv * rows * dim, dim, rows * dim, 0, 0,
                                        _p(req_slot), _p(block_table), block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()),
            "int4_expand")
@@ -676,7 +681,8 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     flag that `raise_if_kernel_gave_up` reads).  window, sink, keep_first: as for `attn_decode`.
 
     `mass` float [pages, kv_heads, page_size]: every key's number grows by the weights that the query heads of its key head, and all of
-    the request's new tokens, have given it (a sink takes its part of them)."""
+    the request's new tokens, have given it (a sink takes its part of them).  The same call gives the same numbers, unless requests of
+    it share a page: that grows by the weights of each, in no certain order."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     tokens, hq, dim = q.shape
     hkv, device = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
@@ -706,16 +712,18 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
                       tile_req: torch.Tensor, tile_q0: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, longest: int, page_size: int,
                       scale: float, window: Optional[int] = None, sink=None, keep_first: int = 0, span: int = PREFILL_TILE,
                       portions: Optional[tuple] = None) -> None:
-    """Attention of portions of prompts over a 4-bit cache: the requests' rows are written out as values once, and the prompt attention
-    of the queries' type runs over those, so codes are turned into operands once per key and not once per tile of queries.
-    Tiles of `span` queries as (request, first query): 64 as for `attn_prefill`, 128 or 256 (bfloat16, head sizes 64 and 128) as for
-    `attn_prefill_wide`.  `longest`: no request that is written out has more rows.  `portions` (requests, places): the requests
-    that are written out, and for every request of the step its place in that list (any number for the others); None: all, in order."""
+    """Attention of portions of prompts over a 4-bit cache: the requests' rows are written out as values once, and a prompt attention
+    runs over those, so codes are turned into operands once per key and not once per tile of queries.
+    Tiles of `span` queries as (request, first query): 128 or 256 (bfloat16, head sizes 64 and 128) as for `attn_prefill_wide`, with float16
+    operands, whose eleven binary digits are those of a held value; 64 (any) as for `attn_prefill`, with float ones.  `longest`: no
+    request that is written out has more rows.  `portions` (requests, places): the requests that are written out, and for every
+    request of the step its place in that list (any number for the others); None: all, in order.  A held value that is NaN reaches
+    the queries before it, too, as it does in those."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     hq, dim = q.shape[1], q.shape[2]
     hkv, device = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
     n_all = q_len.numel()
-    if longest < 1 or hq % hkv or out.shape != q.shape or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.get_device() != device:
+    if longest < 1 or hq % hkv or out.shape != q.shape or req_slot.numel() < n_all or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.get_device() != device:
         raise KernelError("attn_prefill_int4: heads, limits, shapes, devices or the span disagree")
     requests, places = (None, None) if portions is None else portions
     n = n_all if requests is None else requests.numel()
@@ -723,14 +731,28 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         places = torch.arange(n, dtype=torch.int32, device=q.device)
     _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS + ("places",), (req_slot, q_start, q_len, ctx_len, places))
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
-    k, v = torch.empty((2, n, hkv, rows, dim), dtype=q.dtype, device=q.device)
-    int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
     table = places.view(-1, 1) if requests is None else torch.arange(n, dtype=torch.int32, device=q.device).view(-1, 1)
     if span == PREFILL_TILE:
-        attn_prefill(q, out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first)
-    else:
-        attn_prefill_wide(q, out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first,
-                          span=span)
+        k, v = torch.empty((2, n, hkv, rows, dim), device=q.device)
+        int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
+        wide, wide_out = q.float(), out.float()                  # themselves where they are float; rows of other requests stay as they are
+        attn_prefill(wide, wide_out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first)
+        if wide_out is not out:
+            out.copy_(wide_out)
+        return
+    if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
+        raise KernelError(f"attn_prefill_int4: tiles of {span} queries are for bfloat16 and head sizes {TCGEN05_HEAD_DIMS}")
+    for name, t in (("tile_req", tile_req), ("tile_q0", tile_q0)):
+        _need(t, torch.int32, name)
+    lib = _attention_tcgen05(dim, half=True)
+    k, v = torch.empty((2, n, hkv, rows, dim), dtype=torch.float16, device=q.device)
+    halves, factors = torch.empty(q.shape, dtype=torch.float16, device=q.device), torch.empty(n * hkv * 2 + q.shape[0] * hq, device=q.device)
+    q_factor = factors[n * hkv * 2:]
+    _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), _p(k), _p(v), _p(factors), _p(q), _p(halves), _p(q_factor), q.shape[0] * hq, _p(req_slot), _p(block_table),
+                                         block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()), "attn_prefill_int4", own=2)
+    _check(lib.cisr_attn_prefill_tcgen05(_p(halves), _p(out), q.shape[0], _p(k), _p(v), n, _p(places), _p(table), 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
+                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), _p(q_factor),
+                                         _p(factors), _stream()), "attn_prefill_int4")
 
 
 def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,

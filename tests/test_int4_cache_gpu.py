@@ -392,6 +392,13 @@ def test_weights_of_keys(hq, hkv, dim, window, sink, dtype):
 
 
 # ------------------------------------------------------------------ portions of prompts
+def prompt_bound(dtype, span):
+    """Beside `bound`, of the outputs' sizes: float operands (tiles of 64) are exact.  float16 ones are three binary digits of a code times
+    eleven of a step, rounded to eleven, 2^-12: of values once, of keys in scores with terms of 70 units at most, which a weight and the sum
+    that it is divided by are off by; and probabilities are rounded so, as they are in `bound`."""
+    return 0 if span == 64 else 2.0 ** -12 + 2 * 70 * 2.0 ** -12
+
+
 @pytest.mark.parametrize("hq,hkv,dim,dtype,span", [(8, 2, 64, torch.bfloat16, 128), (8, 2, 128, torch.bfloat16, 256), (6, 2, 96, torch.bfloat16, 64), (8, 4, 32, torch.bfloat16, 64),
                                                    (9, 3, 64, torch.float32, 64), (4, 1, 128, torch.float32, 64)])
 @pytest.mark.parametrize("window,keep_first", [(None, 0), (70, 6)])
@@ -405,8 +412,7 @@ def test_portions(hq, hkv, dim, dtype, span, window, keep_first):
         pairs = [(r, a) for r in which for a in range((q_len[r] - 1) // span * span, -1, -span)]
         return i32([r for r, _ in pairs]), i32([a for _, a in pairs])
 
-    # the prompt kernels round probabilities to bfloat16: one more half step of it
-    extra = 0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    extra = prompt_bound(dtype, span)
     for which in (range(4), (3, 1)):
         out = torch.full_like(q, 7.0)
         places = i32([which.index(r) if r in which else -9 for r in range(4)])
@@ -420,9 +426,34 @@ def test_portions(hq, hkv, dim, dtype, span, window, keep_first):
                 assert (got == 7).all()
                 continue
             want, size, _ = plain.attention(q[starts[r]:starts[r] + q_len[r]], *cache.held(r), dim ** -0.5, plain.seen(q_len[r], lens[r], window, keep_first))
-            # values are whole codes of at most 3 binary digits times a step of 11: rounded once more as bfloat16 operands
             off = (got.double() - want).abs()
-            assert (off <= bound(dtype, want, size) + (2 * extra + (0 if dtype == torch.float32 else 70 * 2.0 ** -8 * 2 ** -1)) * size).all(), float((off / size).max())
+            assert (off <= bound(dtype, want, size) + extra * size).all(), float((off / size).max())
+
+
+@pytest.mark.parametrize("dim,span", [(64, 128), (128, 256), (32, 64)])
+@pytest.mark.parametrize("size,query", [(1e-4, 1.5), (1e-2, 1e-20), (30.0, 1e18), (4e5, 1e4)])
+def test_portions_of_any_size(dim, span, size, query):
+    """Values and queries far from 1, some rows of them much smaller than the rest, and one request of zeros."""
+    hq, hkv = 4, 2
+    lens, q_len = [300, 130, 40], [200, 130, 40]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = [torch.randn((n, hkv, dim), generator=g, device="cuda") for n in lens]
+    v = [torch.randn((n, hkv, dim), generator=g, device="cuda") * size / 4 for n in lens]
+    v[0][:100] *= 1e-2
+    k[2].zero_(); v[2].zero_()
+    cache = Cache(lens, hkv, dim, 16, k=k, v=v)
+    q = queries(sum(q_len), hq, dim, torch.bfloat16, std=query)
+    q[3::7] *= 2.0 ** -10
+    starts = [0, 200, 330]
+    pairs = [(r, a) for r in range(3) for a in range(0, q_len[r], span)]
+    out = torch.empty_like(q)
+    kernels.attn_prefill_int4(q, out, cache.k_cache, cache.v_cache, cache.slots, cache.table, i32([r for r, _ in pairs]), i32([a for _, a in pairs]), i32(starts), i32(q_len),
+                              cache.ctx, 300, 16, dim ** -0.5 / query * 1.5, sink=0.3, span=span)
+    for r, n in enumerate(q_len):
+        rows = slice(starts[r], starts[r] + n)
+        want, weight, _ = plain.attention(q[rows], *cache.held(r), dim ** -0.5 / query * 1.5, plain.seen(n, lens[r]), 0.3)
+        off = (out[rows].double() - want).abs()
+        assert (off <= bound(torch.bfloat16, want, weight) + prompt_bound(torch.bfloat16, span) * weight + 1e-30).all(), (r, float((off / weight).max()))
 
 
 # ------------------------------------------------------------------ eviction
@@ -484,6 +515,31 @@ def test_eviction_of_long_requests():
         assert torch.equal(kept[0, 0].long(), want) and kept[1, 0, :301].tolist() == list(range(300)) + [-1]
 
 
+@pytest.mark.parametrize("n", [9000, 10300, 11500, 12300, 13000])
+def test_sums_that_nearly_fill_the_shared_memory_of_a_plain_launch(n):
+    x = torch.zeros((n, 1, 32), device="cuda")
+    cache = Cache([n], 1, 32, 64, spare=4, k=[x], v=[x])
+    mass = torch.rand((cache.pages, 1, 64), device="cuda")
+    sums = torch.cat([mass[p] for p in cache.table[0].tolist()], 1)[0, :n]
+    _, kept = evict(cache, mass, 100, 0, 0)
+    assert torch.equal(kept[0, 0].long(), sums.topk(100).indices.sort().values)
+
+
+def test_a_page_of_two_requests_gets_the_weights_of_both():
+    """One request twice in a call: every weight counts twice, whatever order they come in."""
+    lens = [700, 700]
+    cache = Cache(lens, 2, 64, 16, spare=90)
+    cache.table[1] = cache.table[0]
+    cache.k[1], cache.v[1] = cache.k[0], cache.v[0]
+    cache.store(0, 0, cache.k[0], cache.v[0])
+    for n in (1, 3):                                             # by the kernel itself, and by one of its own
+        q = queries(n, 8, 64, torch.bfloat16)
+        once, twice = torch.zeros((2, cache.pages, 2, 16), device="cuda")
+        cache.attend(q, [n, 0], mass=once)
+        out = cache.attend(torch.cat((q, q)), [n, n], mass=twice)
+        assert torch.equal(out[:n], out[n:]) and torch.equal(twice, 2 * once)
+
+
 def test_a_shared_page_is_not_written():
     """Two requests with the same pages, cut by different rows; the old pages stay as they were."""
     cache = Cache([64, 64], 2, 64, 16, spare=8)
@@ -494,6 +550,90 @@ def test_a_shared_page_is_not_written():
     to, kept = evict(cache, mass, 30, 5, 1)
     old = cache.table[0].tolist()
     assert torch.equal(cache.k_cache[old], k0[old]) and torch.equal(kept[0], kept[1])
+
+
+# ------------------------------------------------------------------ refusals (all by the host, before anything is launched)
+def calls(**change):
+    """Every entry point with good arguments but for the changed ones."""
+    n, hq, hkv, dim, page = 2, 4, 2, 64, 16
+    a = dict(hq=hq, q=queries(n, hq, dim, torch.bfloat16), out=queries(n, hq, dim, torch.bfloat16), k=queries(n, hkv, dim, torch.bfloat16), v=queries(n, hkv, dim, torch.bfloat16),
+             k_cache=torch.zeros((6, hkv, kernels.int4_page_bytes(page, dim)), dtype=torch.uint8, device="cuda"), slots=i32([0, 1]), table=i32([[0, 1], [2, 3]]),
+             req=i32([0, 1]), pos=i32([0, 1]), starts=i32([0, 1]), lens=i32([1, 1]), ctx=i32([20, 5]), most=1, longest=32, page=page, window=None, keep_first=0, sink=None,
+             mass=torch.zeros((6, hkv, page), device="cuda"), to=i32([[4], [5]]), kept=i32([[[0] * 12] * hkv] * n), recent=2, first=1, span=128, tile=i32([0, 1]), zeros=i32([0, 0]),
+             places=None)
+    a["v_cache"] = a["k_cache"].clone()
+    a["whole"], a["whole_v"] = torch.zeros((2, n, hkv, 32, dim), dtype=torch.bfloat16, device="cuda")
+    a.update(change)
+    places = (a["k_cache"], a["v_cache"])
+    return dict(
+        store=lambda: kernels.int4_store(a["k"], a["v"], *places, a["req"], a["pos"], a["slots"], a["table"], a["page"], mass=a["mass"]),
+        read=lambda: kernels.int4_read(*places, a["k"], a["v"], a["req"], a["pos"], a["slots"], a["table"], a["page"]),
+        expand=lambda: kernels.int4_expand(*places, a["whole"], a["whole_v"], a["slots"], a["table"], a["ctx"], a["page"]),
+        decode=lambda: kernels.attn_decode_int4(a["q"], a["out"], *places, a["slots"], a["table"], a["starts"], a["lens"], a["ctx"], a["most"], a["longest"], a["page"], 0.125,
+                                                a["window"], a["sink"], a["keep_first"], a["mass"]),
+        prefill=lambda: kernels.attn_prefill_int4(a["q"], a["out"], *places, a["slots"], a["table"], a["tile"], a["zeros"], a["starts"], a["lens"], a["ctx"], a["longest"], a["page"],
+                                                  0.125, a["window"], a["sink"], a["keep_first"], a["span"], a["places"]),
+        evict=lambda: kernels.int4_evict(*places, a["mass"], a["slots"], a["table"], a["ctx"], a["to"], a["kept"], a["page"], a["longest"], a["recent"], a["first"]))
+
+
+def test_good_arguments_are_taken():
+    for call in calls().values():
+        call()
+    kernels.raise_if_kernel_gave_up()
+
+
+EVERY = ("store", "read", "expand", "decode", "prefill", "evict")
+BAD = [
+    (EVERY, lambda: dict(page=12)), (EVERY, lambda: dict(page=8)), (EVERY, lambda: dict(page=0)), (EVERY, lambda: dict(page=-16)),
+    (EVERY, lambda: dict(k_cache=torch.zeros((6, 2, 576), dtype=torch.int8, device="cuda"))),
+    (EVERY, lambda: dict(k_cache=torch.zeros((7, 2, 576), dtype=torch.uint8, device="cuda"))),
+    (EVERY, lambda: dict(v_cache=torch.zeros((6, 2, 577), dtype=torch.uint8, device="cuda"))),
+    (EVERY, lambda: dict(k_cache=torch.zeros((6, 2, 1152), dtype=torch.uint8, device="cuda")[:, :, ::2])),
+    (EVERY, lambda: dict(v_cache=torch.zeros((6, 2, 576), dtype=torch.uint8))),
+    (EVERY, lambda: dict(table=i32([0, 1]))), (EVERY, lambda: dict(table=i32([[0, 1], [2, 3]]).long())), (EVERY, lambda: dict(table=torch.zeros((2, 2), dtype=torch.int32))),
+    (EVERY, lambda: dict(table=i32([[0, 1, 2, 3], [2, 3, 4, 5]])[:, ::2])),
+    (EVERY, lambda: dict(slots=i32([0, 1]).long())), (EVERY, lambda: dict(slots=torch.zeros(2, dtype=torch.int32))),
+    (("expand", "decode", "prefill", "evict"), lambda: dict(slots=i32([0]))),
+    (("store", "read"), lambda: dict(req=i32([0]))), (("store", "read"), lambda: dict(pos=i32([0, 1, 2]))),
+    (("expand", "decode", "prefill", "evict"), lambda: dict(ctx=i32([20]))), (("decode", "prefill"), lambda: dict(starts=i32([0]))),
+    (("store", "read"), lambda: dict(k=queries(2, 1, 64, torch.bfloat16), v=queries(2, 1, 64, torch.bfloat16))),           # another number of key heads
+    (("store", "read"), lambda: dict(k=queries(2, 2, 32, torch.bfloat16), v=queries(2, 2, 32, torch.bfloat16))),           # another head size
+    (("store", "read"), lambda: dict(v=queries(3, 2, 64, torch.bfloat16))), (("store", "read"), lambda: dict(v=queries(2, 2, 64, torch.float32))),
+    (("store", "read"), lambda: dict(k=queries(2, 2, 64, torch.float16), v=queries(2, 2, 64, torch.float16))),
+    (("store", "read"), lambda: dict(k=queries(2, 2, 64, torch.bfloat16).cpu())),
+    (("store",), lambda: dict(k=queries(2, 2, 128, torch.bfloat16)[:, :, ::2])), (("read",), lambda: dict(k=queries(2, 4, 64, torch.bfloat16)[:, ::2])),
+    (("expand",), lambda: dict(whole=torch.zeros((2, 2, 31, 64), dtype=torch.bfloat16, device="cuda"))),
+    (("decode", "prefill"), lambda: dict(q=queries(2, 4, 64, torch.float16), out=queries(2, 4, 64, torch.float16))), (("decode", "prefill"), lambda: dict(out=queries(2, 4, 64, torch.float32))),
+    (("decode", "prefill"), lambda: dict(q=queries(2, 3, 64, torch.bfloat16), out=queries(2, 3, 64, torch.bfloat16))),     # three query heads for two key heads
+    (("decode", "prefill"), lambda: dict(q=queries(2, 4, 32, torch.bfloat16), out=queries(2, 4, 32, torch.bfloat16))),
+    (("decode", "prefill"), lambda: dict(out=queries(3, 4, 64, torch.bfloat16))), (("decode", "prefill"), lambda: dict(q=queries(2, 8, 64, torch.bfloat16)[:, ::2])),
+    (("decode",), lambda: dict(most=0)), (("decode", "prefill"), lambda: dict(longest=0)), (("evict",), lambda: dict(longest=0)),
+    (("decode",), lambda: dict(window=0)), (("decode",), lambda: dict(keep_first=-1)), (("decode",), lambda: dict(sink=torch.zeros(3, device="cuda"))),
+    (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((6, 2, 8), device="cuda"))), (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((5, 2, 16), device="cuda"))),
+    (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((6, 2, 16), dtype=torch.bfloat16, device="cuda"))),
+    (("prefill",), lambda: dict(span=32)), (("prefill",), lambda: dict(places=(i32([0]), i32([0])))),
+    (("evict",), lambda: dict(to=i32([[4]]))), (("evict",), lambda: dict(kept=i32([[[0] * 20] * 2] * 2))), (("evict",), lambda: dict(kept=i32([[[0] * 12]] * 2))),
+    (("evict",), lambda: dict(recent=-1)), (("evict",), lambda: dict(first=-1)), (("evict",), lambda: dict(recent=8, first=5)),
+    (("evict",), lambda: dict(to=i32([[4], [5]]).long())), (("evict",), lambda: dict(kept=torch.zeros((2, 2, 12), device="cuda"))),
+]
+
+
+@pytest.mark.parametrize("case", range(len(BAD)))
+def test_refusals(case):
+    names, change = BAD[case]
+    made = calls(**change())
+    for name in names:
+        with pytest.raises(KernelError):
+            made[name]()
+
+
+def test_planes_that_do_not_begin_on_16_bytes_are_refused():
+    room = torch.zeros(6 * 2 * 576 + 16, dtype=torch.uint8, device="cuda")
+    odd = room[8:8 + 6 * 2 * 576].view(6, 2, 576)
+    made = calls(k_cache=odd)
+    for name in EVERY:
+        with pytest.raises(KernelError):
+            made[name]()
 
 
 # ------------------------------------------------------------------ together, and as programs run them
