@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 }
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
-// request's end, give zeros.  float16 (three binary digits times eleven, rounded to eleven): divided by the key head's factor (int4_prompt_kernel).
+// request's end, give zeros.  float16 (three binary digits times eleven, rounded to eleven): divided by the key head's factor (int4_top_kernel).
 constexpr int READ_ROWS = 4;         // of a thread, on their way together
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
@@ -259,7 +259,7 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
         T* to = out + (ends ? blockIdx.y * req_stride : 0) + token[i] * token_stride + head[i] * head_stride;
         if (VALUES) from_value_order<NG>(code[i].w);
         float inverse = 1.f;
-        if constexpr (std::is_same<T, __half>::value) inverse = 1.f / factors[((size_t)blockIdx.y * hkv + head[i]) * 2 + VALUES];
+        if constexpr (std::is_same<T, __half>::value) inverse = __uint_as_float((254u << 23) - __float_as_uint(factors[((size_t)blockIdx.y * hkv + head[i]) * 2 + VALUES]));      // (a power of two)
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
             const uint32_t two = VALUES ? held[i].w[j] : held[i].w[j / 2];
@@ -273,67 +273,13 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
     }
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
-                                                            T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
-                                                            Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
-                                                            int tokens, int hkv) {
-    pdl_wait();
-    const long long rows = (long long)tokens * hkv;
-    constexpr int EACH = READ_ROWS * (THREADS / LANES);
-    const int key_units = (int)((rows + EACH - 1) / EACH);
-    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x);
-    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x - key_units);
-    pdl_trigger();
-}
-
-// What a prompt's attention with float16 operands needs before its rows are written out: a power of two for each request's key head, keys and
-// values apart, which brings the largest of them to 2^14 .. 2^15 (a thread block reads all its steps, 1/9 of what is held); and the
-// queries [rows][D] as float16, each row times a power of two to the same end, which is taken back by its factor.  NaN is left out of a largest
-// one, and stays NaN.
-constexpr int PROMPT_THREADS = 512;
-template <int D>
-__global__ void __launch_bounds__(PROMPT_THREADS) int4_prompt_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
-                                                                     const int* __restrict__ req_slot, Pages pages, const int* __restrict__ ends, const int* __restrict__ which,
-                                                                     float* __restrict__ factors, int n_req, const uint4* __restrict__ q, uint4* __restrict__ q_half,
-                                                                     float* __restrict__ q_factor, long long q_rows) {
-    constexpr int NG = D / 32, PARTS = D / 8;                       // threads that share a row of queries
-    __shared__ uint32_t of_warp[PROMPT_THREADS / 32];
-    pdl_wait();
-    const int heads = n_req * pages.hkv, tid = threadIdx.x;
-    if ((int)blockIdx.x < 2 * heads) {
-        const bool values = (int)blockIdx.x >= heads;
-        const int unit = blockIdx.x - (values ? heads : 0), i = unit / pages.hkv, head = unit - i * pages.hkv;
-        const int req = which ? which[i] : i, slot = req_slot[req], end = ends[req];
-        const unsigned char* cache = values ? v_cache : k_cache;
-        uint32_t top = 0;
-        for (int c = tid; c < (end + INT4_BLOCK - 1) / INT4_BLOCK * NG; c += PROMPT_THREADS) {      // eight steps each
-            const int row0 = c / NG * INT4_BLOCK, part = c % NG;
-            const long long block = int4_block_at(pages, slot, row0, head);
-            if (block < 0) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(cache + block * int4_block_bytes(D) + 4 * D + 16 * part);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int at = 8 * part + e, row = row0 + (values ? at / (2 * NG) * 2 + (at & 1) : at / NG);
-                const uint32_t s = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffff;
-                if (row < end && s < 0x7c00u) top = max(top, s);
-            }
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (tid % 32 == 0) of_warp[tid / 32] = top;
-        __syncthreads();
-        if (tid < 32) {
-            top = __reduce_max_sync(0xffffffffu, tid < PROMPT_THREADS / 32 ? of_warp[tid] : 0u);
-            const float most = 7.f * __half2float(__ushort_as_half((unsigned short)top));           // 2^-22 .. 2^19
-            const int exponent = top ? (int)(__float_as_uint(most) >> 23) - 127 - 14 : 0;
-            if (tid == 0) factors[((size_t)i * pages.hkv + head) * 2 + values] = __uint_as_float((uint32_t)(exponent + 127) << 23);
-        }
-        return;
-    }
-    const long long at = (long long)(blockIdx.x - 2 * heads) * PROMPT_THREADS + tid, row = at / PARTS;
-    const bool there = row < q_rows;
-    const uint4 v = there ? q[at] : make_uint4(0, 0, 0, 0);
+// A prompt's queries [rows][D] as float16, each row times a power of two that brings its largest to 2^14 .. 2^15, which its factor takes back.
+struct Queries { const uint4* q; uint4* half; float* factor; long long rows; };
+template <int D> __device__ __forceinline__ void convert_queries(const Queries& a, long long block) {
+    constexpr int PARTS = D / 8;                                    // threads that share a row
+    const long long at = block * blockDim.x + threadIdx.x, row = at / PARTS;
+    const bool there = row < a.rows;
+    const uint4 v = there ? a.q[at] : make_uint4(0, 0, 0, 0);
     const uint32_t x[4] = {v.x, v.y, v.z, v.w};
     uint32_t top = largest<8>(x);
 #pragma unroll
@@ -346,8 +292,77 @@ __global__ void __launch_bounds__(PROMPT_THREADS) int4_prompt_kernel(const unsig
         const __half2 two = __floats2half2_rn(widened(x, 2 * i) * up, widened(x, 2 * i + 1) * up);
         w[i] = *reinterpret_cast<const uint32_t*>(&two);
     }
-    if (there) q_half[at] = make_uint4(w[0], w[1], w[2], w[3]);
-    if (there && at % PARTS == 0) q_factor[row] = __uint_as_float((uint32_t)(127 - exponent) << 23);
+    if (there) a.half[at] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (there && at % PARTS == 0) a.factor[row] = __uint_as_float((uint32_t)(127 - exponent) << 23);
+}
+
+// What a prompt's attention with float16 operands needs before its rows are written out: a power of two for each request's key head, keys
+// and values apart, to the same end (a thread block reads all its steps, 1/9 of what is held; NaN is left out, and stays NaN), and
+// its queries, which the thread blocks behind those take meanwhile.
+constexpr int TOP_THREADS = 1024;
+template <int D>
+__global__ void __launch_bounds__(TOP_THREADS) int4_top_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
+                                                               const int* __restrict__ req_slot, Pages pages, const int* __restrict__ ends, const int* __restrict__ which,
+                                                               float* __restrict__ factors, int* __restrict__ pages_out, int n_req, Queries queries) {
+    constexpr int NG = D / 32, AT_ONCE = 4;
+    __shared__ uint32_t of_warp[TOP_THREADS / 32];
+    pdl_wait();
+    pdl_trigger();
+    if ((int)blockIdx.x >= 2 * n_req * pages.hkv) return convert_queries<D>(queries, blockIdx.x - 2 * n_req * pages.hkv);
+    const int tid = threadIdx.x, unit = blockIdx.x >> 1, i = unit / pages.hkv, head = unit - i * pages.hkv;
+    const bool values = blockIdx.x & 1;
+    if (tid == 0 && head == 0 && !values) pages_out[i] = i;         // the table of the rows written out: a page each
+    const int req = which ? which[i] : i, slot = req_slot[req], end = ends[req];
+    const unsigned char* cache = values ? v_cache : k_cache;
+    uint32_t top = 0;
+    const int chunks = (end + INT4_BLOCK - 1) / INT4_BLOCK * NG;    // of eight steps
+    for (int c0 = tid; c0 < chunks; c0 += AT_ONCE * TOP_THREADS) {
+        uint4 v[AT_ONCE];
+        long long block[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int c = c0 + u * TOP_THREADS;
+            block[u] = c < chunks ? int4_block_at(pages, slot, c / NG * INT4_BLOCK, head) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            v[u] = block[u] < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(cache + block[u] * int4_block_bytes(D) + 4 * D + 16 * ((c0 + u * TOP_THREADS) % NG));
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int c = c0 + u * TOP_THREADS;
+            const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = 8 * (c % NG) + e, row = c / NG * INT4_BLOCK + (values ? at / (2 * NG) * 2 + (at & 1) : at / NG);
+                const uint32_t s = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffff;
+                if (row < end && s < 0x7c00u) top = max(top, s);
+            }
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (tid % 32 == 0) of_warp[tid / 32] = top;
+    __syncthreads();
+    if (tid < 32) {
+        top = __reduce_max_sync(0xffffffffu, of_warp[tid]);
+        const float most = 7.f * __half2float(__ushort_as_half((unsigned short)top));               // 2^-22 .. 2^19
+        const int exponent = top ? (int)(__float_as_uint(most) >> 23) - 127 - 14 : 0;
+        if (tid == 0) factors[((size_t)i * pages.hkv + head) * 2 + values] = __uint_as_float((uint32_t)(exponent + 127) << 23);
+    }
+}
+static_assert(TOP_THREADS == 1024, "a warp joins 32");
+
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
+                                                            T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
+                                                            Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
+                                                            int tokens, int hkv) {
+    pdl_wait();
+    const long long rows = (long long)tokens * hkv;
+    constexpr int EACH = READ_ROWS * (THREADS / LANES);
+    const int key_units = (int)((rows + EACH - 1) / EACH);
+    if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x);
+    else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x - key_units);
+    pdl_trigger();
 }
 
 // ------------------------------------------------------------------ eviction
@@ -585,8 +600,8 @@ CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k
 }
 
 // For a prompt's attention with float16 operands (head sizes 64 and 128): places 0 .. rows - 1 of n_req requests (request which[i], or i without a list) into
-// k, v float16 [n_req][hkv][rows][dim] over `factors` [n_req][hkv][2], and queries bfloat16 [q_rows][dim] into q_half over q_factor [q_rows].
-CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void* k, void* v, float* factors, const void* q, void* q_half, float* q_factor, long long q_rows,
+// k, v float16 [n_req][hkv][rows][dim] over `factors` [n_req][hkv][2] (pages_out becomes 0, 1, .. n_req - 1), and queries bfloat16 [q_rows][dim] into q_half over q_factor [q_rows].
+CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void* k, void* v, float* factors, int* pages_out, const void* q, void* q_half, float* q_factor, long long q_rows,
                                  const int* req_slot, const int* block_table, int width, int page_size, const int* ends, const int* which, int n_req, int rows, int hkv, int dim,
                                  void* stream) {
     if (rows <= 0 || n_req <= 0) return 0;
@@ -595,12 +610,13 @@ CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void*
     const Pages pages = pages_of(block_table, width, page_size, hkv);
     const Place at{nullptr, nullptr, req_slot, pages, Divider((uint32_t)hkv)};
     const dim3 grid((unsigned)units((long long)rows * hkv, READ_ROWS * (THREADS / LANES)), (unsigned)n_req);
+    const Queries queries{(const uint4*)q, (uint4*)q_half, q_factor, q_rows};
+    const long long blocks = 2ll * n_req * hkv + (q_rows * (dim / 8) + TOP_THREADS - 1) / TOP_THREADS;
+    if (blocks >= 1ll << 31) return -2;
     const auto run = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        const long long blocks = 2ll * n_req * hkv + (q_rows * (D / 8) + PROMPT_THREADS - 1) / PROMPT_THREADS;
-        if (blocks >= 1ll << 31) return -2;
-        const int status = launch_kernel(int4_prompt_kernel<D>, dim3((unsigned)blocks), dim3(PROMPT_THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
-                                         (const unsigned char*)v_cache, req_slot, pages, ends, which, factors, n_req, (const uint4*)q, (uint4*)q_half, q_factor, q_rows);
+        const int status = launch_kernel(int4_top_kernel<D>, dim3((unsigned)blocks), dim3(TOP_THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
+                                         (const unsigned char*)v_cache, req_slot, pages, ends, which, factors, pages_out, n_req, queries);
         if (status) return status;
         return launch_kernel(int4_read_kernel<D, __half>, grid, dim3(THREADS), 0, (cudaStream_t)stream, true, (const unsigned char*)k_cache, (const unsigned char*)v_cache, (__half*)k,
                              (__half*)v, (long long)hkv * rows * D, (long long)D, (long long)rows * D, at, Divider((uint32_t)rows), ends, which, (const float*)factors, rows, hkv);

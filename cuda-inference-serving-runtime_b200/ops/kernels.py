@@ -725,14 +725,17 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     n_all = q_len.numel()
     if longest < 1 or hq % hkv or out.shape != q.shape or req_slot.numel() < n_all or span not in (PREFILL_TILE, WIDE_TILE, WIDE_PAIR) or q.get_device() != device:
         raise KernelError("attn_prefill_int4: heads, limits, shapes, devices or the span disagree")
+    if (window is not None and window < 1) or keep_first < 0:
+        raise KernelError("attn_prefill_int4: a window has at least one key, and keep_first is not negative")
     requests, places = (None, None) if portions is None else portions
     n = n_all if requests is None else requests.numel()
-    if places is None:
-        places = torch.arange(n, dtype=torch.int32, device=q.device)
-    _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS + ("places",), (req_slot, q_start, q_len, ctx_len, places))
+    _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS, (req_slot, q_start, q_len, ctx_len))
+    if portions is not None:
+        _int4_lists("attn_prefill_int4", device, block_table, n_all, ("req_slot", "places"), (requests, places))
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
-    table = places.view(-1, 1) if requests is None else torch.arange(n, dtype=torch.int32, device=q.device).view(-1, 1)
     if span == PREFILL_TILE:
+        table = torch.arange(n, dtype=torch.int32, device=q.device).view(-1, 1)
+        places = table.view(-1) if places is None else places
         k, v = torch.empty((2, n, hkv, rows, dim), device=q.device)
         int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
         wide, wide_out = q.float(), out.float()                  # themselves where they are float; rows of other requests stay as they are
@@ -746,12 +749,12 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         _need(t, torch.int32, name)
     lib = _attention_tcgen05(dim, half=True)
     k, v = torch.empty((2, n, hkv, rows, dim), dtype=torch.float16, device=q.device)
-    halves, factors = torch.empty(q.shape, dtype=torch.float16, device=q.device), torch.empty(n * hkv * 2 + q.shape[0] * hq, device=q.device)
-    q_factor = factors[n * hkv * 2:]
-    _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), _p(k), _p(v), _p(factors), _p(q), _p(halves), _p(q_factor), q.shape[0] * hq, _p(req_slot), _p(block_table),
+    halves, factors = torch.empty(q.shape, dtype=torch.float16, device=q.device), torch.empty(n * hkv * 2 + n + q.shape[0] * hq, device=q.device)
+    table, q_factor = factors.data_ptr() + 8 * n * hkv, factors.data_ptr() + 8 * n * hkv + 4 * n
+    _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), _p(k), _p(v), _p(factors), table, _p(q), _p(halves), q_factor, q.shape[0] * hq, _p(req_slot), _p(block_table),
                                          block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()), "attn_prefill_int4", own=2)
-    _check(lib.cisr_attn_prefill_tcgen05(_p(halves), _p(out), q.shape[0], _p(k), _p(v), n, _p(places), _p(table), 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
-                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), _p(q_factor),
+    _check(lib.cisr_attn_prefill_tcgen05(_p(halves), _p(out), q.shape[0], _p(k), _p(v), n, table if places is None else _p(places), table, 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
+                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor,
                                          _p(factors), _stream()), "attn_prefill_int4")
 
 

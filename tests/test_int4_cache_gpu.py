@@ -608,10 +608,10 @@ BAD = [
     (("decode", "prefill"), lambda: dict(q=queries(2, 4, 32, torch.bfloat16), out=queries(2, 4, 32, torch.bfloat16))),
     (("decode", "prefill"), lambda: dict(out=queries(3, 4, 64, torch.bfloat16))), (("decode", "prefill"), lambda: dict(q=queries(2, 8, 64, torch.bfloat16)[:, ::2])),
     (("decode",), lambda: dict(most=0)), (("decode", "prefill"), lambda: dict(longest=0)), (("evict",), lambda: dict(longest=0)),
-    (("decode",), lambda: dict(window=0)), (("decode",), lambda: dict(keep_first=-1)), (("decode",), lambda: dict(sink=torch.zeros(3, device="cuda"))),
+    (("decode", "prefill"), lambda: dict(window=0)), (("decode", "prefill"), lambda: dict(keep_first=-1)), (("decode",), lambda: dict(sink=torch.zeros(3, device="cuda"))),
     (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((6, 2, 8), device="cuda"))), (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((5, 2, 16), device="cuda"))),
     (("store", "decode", "evict"), lambda: dict(mass=torch.zeros((6, 2, 16), dtype=torch.bfloat16, device="cuda"))),
-    (("prefill",), lambda: dict(span=32)), (("prefill",), lambda: dict(places=(i32([0]), i32([0])))),
+    (("prefill",), lambda: dict(span=32)), (("prefill",), lambda: dict(q=queries(2, 4, 64, torch.float32), out=queries(2, 4, 64, torch.float32))), (("prefill",), lambda: dict(places=(i32([0]), i32([0])))),
     (("evict",), lambda: dict(to=i32([[4]]))), (("evict",), lambda: dict(kept=i32([[[0] * 20] * 2] * 2))), (("evict",), lambda: dict(kept=i32([[[0] * 12]] * 2))),
     (("evict",), lambda: dict(recent=-1)), (("evict",), lambda: dict(first=-1)), (("evict",), lambda: dict(recent=8, first=5)),
     (("evict",), lambda: dict(to=i32([[4], [5]]).long())), (("evict",), lambda: dict(kept=torch.zeros((2, 2, 12), device="cuda"))),
