@@ -46,10 +46,10 @@ template <int NT> constexpr int tile_keys() { return NT == 1 ? 64 : 32; }
 constexpr int BLOCK_BYTES = int4_block_bytes(D);
 constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum follows a score only where that is 2^SLACK times its weight above it, which after a warp's first tile is rare (each time
-// costs 50 multiplications a lane).  Probabilities are held times 2^5 (for float queries, whose second terms are 2^-11 of the first, 2^9): with
-// steps of V below 128 (8; values below 896 or 56) no product of the two overflows a float16, and small ones keep their digits.  A warp whose sums come out not finite does its keys
-// again with probabilities times 2^-5, where no step can overflow.  (Looking at every step instead took 8 instructions per 16 keys.)
-constexpr float SLACK = 4.f, USUAL_SHIFT = TERMS == 1 ? 5.f : 9.f, LARGE_SHIFT = -5.f;
+// costs 50 multiplications a lane).  Probabilities are held times 2^9: with steps of V below 8 (values below 56) no product of the two overflows
+// a float16, and products down to 2^-23 keep all their digits (smaller ones are off by 2^-34 at most).  A warp whose sums come out not finite
+// does its keys again with probabilities times 2^-5, where no step can overflow.  (Looking at every step instead took 8 instructions per 16 keys.)
+constexpr float SLACK = 4.f, USUAL_SHIFT = 9.f, LARGE_SHIFT = -5.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 constexpr int MAX_RANKED = 128;                                    // requests that are put in order of length, a thread each
 

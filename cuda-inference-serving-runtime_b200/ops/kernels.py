@@ -531,7 +531,11 @@ INT4_GROUP = 32                  # values along a head that share a step
 INT4_BLOCK = 8                   # rows of a block; a page is whole blocks
 INT4_HEAD_DIMS = (32, 64, 96, 128)
 INT4_MAX_BYTES = 1 << 36         # of a plane: places in it are counted in 16 bytes, as 32-bit numbers
-INT4_FEW = 16                    # new tokens of a request up to which attn_decode_int4 is the faster call (see attn_prefill_int4)
+# New tokens of a request up to which `attn_decode_int4` is the faster call also where `attn_prefill_int4` takes tiles of 128: us at 32 and at 64
+# tokens, 32 requests of 2500 rows, 64 heads over 8 of 128: 464 against 490, 902 against 503; 32 over 8: 239 against 297, 463 against 304;
+# 9 over 3 of 64: 51 against 80, 96 against 81; one request of 6000 rows, 32 over 8 of 128: 29 against 70, 47 against 70.
+INT4_FEW = 32
+INT4_WEIGHED = 16                # the latest tokens of a portion by whose weights keys are judged (a score per query and key is kept meanwhile)
 _int4_rows_state = {}
 _attention_int4_libs = {}
 _attention_int4_calls = {}       # by the sizes of a call: the function, the floats of scratch it takes, the kernels it launches
@@ -539,9 +543,9 @@ _attention_int4_calls = {}       # by the sizes of a call: the function, the flo
 
 def int4_jobs(head_dim: int, dtype: torch.dtype):
     """The build jobs of a 4-bit cache for this head size and type of queries."""
-    half = dtype == torch.bfloat16 and head_dim in TCGEN05_HEAD_DIMS
+    wide = dtype == torch.bfloat16 and head_dim in TCGEN05_HEAD_DIMS
     return ([("int4_rows.cu", {}, ()), ("attention_int4.cu", {"HEAD_DIM": head_dim, "STORAGE_BF16": dtype_code(dtype)}, ())]
-            + ([("attention_tcgen05.cu", {"HEAD_DIM": head_dim, "HALF_OPERANDS": 1}, ())] if half else attention_tcgen05_jobs(head_dim, torch.float32)))
+            + ([("attention_tcgen05.cu", {"HEAD_DIM": head_dim, "HALF_OPERANDS": 1}, ())] if wide else []))
 
 
 def _int4_rows():
@@ -675,7 +679,7 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
 def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
                      q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_queries: int, longest: int, page_size: int, scale: float,
                      window: Optional[int] = None, sink=None, keep_first: int = 0, mass: Optional[torch.Tensor] = None) -> None:
-    """Attention of a few new tokens per request (one in a decode step) over a 4-bit cache: q, out [tokens, heads, head_dim].
+    """Attention of new tokens, few per request (one in a decode step), over a 4-bit cache: q, out [tokens, heads, head_dim].
     Request r brings q_len[r] tokens from row q_start[r] of q on and has ctx_len[r] rows in the cache, theirs included; requests that
     bring none, or more than `max_queries`, are left alone.  `longest`: no request has more rows (a bound will do; one that has sets the
     flag that `raise_if_kernel_gave_up` reads).  window, sink, keep_first: as for `attn_decode`.
@@ -711,14 +715,17 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
 def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
                       tile_req: torch.Tensor, tile_q0: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, longest: int, page_size: int,
                       scale: float, window: Optional[int] = None, sink=None, keep_first: int = 0, span: int = PREFILL_TILE,
-                      portions: Optional[tuple] = None) -> None:
+                      portions: Optional[tuple] = None, max_queries: Optional[int] = None) -> None:
     """Attention of portions of prompts over a 4-bit cache: the requests' rows are written out as values once, and a prompt attention
     runs over those, so codes are turned into operands once per key and not once per tile of queries.
-    Tiles of `span` queries as (request, first query): 128 or 256 (bfloat16, head sizes 64 and 128) as for `attn_prefill_wide`, with float16
-    operands, whose eleven binary digits are those of a held value; 64 (any) as for `attn_prefill`, with float ones.  `longest`: no
-    request that is written out has more rows.  `portions` (requests, places): the requests that are written out, and for every
-    request of the step its place in that list (any number for the others); None: all, in order.  A held value that is NaN reaches
-    the queries before it, too, as it does in those."""
+    Tiles of `span` queries, 128 or 256 (bfloat16, head sizes 64 and 128), as (request, first query) as for `attn_prefill_wide`, with float16
+    operands, whose eleven binary digits are those of a held value; a held value that is NaN reaches the queries before it, too, as
+    it does there.  `longest`: no request that is written out has more rows.  `portions` (requests, places): the requests that are
+    written out, and for every request of the step its place in that list (any number for the others); None: all, in order.
+
+    `span` 64 is for the other types and head sizes: `attn_decode_int4` of the requests that are listed (the tiles are not looked at), no
+    portion longer than `max_queries` (None: than q).  The rows written out in float for a kernel of its own took two to five
+    times as long (us, 4 requests of 1000 queries: 440 against 966, float with 32 heads over 8 of 128; 144 against 463, bfloat16 with 16 over 8 of 96)."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     hq, dim = q.shape[1], q.shape[2]
     hkv, device = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
@@ -734,14 +741,9 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         _int4_lists("attn_prefill_int4", device, block_table, n_all, ("req_slot", "places"), (requests, places))
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     if span == PREFILL_TILE:
-        table = torch.arange(n, dtype=torch.int32, device=q.device).view(-1, 1)
-        places = table.view(-1) if places is None else places
-        k, v = torch.empty((2, n, hkv, rows, dim), device=q.device)
-        int4_expand(k_cache, v_cache, k, v, req_slot[:n_all], block_table, ctx_len, page_size, requests)
-        wide, wide_out = q.float(), out.float()                  # themselves where they are float; rows of other requests stay as they are
-        attn_prefill(wide, wide_out, k, v, places, table, tile_req, tile_q0, q_start, q_len, ctx_len, hq, hkv, rows, scale, window, sink=sink, keep_first=keep_first)
-        if wide_out is not out:
-            out.copy_(wide_out)
+        lists = (req_slot, q_start, q_len, ctx_len) if requests is None else [t[requests.long()] for t in (req_slot, q_start, q_len, ctx_len)]
+        attn_decode_int4(q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], min(max_queries or q.shape[0], max(1, q.shape[0])), longest, page_size, scale, window, sink,
+                         keep_first)
         return
     if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
         raise KernelError(f"attn_prefill_int4: tiles of {span} queries are for bfloat16 and head sizes {TCGEN05_HEAD_DIMS}")

@@ -204,14 +204,18 @@ def token_rows(ctx, cache) -> torch.Tensor:
 
 
 def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, window) -> torch.Tensor:
-    """Attention of a step's queries over pages held in 4 bits: portions of more than a few tokens by the prompt kernels over the rows written
-    out as values, all others straight over the pages.  Where keys are weighed, what counts are the latest tokens of every
-    portion, a few at most: those run over the pages, too."""
+    """Attention of a step's queries over pages held in 4 bits: portions of more than a few tokens by the prompt kernel over the rows written
+    out as values, where the queries' type and head size have one, all others straight over the pages.  Where keys are weighed,
+    what counts are the latest tokens of every portion: those run over the pages, too."""
     out = torch.empty_like(q)
-    few = kernels.INT4_FEW
     lens, ends = ctx.host.q_len, ctx.host.ctx_len
-    most = max(lens)
-    by_portions = most > few
+    most, weighed = max(lens), kernels.INT4_WEIGHED
+
+    def over_pages(q_start, q_len, queries, longest, mass):
+        kernels.attn_decode_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, q_start, q_len, ctx.ctx_len, queries, max(longest, ctx.host.ctx_bound or 0),
+                                 cache.page_size, scale, window, mass=mass)
+
+    by_portions = most > kernels.INT4_FEW and q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS
     if by_portions:
         step = ctx.shared.get("int4_portions")
         if step is None:                     # once per step: which requests bring portions, and the place of each among them
@@ -219,24 +223,22 @@ def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, win
             places = [which.index(r) if n > 1 else 0 for r, n in enumerate(lens)]
             lists = torch.tensor(which + places, dtype=torch.int32, device=ctx.device)
             step = ctx.shared["int4_portions"] = (lists[:len(which)], lists[len(which):], max(ends[r] for r in which))
-        if q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS:
-            (tile_req, tile_q0), span = wide_tiles(plan, ctx, hq, window)
-        else:
-            tile_req, tile_q0, span = plan["tile_req"], plan["tile_q0"], kernels.PREFILL_TILE
+        (tile_req, tile_q0), span = wide_tiles(plan, ctx, hq, window)
         kernels.attn_prefill_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, tile_req, tile_q0, ctx.q_start, ctx.q_len, ctx.ctx_len, step[2],
                                   cache.page_size, scale, window, span=span, portions=step[:2])
-        if cache.mass is None and not plan.info["n_decode"]:
-            return out
-    q_start, q_len, queries = ctx.q_start, ctx.q_len, 1 if by_portions else most
-    if by_portions and cache.mass is not None:
-        latest = ctx.shared.get("int4_latest")
-        if latest is None:
-            n = ctx.q_len.clamp(max=few)
-            latest = ctx.shared["int4_latest"] = (ctx.q_start + ctx.q_len - n, n)
-        (q_start, q_len), queries = latest, few
-    longest = max(max(c for n, c in zip(lens, ends) if n <= queries or cache.mass is not None), ctx.host.ctx_bound or 0)
-    kernels.attn_decode_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, q_start, q_len, ctx.ctx_len, queries, longest, cache.page_size, scale, window,
-                             mass=cache.mass)
+    if cache.mass is None or most <= weighed:
+        if not by_portions:
+            over_pages(ctx.q_start, ctx.q_len, most, max(ends), cache.mass)
+        elif plan.info["n_decode"]:
+            over_pages(ctx.q_start, ctx.q_len, 1, max(c for n, c in zip(lens, ends) if n == 1), None)
+        return out
+    if not by_portions:
+        over_pages(ctx.q_start, ctx.q_len, most, max(ends), None)
+    latest = ctx.shared.get("int4_latest")
+    if latest is None:
+        n = ctx.q_len.clamp(max=weighed)
+        latest = ctx.shared["int4_latest"] = (ctx.q_start + ctx.q_len - n, n)
+    over_pages(*latest, weighed, max(ends), cache.mass)
     return out
 
 

@@ -393,7 +393,7 @@ def test_weights_of_keys(hq, hkv, dim, window, sink, dtype):
 
 # ------------------------------------------------------------------ portions of prompts
 def prompt_bound(dtype, span):
-    """Beside `bound`, of the outputs' sizes: float operands (tiles of 64) are exact.  float16 ones are three binary digits of a code times
+    """Beside `bound`, of the outputs' sizes: over the pages (tiles of 64) nothing.  float16 operands are three binary digits of a code times
     eleven of a step, rounded to eleven, 2^-12: of values once, of keys in scores with terms of 70 units at most, which a weight and the sum
     that it is divided by are off by; and probabilities are rounded so, as they are in `bound`."""
     return 0 if span == 64 else 2.0 ** -12 + 2 * 70 * 2.0 ** -12
@@ -453,7 +453,9 @@ def test_portions_of_any_size(dim, span, size, query):
         rows = slice(starts[r], starts[r] + n)
         want, weight, _ = plain.attention(q[rows], *cache.held(r), dim ** -0.5 / query * 1.5, plain.seen(n, lens[r]), 0.3)
         off = (out[rows].double() - want).abs()
-        assert (off <= bound(torch.bfloat16, want, weight) + prompt_bound(torch.bfloat16, span) * weight + 1e-30).all(), (r, float((off / weight).max()))
+        # products of a probability (times 2^9) and a step are float16: below its normal numbers they are off by half of 2^-24, times codes up to 7
+        small = 7 * lens[r] * 2.0 ** -34 if span == 64 else 1e-30
+        assert (off <= bound(torch.bfloat16, want, weight) + prompt_bound(torch.bfloat16, span) * weight + small).all(), (r, float((off / weight).max()))
 
 
 # ------------------------------------------------------------------ eviction

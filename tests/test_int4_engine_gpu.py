@@ -169,7 +169,7 @@ def test_a_fork_of_a_request_that_is_cut(graph):
         one, other = (torch.cat([group.mass[:, p] for p in stepper.cache.requests[k].tables[0]], -1)[..., :n] for k in ("a", "b"))
         assert torch.equal(one, other) and n < 32
         if i < 10:           # not cut yet: every query head has given one in all for each of the portion's latest tokens and each token since
-            given = mixer.hq // mixer.hkv * (min(21, kernels.INT4_FEW) + i + 1)
+            given = mixer.hq // mixer.hkv * (min(21, kernels.INT4_WEIGHED) + i + 1)
             assert ((one.double().sum(-1) - given).abs() < 1e-3 * given).all()
 
 
