@@ -115,7 +115,7 @@ struct Args {
     const int* req_slot; const int* table; int width;
     const int* q_start; const int* q_len; const int* ctx_len;
     float* partial;      // [tile][kv head][row][split][D], where the splits are not one cluster
-    float* stats;        // [tile][kv head][row][split or 1][2]: largest score (base 2, less the shift), sum
+    float* stats;        // [tile][kv head][row][split or 1][2]: largest score (base 2, less the shift), sum; null where no other kernel wants them
     float* scores;       // [tile][kv head][longest][row_stride], base 2, or null
     float* mass;         // added to by this kernel itself, or null
     int max_queries, tiles, row_stride, n_splits, cluster, longest;
@@ -643,8 +643,10 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             for (int i = 0; i < WARPS; ++i) j.add(merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D], 0.f, merge[((size_t)i * ROWS + r) * MERGE_STRIDE + D + 1]);
             sums[r * MERGE_STRIDE + D] = j.m; sums[r * MERGE_STRIDE + D + 1] = j.den;
             if (!clustered && r < span.rows) {
-                float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
-                st[0] = j.m; st[1] = j.den;
+                if (a.stats) {
+                    float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
+                    st[0] = j.m; st[1] = j.den;
+                }
                 lse[r] = j.m + log2f(j.whole(sink_of(r)));
             }
         }
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int
             for (int p = 0; p < parts; ++p) j.m = fmaxf(j.m, others[p][tid][0]);
             for (int p = 0; p < parts; ++p) j.add(others[p][tid][0], 0.f, others[p][tid][1]);
             lse[tid] = j.m + log2f(j.whole(sink_of(tid)));
-            if (rank == 0) {
+            if (a.stats && rank == 0) {
                 float* st = a.stats + (base_row + tid) * 2;
                 st[0] = j.m; st[1] = j.den;
             }
@@ -825,29 +827,37 @@ template <int NT> constexpr size_t dynamic_smem() {
     return ring > merge ? ring : merge;
 }
 
-int sm_count() {                                                    // of the current device
-    static int known[64] = {};
-    int device = 0, n = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) return 1;
-    if (device < 64 && known[device]) return known[device];
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return 1;
-    if (device < 64) known[device] = n;
-    return n;
+constexpr int MAX_DEVICES = 64;
+int sm_count(int device) {
+    static int known[MAX_DEVICES] = {};
+    if (!known[device]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return 1;
+        known[device] = n;
+    }
+    return known[device];
 }
 
-// Thread blocks of the kernel that run at once on the current device in clusters of `size`: a cluster lies in one part of the chip, whose
+// Lets the kernel take its shared memory on a device, once.
+template <int NT> cudaError_t prepare_kernel(int device) {
+    static bool done[MAX_DEVICES] = {};
+    if (done[device]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_smem<NT>());
+    done[device] = e == cudaSuccess;
+    return e;
+}
+
+// Thread blocks of the kernel that run at once on a device in clusters of `size`: a cluster lies in one part of the chip, whose
 // last places it may not fill (48 clusters of 6 took two rounds where 296 blocks have places).
-template <int NT> int places(int size) {
-    static int known[64][MAX_CLUSTER + 1] = {};
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return size;
+template <int NT> int places(int device, int size) {
+    static int known[MAX_DEVICES][MAX_CLUSTER + 1] = {};
     if (!known[device][size]) {
         constexpr size_t SMEM = dynamic_smem<NT>();
         int n = 0;
-        if (cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM) != cudaSuccess) return size;
+        if (prepare_kernel<NT>(device) != cudaSuccess) return size;
         if (size == 1) {
             if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_int4_kernel<NT>, 32 * warps_of<NT>(), SMEM) != cudaSuccess) n = 0;
-            n *= sm_count();
+            n *= sm_count(device);
         } else {
             cudaLaunchConfig_t config = {};
             config.gridDim = dim3(1, 1, size); config.blockDim = dim3(32 * warps_of<NT>()); config.dynamicSmemBytes = SMEM;
@@ -871,13 +881,13 @@ struct Shape {
     bool ranked;
     long long units;                 // requests by tiles by key heads by rows
     long long keys;
-    Shape(int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
+    Shape(int device, int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
         const int needed = max_queries * (hq / hkv);
         rows = needed > 8 ? 16 : 8;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
         const int warps = rows == 8 ? warps_of<1>() : warps_of<2>(), TK = rows == 8 ? tile_keys<1>() : tile_keys<2>();
-        const auto room_of = [&](int size) { return rows == 8 ? places<1>(size) : places<2>(size); };
+        const auto room_of = [&](int size) { return rows == 8 ? places<1>(device, size) : places<2>(device, size); };
         const long long pairs = (long long)n_req * tiles * hkv, room = room_of(1);
         long long reach = longest;
         if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
@@ -903,20 +913,17 @@ struct Shape {
         keys = longest;
     }
     bool merged_by_kernel() const { return splits > 1 && cluster == 1; }
-    long long partial() const { return merged_by_kernel() ? units * splits * D : 0; }
-    long long stats() const { return units * (merged_by_kernel() ? splits : 1) * 2; }
-    long long scores() const { return units * keys; }
     bool mass_by_kernel() const { return merged_by_kernel() || tiles > 1; }
+    long long partial() const { return merged_by_kernel() ? units * splits * D : 0; }
+    long long stats(bool mass) const { return merged_by_kernel() ? units * splits * 2 : mass && tiles > 1 ? units * 2 : 0; }
+    long long scores(bool mass) const { return mass ? units * keys : 0; }
     int launches(bool mass) const { return 1 + merged_by_kernel() + (mass && mass_by_kernel()); }
 };
 
-template <int NT> int launch(Args a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
+template <int NT> int launch(int device, Args& a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
     constexpr int WARPS = warps_of<NT>();
     constexpr size_t SMEM = dynamic_smem<NT>();
-    if constexpr (SMEM > 48 * 1024 - 20480) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const cudaError_t e = prepare_kernel<NT>(device); e != cudaSuccess) return (int)e;
     const dim3 grid((unsigned)(n_req * a.tiles), (unsigned)a.hkv, (unsigned)a.n_splits);
     a.mass = shape.mass_by_kernel() ? nullptr : mass;
     int status = launch_kernel_cluster(attn_int4_kernel<NT>, grid, dim3(32 * WARPS), SMEM, s, g_pdl, a.cluster, a);
@@ -938,36 +945,48 @@ CISR_EXPORT int cisr_attn_int4_head_dim() { return D; }
 // `error_flag`: one zeroed int in device memory that the kernels set when a request is longer than they were told.
 CISR_EXPORT int cisr_attn_int4_init(int* error_flag) { g_error = error_flag; return 0; }
 
-// Floats of scratch that a call with these sizes takes (partial sums and statistics of the ranges, with `mass` also the scores).
-// The kernels that it launches: a million million times their number is added.
+// Floats of scratch that a call with these sizes on the current device takes (partial sums and statistics of the ranges, with `mass` also the
+// scores).  The kernels that it launches: a million million times their number is added.
 CISR_EXPORT long long cisr_attn_int4_scratch(int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first, int with_mass) {
-    if (n_req <= 0 || max_queries <= 0 || hkv <= 0 || longest <= 0) return 0;
-    const Shape s(n_req, max_queries, longest, hq, hkv, window, keep_first);
-    return s.partial() + s.stats() + (with_mass ? s.scores() : 0) + 1000000000000ll * s.launches(with_mass != 0);
+    int device = 0;
+    if (n_req <= 0 || max_queries <= 0 || hkv <= 0 || longest <= 0 || cudaGetDevice(&device) != cudaSuccess || device >= MAX_DEVICES) return 0;
+    const Shape s(device, n_req, max_queries, longest, hq, hkv, window, keep_first);
+    return s.partial() + s.stats(with_mass != 0) + s.scores(with_mass != 0) + 1000000000000ll * s.launches(with_mass != 0);
 }
+
+// A call's arguments, packed by the host in this order (as one address it is a third of the time in the interpreter).
+struct AttnInt4Call {
+    const void *q; void* out; const void *k_cache, *v_cache; const int *req_slot, *block_table, *q_start, *q_len, *ctx_len; float *scratch, *mass; const float* sink_heads;
+    void* stream;
+    double scale, sink;
+    int width, n_req, max_queries, longest, hq, hkv, page_size, window, keep_first;
+};
 
 // q, out [tokens][hq][D]; request r brings q_len[r] tokens from row q_start[r] on and has ctx_len[r] rows with them; those with more than
 // `max_queries` are left alone, and none may have more than `longest` rows (one that has sets the error flag).
-CISR_EXPORT int cisr_attn_int4(const void* q, void* out, const void* k_cache, const void* v_cache, const int* req_slot, const int* block_table, int width,
-                               const int* q_start, const int* q_len, const int* ctx_len, float* scratch, float* mass, int n_req, int max_queries, int longest,
-                               int hq, int hkv, int page_size, float scale, int window, int keep_first, float sink, const float* sink_heads, void* stream) {
-    if (n_req <= 0 || max_queries <= 0) return 0;
+CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
+    const AttnInt4Call& c = *call;
+    if (c.n_req <= 0 || c.max_queries <= 0) return 0;
     if (!g_error) return -13;
-    if (hkv <= 0 || hkv > 65535 || hq % hkv || !isfinite(scale) || longest <= 0 || page_size <= 0 || page_size % INT4_BLOCK || (long long)max_queries * (hq / hkv) > 1 << 20) return -2;
-    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 || (uintptr_t)scratch & 15) return -2;      // rows are read by 16 bytes
-    const Shape shape(n_req, max_queries, longest, hq, hkv, window, keep_first);
-    if (shape.splits > 65535 || (long long)n_req * shape.tiles >= 1ll << 31) return -2;
-    const int group = hq / hkv;
+    if (c.hkv <= 0 || c.hkv > 65535 || c.hq % c.hkv || !isfinite((float)c.scale) || c.longest <= 0 || c.page_size <= 0 || c.page_size % INT4_BLOCK ||
+        (long long)c.max_queries * (c.hq / c.hkv) > 1 << 20) return -2;
+    if (((uintptr_t)c.q | (uintptr_t)c.k_cache | (uintptr_t)c.v_cache) & 15 || (uintptr_t)c.scratch & 15) return -2;      // rows are read by 16 bytes
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= MAX_DEVICES) return -2;
+    const Shape shape(device, c.n_req, c.max_queries, c.longest, c.hq, c.hkv, c.window, c.keep_first);
+    if (shape.splits > 65535 || (long long)c.n_req * shape.tiles >= 1ll << 31) return -2;
+    const int group = c.hq / c.hkv;
+    const bool mass = c.mass != nullptr;
     Args a{};
-    a.q = (const T*)q; a.out = (T*)out; a.k_cache = (const unsigned char*)k_cache; a.v_cache = (const unsigned char*)v_cache;
-    a.req_slot = req_slot; a.table = block_table; a.width = width; a.q_start = q_start; a.q_len = q_len; a.ctx_len = ctx_len;
-    a.partial = scratch; a.stats = scratch + shape.partial(); a.scores = mass ? a.stats + shape.stats() : nullptr;
-    a.max_queries = max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
-    a.by_page = Divider((uint32_t)page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.by_heads = Divider((uint32_t)hkv);
-    a.group = group; a.n_req = n_req; a.ranked = shape.ranked;
+    a.q = (const T*)c.q; a.out = (T*)c.out; a.k_cache = (const unsigned char*)c.k_cache; a.v_cache = (const unsigned char*)c.v_cache;
+    a.req_slot = c.req_slot; a.table = c.block_table; a.width = c.width; a.q_start = c.q_start; a.q_len = c.q_len; a.ctx_len = c.ctx_len;
+    a.partial = c.scratch; a.stats = shape.stats(mass) ? c.scratch + shape.partial() : nullptr; a.scores = mass ? c.scratch + shape.partial() + shape.stats(mass) : nullptr;
+    a.max_queries = c.max_queries; a.tiles = shape.tiles; a.row_stride = shape.stride; a.n_splits = shape.splits; a.cluster = shape.cluster;
+    a.by_page = Divider((uint32_t)c.page_size); a.by_group = Divider((uint32_t)group); a.by_tiles = Divider((uint32_t)shape.tiles); a.by_heads = Divider((uint32_t)c.hkv);
+    a.group = group; a.n_req = c.n_req; a.ranked = shape.ranked;
     a.rank_threads = 1;
-    while (a.rank_threads < n_req && a.rank_threads < MAX_RANKED) a.rank_threads *= 2;
-    a.longest = longest; a.hq = hq; a.hkv = hkv; a.page_size = page_size; a.window = window; a.keep_first = keep_first;
-    a.scale = scale; a.sink_all = sink; a.sink_heads = sink_heads; a.error = g_error;
-    return shape.rows == 8 ? launch<1>(a, shape, n_req, mass, (cudaStream_t)stream) : launch<2>(a, shape, n_req, mass, (cudaStream_t)stream);
+    while (a.rank_threads < c.n_req && a.rank_threads < MAX_RANKED) a.rank_threads *= 2;
+    a.longest = c.longest; a.hq = c.hq; a.hkv = c.hkv; a.page_size = c.page_size; a.window = c.window; a.keep_first = c.keep_first;
+    a.scale = (float)c.scale; a.sink_all = (float)c.sink; a.sink_heads = c.sink_heads; a.error = g_error;
+    return shape.rows == 8 ? launch<1>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream) : launch<2>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
 }

@@ -556,46 +556,62 @@ long long units(long long rows, int each) { return 2 * ((rows + each - 1) / each
 
 CISR_EXPORT void cisr_int4_rows_set_pdl(int on) { g_pdl = on != 0; }
 
+// Calls' arguments, packed by the host in this order (as one address they are a third of the time in the interpreter).
+struct Int4StoreCall {
+    const void *k, *v; void *k_cache, *v_cache; float* mass; const int *token_req, *positions, *req_slot, *block_table; void* stream;
+    long long k_token, k_head, v_token, v_head;
+    int dtype, width, page_size, tokens, hkv, dim;
+};
+struct Int4ReadCall {
+    const void *k_cache, *v_cache; void *k, *v; const int *token_req, *positions, *req_slot, *block_table, *ends, *which; void* stream;
+    long long req_stride, token_stride, head_stride;
+    int dtype, width, page_size, n_req, tokens, hkv, dim;
+};
+struct Int4EvictCall {
+    void *k_cache, *v_cache; float* mass; const int *req_slot, *block_table, *ctx_len; int* kept; const int* to_table; void* stream;
+    int width, to_width, n_req, hkv, dim, page_size, keep, recent, first, longest;
+};
+
 // k, v [tokens][hkv][dim] with strides in values; codes go to place positions[t] of request token_req[t], whose number in `mass` (if any) becomes 0.
-CISR_EXPORT int cisr_int4_store(const void* k, const void* v, int dtype, long long k_token, long long k_head, long long v_token, long long v_head, void* k_cache,
-                                void* v_cache, float* mass, const int* token_req, const int* positions, const int* req_slot, const int* block_table, int width, int page_size,
-                                int tokens, int hkv, int dim, void* stream) {
-    if (tokens <= 0) return 0;
-    if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || ((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
-    if ((long long)tokens * hkv >= 1ll << 30) return -2;
-    const long long blocks = units((long long)tokens * hkv, THREADS / LANES);
-    const int per16 = dtype == CISR_F32 ? 4 : 8;
-    const int wide = (((uintptr_t)k & 15) == 0 && k_token % per16 == 0 && k_head % per16 == 0 ? 1 : 0) | (((uintptr_t)v & 15) == 0 && v_token % per16 == 0 && v_head % per16 == 0 ? 2 : 0);
-    const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
-    return by_head_size(dim, [&](auto d) {
+CISR_EXPORT int cisr_int4_store(const Int4StoreCall* call) {
+    const Int4StoreCall& c = *call;
+    if (c.tokens <= 0) return 0;
+    if (c.hkv <= 0 || c.page_size <= 0 || c.page_size % INT4_BLOCK || ((uintptr_t)c.k_cache | (uintptr_t)c.v_cache) & 15) return -2;
+    if ((long long)c.tokens * c.hkv >= 1ll << 30) return -2;
+    const long long blocks = units((long long)c.tokens * c.hkv, THREADS / LANES);
+    const int per16 = c.dtype == CISR_F32 ? 4 : 8;
+    const int wide = (((uintptr_t)c.k & 15) == 0 && c.k_token % per16 == 0 && c.k_head % per16 == 0 ? 1 : 0) |
+                     (((uintptr_t)c.v & 15) == 0 && c.v_token % per16 == 0 && c.v_head % per16 == 0 ? 2 : 0);
+    const Place at{c.token_req, c.positions, c.req_slot, pages_of(c.block_table, c.width, c.page_size, c.hkv), Divider((uint32_t)c.hkv)};
+    return by_head_size(c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (dtype == CISR_F32)
-            return launch_kernel(int4_store_kernel<D, float>, dim3((unsigned)blocks), dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const float*)k, (const float*)v, k_token,
-                                 k_head, v_token, v_head, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, at, tokens, hkv, wide);
-        return launch_kernel(int4_store_kernel<D, __nv_bfloat16>, dim3((unsigned)blocks), dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const __nv_bfloat16*)k,
-                             (const __nv_bfloat16*)v, k_token, k_head, v_token, v_head, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, at, tokens, hkv, wide);
+        const auto run = [&](auto* kernel, auto* k, auto* v) {
+            return launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), 0, (cudaStream_t)c.stream, g_pdl, k, v, c.k_token, c.k_head, c.v_token, c.v_head,
+                                 (unsigned char*)c.k_cache, (unsigned char*)c.v_cache, c.mass, at, c.tokens, c.hkv, wide);
+        };
+        return c.dtype == CISR_F32 ? run(int4_store_kernel<D, float>, (const float*)c.k, (const float*)c.v)
+                                   : run(int4_store_kernel<D, __nv_bfloat16>, (const __nv_bfloat16*)c.k, (const __nv_bfloat16*)c.v);
     });
 }
 
 // The reverse: rows (token_req[t], positions[t]) into k, v [tokens][hkv][dim]; or, with `ends`, places 0 .. tokens - 1 of each of n_req
 // requests (request which[i], or i without a list) into [n_req][..] with the strides given; places from ends[request] on give zeros.
-CISR_EXPORT int cisr_int4_read(const void* k_cache, const void* v_cache, void* k, void* v, int dtype, long long req_stride, long long token_stride, long long head_stride,
-                               const int* token_req, const int* positions, const int* req_slot, const int* block_table, int width, int page_size, const int* ends,
-                               const int* which, int n_req, int tokens, int hkv, int dim, void* stream) {
-    if (tokens <= 0 || n_req <= 0) return 0;
-    if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535) return -2;
-    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v) & 15 || token_stride % 8 || head_stride % 8 || req_stride % 8) return -2;
-    if ((long long)tokens * hkv >= 1ll << 30) return -2;
-    const long long blocks = units((long long)tokens * hkv, READ_ROWS * (THREADS / LANES));
-    const Place at{token_req, positions, req_slot, pages_of(block_table, width, page_size, hkv), Divider((uint32_t)hkv)};
-    const dim3 grid((unsigned)blocks, (unsigned)n_req);
-    return by_head_size(dim, [&](auto d) {
+CISR_EXPORT int cisr_int4_read(const Int4ReadCall* call) {
+    const Int4ReadCall& c = *call;
+    if (c.tokens <= 0 || c.n_req <= 0) return 0;
+    if (c.hkv <= 0 || c.page_size <= 0 || c.page_size % INT4_BLOCK || c.n_req > 65535) return -2;
+    if (((uintptr_t)c.k_cache | (uintptr_t)c.v_cache | (uintptr_t)c.k | (uintptr_t)c.v) & 15 || c.token_stride % 8 || c.head_stride % 8 || c.req_stride % 8) return -2;
+    if ((long long)c.tokens * c.hkv >= 1ll << 30) return -2;
+    const long long blocks = units((long long)c.tokens * c.hkv, READ_ROWS * (THREADS / LANES));
+    const Place at{c.token_req, c.positions, c.req_slot, pages_of(c.block_table, c.width, c.page_size, c.hkv), Divider((uint32_t)c.hkv)};
+    const dim3 grid((unsigned)blocks, (unsigned)c.n_req);
+    return by_head_size(c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (dtype == CISR_F32)
-            return launch_kernel(int4_read_kernel<D, float>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache, (const unsigned char*)v_cache,
-                                 (float*)k, (float*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, (const float*)nullptr, tokens, hkv);
-        return launch_kernel(int4_read_kernel<D, __nv_bfloat16>, grid, dim3(THREADS), 0, (cudaStream_t)stream, g_pdl, (const unsigned char*)k_cache,
-                             (const unsigned char*)v_cache, (__nv_bfloat16*)k, (__nv_bfloat16*)v, req_stride, token_stride, head_stride, at, Divider((uint32_t)tokens), ends, which, (const float*)nullptr, tokens, hkv);
+        const auto run = [&](auto* kernel, auto* k, auto* v) {
+            return launch_kernel(kernel, grid, dim3(THREADS), 0, (cudaStream_t)c.stream, g_pdl, (const unsigned char*)c.k_cache, (const unsigned char*)c.v_cache, k, v, c.req_stride,
+                                 c.token_stride, c.head_stride, at, Divider((uint32_t)c.tokens), c.ends, c.which, (const float*)nullptr, c.tokens, c.hkv);
+        };
+        return c.dtype == CISR_F32 ? run(int4_read_kernel<D, float>, (float*)c.k, (float*)c.v) : run(int4_read_kernel<D, __nv_bfloat16>, (__nv_bfloat16*)c.k, (__nv_bfloat16*)c.v);
     });
 }
 
@@ -626,27 +642,28 @@ CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void*
 
 // Places that stay into kept [n_req][hkv][keep] (-1 behind the last), their rows and sums to the pages of to_table [n_req][to_width].
 // `longest`: no request has more rows.
-CISR_EXPORT int cisr_int4_evict(void* k_cache, void* v_cache, float* mass, const int* req_slot, const int* block_table, int width, const int* ctx_len, int* kept,
-                                const int* to_table, int to_width, int n_req, int hkv, int dim, int page_size, int keep, int recent, int first, int longest, void* stream) {
-    if (n_req <= 0 || keep <= 0) return 0;
-    if (hkv <= 0 || hkv > 65535 || n_req > 65535 || page_size <= 0 || page_size % INT4_BLOCK || recent < 0 || first < 0 || recent > keep || first > keep - recent) return -2;
-    if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return -2;
-    const Pages pages = pages_of(block_table, width, page_size, hkv);
-    const int between = longest - recent - first;
+CISR_EXPORT int cisr_int4_evict(const Int4EvictCall* call) {
+    const Int4EvictCall& c = *call;
+    if (c.n_req <= 0 || c.keep <= 0) return 0;
+    if (c.hkv <= 0 || c.hkv > 65535 || c.n_req > 65535 || c.page_size <= 0 || c.page_size % INT4_BLOCK || c.recent < 0 || c.first < 0 || c.recent > c.keep ||
+        c.first > c.keep - c.recent) return -2;
+    if (((uintptr_t)c.k_cache | (uintptr_t)c.v_cache) & 15) return -2;
+    const Pages pages = pages_of(c.block_table, c.width, c.page_size, c.hkv);
+    const int between = c.longest - c.recent - c.first;
     const int cached = between < 0 ? 0 : between < SELECT_CACHED ? between : SELECT_CACHED;
-    const size_t smem = sizeof(uint32_t) * (size_t)(cached < SELECT_CACHED ? cached : SELECT_CACHED);
+    const size_t smem = sizeof(uint32_t) * (size_t)cached;
     if (smem > 32 * 1024) {          // with the counts more than the 48 KB that need no leave
         const cudaError_t e = cudaFuncSetAttribute(int4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(uint32_t) * SELECT_CACHED));
         if (e != cudaSuccess) return (int)e;
     }
-    const cudaStream_t s = (cudaStream_t)stream;
-    const int status = launch_kernel(int4_select_kernel, dim3(hkv, n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)mass, req_slot, pages, ctx_len, kept, keep,
-                                     recent, first, cached);
+    const cudaStream_t s = (cudaStream_t)c.stream;
+    const int status = launch_kernel(int4_select_kernel, dim3(c.hkv, c.n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)c.mass, c.req_slot, pages, c.ctx_len, c.kept,
+                                     c.keep, c.recent, c.first, cached);
     if (status) return status;
     constexpr int rows = MOVE_BLOCKS * INT4_BLOCK * (THREADS / 32);
-    const dim3 grid((unsigned)((keep + rows - 1) / rows), hkv, n_req);
-    return by_head_size(dim, [&](auto d) {
-        return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)k_cache, (unsigned char*)v_cache, mass, req_slot, pages,
-                             pages_of(to_table, to_width, page_size, hkv), (const int*)kept, keep);
+    const dim3 grid((unsigned)((c.keep + rows - 1) / rows), c.hkv, c.n_req);
+    return by_head_size(c.dim, [&](auto d) {
+        return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)c.k_cache, (unsigned char*)c.v_cache, c.mass, c.req_slot, pages,
+                             pages_of(c.to_table, c.to_width, c.page_size, c.hkv), (const int*)c.kept, c.keep);
     });
 }

@@ -582,7 +582,7 @@ def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_si
     shape, device = k_cache.shape, k_cache.get_device()
     if (len(shape) == 3 and v_cache.shape == shape and k_cache.dtype is torch.uint8 and v_cache.dtype is torch.uint8 and device >= 0 and v_cache.get_device() == device
             and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[2] == page_size * 9 * dim // 16 and not page_size % INT4_BLOCK and dim in INT4_HEAD_DIMS
-            and (hkv is None or shape[1] == hkv) and (_device is None or device == _device()) and shape[0] * shape[1] * shape[2] < INT4_MAX_BYTES):
+            and (hkv is None or shape[1] == hkv) and (_device is None or device == _device()) and k_cache.numel() < INT4_MAX_BYTES):
         return shape[1], device
     _need(k_cache, torch.uint8, "k_cache", 3); _need(v_cache, torch.uint8, "v_cache", 3)
     if k_cache.numel() >= INT4_MAX_BYTES:
@@ -593,21 +593,33 @@ def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_si
                       f"got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
 
 
-def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, names: tuple, lists: tuple) -> None:
-    """Checks int32 lists of `count` entries each (`req_slot`: any number) and the block table, all on the cache's device."""
-    if not (table.dtype is torch.int32 and table.dim() == 2 and table.is_contiguous() and table.get_device() == device):
-        _need(table, torch.int32, "block_table", 2)
+_int32 = torch.int32
+
+
+def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, names: tuple, req_slot: torch.Tensor, *lists: torch.Tensor) -> None:
+    """Checks req_slot (any number of entries), int32 lists of `count` entries each and the block table, all on the cache's device."""
+    good = (table.dtype is _int32 and table.dim() == 2 and table.is_contiguous() and table.get_device() == device
+            and req_slot.dtype is _int32 and req_slot.dim() == 1 and req_slot.is_contiguous() and req_slot.get_device() == device)
+    for t in lists:
+        good = good and t.dtype is _int32 and t.dim() == 1 and t.numel() == count and t.is_contiguous() and t.get_device() == device
+    if good:
+        return
+    _need(table, _int32, "block_table", 2)
+    if table.get_device() != device:
         raise KernelError(f"{what}: block_table is on {table.device}, the cache on cuda:{device}")
-    for name, t in zip(names, lists):
-        if t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous() and t.get_device() == device and (t.shape[0] == count or name == "req_slot"):
-            continue
-        _need(t, torch.int32, name, 1)
+    for name, t in zip(names, (req_slot,) + lists):
+        _need(t, _int32, name, 1)
         if t.get_device() != device:
             raise KernelError(f"{what}: {name} is on {t.device}, the cache on cuda:{device}")
-        raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
+        if t.numel() != count and name != "req_slot":
+            raise KernelError(f"{what}: {name} must have {count} entries, got {t.numel()}")
 
 
-_ROW_LISTS, _REQUEST_LISTS = ("token_req", "positions", "req_slot"), ("req_slot", "q_start", "q_len", "ctx_len")
+_ROW_LISTS, _REQUEST_LISTS = ("req_slot", "token_req", "positions"), ("req_slot", "q_start", "q_len", "ctx_len")
+# The calls' arguments in the order of csrc/int4_rows.cu and csrc/attention_int4.cu.
+_STORE_CALL, _READ_CALL, _EVICT_CALL = struct.Struct("@10P4q6i").pack, struct.Struct("@11P3q7i").pack, struct.Struct("@9P10i").pack
+_ATTN_INT4_CALL = struct.Struct("@13P2d9i").pack
+_NO_SINK = (float("-inf"), 0)
 
 
 def _int4_mass(what: str, mass: torch.Tensor, k_cache: torch.Tensor, page_size: int) -> None:
@@ -632,13 +644,26 @@ def int4_store(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
         raise KernelError("int4_store: k and v must be alike, float32 or bfloat16 [tokens, kv_heads, head_dim] with neighbouring values, on the cache's device")
     tokens, hkv, dim = shape
     _int4_cache("int4_store", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_store", device, block_table, tokens, _ROW_LISTS, (token_req, positions, req_slot))
+    _int4_lists("int4_store", device, block_table, tokens, _ROW_LISTS, req_slot, token_req, positions)
     if mass is not None:
         _int4_mass("int4_store", mass, k_cache, page_size)
     (k_token, k_head, _), (v_token, v_head, _) = k.stride(), v.stride()
-    _check(_int4_rows().cisr_int4_store(k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], k_token, k_head, v_token, v_head, k_cache.data_ptr(), v_cache.data_ptr(), _p(mass),
-                                        token_req.data_ptr(), positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, tokens, hkv,
-                                        dim, _stream()), "int4_store")
+    try:
+        call = _STORE_CALL(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), 0 if mass is None else mass.data_ptr(), token_req.data_ptr(), positions.data_ptr(),
+                           req_slot.data_ptr(), block_table.data_ptr(), _stream(), k_token, k_head, v_token, v_head, _DTYPE_CODE[k.dtype], block_table.size(1), page_size, tokens,
+                           hkv, dim)
+    except struct.error as err:          # a number that is none, or beyond what the kernels take
+        raise KernelError(f"int4_store: {err}") from err
+    _check(_int4_rows().cisr_int4_store(call), "int4_store")
+
+
+def _read_call(what: str, k_cache, v_cache, k_out, v_out, token_req, positions, req_slot, block_table, ends, which, strides: tuple, page_size, n_req, tokens, hkv, dim) -> None:
+    try:
+        call = _READ_CALL(k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), token_req, positions, req_slot.data_ptr(), block_table.data_ptr(), ends, which,
+                          _stream(), *strides, dtype_code(k_out.dtype), block_table.size(1), page_size, n_req, tokens, hkv, dim)
+    except struct.error as err:
+        raise KernelError(f"{what}: {err}") from err
+    _check(_int4_rows().cisr_int4_read(call), what)
 
 
 def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, token_req: torch.Tensor, positions: torch.Tensor,
@@ -650,9 +675,9 @@ def int4_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor,
     _, device = _int4_cache("int4_read", k_cache, v_cache, page_size, hkv, dim)
     if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_read: k_out and v_out differ in shape, or lie elsewhere than the cache")
-    _int4_lists("int4_read", device, block_table, tokens, _ROW_LISTS, (token_req, positions, req_slot))
-    _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), 0, hkv * dim, dim, _p(token_req),
-                                       _p(positions), _p(req_slot), _p(block_table), block_table.shape[1], page_size, 0, 0, 1, tokens, hkv, dim, _stream()), "int4_read")
+    _int4_lists("int4_read", device, block_table, tokens, _ROW_LISTS, req_slot, token_req, positions)
+    _read_call("int4_read", k_cache, v_cache, k_out, v_out, token_req.data_ptr(), positions.data_ptr(), req_slot, block_table, 0, 0, (0, hkv * dim, dim), page_size, 1, tokens,
+               hkv, dim)
 
 
 def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
@@ -665,15 +690,14 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
     if v_out.shape != k_out.shape or k_out.get_device() != device or v_out.get_device() != device:
         raise KernelError("int4_expand: k_out and v_out differ in shape, or lie elsewhere than the cache")
     if requests is None:
-        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "ctx_len"), (req_slot, ctx_len))
+        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "ctx_len"), req_slot, ctx_len)
     else:
-        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "requests"), (req_slot, requests))
-        _int4_lists("int4_expand", device, block_table, req_slot.numel(), ("ctx_len",), (ctx_len,))
+        _int4_lists("int4_expand", device, block_table, n, ("req_slot", "requests"), req_slot, requests)
+        _int4_lists("int4_expand", device, block_table, req_slot.numel(), ("req_slot", "ctx_len"), req_slot, ctx_len)
     if requests is None and req_slot.numel() < n:
         raise KernelError(f"int4_expand: req_slot has {req_slot.numel()} entries for {n} requests")
-    _check(_int4_rows().cisr_int4_read(_p(k_cache), _p(v_cache), _p(k_out), _p(v_out), dtype_code(k_out.dtype), hkv * rows * dim, dim, rows * dim, 0, 0,
-                                       _p(req_slot), _p(block_table), block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()),
-           "int4_expand")
+    _read_call("int4_expand", k_cache, v_cache, k_out, v_out, 0, 0, req_slot, block_table, ctx_len.data_ptr(), 0 if requests is None else requests.data_ptr(),
+               (hkv * rows * dim, dim, rows * dim), page_size, n, rows, hkv, dim)
 
 
 def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
@@ -691,7 +715,7 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     tokens, hq, dim = q.shape
     hkv, device = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
     n = q_len.numel()
-    _int4_lists("attn_decode_int4", device, block_table, n, _REQUEST_LISTS, (req_slot, q_start, q_len, ctx_len))
+    _int4_lists("attn_decode_int4", device, block_table, n, _REQUEST_LISTS, req_slot, q_start, q_len, ctx_len)
     if out.shape != q.shape or hq % hkv or max_queries < 1 or longest < 1 or req_slot.numel() < n or q.get_device() != device or out.get_device() != device:
         raise KernelError("attn_decode_int4: shapes, heads, limits, lists or devices disagree")
     if (window is not None and window < 1) or keep_first < 0:
@@ -706,10 +730,15 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
         lib = _attention_int4(dim, q.dtype)
         launches, floats = divmod(lib.cisr_attn_int4_scratch(n, max_queries, longest, hq, hkv, window or 0, keep_first, mass is not None), 10 ** 12)
         call = _attention_int4_calls[key] = (lib.cisr_attn_int4, floats, launches)
-    scratch = torch.empty(call[1], dtype=torch.float32, device=q.device)
-    _check(call[0](q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-                   q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), scratch.data_ptr(), _p(mass), n, max_queries, longest, hq, hkv, page_size, scale,
-                   window or 0, keep_first, *_sink(sink, hq), _stream()), "attn_decode_int4", own=call[2])
+    scratch = torch.empty(call[1], dtype=torch.float32, device=q.device) if call[1] else None
+    number, per_head = _NO_SINK if sink is None else _sink(sink, hq)
+    try:
+        packed = _ATTN_INT4_CALL(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
+                                 q_len.data_ptr(), ctx_len.data_ptr(), 0 if scratch is None else scratch.data_ptr(), 0 if mass is None else mass.data_ptr(), per_head, _stream(),
+                                 scale, number, block_table.size(1), n, max_queries, longest, hq, hkv, page_size, window or 0, keep_first)
+    except struct.error as err:
+        raise KernelError(f"attn_decode_int4: {err}") from err
+    _check(call[0](packed), "attn_decode_int4", own=call[2])
 
 
 def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
@@ -736,9 +765,9 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         raise KernelError("attn_prefill_int4: a window has at least one key, and keep_first is not negative")
     requests, places = (None, None) if portions is None else portions
     n = n_all if requests is None else requests.numel()
-    _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS, (req_slot, q_start, q_len, ctx_len))
+    _int4_lists("attn_prefill_int4", device, block_table, n_all, _REQUEST_LISTS, req_slot, q_start, q_len, ctx_len)
     if portions is not None:
-        _int4_lists("attn_prefill_int4", device, block_table, n_all, ("req_slot", "places"), (requests, places))
+        _int4_lists("attn_prefill_int4", device, block_table, n_all, ("req_slot", "places"), requests, places)
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     if span == PREFILL_TILE:
         lists = (req_slot, q_start, q_len, ctx_len) if requests is None else [t[requests.long()] for t in (req_slot, q_start, q_len, ctx_len)]
@@ -774,7 +803,7 @@ def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor,
     bytes_ = k_cache.shape[2] if k_cache.dim() == 3 else 0
     dim = bytes_ * 16 // (9 * page_size) if page_size > 0 else 0
     _, device = _int4_cache("int4_evict", k_cache, v_cache, page_size, hkv, dim)
-    _int4_lists("int4_evict", device, block_table, n, ("req_slot", "ctx_len"), (req_slot, ctx_len))
+    _int4_lists("int4_evict", device, block_table, n, ("req_slot", "ctx_len"), req_slot, ctx_len)
     _int4_mass("int4_evict", mass, k_cache, page_size)
     if kept.get_device() != device or to_table.get_device() != device:
         raise KernelError("int4_evict: kept and to_table must lie on the cache's device")
@@ -782,8 +811,12 @@ def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor,
         raise KernelError("int4_evict: req_slot and to_table need an entry per request, and to_table room for the rows that stay")
     if recent < 0 or first < 0 or first + recent > keep:
         raise KernelError(f"int4_evict: {first} first and {recent} recent rows do not fit {keep} that stay")
-    _check(_int4_rows().cisr_int4_evict(_p(k_cache), _p(v_cache), _p(mass), _p(req_slot), _p(block_table), block_table.shape[1], _p(ctx_len), _p(kept), _p(to_table),
-                                        to_table.shape[1], n, hkv, dim, page_size, keep, recent, first, longest, _stream()), "int4_evict", own=2)
+    try:
+        call = _EVICT_CALL(k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), ctx_len.data_ptr(), kept.data_ptr(),
+                           to_table.data_ptr(), _stream(), block_table.size(1), to_table.size(1), n, hkv, dim, page_size, keep, recent, first, longest)
+    except struct.error as err:
+        raise KernelError(f"int4_evict: {err}") from err
+    _check(_int4_rows().cisr_int4_evict(call), "int4_evict", own=2)
 
 
 # ------------------------------------------------------------------ merge of the key ranges + output projection (decode steps)
