@@ -53,9 +53,9 @@ constexpr float SLACK = 4.f, USUAL_SHIFT = 9.f, LARGE_SHIFT = -5.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 constexpr int MAX_RANKED = 128;                                    // requests that are put in order of length, a thread each
 
-// Warps of a thread block: eight where a warp's registers let two such blocks share an SM.
-template <int NT> constexpr int warps_of() { return NT == 1 && TERMS == 1 ? 8 : 4; }
-template <int NT> constexpr int blocks_of() { return NT == 1 ? (TERMS == 1 ? 2 : 3) : 2; }
+// Thread blocks of four warps, and for bfloat16 queries of up to 8 rows also of eight (`Shape` chooses); blocks of an SM by a warp's registers.
+constexpr int MOST_WARPS = TERMS == 1 ? 8 : 4;
+template <int NT, int WARPS> constexpr int blocks_of() { return NT == 1 ? (TERMS == 1 ? 16 / WARPS : 3) : 2; }
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -196,9 +196,9 @@ struct Joined {
 // subtracted from them (and the subnormals made normal) by one instruction for two.  The matrix instructions align their
 // products by the operands' exponent fields, so that a sum over subnormals keeps some 2^-18 of its largest term only: far below the
 // rounding of a bfloat16 output, but not of a float one.
-template <int NT>
-__global__ void __launch_bounds__(32 * warps_of<NT>(), blocks_of<NT>()) attn_int4_kernel(const __grid_constant__ Args a) {
-    constexpr int ROWS = 8 * NT, WARPS = warps_of<NT>(), THREADS = 32 * WARPS;
+template <int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT, THREADS = 32 * WARPS;
     constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
     constexpr int MERGE_STRIDE = D + 4;                  // rows of whole 16 bytes
@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
 bool g_pdl = false;
 int* g_error = nullptr;
 
-template <int NT> constexpr size_t dynamic_smem() {
-    constexpr size_t ring = (size_t)warps_of<NT>() * 2 * (tile_keys<NT>() / INT4_BLOCK) * BLOCK_BYTES, merge = sizeof(float) * warps_of<NT>() * 8 * NT * (D + 4);
+template <int NT, int WARPS> constexpr size_t dynamic_smem() {
+    constexpr size_t ring = (size_t)WARPS * 2 * (tile_keys<NT>() / INT4_BLOCK) * BLOCK_BYTES, merge = sizeof(float) * WARPS * 8 * NT * (D + 4);
     return ring > merge ? ring : merge;
 }
 
@@ -839,33 +839,33 @@ int sm_count(int device) {
 }
 
 // Lets the kernel take its shared memory on a device, once.
-template <int NT> cudaError_t prepare_kernel(int device) {
+template <int NT, int WARPS> cudaError_t prepare_kernel(int device) {
     static bool done[MAX_DEVICES] = {};
     if (done[device]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_smem<NT>());
+    const cudaError_t e = cudaFuncSetAttribute(attn_int4_kernel<NT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_smem<NT, WARPS>());
     done[device] = e == cudaSuccess;
     return e;
 }
 
 // Thread blocks of the kernel that run at once on a device in clusters of `size`: a cluster lies in one part of the chip, whose
 // last places it may not fill (48 clusters of 6 took two rounds where 296 blocks have places).
-template <int NT> int places(int device, int size) {
+template <int NT, int WARPS> int places(int device, int size) {
     static int known[MAX_DEVICES][MAX_CLUSTER + 1] = {};
     if (!known[device][size]) {
-        constexpr size_t SMEM = dynamic_smem<NT>();
+        constexpr size_t SMEM = dynamic_smem<NT, WARPS>();
         int n = 0;
-        if (prepare_kernel<NT>(device) != cudaSuccess) return size;
+        if (prepare_kernel<NT, WARPS>(device) != cudaSuccess) return size;
         if (size == 1) {
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_int4_kernel<NT>, 32 * warps_of<NT>(), SMEM) != cudaSuccess) n = 0;
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_int4_kernel<NT, WARPS>, 32 * WARPS, SMEM) != cudaSuccess) n = 0;
             n *= sm_count(device);
         } else {
             cudaLaunchConfig_t config = {};
-            config.gridDim = dim3(1, 1, size); config.blockDim = dim3(32 * warps_of<NT>()); config.dynamicSmemBytes = SMEM;
+            config.gridDim = dim3(1, 1, size); config.blockDim = dim3(32 * WARPS); config.dynamicSmemBytes = SMEM;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
             attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = (unsigned)size;
             config.attrs = attr; config.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, attn_int4_kernel<NT>, &config) != cudaSuccess) n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, attn_int4_kernel<NT, WARPS>, &config) != cudaSuccess) n = 0;
             n *= size;
         }
         cudaGetLastError();
@@ -877,32 +877,55 @@ template <int NT> int places(int device, int size) {
 // What a launch has of everything: query rows of a tile (8, or 16 where requests bring more), tiles per request, rows that scratch is kept
 // for (even, so that pairs are aligned), splits of a request's keys and whether they are one cluster.
 struct Shape {
-    int rows, tiles, stride, splits, cluster;
+    int rows, tiles, stride, splits, cluster, warps;
     bool ranked;
     long long units;                 // requests by tiles by key heads by rows
     long long keys;
+    int room_of(int device, int w, int size) const {
+        if (rows == 16) return places<2, 4>(device, size);
+        return w == MOST_WARPS ? places<1, MOST_WARPS>(device, size) : places<1, 4>(device, size);
+    }
+    // How long `blocks` of w warps take, `tiles` to a warp, in the time that an SM takes for one warp's tile when it is full (0.22 us of 64
+    // keys of 128 for bfloat16, 0.38 for float, 0.16 and 0.27 of 32 keys for 16 rows).  A tile of a warp alone takes LATENCY of that, a
+    // block's start and end FIXED, the launch and a cluster's joining some more.  Blocks beyond those that run at once come in rounds.
+    // Fitted to 1 to 128 requests of 150 to 8000 keys in 1 to 8 splits; right within a fifth, and in the order of what it compares: us of
+    // 8 and 4 warps, 8 key heads of 128: 48 x 3000 keys 49 and 41, 64 x 500 22.6 and 16.1, 32 x 4000 38 and 41, in two splits 49 and 41.
+    double estimate(long long blocks, int room, int sms, int w, double tiles_of_warp, int parts) const {
+        const double FIXED = rows == 8 ? (TERMS == 1 ? 29 : 18) : (TERMS == 1 ? 63 : 51), LATENCY = rows == 8 ? (TERMS == 1 ? 8 : 5) : 5;
+        const auto round = [&](long long n) {                       // of n blocks
+            const double sharing = (double)w * ((n + sms - 1) / sms);
+            return FIXED + tiles_of_warp * (sharing > LATENCY ? sharing : LATENCY);
+        };
+        return 12 + (parts > 1 ? 10 : 0) + (double)(blocks / room) * round(room) + (blocks % room ? round(blocks % room) : 0);
+    }
+    // Eight warps unless four are clearly better: of requests of unlike lengths the larger blocks' last round is shorter than estimated (64 of 4000
+    // to 8000 keys: 95 us, with four warps 104 to 114, where equal ones are 123 and 117).
+    static constexpr double FEWER_WARPS = 0.9;
     Shape(int device, int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
         const int needed = max_queries * (hq / hkv);
         rows = needed > 8 ? 16 : 8;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
-        const int warps = rows == 8 ? warps_of<1>() : warps_of<2>(), TK = rows == 8 ? tile_keys<1>() : tile_keys<2>();
-        const auto room_of = [&](int size) { return rows == 8 ? places<1>(device, size) : places<2>(device, size); };
-        const long long pairs = (long long)n_req * tiles * hkv, room = room_of(1);
+        const long long pairs = (long long)n_req * tiles * hkv;
         long long reach = longest;
         if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
-        // A block takes as long as its warps' tiles and some five more for its start and end (fitted to the times of 1 to 3 splits); blocks beyond
-        // those that run at once come in rounds, of which the last is not even.  The count of splits with the least of it; up to a cluster's size,
-        // where that leaves no SM idle, else more, which another kernel joins.
-        const double tiles_of_warp = (double)reach / (TK * warps);
-        const int most = (int)((reach + (long long)TK * warps - 1) / (TK * warps));      // a tile for every warp
-        splits = 1;
+        const int sms = sm_count(device);
         double best = 0;
-        for (int s = 1; s <= (most < MAX_CLUSTER ? most : MAX_CLUSTER); ++s) {
-            const double rounds = (double)pairs * s / room_of(s), time = (rounds > 1 ? rounds + 0.4 : 1) * (5 + tiles_of_warp / s);
-            if (s == 1 || time < best) { best = time; splits = s; }
+        long long most = 0;
+        warps = 0;
+        for (int w = rows == 8 ? MOST_WARPS : 4; w >= 4; w /= 2) {
+            const int per_block = (rows == 8 ? tile_keys<1>() : tile_keys<2>()) * w;                  // keys of a tile for every warp
+            const long long parts = (reach + per_block - 1) / per_block;
+            double least = 0;
+            int n_least = 1;
+            for (int n = 1; n <= (parts < MAX_CLUSTER ? parts : MAX_CLUSTER); ++n) {
+                const double time = estimate(pairs * n, room_of(device, w, n), sms, w, (parts + n - 1) / n, n);
+                if (n == 1 || time < least) { least = time; n_least = n; }
+            }
+            if (warps == 0 || least < FEWER_WARPS * best) { best = least; splits = n_least; warps = w; most = parts; }
         }
-        if (splits == MAX_CLUSTER && pairs * MAX_CLUSTER < room / 2) {
+        const long long room = room_of(device, warps, 1);
+        if (splits == MAX_CLUSTER && pairs * MAX_CLUSTER < room / 2) {                                // SMs idle: as many as there are places for
             const long long want = (room + pairs - 1) / pairs;
             splits = (int)(want < most ? want : most);
             if (splits > 64) splits = 64;
@@ -920,13 +943,12 @@ struct Shape {
     int launches(bool mass) const { return 1 + merged_by_kernel() + (mass && mass_by_kernel()); }
 };
 
-template <int NT> int launch(int device, Args& a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
-    constexpr int WARPS = warps_of<NT>();
-    constexpr size_t SMEM = dynamic_smem<NT>();
-    if (const cudaError_t e = prepare_kernel<NT>(device); e != cudaSuccess) return (int)e;
+template <int NT, int WARPS> int launch(int device, Args& a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
+    constexpr size_t SMEM = dynamic_smem<NT, WARPS>();
+    if (const cudaError_t e = prepare_kernel<NT, WARPS>(device); e != cudaSuccess) return (int)e;
     const dim3 grid((unsigned)(n_req * a.tiles), (unsigned)a.hkv, (unsigned)a.n_splits);
     a.mass = shape.mass_by_kernel() ? nullptr : mass;
-    int status = launch_kernel_cluster(attn_int4_kernel<NT>, grid, dim3(32 * WARPS), SMEM, s, g_pdl, a.cluster, a);
+    int status = launch_kernel_cluster(attn_int4_kernel<NT, WARPS>, grid, dim3(32 * WARPS), SMEM, s, g_pdl, a.cluster, a);
     if (status) return status;
     if (shape.merged_by_kernel()) {
         status = launch_kernel(attn_int4_merge_kernel<8 * NT>, dim3(grid.x, grid.y, (unsigned)a.row_stride), dim3(D), 0, s, true, a);
@@ -988,5 +1010,6 @@ CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
     while (a.rank_threads < c.n_req && a.rank_threads < MAX_RANKED) a.rank_threads *= 2;
     a.longest = c.longest; a.hq = c.hq; a.hkv = c.hkv; a.page_size = c.page_size; a.window = c.window; a.keep_first = c.keep_first;
     a.scale = (float)c.scale; a.sink_all = (float)c.sink; a.sink_heads = c.sink_heads; a.error = g_error;
-    return shape.rows == 8 ? launch<1>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream) : launch<2>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
+    const auto run = shape.rows == 16 ? launch<2, 4> : shape.warps == MOST_WARPS ? launch<1, MOST_WARPS> : launch<1, 4>;
+    return run(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
 }
