@@ -19,6 +19,12 @@
 // Operands other than codes are float16: of queries, normed by a power of two per row, exactly what bfloat16 holds (elements below 2^-24 of
 // the row's largest lose digits); of probabilities 11 bits.  Float queries take two float16 terms (22 bits) for both.
 // Scores, running maxima, sums and outputs are float.
+//
+// What bounds it: with many long requests the instructions around the products (219 per 16 keys and warp at head size 128 and up to 8
+// rows) at 71 % of the rate of memory: 64 requests of 4000 to 8000 rows, 32 heads over 8 of 128, 96 us of 68; float queries, whose
+// products are two, half of that rate; with few or short requests the way from one trip to memory to the next, some 5 us of a block
+// (one request of 700 rows 8 to 10 us, of 8000 12).  Besides (us, 32 heads over 8 of 128): 32 x 4000 rows 38 (memory 22), 48 x 3000 41 (25), 64 x 500 16 (6);
+// five tokens each of 8 requests of 3000 rows 29: 20 rows are two tiles of 16, and each reads and unpacks the keys again.
 #include <climits>
 
 #include "int4_cache.cuh"
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     // The key heads of a request's tile of rows are neighbours in the order of thread blocks (a page's heads lie side by side), and where
     // not all blocks run at once the longest requests come first, so that the last blocks to end are short ones: 64 requests of 4000 to
-    // 8000 rows 111 us in the order of requests.
+    // 8000 rows 96 us, in the order of requests 111.
     const int split = blockIdx.z, id = blockIdx.x + gridDim.x * blockIdx.y;
     int unit_of = a.by_heads(id);
     const int kvh = id - unit_of * a.hkv;

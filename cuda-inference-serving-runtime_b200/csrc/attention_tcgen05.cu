@@ -262,7 +262,8 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             for (int b = lane; b < NSUB * boxes; b += 32) {       // lane b: box b (64-column half, run of box_rows keys)
                 const int i = b % boxes, sub = b / boxes;
                 const int kpos = tile_k0(j) + i * box_rows;
-                const int page = kpos < k_end ? __ldg(table + kpos / page_size) : -1;     // the table is older than the kernel before
+                // the table is older than the kernel before; rows written out for this call are one page, and a request that has more gets zeros
+                const int page = kpos < k_end && (!HALF_OPERANDS || kpos < page_size) ? __ldg(table + kpos / page_size) : -1;
                 const int row = page < 0 ? cache_rows : (page * hkv + kvh) * page_size + kpos % page_size;   // beyond the cache: zeros
                 tma_load_2d(ring + s * KV_BYTES + sub * KV_SUB + i * box_rows * 128, map, sub * 64, row, full + s);
             }

@@ -749,7 +749,8 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     runs over those, so codes are turned into operands once per key and not once per tile of queries.
     Tiles of `span` queries, 128 or 256 (bfloat16, head sizes 64 and 128), as (request, first query) as for `attn_prefill_wide`, with float16
     operands, whose eleven binary digits are those of a held value; a held value that is NaN reaches the queries before it, too, as
-    it does there.  `longest`: no request that is written out has more rows.  `portions` (requests, places): the requests that are
+    it does there.  `longest`: no request that is written out has more rows (a bound will do; one that has sets the
+    flag that `raise_if_kernel_gave_up` reads).  `portions` (requests, places): the requests that are
     written out, and for every request of the step its place in that list (any number for the others); None: all, in order.
 
     `span` 64 is for the other types and head sizes: `attn_decode_int4` of the requests that are listed (the tiles are not looked at), no
@@ -771,7 +772,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     if span == PREFILL_TILE:
         lists = (req_slot, q_start, q_len, ctx_len) if requests is None else [t[requests.long()] for t in (req_slot, q_start, q_len, ctx_len)]
-        attn_decode_int4(q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], min(max_queries or q.shape[0], max(1, q.shape[0])), longest, page_size, scale, window, sink,
+        attn_decode_int4(q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], max(1, min(max_queries or q.shape[0], q.shape[0])), longest, page_size, scale, window, sink,
                          keep_first)
         return
     if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
@@ -783,7 +784,8 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     halves, factors = torch.empty(q.shape, dtype=torch.float16, device=q.device), torch.empty(n * hkv * 2 + n + q.shape[0] * hq, device=q.device)
     table, q_factor = factors.data_ptr() + 8 * n * hkv, factors.data_ptr() + 8 * n * hkv + 4 * n
     _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), _p(k), _p(v), _p(factors), table, _p(q), _p(halves), q_factor, q.shape[0] * hq, _p(req_slot), _p(block_table),
-                                         block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _stream()), "attn_prefill_int4", own=2)
+                                         block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim,
+                                         _p(_error_flag()), _stream()), "attn_prefill_int4", own=2)
     _check(lib.cisr_attn_prefill_tcgen05(_p(halves), _p(out), q.shape[0], _p(k), _p(v), n, table if places is None else _p(places), table, 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
                                          _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor,
                                          _p(factors), _stream()), "attn_prefill_int4")

@@ -391,6 +391,38 @@ def test_weights_of_keys(hq, hkv, dim, window, sink, dtype):
     assert torch.equal(cache.attend(q, q_len, window=window, sink=sink), got)
 
 
+def test_nothing_to_do():
+    """No tokens, no requests, no rows: nothing is written, nothing fails."""
+    cache = Cache([20], 2, 64, 16)
+    none, empty = i32([]), torch.empty((0, 2, 64), device="cuda")
+    before = cache.k_cache.clone()
+    places = (cache.k_cache, cache.v_cache)
+    kernels.int4_store(empty, empty, *places, none, none, cache.slots, cache.table, 16)
+    kernels.int4_read(*places, empty, empty, none, none, cache.slots, cache.table, 16)
+    kernels.int4_expand(*places, empty.view(0, 2, 0, 64), empty.view(0, 2, 0, 64), none, cache.table, none, 16)
+    for dtype, span in ((torch.float32, 64), (torch.bfloat16, 128)):
+        q = torch.empty((0, 4, 64), dtype=dtype, device="cuda")
+        kernels.attn_decode_int4(q, q, *places, none, cache.table, none, none, none, 1, 20, 16, 0.125)
+        kernels.attn_prefill_int4(q, q, *places, none, cache.table, none, none, none, none, none, 20, 16, 0.125, span=span)
+        kernels.attn_prefill_int4(q, q, *places, cache.slots, cache.table, none, none, i32([0]), i32([0]), cache.ctx, 20, 16, 0.125, span=span)
+    mass = torch.zeros((cache.pages, 2, 16), device="cuda")
+    kernels.int4_evict(*places, mass, none, cache.table, none, torch.empty((0, 1), dtype=torch.int32, device="cuda"), torch.empty((0, 2, 8), dtype=torch.int32, device="cuda"), 16, 20, 2)
+    kernels.int4_evict(*places, mass, cache.slots, cache.table, cache.ctx, i32([[0]]), torch.empty((1, 2, 0), dtype=torch.int32, device="cuda"), 16, 20, 0)
+    kernels.raise_if_kernel_gave_up()
+    assert torch.equal(cache.k_cache, before)
+
+
+def test_a_prompt_longer_than_the_bound_is_reported():
+    cache = Cache([300], 2, 64, 16)
+    q = queries(40, 4, 64, torch.bfloat16)
+    for longest in (128, 256):
+        kernels.attn_prefill_int4(q, torch.empty_like(q), cache.k_cache, cache.v_cache, cache.slots, cache.table, i32([0]), i32([0]), i32([0]), i32([40]), cache.ctx, longest, 16,
+                                  0.125, span=128)
+        with pytest.raises(KernelError, match="longer than the bound"):
+            kernels.raise_if_kernel_gave_up()
+    kernels.raise_if_kernel_gave_up()
+
+
 # ------------------------------------------------------------------ portions of prompts
 def prompt_bound(dtype, span):
     """Beside `bound`, of the outputs' sizes: over the pages (tiles of 64) nothing.  float16 operands are three binary digits of a code times
