@@ -24,7 +24,7 @@
 // rows) at 71 % of the rate of memory: 64 requests of 4000 to 8000 rows, 32 heads over 8 of 128, 96 us of 68; float queries, whose
 // products are two, half of that rate; with few or short requests the way from one trip to memory to the next, some 5 us of a block
 // (one request of 700 rows 8 to 10 us, of 8000 12).  Besides (us, 32 heads over 8 of 128): 32 x 4000 rows 38 (memory 22), 48 x 3000 41 (25), 64 x 500 16 (6);
-// five tokens each of 8 requests of 3000 rows 29: 20 rows are two tiles of 16, and each reads and unpacks the keys again.
+// five tokens each of 8 requests of 3000 rows 24.
 #include <climits>
 
 #include "int4_cache.cuh"
@@ -198,7 +198,7 @@ struct Joined {
     __device__ __forceinline__ float whole(float sink) const { return sink > -INFINITY ? den + exp2f(fmaf(sink, LOG2E, -m)) : den; }
 };
 
-// NT: columns of 8 query rows.  Where there are two, or float queries, codes serve two matrix instructions, and the offset is
+// NT: columns of 8 query rows.  Where there are two or three, or float queries, codes serve two matrix instructions, and the offset is
 // subtracted from them (and the subnormals made normal) by one instruction for two.  The matrix instructions align their
 // products by the operands' exponent fields, so that a sum over subnormals keeps some 2^-18 of its largest term only: far below the
 // rounding of a bfloat16 output, but not of a float one.
@@ -206,6 +206,7 @@ template <int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_kernel(const __grid_constant__ Args a) {
     constexpr int ROWS = 8 * NT, THREADS = 32 * WARPS;
     constexpr bool OFFSET = NT == 1 && TERMS == 1;       // the offset as a product with a constant
+    constexpr bool Q_SHARED = NT > 2;                    // the queries' operands stay in shared memory
     constexpr float SECOND = OFFSET ? 0.0625f : 1.f;     // of operands that meet codes n 2^-20
     constexpr int MERGE_STRIDE = D + 4;                  // rows of whole 16 bytes
     constexpr int TK = tile_keys<NT>(), HALVES = TK / 16, PLANE_BYTES = TK / INT4_BLOCK * BLOCK_BYTES;
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         if (c == 0) group_sum[r][j] = sum;
     }
     __syncthreads();
-    uint32_t qf[NT][NG][2][TERMS][2];
+    uint4 qf[Q_SHARED ? 1 : NT][NG][TERMS];
     uint32_t qs[NT];                                                // -8 2^-24 sum q of two groups, the first float16 term (c below 2) or the second
     float unit[NT][2];                                              // of a column's sums, in the softmax's exponent (base 2); positive
 #pragma unroll
@@ -362,10 +363,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
 #pragma unroll
         for (int j = 0; j < NG; ++j)
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                const uint4 w = operand[nt * NG + j][term][lane];
-                qf[nt][j][0][term][0] = w.x; qf[nt][j][0][term][1] = w.y; qf[nt][j][1][term][0] = w.z; qf[nt][j][1][term][1] = w.w;
-            }
+            for (int term = 0; term < TERMS; ++term)
+                if constexpr (!Q_SHARED) qf[nt][j][term] = operand[nt * NG + j][term][lane];
         if constexpr (OFFSET) {
             const int j0 = 2 * (c & 1);
             const float s0 = j0 < NG ? -0x1p-21f * group_sum[nt * 8 + g][j0 < NG ? j0 : 0] : 0.f, s1 = j0 + 1 < NG ? -0x1p-21f * group_sum[nt * 8 + g][j0 + 1 < NG ? j0 + 1 : 0] : 0.f;
@@ -416,6 +415,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 float acc[NT][4];
+                uint4 query[NT][TERMS];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int term = 0; term < TERMS; ++term) query[nt][term] = Q_SHARED ? operand[nt * NG + j][term][lane] : qf[Q_SHARED ? 0 : nt][j][term];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t x = k ? w0.w[j] >> 8 : w0.w[j], y = k ? w1.w[j] >> 8 : w1.w[j];
@@ -425,8 +429,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int term = 0; term < TERMS; ++term) {
-                            if (k || term) mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
-                            else mma_f16_new(acc[nt], a0, a1, a2, a3, qf[nt][j][k][term][0], qf[nt][j][k][term][1]);
+                            const uint4& q = query[nt][term];
+                            if (k || term) mma_f16(acc[nt], a0, a1, a2, a3, k ? q.z : q.x, k ? q.w : q.y);
+                            else mma_f16_new(acc[nt], a0, a1, a2, a3, q.x, q.y);
                         }
                 }
                 const float f0 = j & 1 ? high_half(s0.w[j / 2]) : low_half(s0.w[j / 2]), f1 = j & 1 ? high_half(s1.w[j / 2]) : low_half(s1.w[j / 2]);
@@ -880,14 +885,18 @@ template <int NT, int WARPS> int places(int device, int size) {
     return known[device][size];
 }
 
-// What a launch has of everything: query rows of a tile (8, or 16 where requests bring more), tiles per request, rows that scratch is kept
+// What a launch has of everything: query rows of a tile (8, or 16 or 24 where requests bring more), tiles per request, rows that scratch is kept
 // for (even, so that pairs are aligned), splits of a request's keys and whether they are one cluster.
 struct Shape {
     int rows, tiles, stride, splits, cluster, warps;
     bool ranked;
+    int room;                        // thread blocks that run at once, without clusters
     long long units;                 // requests by tiles by key heads by rows
     long long keys;
     int room_of(int device, int w, int size) const {
+#if STORAGE_BF16
+        if (rows == 24) return places<3, 4>(device, size);
+#endif
         if (rows == 16) return places<2, 4>(device, size);
         return w == MOST_WARPS ? places<1, MOST_WARPS>(device, size) : places<1, 4>(device, size);
     }
@@ -897,7 +906,7 @@ struct Shape {
     // Fitted to 1 to 128 requests of 150 to 8000 keys in 1 to 8 splits; right within a fifth, and in the order of what it compares: us of
     // 8 and 4 warps, 8 key heads of 128: 48 x 3000 keys 49 and 41, 64 x 500 22.6 and 16.1, 32 x 4000 38 and 41, in two splits 49 and 41.
     double estimate(long long blocks, int room, int sms, int w, double tiles_of_warp, int parts) const {
-        const double FIXED = rows == 8 ? (TERMS == 1 ? 29 : 18) : (TERMS == 1 ? 63 : 51), LATENCY = rows == 8 ? (TERMS == 1 ? 8 : 5) : 5;
+        const double FIXED = rows == 8 ? (TERMS == 1 ? 29 : 18) : rows == 24 ? 50 : (TERMS == 1 ? 63 : 51), LATENCY = rows == 8 ? (TERMS == 1 ? 8 : 5) : 5;
         const auto round = [&](long long n) {                       // of n blocks
             const double sharing = (double)w * ((n + sms - 1) / sms);
             return FIXED + tiles_of_warp * (sharing > LATENCY ? sharing : LATENCY);
@@ -907,14 +916,12 @@ struct Shape {
     // Eight warps unless four are clearly better: of requests of unlike lengths the larger blocks' last round is shorter than estimated (64 of 4000
     // to 8000 keys: 95 us, with four warps 104 to 114, where equal ones are 123 and 117).
     static constexpr double FEWER_WARPS = 0.9;
-    Shape(int device, int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
-        const int needed = max_queries * (hq / hkv);
-        rows = needed > 8 ? 16 : 8;
+    // Warps and splits for tiles of `height` rows, and how long they take.
+    double choose(int device, int height, int needed, int n_req, int hkv, long long reach) {
+        rows = height;
         tiles = (needed + rows - 1) / rows;
         stride = ((needed < rows ? needed : rows) + 1) & ~1;
         const long long pairs = (long long)n_req * tiles * hkv;
-        long long reach = longest;
-        if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
         const int sms = sm_count(device);
         double best = 0;
         long long most = 0;
@@ -930,12 +937,28 @@ struct Shape {
             }
             if (warps == 0 || least < FEWER_WARPS * best) { best = least; splits = n_least; warps = w; most = parts; }
         }
-        const long long room = room_of(device, warps, 1);
+        room = room_of(device, warps, 1);
         if (splits == MAX_CLUSTER && pairs * MAX_CLUSTER < room / 2) {                                // SMs idle: as many as there are places for
             const long long want = (room + pairs - 1) / pairs;
             splits = (int)(want < most ? want : most);
             if (splits > 64) splits = 64;
         }
+        return best;
+    }
+    Shape(int device, int n_req, int max_queries, int longest, int hq, int hkv, int window, int keep_first) {
+        const int needed = max_queries * (hq / hkv);
+        long long reach = longest;
+        if (window > 0 && (long long)window + keep_first + max_queries < reach) reach = (long long)window + keep_first + max_queries;
+        const double time = choose(device, needed > 8 ? 16 : 8, needed, n_req, hkv, reach);
+#if STORAGE_BF16
+        // A tile of 24 rows takes 1.3 times as long as one of 16 and unpacks the keys once for all: us, 32 heads over 8 of 128, 20 rows of 32
+        // requests of 2500 keys 47 and 72, of 8 of 3000 23.5 and 29; 56 rows (64 over 8 of 64) of 8 of 3000 37 and 31.
+        if (needed > 16) {
+            Shape high = *this;
+            if (1.3 * high.choose(device, 24, needed, n_req, hkv, reach) < time) *this = high;
+        }
+#endif
+        const long long pairs = (long long)n_req * tiles * hkv;
         cluster = splits <= MAX_CLUSTER ? splits : 1;
         ranked = n_req > 1 && n_req <= MAX_RANKED && pairs * splits > room;
         units = pairs * stride;
@@ -1016,6 +1039,9 @@ CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
     while (a.rank_threads < c.n_req && a.rank_threads < MAX_RANKED) a.rank_threads *= 2;
     a.longest = c.longest; a.hq = c.hq; a.hkv = c.hkv; a.page_size = c.page_size; a.window = c.window; a.keep_first = c.keep_first;
     a.scale = (float)c.scale; a.sink_all = (float)c.sink; a.sink_heads = c.sink_heads; a.error = g_error;
+#if STORAGE_BF16
+    if (shape.rows == 24) return launch<3, 4>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
+#endif
     const auto run = shape.rows == 16 ? launch<2, 4> : shape.warps == MOST_WARPS ? launch<1, MOST_WARPS> : launch<1, 4>;
     return run(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
 }
