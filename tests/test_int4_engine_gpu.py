@@ -58,7 +58,10 @@ class Plain:
             q, k, v = self.rounded(turned[:hq]), self.rounded(turned[hq:]), self.rounded(qkv[hq + hkv:])
             keys.append(plain_int4.held(k)); values.append(plain_int4.held(v))
             ks, vs = torch.stack(keys, 1).repeat_interleave(hq // hkv, 0), torch.stack(values, 1).repeat_interleave(hq // hkv, 0)
-            p = torch.softmax(torch.einsum("hd,hjd->hj", q, ks) * dim ** -0.5, -1)
+            scores = torch.einsum("hd,hjd->hj", q, ks) * dim ** -0.5
+            if mixer.window:
+                scores[:, :max(0, len(keys) - mixer.window)] = -torch.inf
+            p = torch.softmax(scores, -1)
             out = self.rounded(torch.einsum("hj,hjd->hd", p, vs).reshape(-1))
             x = x + mixer.o.double() @ out
             h = self.rounded(self.norm(x, n2))
@@ -110,6 +113,35 @@ def test_logits_are_those_of_a_cache_in_4_bits(dtype, heads, kv_heads, hidden, g
         stepper.release("a"); stepper.release("b")
         stepper.cache.check()
     assert ((results[0] - results[1]).square().mean(-1).sqrt() / spread).median() < (6.8e-2 if dtype == "bfloat16" else 2e-4)
+
+
+@pytest.mark.parametrize("dtype,dim", [("float32", 32), ("bfloat16", 64), ("bfloat16", 96)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_layer_with_a_window(dtype, dim, graph):
+    """A layer that sees 40 keys, whose pages go back as they are passed, behind one that sees all."""
+    from cisr_b200 import Model, StepEntry
+    from test_toy_parts_gpu import W_CONFIG, register_windowed_toy
+
+    register_windowed_toy()
+    model = Model.from_config(dict(W_CONFIG, hidden_size=4 * dim, head_dim=dim, vocab_size=256), seed=5, dtype=dtype)
+    prompt, reply = tokens_of(100, 1), tokens_of(60, 2)
+    plain = Plain(model)
+    want = torch.stack([plain.token(t, i) for i, t in enumerate(prompt + reply)])
+    for portions in ([100], [45, 3, 52]):
+        stepper = stepper_of(model, graph=graph)
+        stepper.create("a")
+        got, at = [], 0
+        for n in portions:
+            got.append(stepper.step([StepEntry("a", prompt[at:at + n], list(range(n)))]).clone())
+            at += n
+        for t in reply:
+            got.append(stepper.step([StepEntry("a", [t], [0])]).clone())
+            stepper.cache.check()
+        stepper.check_kernels()
+        windowed = next(g for g in stepper.cache.page_groups if g.use.window)
+        assert windowed.pool.n_used <= 40 // 8 + 1
+        off = (torch.cat(got).double() - want).square().mean(-1).sqrt() / want.std()
+        assert off.median() < (6.8e-2 if dtype == "bfloat16" else 2e-4), off
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
