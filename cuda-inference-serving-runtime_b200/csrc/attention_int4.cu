@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     const int split = blockIdx.z, id = blockIdx.x + gridDim.x * blockIdx.y;
     int unit_of = a.by_heads(id);
     const int kvh = id - unit_of * a.hkv;
-    pdl_wait();
+    pdl_trigger();
+    // Lengths, places in q and the table are older than the kernel before this one (which brings queries and rows): they are read beside its end.
     if (a.ranked) {
         __shared__ int lens[MAX_RANKED], before[MAX_RANKED], chosen;
         for (int i = tid; i < a.n_req; i += THREADS) { lens[i] = a.ctx_len[i]; before[i] = 0; }
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         unit_of += (chosen - rank) * a.tiles;
     }
     Span<TK> span;
-    if (!find_span<ROWS>(span, a, unit_of)) return;                 // the same for a whole cluster
+    if (!find_span<ROWS>(span, a, unit_of)) return pdl_wait();      // the same for a whole cluster
     const size_t base_row = ((size_t)unit_of * a.hkv + kvh) * a.row_stride;
     const int* pages = a.table + (size_t)span.slot * a.width;
     const int tok0 = span.tok0;
@@ -271,8 +272,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     uint32_t here, next;                                            // of this tile, of the next one
+    here = look_up(warp); next = look_up(warp + WARPS);             // on their way at once
+    pdl_wait();
     const auto begin = [&] {
-        here = look_up(warp); next = look_up(warp + WARPS);         // on their way at once
         fetch(a.k_cache, landing, here, warp < n_tiles);
         fetch(a.v_cache, landing + PLANE_BYTES, here, warp < n_tiles);
     };
@@ -611,6 +613,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
             }
         if (shift == LARGE_SHIFT || !__any_sync(0xffffffffu, all != 0.f)) break;
         shift = LARGE_SHIFT;
+        here = look_up(warp); next = look_up(warp + WARPS);
         begin();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -203,11 +203,11 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
                                                              long long v_head, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
                                                              Place at, int tokens, int hkv, int wide) {
     pdl_wait();
+    pdl_trigger();
     const long long rows = (long long)tokens * hkv;
     const int key_units = (int)((rows + THREADS / LANES - 1) / (THREADS / LANES));
     if ((int)blockIdx.x < key_units) store_rows<D, T, false>(k, k_token, k_head, k_cache, mass, at, tokens, hkv, wide & 1, blockIdx.x);
     else store_rows<D, T, true>(v, v_token, v_head, v_cache, mass, at, tokens, hkv, wide & 2, blockIdx.x - key_units);
-    pdl_trigger();
 }
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
@@ -363,12 +363,12 @@ __global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char*
                                                             Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
                                                             int tokens, int hkv) {
     pdl_wait();
+    pdl_trigger();
     const long long rows = (long long)tokens * hkv;
     constexpr int EACH = READ_ROWS * (THREADS / LANES);
     const int key_units = (int)((rows + EACH - 1) / EACH);
     if ((int)blockIdx.x < key_units) read_rows<D, T, false>(k_cache, k, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x);
     else read_rows<D, T, true>(v_cache, v, req_stride, token_stride, head_stride, at, by_tokens, ends, which, factors, tokens, hkv, blockIdx.x - key_units);
-    pdl_trigger();
 }
 
 // ------------------------------------------------------------------ eviction
