@@ -772,7 +772,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     rows = -(-longest // WIDE_TILE) * WIDE_TILE                  # one page per request, of whole key tiles
     if span == PREFILL_TILE:
         lists = (req_slot, q_start, q_len, ctx_len) if requests is None else [t[requests.long()] for t in (req_slot, q_start, q_len, ctx_len)]
-        attn_decode_int4(q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], max(1, min(max_queries or q.shape[0], q.shape[0])), longest, page_size, scale, window, sink,
+        _untimed["attn_decode_int4"](q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], max(1, min(max_queries or q.shape[0], q.shape[0])), longest, page_size, scale, window, sink,
                          keep_first)
         return
     if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
@@ -2746,6 +2746,8 @@ _DESCRIBE = {
     "int4_read": lambda k_cache, v_cache, k_out, *a, **kw: tuple(int(n) for n in k_out.shape),
     "int4_expand": lambda k_cache, v_cache, k_out, *a, **kw: tuple(int(n) for n in k_out.shape),
     "attn_decode_int4": lambda q, out, k_cache, v_cache, req_slot, block_table, q_start, q_len, ctx_len, max_queries, longest, *a, **kw:
+        (int(q.shape[0]), int(q.shape[1]), int(k_cache.shape[1]), int(q.shape[2]), int(longest)),
+    "attn_prefill_int4": lambda q, out, k_cache, v_cache, req_slot, block_table, tile_req, tile_q0, q_start, q_len, ctx_len, longest, *a, **kw:
         (int(q.shape[0]), int(q.shape[1]), int(k_cache.shape[1]), int(q.shape[2]), int(longest)),
     "int4_evict": lambda k_cache, v_cache, mass, req_slot, block_table, ctx_len, to_table, kept, *a, **kw: tuple(int(n) for n in kept.shape),
     "merge_out_proj": lambda partial, stats, n_splits, dec_req, q_start, n_dec, hq, dim, w, out, **kw:

@@ -764,6 +764,44 @@ def test_captured_replayed_and_on_two_streams():
     kernels.raise_if_kernel_gave_up()
 
 
+@pytest.mark.parametrize("dtype,span", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_prompts_and_cuts_captured_and_replayed(dtype, span):
+    """A portion's attention, a weighed step and a cut in one capture, replayed with other contents, lengths and pages."""
+    hq, hkv, dim, page = 8, 2, 64, 16
+    cache = Cache([300, 180], hkv, dim, page, spare=20)
+    q = queries(80, hq, dim, dtype)
+    mass, kept = torch.zeros((cache.pages, hkv, page), device="cuda"), torch.empty((2, hkv, 64), dtype=torch.int32, device="cuda")
+    to = i32(cache.free[:8]).view(2, 4)
+    tiles = [(r, a) for r, n in ((0, 50), (1, 30)) for a in range(0, n, span)]
+    lists = [i32(x) for x in ([r for r, _ in tiles], [a for _, a in tiles], [0, 50], [50, 30], [49, 79], [1, 1])]
+    k_out, v_out = torch.empty((2, 2, hkv, 64, dim), device="cuda")
+
+    def turn():
+        out, last = torch.empty_like(q), torch.zeros_like(q)
+        places = (cache.k_cache, cache.v_cache, cache.slots, cache.table)
+        kernels.attn_prefill_int4(q, out, *places, *lists[:4], cache.ctx, 320, page, dim ** -0.5, span=span)
+        kernels.attn_decode_int4(q, last, *places, lists[4], lists[5], cache.ctx, 1, 320, page, dim ** -0.5, mass=mass)
+        kernels.int4_evict(cache.k_cache, cache.v_cache, mass, cache.slots, cache.table, cache.ctx, to, kept, page, 320, 8, 2)
+        kernels.int4_expand(cache.k_cache, cache.v_cache, k_out, v_out, cache.slots, to, new, page)
+        return out, last
+
+    new = i32([64, 64])
+    turn()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = turn()
+    for i in range(3):
+        q.copy_(queries(80, hq, dim, dtype, seed=30 + i))
+        cache.ctx.copy_(i32([300 - 9 * i, 180 - i]))
+        results = []
+        for run in (lambda: (graph.replay(), held)[1], turn):
+            mass.zero_()
+            results.append([x.clone() for x in (*run(), mass, kept, k_out, v_out)])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+    kernels.raise_if_kernel_gave_up()
+
+
 def test_far_places_pass_32_bits():
     """A pool of more than 2^31 bytes: the last page's rows are where they should be."""
     hkv, dim, page = 8, 128, 64
