@@ -497,68 +497,50 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) int4_select_kernel(const fl
     for (int i = tid; i < recent; i += SELECT_THREADS) out[keep - recent + i] = len - recent + i;
 }
 
-// A warp moves the rows of MOVE_BLOCKS new blocks of 8, all of them on their way at once: lane (r, c) a quarter of row r of the keys, of the row
-// in slot r of the values, a step of each, and (c = 0) the row's sum.
-// Bound by memory, of which a kept row's neighbours come along: 2048 of 4096 rows of 24 requests, 8 heads of 128, 33 us (17 for the rows
-// alone, 26 with all that is read).
-constexpr int MOVE_BLOCKS = 4;
+// A warp moves the rows of a new block of 8: lane (r, c) a quarter of row r of the keys, of the row in slot r of the values, a step of each, and
+// (c = 0) the row's sum.  Bound by memory, of which a kept row's neighbours come along, and by three trips to it, one behind another, which
+// eight thread blocks of an SM hide (with four blocks of rows to a warp, and so fewer warps, it took 35 us): 2048 of 4096 rows of
+// 24 requests, 8 heads of 128, 27 us (17 for the rows alone, 26 with all that is read).
 template <int D>
-__global__ void __launch_bounds__(THREADS) int4_move_kernel(unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
-                                                            const int* __restrict__ req_slot, Pages pages, Pages to_pages, const int* __restrict__ kept, int keep) {
+__global__ void __launch_bounds__(THREADS, 8) int4_move_kernel(unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
+                                                               const int* __restrict__ req_slot, Pages pages, Pages to_pages, const int* __restrict__ kept, int keep) {
     constexpr int NG = D / 32;
     pdl_wait();
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = blockIdx.y, req = blockIdx.z, slot = req_slot[req];
     const int* places = kept + ((size_t)req * pages.hkv + head) * keep;
     const int slot_row = 2 * (r & 3) + (r >> 2);                    // the row in slot r of the values
-    const int warp_row = (blockIdx.x * (THREADS / 32) + threadIdx.x / 32) * MOVE_BLOCKS * INT4_BLOCK;
-    long long to[MOVE_BLOCKS], key_at[MOVE_BLOCKS], value_at[MOVE_BLOCKS];
-    int key_pos[MOVE_BLOCKS], value_pos[MOVE_BLOCKS];
-#pragma unroll
-    for (int b = 0; b < MOVE_BLOCKS; ++b) {
-        const int row = warp_row + b * INT4_BLOCK;
-        key_pos[b] = row + r < keep ? places[row + r] : -1;
-        value_pos[b] = row + slot_row < keep ? places[row + slot_row] : -1;
-        to[b] = row < keep ? int4_block_at(to_pages, req, row, head) : -1;
-    }
-#pragma unroll
-    for (int b = 0; b < MOVE_BLOCKS; ++b) {
-        key_at[b] = to[b] < 0 ? -1 : int4_block_at(pages, slot, key_pos[b], head);
-        value_at[b] = to[b] < 0 ? -1 : int4_block_at(pages, slot, value_pos[b], head);
-    }
+    const int row = (blockIdx.x * (THREADS / 32) + threadIdx.x / 32) * INT4_BLOCK;
+    const int key_pos = row + r < keep ? places[row + r] : -1, value_pos = row + slot_row < keep ? places[row + slot_row] : -1;
+    const long long to = row < keep ? int4_block_at(to_pages, req, row, head) : -1;
+    const long long key_at = to < 0 ? -1 : int4_block_at(pages, slot, key_pos, head), value_at = to < 0 ? -1 : int4_block_at(pages, slot, value_pos, head);
     struct alignas(16) Part { uint32_t w[NG]; };
-    Part k[MOVE_BLOCKS], v[MOVE_BLOCKS];
-    __half k_step[MOVE_BLOCKS], v_step[MOVE_BLOCKS];
-    float sum[MOVE_BLOCKS];
-#pragma unroll
-    for (int b = 0; b < MOVE_BLOCKS; ++b) {
-        if (key_at[b] >= 0) {
-            const unsigned char* from = k_cache + key_at[b] * int4_block_bytes(D);
-            const int from_r = key_pos[b] % INT4_BLOCK;
-            copy_share<4 * NG>(&k[b], from + from_r * (D / 2) + c * 4 * NG);
-            if (c < NG) k_step[b] = reinterpret_cast<const __half*>(from + 4 * D)[from_r * NG + c];
-            if (c == 0) sum[b] = mass[key_at[b] * INT4_BLOCK + from_r];
-        }
-        if (value_at[b] >= 0) {
-            const unsigned char* from = v_cache + value_at[b] * int4_block_bytes(D);
-            const int from_r = value_pos[b] % INT4_BLOCK, from_slot = int4_value_slot(from_r);
-            const int turned = int4_value_turn<D>(r) != int4_value_turn<D>(from_slot) ? 2 : 0;      // eighths exchanged four by four: quarters two by two
-            copy_share<4 * NG>(&v[b], from + from_slot * (D / 2) + (c ^ turned) * 4 * NG);
-            if (c < NG) v_step[b] = reinterpret_cast<const __half*>(from + 4 * D)[((from_r >> 1) * NG + c) * 2 + (from_r & 1)];
-        }
+    Part k, v;
+    __half k_step, v_step;
+    float sum;
+    if (key_at >= 0) {
+        const unsigned char* from = k_cache + key_at * int4_block_bytes(D);
+        const int from_r = key_pos % INT4_BLOCK;
+        copy_share<4 * NG>(&k, from + from_r * (D / 2) + c * 4 * NG);
+        if (c < NG) k_step = reinterpret_cast<const __half*>(from + 4 * D)[from_r * NG + c];
+        if (c == 0) sum = mass[key_at * INT4_BLOCK + from_r];
     }
-#pragma unroll
-    for (int b = 0; b < MOVE_BLOCKS; ++b) {
-        if (key_at[b] >= 0) {
-            unsigned char* dest = k_cache + to[b] * int4_block_bytes(D);
-            copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &k[b]);
-            if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[r * NG + c] = k_step[b];
-            if (c == 0) mass[to[b] * INT4_BLOCK + r] = sum[b];
-        }
-        if (value_at[b] >= 0) {
-            unsigned char* dest = v_cache + to[b] * int4_block_bytes(D);
-            copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &v[b]);
-            if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[((slot_row >> 1) * NG + c) * 2 + (slot_row & 1)] = v_step[b];
-        }
+    if (value_at >= 0) {
+        const unsigned char* from = v_cache + value_at * int4_block_bytes(D);
+        const int from_r = value_pos % INT4_BLOCK, from_slot = int4_value_slot(from_r);
+        const int turned = int4_value_turn<D>(r) != int4_value_turn<D>(from_slot) ? 2 : 0;      // eighths exchanged four by four: quarters two by two
+        copy_share<4 * NG>(&v, from + from_slot * (D / 2) + (c ^ turned) * 4 * NG);
+        if (c < NG) v_step = reinterpret_cast<const __half*>(from + 4 * D)[((from_r >> 1) * NG + c) * 2 + (from_r & 1)];
+    }
+    if (key_at >= 0) {
+        unsigned char* dest = k_cache + to * int4_block_bytes(D);
+        copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &k);
+        if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[r * NG + c] = k_step;
+        if (c == 0) mass[to * INT4_BLOCK + r] = sum;
+    }
+    if (value_at >= 0) {
+        unsigned char* dest = v_cache + to * int4_block_bytes(D);
+        copy_share<4 * NG>(dest + r * (D / 2) + c * 4 * NG, &v);
+        if (c < NG) reinterpret_cast<__half*>(dest + 4 * D)[((slot_row >> 1) * NG + c) * 2 + (slot_row & 1)] = v_step;
     }
 }
 
@@ -686,7 +668,7 @@ CISR_EXPORT int cisr_int4_evict(const Int4EvictCall* call) {
     const int status = launch_kernel(int4_select_kernel, dim3(c.hkv, c.n_req), dim3(SELECT_THREADS), smem, s, g_pdl, (const float*)c.mass, c.req_slot, pages, c.ctx_len, c.kept,
                                      c.keep, c.recent, c.first, cached);
     if (status) return status;
-    constexpr int rows = MOVE_BLOCKS * INT4_BLOCK * (THREADS / 32);
+    constexpr int rows = INT4_BLOCK * (THREADS / 32);
     const dim3 grid((unsigned)((c.keep + rows - 1) / rows), c.hkv, c.n_req);
     return by_head_size(c.dim, [&](auto d) {
         return launch_kernel(int4_move_kernel<decltype(d)::value>, grid, dim3(THREADS), 0, s, true, (unsigned char*)c.k_cache, (unsigned char*)c.v_cache, c.mass, c.req_slot, pages,
