@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
 // request's end, give zeros.  float16 (three binary digits times eleven, rounded to eleven): divided by the key head's factor (int4_top_kernel).
-// Bound by memory: 8192 rows of 8 heads of 128 as bfloat16 10.8 us of 6.6, as float 24.6 of 11.7; 24 x 2048 rows 46.6 of 39.4.
-constexpr int READ_ROWS = 4;         // of a thread, on their way together
+// Bound by memory: 8192 rows of 8 heads of 128 as bfloat16 10.4 us of 6.6, as float 20.6 of 11.7; 24 x 2048 rows 43 of 39 and 101 of 70.
+constexpr int READ_ROWS = 1;         // of a thread, and eight thread blocks to an SM: with four rows on their way together, and so fewer threads, 47 and 130
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
                                           const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(TOP_THREADS) int4_top_kernel(const unsigned ch
 static_assert(TOP_THREADS == 1024, "a warp joins 32");
 
 template <int D, typename T>
-__global__ void __launch_bounds__(THREADS) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
+__global__ void __launch_bounds__(THREADS, 8) int4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache, T* __restrict__ k,
                                                             T* __restrict__ v, long long req_stride, long long token_stride, long long head_stride, Place at,
                                                             Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,
                                                             int tokens, int hkv) {
