@@ -780,15 +780,17 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     for name, t in (("tile_req", tile_req), ("tile_q0", tile_q0)):
         _need(t, torch.int32, name)
     lib = _attention_tcgen05(dim, half=True)
-    k, v = torch.empty((2, n, hkv, rows, dim), dtype=torch.float16, device=q.device)
-    halves, factors = torch.empty(q.shape, dtype=torch.float16, device=q.device), torch.empty(n * hkv * 2 + n + q.shape[0] * hq, device=q.device)
-    table, q_factor = factors.data_ptr() + 8 * n * hkv, factors.data_ptr() + 8 * n * hkv + 4 * n
-    _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), _p(k), _p(v), _p(factors), table, _p(q), _p(halves), q_factor, q.shape[0] * hq, _p(req_slot), _p(block_table),
-                                         block_table.shape[1], page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim,
-                                         _p(_error_flag()), _stream()), "attn_prefill_int4", own=2)
-    _check(lib.cisr_attn_prefill_tcgen05(_p(halves), _p(out), q.shape[0], _p(k), _p(v), n, table if places is None else _p(places), table, 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
-                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor,
-                                         _p(factors), _stream()), "attn_prefill_int4")
+    # one allocation: keys, values, queries in float16, then the factors of key heads, the rows' table and the factors of queries
+    tokens, plane = q.shape[0], 2 * n * hkv * rows * dim
+    room = torch.empty(2 * plane + 2 * q.numel() + 8 * n * hkv + 4 * n + 4 * tokens * hq, dtype=torch.uint8, device=q.device)
+    k = room.data_ptr()
+    v, halves, factors = k + plane, k + 2 * plane, k + 2 * plane + 2 * q.numel()
+    table, q_factor, stream = factors + 8 * n * hkv, factors + 8 * n * hkv + 4 * n, _stream()
+    _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), k, v, factors, table, _p(q), halves, q_factor, tokens * hq, _p(req_slot), _p(block_table), block_table.size(1),
+                                         page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _p(_error_flag()), stream), "attn_prefill_int4", own=2)
+    _check(lib.cisr_attn_prefill_tcgen05(halves, _p(out), tokens, k, v, n, table if places is None else _p(places), table, 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
+                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor, factors,
+                                         stream), "attn_prefill_int4")
 
 
 def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,
@@ -797,7 +799,7 @@ def int4_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor,
     `recent`, and of those between the ones with the largest `mass` (of equal ones the lowest place; NaN counts as the largest), in
     their order.  kept int32 [requests, kv_heads, keep] becomes the places that stay (-1 behind the last; a request of
     `keep` rows or fewer keeps all), and the rows go, with their mass, to the pages that row r of to_table [requests, width] names
-    for request r.  Those must be no page that any request still reads (the request's own old pages among them): nothing is
+    for request r.  Those must be no page twice, and none that any request still reads (the request's own old pages among them): nothing is
     moved in place, so shared pages stay as they are.  Rows of the new pages behind the last kept one are left as they were.
     `longest`: no request has more rows (longer ones are right, but slower)."""
     _need(kept, torch.int32, "kept", 3); _need(to_table, torch.int32, "to_table", 2)
