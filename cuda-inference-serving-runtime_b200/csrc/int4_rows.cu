@@ -300,10 +300,11 @@ template <int D> __device__ __forceinline__ void convert_queries(const Queries& 
 
 // What a prompt's attention with float16 operands needs before its rows are written out: a power of two for each request's key head, keys
 // and values apart, to the same end (a thread block reads all its steps, 1/9 of what is held; NaN is left out, and stays NaN), and
-// its queries, which the thread blocks behind those take meanwhile.  2 requests of 3500 rows, 8 heads, and 2000 queries of 32 heads of 128: 11.5 us.
+// its queries, which the thread blocks behind those take meanwhile.  2 requests of 3500 rows, 8 heads, and 2000 queries of 32 heads of 128: 8.6 us (with one
+// thread block to an SM, for its registers, 12).
 constexpr int TOP_THREADS = 1024;
 template <int D>
-__global__ void __launch_bounds__(TOP_THREADS) int4_top_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
+__global__ void __launch_bounds__(TOP_THREADS, 2) int4_top_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
                                                                const int* __restrict__ req_slot, Pages pages, const int* __restrict__ ends, const int* __restrict__ which,
                                                                float* __restrict__ factors, int* __restrict__ pages_out, int n_req, int rows, int* __restrict__ error,
                                                                Queries queries) {
