@@ -53,6 +53,30 @@ class PagedBinding:
     state: Optional[torch.Tensor] = None     # the entry's own side state [slots, ...], where its mixer asked for one
     held: str = ""                           # "int4": k and v are uint8 [pages, kv_heads, bytes of a page]
     mass: Optional[torch.Tensor] = None      # float [pages, kv_heads, page_size], where keys are weighed
+    places: Optional["StepPlaces"] = None    # where `held` says something: a step's own page
+
+
+class StepPlaces:
+    """The places of a step's tokens in a page of the step's own (token t in row t of page 0), which its products write where the cache is held
+    in another form.  The products look their places up before they wait for the kernel ahead of them, so in a captured step these
+    lists have to be older than the step: they are constants of the cache, made when it is made.  Longer steps than any before get longer
+    lists, and the shorter ones stay, since captured steps read them."""
+
+    def __init__(self, tokens: int, device):
+        self.device, self.lists = device, []
+        self._longer(tokens)
+
+    def _longer(self, tokens: int) -> None:
+        self.lists.append((torch.arange(tokens, dtype=torch.int32, device=self.device), torch.zeros(tokens, dtype=torch.int32, device=self.device)))
+
+    def __call__(self, tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Rows 0 .. tokens - 1, and as many zeros (requests, slots and pages)."""
+        if tokens > self.lists[-1][0].numel():
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"a step of {tokens} tokens is captured before any step of as many tokens has run")
+            self._longer(max(tokens, 2 * self.lists[-1][0].numel()))
+        rows, zeros = self.lists[-1]
+        return rows[:tokens], zeros[:tokens]
 
 
 @dataclass
@@ -137,6 +161,8 @@ class CacheManager:
                 raise ValueError(f"unknown form of a cache {use.held!r}")
             if weigh and not isinstance(use, int) and use.kind == "pages" and (use.held != "int4" or use.window is not None):
                 raise ValueError("keys are weighed, and requests cut by their weights, in caches held in 4 bits without a window")
+        held = any(not isinstance(use, int) and use.kind == "pages" and use.held for use in uses)
+        self.places = StepPlaces(max(1024, 2 * max_slots), device) if held and device is not None else None      # (a captured step has fewer than twice the slots)
         self.page_groups: List[PageGroup] = []
         self.state_groups: List[StateGroup] = []
         self.entry_group: Dict[int, Tuple[str, int]] = {}   # run entry -> ("pages"|"state", group index)
@@ -378,7 +404,8 @@ class CacheManager:
             k, v = g.planes[g.entry_slot[source]]
             return PagedBinding(k, v, g.device_table, g.page_size,
                                 write=reads_from is None, window=g.use.window, keep_first=g.use.keep_first, state=self.side_state(entry),
-                                held=g.use.held, mass=None if g.mass is None else g.mass[g.entry_slot[source]])
+                                held=g.use.held, mass=None if g.mass is None else g.mass[g.entry_slot[source]],
+                                places=self.places if g.use.held else None)
         g = self.state_groups[gi]
         return StateBinding(g.states[g.entry_slot[source]])
 

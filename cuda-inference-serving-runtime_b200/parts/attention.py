@@ -93,7 +93,7 @@ class GQAAttention(Mixer):
         rot = self.position.rotation(ctx)
         q = torch.empty((tokens, hq, dim), dtype=self.dtype, device=device)
         # where the new keys and values go: straight into the cache, or, where that is held in 4 bits, into a page of this step first
-        to = staged_rows(ctx, hkv, dim, self.dtype) if cache.held else StepRows(cache.k, cache.v, ctx.positions, ctx.token_req, ctx.req_slot, cache.block_table,
+        to = staged_rows(ctx, cache, hkv, dim, self.dtype) if cache.held else StepRows(cache.k, cache.v, ctx.positions, ctx.token_req, ctx.req_slot, cache.block_table,
                                                                                cache.page_size)
         turn = (dim, rot.rot_half, rot.interleaved) if rot else (dim, 0, False)
         if cache.write and kernels.skinny_ok(tokens, self.qkv, turn):
@@ -179,16 +179,13 @@ class StepRows(NamedTuple):
     page_size: int
 
 
-def staged_rows(ctx, hkv: int, dim: int, dtype: torch.dtype) -> StepRows:
+def staged_rows(ctx, cache, hkv: int, dim: int, dtype: torch.dtype) -> StepRows:
     """One page per plane that holds a step's new keys and values [1, kv_heads, tokens, head_dim], token t in row t: what the products'
-    epilogues write into where the cache itself is held in another form."""
-    tokens, device = ctx.n_tokens, ctx.device
-    k, v = torch.empty((2, 1, hkv, tokens, dim), dtype=dtype, device=device)
-    places = ctx.shared.get("staged")
-    if places is None:
-        zeros = torch.zeros(tokens, dtype=torch.int32, device=device)
-        places = ctx.shared["staged"] = (torch.arange(tokens, dtype=torch.int32, device=device), zeros, zeros[:1], zeros[:1].view(1, 1))
-    return StepRows(k, v, *places, tokens)
+    epilogues write into where the cache itself is held in another form.  The places are the cache's (`StepPlaces` says why)."""
+    tokens = ctx.n_tokens
+    k, v = torch.empty((2, 1, hkv, tokens, dim), dtype=dtype, device=ctx.device)
+    rows, zeros = cache.places(tokens)
+    return StepRows(k, v, rows, zeros, zeros[:1], zeros[:1].view(1, 1), tokens)
 
 
 def token_rows(ctx, cache) -> torch.Tensor:

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+import torch.utils._python_dispatch
 
 from cisr_b200.cache import CacheManager, OutOfPages
 from cisr_b200.config.spec import CacheUse
@@ -114,6 +115,42 @@ def test_a_fork_of_weighed_pages_gets_its_own():
     step(shared, "a", 20)
     shared.fork("a", "b")
     assert shared.requests["a"].tables[0] == shared.requests["b"].tables[0]
+
+
+class Launching(torch.utils._python_dispatch.TorchDispatchMode):
+    """Names torch's operations that put something on the stream: all but views and new tensors."""
+    QUIET = ("empty", "new_empty", "empty_like", "empty_strided", "unbind", "select", "slice", "view", "_unsafe_view", "as_strided", "transpose", "detach", "alias", "split", "t",
+             "squeeze", "unsqueeze", "expand", "_reshape_alias", "chunk", "permute")
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        name = func.overloadpacket.__name__
+        if name not in self.QUIET:
+            self.seen.append(name)
+        return func(*args, **(kwargs or {}))
+
+
+def test_a_steps_own_places_are_older_than_the_step():
+    """The products look them up before they wait for the kernel ahead of them: no kernel of the step may write them, and what a captured step
+    reads stays where it is when longer steps come."""
+    from types import SimpleNamespace
+
+    from cisr_b200.cache.manager import StepPlaces
+    from cisr_b200.parts.attention import staged_rows
+
+    places = StepPlaces(8, "cpu")
+    with Launching() as mode:
+        to = staged_rows(SimpleNamespace(n_tokens=5, device="cpu", shared={}), SimpleNamespace(places=places), 2, 32, torch.float32)
+    assert mode.seen == [], mode.seen
+    assert to.k.shape == to.v.shape == (1, 2, 5, 32) and to.page_size == 5 and to.block_table.tolist() == [[0]] and to.req_slot.tolist() == [0]
+    assert to.positions.tolist() == [0, 1, 2, 3, 4] and to.token_req.tolist() == [0] * 5
+    assert places(5)[0].data_ptr() == to.positions.data_ptr() and places(8)[0].data_ptr() == to.positions.data_ptr()
+    rows, zeros = places(9)
+    assert rows.tolist() == list(range(9)) and zeros.tolist() == [0] * 9 and places.lists[0][0].data_ptr() == to.positions.data_ptr()
+    assert places(300)[0].tolist() == list(range(300)) and len(places.lists) == 3
 
 
 def test_what_is_kept():
