@@ -377,7 +377,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         if (HALF_OPERANDS) {
             const int mine = (shared ? 0 : stream * BM) + row;
             const float* of_head = kv_factor + ((size_t)req_slot[req] * hkv + kvh) * 2;
-            scale2 *= (mine < rows ? q_factor[(size_t)(tok0 + mine) * hq + head] : 0.f) * of_head[0];
+            // not 0, which a row of zeros (whose factor is 2^-120) or a tiny scale would make of it: a masked score, -inf, stays one.  (Raw scores are
+            // below 2^38, so that nothing of a weight shows where the bound is the larger.)
+            scale2 = fmaxf(scale2 * (mine < rows ? q_factor[(size_t)(tok0 + mine) * hq + head] : 0.f) * of_head[0], 0x1p-126f);
             v_factor = of_head[1];
         }
         // bent scores lie in (-cap, cap): where 2^(cap log2 e) is far from a float's range they need no running max, and

@@ -1,0 +1,45 @@
+"""Attention over a cache held in 4 bits where numbers, scales or lengths are unusual."""
+import pytest
+import torch
+
+import plain_int4 as plain
+from cisr_b200.ops import kernels
+from test_int4_cache_gpu import Cache, bound, check, i32, prompt_bound, queries
+
+pytestmark = pytest.mark.gpu
+
+
+def portions(cache, q, q_len, span, scale, **kw):
+    """Every request's portion, in tiles of `span`."""
+    starts = [sum(q_len[:r]) for r in range(len(q_len))]
+    pairs = [(r, a) for r, n in enumerate(q_len) for a in range(0, n, span)]
+    out = torch.full_like(q, 7.0)
+    kernels.attn_prefill_int4(q, out, cache.k_cache, cache.v_cache, cache.slots, cache.table, i32([r for r, _ in pairs]), i32([a for _, a in pairs]), i32(starts), i32(q_len),
+                              cache.ctx, max(cache.lens), cache.page, scale, span=span, **kw)
+    kernels.raise_if_kernel_gave_up()
+    return out
+
+
+def check_portions(cache, q, got, q_len, span, scale, sink=None):
+    at = 0
+    for r, n in enumerate(q_len):
+        want, size, p = plain.attention(q[at:at + n], *cache.held(r), scale, plain.seen(n, cache.lens[r]), sink)
+        off = (got[at:at + n].double() - want).abs()
+        most = bound(q.dtype, want, size, plain.stepped(p, cache.v[r]) if span == 64 else 0) + prompt_bound(q.dtype, span) * size
+        assert (off <= most).all(), (r, float(torch.nan_to_num(off / most, 1e9).max()))
+        at += n
+
+
+@pytest.mark.parametrize("dim,span", [(64, 128), (64, 256), (128, 128), (128, 256), (96, 64), (32, 64)])
+@pytest.mark.parametrize("size,scale", [(1.0, 0.125), (1e-4, 0.125), (1e-5, 1e-3), (1.0, 1e-19), (1e-4, 1e-30), (1.0, 0.0)])
+def test_queries_of_zeros(dim, span, size, scale):
+    """The mean of what such a row sees, whatever the sizes of keys and scale, with keys out of sight among a tile's."""
+    hq, hkv = 4, 2
+    lens, q_len = [300, 130], [200, 130]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = [torch.randn((n, hkv, dim), generator=g, device="cuda") * size for n in lens]
+    cache = Cache(lens, hkv, dim, 16, k=k, v=[torch.randn((n, hkv, dim), generator=g, device="cuda") for n in lens])
+    q = queries(sum(q_len), hq, dim, torch.bfloat16)
+    q[::3] = 0
+    q[1::3, 1] = 0
+    check_portions(cache, q, portions(cache, q, q_len, span, scale), q_len, span, scale)
