@@ -275,8 +275,9 @@ __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cach
     }
 }
 
-// A prompt's queries [rows][D] as float16, each row times a power of two that brings its largest to 2^14 .. 2^15, which its factor takes back.
-struct Queries { const uint4* q; uint4* half; float* factor; long long rows; };
+// A prompt's queries [rows][D] as float16, each row times a power of two that brings its largest to 2^14 .. 2^15, which its factor takes back, and with
+// the sign of the scale (the softmax behind takes its maximum before it scales, so its scale is positive).
+struct Queries { const uint4* q; uint4* half; float* factor; long long rows; float scale; };
 template <int D> __device__ __forceinline__ void convert_queries(const Queries& a, long long block) {
     constexpr int PARTS = D / 8;                                    // threads that share a row
     const long long at = block * blockDim.x + threadIdx.x, row = at / PARTS;
@@ -287,7 +288,7 @@ template <int D> __device__ __forceinline__ void convert_queries(const Queries& 
 #pragma unroll
     for (int o = 1; o < PARTS; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int exponent = min(14 - ((int)(top >> 23) - 127), 120);
-    const float up = __uint_as_float((uint32_t)(exponent + 127) << 23);
+    const float up = copysignf(__uint_as_float((uint32_t)(exponent + 127) << 23), a.scale);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -624,18 +625,20 @@ CISR_EXPORT int cisr_int4_read(const Int4ReadCall* call) {
 }
 
 // For a prompt's attention with float16 operands (head sizes 64 and 128): places 0 .. rows - 1 of n_req requests (request which[i], or i without a list) into
-// k, v float16 [n_req][hkv][rows][dim] over `factors` [n_req][hkv][2] (pages_out becomes 0, 1, .. n_req - 1), and queries bfloat16 [q_rows][dim] into q_half over q_factor [q_rows].
+// k, v float16 [n_req][hkv][rows][dim] over `factors` [n_req][hkv][2] (pages_out becomes 0, 1, .. n_req - 1), and queries bfloat16 [q_rows][dim] into q_half over q_factor [q_rows],
+// with the sign of `scale`.
 // A request with more rows sets the error flag.
 CISR_EXPORT int cisr_int4_prompt(const void* k_cache, const void* v_cache, void* k, void* v, float* factors, int* pages_out, const void* q, void* q_half, float* q_factor, long long q_rows,
                                  const int* req_slot, const int* block_table, int width, int page_size, const int* ends, const int* which, int n_req, int rows, int hkv, int dim,
-                                 int* error, void* stream) {
+                                 float scale, int* error, void* stream) {
+    if (!isfinite(scale)) return -2;
     if (rows <= 0 || n_req <= 0) return 0;
     if (hkv <= 0 || page_size <= 0 || page_size % INT4_BLOCK || n_req > 65535 || (long long)rows * hkv >= 1ll << 30) return -2;
     if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_half) & 15) return -2;
     const Pages pages = pages_of(block_table, width, page_size, hkv);
     const Place at{nullptr, nullptr, req_slot, pages, Divider((uint32_t)hkv)};
     const dim3 grid((unsigned)units((long long)rows * hkv, READ_ROWS * (THREADS / LANES)), (unsigned)n_req);
-    const Queries queries{(const uint4*)q, (uint4*)q_half, q_factor, q_rows};
+    const Queries queries{(const uint4*)q, (uint4*)q_half, q_factor, q_rows, scale};
     const long long blocks = 2ll * n_req * hkv + (q_rows * (dim / 8) + TOP_THREADS - 1) / TOP_THREADS;
     if (blocks >= 1ll << 31) return -2;
     const auto run = [&](auto d) {

@@ -706,7 +706,7 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     """Attention of new tokens, few per request (one in a decode step), over a 4-bit cache: q, out [tokens, heads, head_dim].
     Request r brings q_len[r] tokens from row q_start[r] of q on and has ctx_len[r] rows in the cache, theirs included; requests that
     bring none, or more than `max_queries`, are left alone.  `longest`: no request has more rows (a bound will do; one that has sets the
-    flag that `raise_if_kernel_gave_up` reads).  window, sink, keep_first: as for `attn_decode`.
+    flag that `raise_if_kernel_gave_up` reads).  scale: any finite float, of either sign.  window, sink, keep_first: as for `attn_decode`.
 
     `mass` float [pages, kv_heads, page_size]: every key's number grows by the weights that the query heads of its key head, and all of
     the request's new tokens, have given it (a sink takes its part of them).  The same call gives the same numbers, unless requests of
@@ -787,9 +787,9 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     v, halves, factors = k + plane, k + 2 * plane, k + 2 * plane + 2 * q.numel()
     table, q_factor, stream = factors + 8 * n * hkv, factors + 8 * n * hkv + 4 * n, _stream()
     _check(_int4_rows().cisr_int4_prompt(_p(k_cache), _p(v_cache), k, v, factors, table, _p(q), halves, q_factor, tokens * hq, _p(req_slot), _p(block_table), block_table.size(1),
-                                         page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, _p(_error_flag()), stream), "attn_prefill_int4", own=2)
+                                         page_size, _p(ctx_len), _p(requests), n, rows, hkv, dim, scale, _p(_error_flag()), stream), "attn_prefill_int4", own=2)
     _check(lib.cisr_attn_prefill_tcgen05(halves, _p(out), tokens, k, v, n, table if places is None else _p(places), table, 1, _p(tile_req), _p(tile_q0), tile_req.numel(), span,
-                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, scale, 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor, factors,
+                                         _p(q_start), _p(q_len), _p(ctx_len), hq, hkv, rows, abs(scale), 0.0, int(window or 0), keep_first, *_sink(sink, hq), q_factor, factors,
                                          stream), "attn_prefill_int4")
 
 

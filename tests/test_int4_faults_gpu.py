@@ -1,9 +1,12 @@
 """Attention over a cache held in 4 bits where numbers, scales or lengths are unusual."""
+import math
+
 import pytest
 import torch
 
 import plain_int4 as plain
 from cisr_b200.ops import kernels
+from cisr_b200.ops.kernels import KernelError
 from test_int4_cache_gpu import Cache, bound, check, i32, prompt_bound, queries
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +46,26 @@ def test_queries_of_zeros(dim, span, size, scale):
     q[::3] = 0
     q[1::3, 1] = 0
     check_portions(cache, q, portions(cache, q, q_len, span, scale), q_len, span, scale)
+
+
+@pytest.mark.parametrize("dtype,dim,span", [(torch.bfloat16, 64, 128), (torch.bfloat16, 128, 256), (torch.bfloat16, 32, 64), (torch.float32, 64, 64)])
+@pytest.mark.parametrize("scale", [-0.125, -2.0, -1e-19, 3.0, 0.0])
+@pytest.mark.parametrize("sink", [None, 0.5])
+def test_scales_of_either_sign(dtype, dim, span, scale, sink):
+    hq, hkv = 4, 2
+    lens, q_len = [300, 130], [200, 130]
+    cache = Cache(lens, hkv, dim, 16)
+    q = queries(sum(q_len), hq, dim, dtype, std=1.0 if abs(scale) < 1 else 0.1)
+    check_portions(cache, q, portions(cache, q, q_len, span, scale, sink=sink), q_len, span, scale, sink)
+
+
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan, 1e39])
+def test_scales_that_are_no_numbers_are_refused(scale):
+    for dtype, span in ((torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)):
+        cache = Cache([20], 2, 64, 16)
+        q = queries(3, 4, 64, dtype)
+        with pytest.raises(KernelError):
+            portions(cache, q, [3], span, scale)
+        with pytest.raises(KernelError):
+            cache.attend(q, [3], scale=scale)
+    kernels.raise_if_kernel_gave_up()
