@@ -777,8 +777,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
         return
     if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
         raise KernelError(f"attn_prefill_int4: tiles of {span} queries are for bfloat16 and head sizes {TCGEN05_HEAD_DIMS}")
-    for name, t in (("tile_req", tile_req), ("tile_q0", tile_q0)):
-        _need(t, torch.int32, name)
+    _int4_lists("attn_prefill_int4", device, block_table, tile_req.numel(), ("req_slot", "tile_req", "tile_q0"), req_slot, tile_req, tile_q0)
     lib = _attention_tcgen05(dim, half=True)
     # one allocation: keys, values, queries in float16, then the factors of key heads, the rows' table and the factors of queries
     tokens, plane = q.shape[0], 2 * n * hkv * rows * dim

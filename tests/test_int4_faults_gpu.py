@@ -69,3 +69,14 @@ def test_scales_that_are_no_numbers_are_refused(scale):
         with pytest.raises(KernelError):
             cache.attend(q, [3], scale=scale)
     kernels.raise_if_kernel_gave_up()
+
+
+def test_tile_lists_have_the_same_length_and_place():
+    cache = Cache([300, 40], 2, 64, 16)
+    q = queries(100, 4, 64, torch.bfloat16)
+    one, two = i32([0]), i32([0, 0])
+    for req, q0 in ((two, one), (one, two), (two.cpu(), two), (two, two.cpu()), (two[None], two[None]), (two.long(), two), (two, i32([0, 0, 0, 0])[::2])):
+        with pytest.raises(KernelError):
+            kernels.attn_prefill_int4(q, torch.empty_like(q), cache.k_cache, cache.v_cache, cache.slots, cache.table, req, q0, i32([0, 60]), i32([60, 40]), cache.ctx, 300, 16, 0.125,
+                                      span=128)
+    kernels.raise_if_kernel_gave_up()
