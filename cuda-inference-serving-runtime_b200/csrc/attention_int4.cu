@@ -54,8 +54,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 // The running maximum follows a score only where that is 2^SLACK times its weight above it, which after a warp's first tile is rare (each time
 // costs 50 multiplications a lane).  Probabilities are held times 2^9: with steps of V below 8 (values below 56) no product of the two overflows
 // a float16, and products down to 2^-23 keep all their digits (smaller ones are off by 2^-34 at most).  A warp whose sums come out not finite
-// does its keys again with probabilities times 2^-5, where no step can overflow.  (Looking at every step instead took 8 instructions per 16 keys.)
-constexpr float SLACK = 4.f, USUAL_SHIFT = 9.f, LARGE_SHIFT = -5.f;
+// does its keys again with bfloat16 operands, which no step can overflow: codes, which they hold exactly, and products of a probability and a
+// step, made in float, as two terms (16 digits; for float queries three, 24).  So it does not matter to a small group that another one is large.
+// (Looking at every step instead took 8 instructions per 16 keys.)
+constexpr float SLACK = 4.f, SHIFT = 9.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 constexpr int MAX_RANKED = 128;                                    // requests that are put in order of length, a thread each
 
@@ -72,6 +74,10 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 __device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16_8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
@@ -94,6 +100,16 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 template <int EXPONENT> __device__ __forceinline__ uint32_t centred(uint32_t n) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&n), __float2half2_rn((float)(1 << EXPONENT)), __float2half2_rn(-8.f / 512.f));
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two codes n, one in each half's low four bits, as bfloat16 n - 8: 128 + n is one by its bits, and 136 less is exact.
+__device__ __forceinline__ uint32_t centred_bf16(uint32_t n) {
+    const uint32_t x = n | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(136.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float low_half(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x & 0xffff))); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x >> 16))); }
@@ -380,7 +396,6 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     float o[D / 16][NT][4], r_off[OFFSET ? NG : 1][NT][4], m_run[NT][2], l_run[NT][2];
     float limit[NT][2];                                             // scores above it move the maximum
     int own_pos[NT][2];                                             // a column's place, for tiles with masks
-    float shift = USUAL_SHIFT;
     uint32_t eights[4];                                             // the constant operand, kept in registers: as an immediate it was loaded again for every product
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, 0x00080008;" : "=r"(eights[i]));
@@ -396,9 +411,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     };
 
     float* scores = a.scores ? a.scores + ((size_t)unit_of * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
-    // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.
-    const auto step = [&](auto is_edge, int t) {
-        constexpr bool EDGE = decltype(is_edge)::value;
+    // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.  LARGE: products with steps as bfloat16.
+    const auto step = [&](auto is_edge, auto is_large, int t) {
+        constexpr bool EDGE = decltype(is_edge)::value, LARGE = decltype(is_large)::value;
+        constexpr int PARTS = LARGE ? TERMS + 1 : TERMS;
+        constexpr bool HALVES_PRODUCT = TERMS == 1 && !LARGE;       // of probability and step, in float16
         const int k0 = span.key(t0 + t);
         float s[HALVES][NT][4];
         asm volatile("cp.async.wait_group 1;" ::: "memory");        // the keys
@@ -496,7 +513,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float top = shift - (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e] * unit[nt][e]);
+                const float top = SHIFT - (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e] * unit[nt][e]);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
                     float p0 = exp2_fast(fmaf(s[h][nt][e], unit[nt][e], top)), p1 = exp2_fast(fmaf(s[h][nt][e + 2], unit[nt][e], top));
@@ -514,13 +531,13 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         for (int h = 0; h < HALVES; ++h) {
             // probabilities as B: rows of the product above are keys, here columns: two 8 x 8 transpositions per 16 keys
             uint32_t pt[NT][2];
-#if STORAGE_BF16
+            if constexpr (HALVES_PRODUCT) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                pt[nt][0] = transposed(pack_f16(s[h][nt][0], s[h][nt][1]));
-                pt[nt][1] = transposed(pack_f16(s[h][nt][2], s[h][nt][3]));
+                for (int nt = 0; nt < NT; ++nt) {
+                    pt[nt][0] = transposed(pack_f16(s[h][nt][0], s[h][nt][1]));
+                    pt[nt][1] = transposed(pack_f16(s[h][nt][2], s[h][nt][3]));
+                }
             }
-#endif
             const unsigned char* b0 = vs + 2 * h * BLOCK_BYTES;
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             Share<4 * NG> sv[2];                                    // the steps of two neighbouring keys side by side
@@ -532,38 +549,47 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 // B of this group: probability times step, of two keys a register
-                uint32_t pb[NT][TERMS][2];
+                uint32_t pb[NT][PARTS][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#if STORAGE_BF16
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t v = mul_f16x2(pt[nt][b], sv[b].w[j]);
-                        if constexpr (EDGE) v &= ~__vcmpeq2(pt[nt][b], 0x80008000u);      // out of sight: nothing, whatever the step there is
-                        pb[nt][0][b] = v;
-                    }
-#else
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        // before the transposition a lane has keys of row g: its step is half of the word of the pair of rows g / 2
-                        const uint32_t pair = __shfl_sync(0xffffffffu, sv[b].w[j], g >> 1);
-                        const float step = g & 1 ? high_half(pair) : low_half(pair);
-                        float v0 = s[h][nt][2 * b] * step, v1 = s[h][nt][2 * b + 1] * step;
-                        if constexpr (EDGE) {
-                            if (__float_as_uint(s[h][nt][2 * b]) == 0x80000000u) v0 = 0.f;
-                            if (__float_as_uint(s[h][nt][2 * b + 1]) == 0x80000000u) v1 = 0.f;
+                        if constexpr (HALVES_PRODUCT) {
+                            uint32_t v = mul_f16x2(pt[nt][b], sv[b].w[j]);
+                            if constexpr (EDGE) v &= ~__vcmpeq2(pt[nt][b], 0x80008000u);      // out of sight: nothing, whatever the step there is
+                            pb[nt][0][b] = v;
+                        } else {
+                            // before the transposition a lane has keys of row g: its step is half of the word of the pair of rows g / 2
+                            const uint32_t pair = __shfl_sync(0xffffffffu, sv[b].w[j], g >> 1);
+                            const float step = g & 1 ? high_half(pair) : low_half(pair);
+                            float v0 = s[h][nt][2 * b] * step, v1 = s[h][nt][2 * b + 1] * step;
+                            if constexpr (EDGE) {
+                                if (__float_as_uint(s[h][nt][2 * b]) == 0x80000000u) v0 = 0.f;
+                                if (__float_as_uint(s[h][nt][2 * b + 1]) == 0x80000000u) v1 = 0.f;
+                            }
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part) {
+                                const uint32_t term = LARGE ? pack_bf16(v0, v1) : pack_f16(v0, v1);
+                                pb[nt][part][b] = transposed(term);
+                                v0 -= LARGE ? __uint_as_float(term << 16) : low_half(term);
+                                v1 -= LARGE ? __uint_as_float(term & 0xffff0000u) : high_half(term);
+                            }
                         }
-                        const uint32_t hi = pack_f16(v0, v1);
-                        pb[nt][0][b] = transposed(hi);
-                        pb[nt][TERMS - 1][b] = transposed(pack_f16(v0 - low_half(hi), v1 - high_half(hi)));
                     }
-#endif
-                }
                 const uint32_t r0 = __byte_perm(u0.w[j / 2], u1.w[j / 2], j & 1 ? 0x7632 : 0x5410);      // keys 2 c and 2 c + 1 of the first block
                 const uint32_t r1 = __byte_perm(u2.w[j / 2], u3.w[j / 2], j & 1 ? 0x7632 : 0x5410);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t x = k ? r0 >> 8 : r0, y = k ? r1 >> 8 : r1;
+                    if constexpr (LARGE) {
+                        const uint32_t a0 = centred_bf16(x & 0x000f000fu), a1 = centred_bf16((x >> 4) & 0x000f000fu), a2 = centred_bf16(y & 0x000f000fu),
+                                       a3 = centred_bf16((y >> 4) & 0x000f000fu);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part) mma_bf16(o[2 * j + k][nt], a0, a1, a2, a3, pb[nt][part][0], pb[nt][part][1]);
+                        continue;
+                    }
                     uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
                     if constexpr (!OFFSET) { a0 = centred<15>(a0); a1 = centred<11>(a1); a2 = centred<15>(a2); a3 = centred<11>(a3); }
 #pragma unroll
@@ -571,7 +597,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
 #pragma unroll
                         for (int term = 0; term < TERMS; ++term) mma_f16(o[2 * j + k][nt], a0, a1, a2, a3, pb[nt][term][0], pb[nt][term][1]);
                 }
-                if constexpr (OFFSET) {
+                if constexpr (OFFSET && !LARGE) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -586,7 +612,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
         next = look_up(t + 2 * WARPS);
     };
 
-    for (;;) {
+    const auto clear = [&] {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -596,25 +622,35 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
             m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
             l_run[nt][0] = l_run[nt][1] = 0.f;
         }
-        int t = warp;
-        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), t);
+    };
+    clear();
+    int t = warp;
+    for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), std::false_type(), t);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
-        for (; t < n_tiles; t += WARPS) step(std::true_type(), t);
-        float all = 0.f;                                            // an overflow is in the sums of the constant operand too
+        for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
+    for (; t < n_tiles; t += WARPS) step(std::true_type(), std::false_type(), t);
+    float all = 0.f;                                                // an overflow is in the sums of the constant operand too
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < (OFFSET ? NG : D / 16); ++i) {
-                const float* v = OFFSET ? r_off[OFFSET ? i : 0][nt] : o[i][nt];
-                all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
-            }
-        if (shift == LARGE_SHIFT || !__any_sync(0xffffffffu, all != 0.f)) break;
-        shift = LARGE_SHIFT;
+        for (int i = 0; i < (OFFSET ? NG : D / 16); ++i) {
+            const float* v = OFFSET ? r_off[OFFSET ? i : 0][nt] : o[i][nt];
+            all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
+        }
+    if (__any_sync(0xffffffffu, all != 0.f)) {
+        clear();
         here = look_up(warp); next = look_up(warp + WARPS);
         begin();
+        for (t = warp; t < n_tiles; t += WARPS) step(std::true_type(), std::true_type(), t);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)                             // in the units of the usual sums
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                o[i][nt][0] *= OFFSET ? 0x1p-24f : 0x1p-9f; o[i][nt][1] *= OFFSET ? 0x1p-24f : 0x1p-9f;
+                o[i][nt][2] *= OFFSET ? 0x1p-20f : 0x1p-9f; o[i][nt][3] *= OFFSET ? 0x1p-20f : 0x1p-9f;
+            }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                                // every warp is done with its tiles: their place becomes the merge area
@@ -636,7 +672,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     make_float4((o[2 * j][nt][h] - off) * whole, (o[2 * j][nt][2 + h] * SECOND - off) * whole, (o[2 * j + 1][nt][h] - off) * whole,
                                 (o[2 * j + 1][nt][2 + h] * SECOND - off) * whole);
             }
-            if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : fmaf(m_run[nt][h], unit[nt][h], -shift); row[D + 1] = l; }
+            if (g == 0) { row[D] = m_run[nt][h] == -INFINITY ? -INFINITY : fmaf(m_run[nt][h], unit[nt][h], -SHIFT); row[D + 1] = l; }
         }
     __syncthreads();
     // The warps' sums joined, in their order: into the first warp's place for the cluster, or to where they go.

@@ -7,7 +7,7 @@ import torch
 import plain_int4 as plain
 from cisr_b200.ops import kernels
 from cisr_b200.ops.kernels import KernelError
-from test_int4_cache_gpu import Cache, bound, check, i32, prompt_bound, queries
+from test_int4_cache_gpu import Cache, bound, i32, prompt_bound, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,28 @@ def test_tile_lists_have_the_same_length_and_place():
             kernels.attn_prefill_int4(q, torch.empty_like(q), cache.k_cache, cache.v_cache, cache.slots, cache.table, req, q0, i32([0, 60]), i32([60, 40]), cache.ctx, 300, 16, 0.125,
                                       span=128)
     kernels.raise_if_kernel_gave_up()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,dim", [(8, 2, 64), (8, 2, 128), (4, 2, 96)])
+@pytest.mark.parametrize("n", [1, 3, 5])
+@pytest.mark.parametrize("large,small", [(2000.0, 1e-3), (4e5, 1.0), (60.0, 1e-2)])
+def test_a_large_group_among_small_ones(dtype, hq, hkv, dim, n, large, small):
+    """One key of a tile has a large group of 32 values; every other group is held and weighed as exactly as beside small ones."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = torch.randn((2, 700, hkv, dim), generator=g, device="cuda")
+    v = v * small
+    v[100, :, 32:64] = large * torch.randn((hkv, 32), generator=g, device="cuda")
+    v[650, 0, :32] = large
+    q = queries(n, hq, dim, dtype)
+    for again in (False, True):
+        if again:
+            k[100] = -3 * q[0, ::hq // hkv].float()              # the key itself has next to no weight with some rows, and all of it with others
+        cache = Cache([700], hkv, dim, 16, k=[k], v=[v])
+        out, size, p = plain.attention(q, *cache.held(0), dim ** -0.5, plain.seen(n, 700))
+        # Float: the second float16 term of a product below 2^-14 is off by half of the smallest float16, 2^-25, which is 2^-34 of a weight times a
+        # step since weights are held times 2^9, and codes are 7 at most: where one key takes nearly all the weight and has
+        # code 0, that is what is left of the others.
+        small = 0 if dtype == torch.bfloat16 else 7 * 700 * 2.0 ** -34
+        off, most = (cache.attend(q, [n]).double() - out).abs(), bound(dtype, out, size, plain.stepped(p, cache.v[0])) + small
+        assert (off <= most).all(), (again, float((off / most).max()))
