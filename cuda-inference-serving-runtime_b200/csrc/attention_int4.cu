@@ -212,6 +212,8 @@ struct Joined {
     }
     // with the sink: one more term of the denominator, no value
     __device__ __forceinline__ float whole(float sink) const { return sink > -INFINITY ? den + exp2f(fmaf(sink, LOG2E, -m)) : den; }
+    // the logarithm (base 2) of that, by which a score becomes a weight; of a row that sees nothing one by which every weight is 0
+    __device__ __forceinline__ float logarithm(float sink) const { return den == 0.f ? INFINITY : m + log2f(whole(sink)); }
 };
 
 // NT: columns of 8 query rows.  Where there are two or three, or float queries, codes serve two matrix instructions, and the offset is
@@ -697,7 +699,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     float* st = a.stats + ((base_row + r) * a.n_splits + split) * 2;
                     st[0] = j.m; st[1] = j.den;
                 }
-                lse[r] = j.m + log2f(j.whole(sink_of(r)));
+                lse[r] = j.logarithm(sink_of(r));
             }
         }
     }
@@ -751,7 +753,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
             Joined j;
             for (int p = 0; p < parts; ++p) j.m = fmaxf(j.m, others[p][tid][0]);
             for (int p = 0; p < parts; ++p) j.add(others[p][tid][0], 0.f, others[p][tid][1]);
-            lse[tid] = j.m + log2f(j.whole(sink_of(tid)));
+            lse[tid] = j.logarithm(sink_of(tid));
             if (a.stats && rank == 0) {
                 float* st = a.stats + (base_row + tid) * 2;
                 st[0] = j.m; st[1] = j.den;
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(MASS_THREADS) attn_int4_mass_kernel(const __gr
             for (int i = 0; i < parts; ++i) j.m = fmaxf(j.m, stats[i].x);
             for (int i = 0; i < parts; ++i) j.add(stats[i].x, 0.f, stats[i].y);
             const int head = kvh * group + row % group;
-            lse[r] = j.m + log2f(j.whole(a.sink_heads ? a.sink_heads[head] : a.sink_all));
+            lse[r] = j.logarithm(a.sink_heads ? a.sink_heads[head] : a.sink_all);
         }
         __syncthreads();
 #pragma unroll

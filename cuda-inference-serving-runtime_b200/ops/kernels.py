@@ -705,7 +705,8 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
                      window: Optional[int] = None, sink=None, keep_first: int = 0, mass: Optional[torch.Tensor] = None) -> None:
     """Attention of new tokens, few per request (one in a decode step), over a 4-bit cache: q, out [tokens, heads, head_dim].
     Request r brings q_len[r] tokens from row q_start[r] of q on and has ctx_len[r] rows in the cache, theirs included; requests that
-    bring none, or more than `max_queries`, are left alone.  `longest`: no request has more rows (a bound will do; one that has sets the
+    bring none, or more than `max_queries`, are left alone; tokens before a request's first row (it brings more than it has) see nothing and
+    get zeros.  `longest`: no request has more rows (a bound will do; one that has sets the
     flag that `raise_if_kernel_gave_up` reads).  scale: any finite float, of either sign.  window, sink, keep_first: as for `attn_decode`.
 
     `mass` float [pages, kv_heads, page_size]: every key's number grows by the weights that the query heads of its key head, and all of

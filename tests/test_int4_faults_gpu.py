@@ -105,3 +105,28 @@ def test_a_large_group_among_small_ones(dtype, hq, hkv, dim, n, large, small):
         small = 0 if dtype == torch.bfloat16 else 7 * 700 * 2.0 ** -34
         off, most = (cache.attend(q, [n]).double() - out).abs(), bound(dtype, out, size, plain.stepped(p, cache.v[0])) + small
         assert (off <= most).all(), (again, float((off / most).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2), (16, 2)])
+@pytest.mark.parametrize("sink", [None, 0.3])
+def test_tokens_that_see_nothing_give_no_weight(dtype, hq, hkv, sink):
+    """More tokens than rows: the first ones lie before the first row, see nothing, give zeros and add nothing."""
+    lens, q_len, dim, page = [3, 200, 1], [5, 6, 4], 64, 16
+    cache = Cache(lens, hkv, dim, page)
+    q = queries(sum(q_len), hq, dim, dtype)
+    mass = torch.full((cache.pages, hkv, page), 0.25, device="cuda")
+    got = cache.attend(q, q_len, mass=mass, sink=sink)
+    at = 0
+    for r, n in enumerate(q_len):
+        blind = max(0, n - lens[r])
+        assert not got[at:at + blind].any()
+        ok = plain.seen(n, lens[r])[blind:]
+        out, size, p = plain.attention(q[at + blind:at + n], *cache.held(r), dim ** -0.5, ok, sink)
+        off = (got[at + blind:at + n].double() - out).abs()
+        assert (off <= bound(dtype, out, size, plain.stepped(p, cache.v[r]))).all()
+        sums = torch.cat([mass[i] for i in cache.table[r].tolist() if i >= 0], 1)[:, :lens[r]].double() - 0.25
+        want = p.view(hkv, -1, lens[r]).sum(1)
+        # weights as far off as `bound` says of scores, and float sums beside 0.25
+        assert ((sums - want).abs() <= 2 * 70 * 8 * 2.0 ** -23 * want + 2.0 ** -22).all(), (r, sums, want)
+        at += n
