@@ -1013,12 +1013,12 @@ struct Shape {
     int launches(bool mass) const { return 1 + merged_by_kernel() + (mass && mass_by_kernel()); }
 };
 
-template <int NT, int WARPS> int launch(int device, Args& a, const Shape& shape, int n_req, float* mass, cudaStream_t s) {
+template <int NT, int WARPS> int launch(int device, Args& a, const Shape& shape, int n_req, float* mass, bool early, cudaStream_t s) {
     constexpr size_t SMEM = dynamic_smem<NT, WARPS>();
     if (const cudaError_t e = prepare_kernel<NT, WARPS>(device); e != cudaSuccess) return (int)e;
     const dim3 grid((unsigned)(n_req * a.tiles), (unsigned)a.hkv, (unsigned)a.n_splits);
     a.mass = shape.mass_by_kernel() ? nullptr : mass;
-    int status = launch_kernel_cluster(attn_int4_kernel<NT, WARPS>, grid, dim3(32 * WARPS), SMEM, s, g_pdl, a.cluster, a);
+    int status = launch_kernel_cluster(attn_int4_kernel<NT, WARPS>, grid, dim3(32 * WARPS), SMEM, s, early, a.cluster, a);
     if (status) return status;
     if (shape.merged_by_kernel()) {
         status = launch_kernel(attn_int4_merge_kernel<8 * NT>, dim3(grid.x, grid.y, (unsigned)a.row_stride), dim3(D), 0, s, true, a);
@@ -1051,11 +1051,12 @@ struct AttnInt4Call {
     const void *q; void* out; const void *k_cache, *v_cache; const int *req_slot, *block_table, *q_start, *q_len, *ctx_len; float *scratch, *mass; const float* sink_heads;
     void* stream;
     double scale, sink;
-    int width, n_req, max_queries, longest, hq, hkv, page_size, window, keep_first;
+    int width, n_req, max_queries, longest, hq, hkv, page_size, window, keep_first, new_lists;
 };
 
 // q, out [tokens][hq][D]; request r brings q_len[r] tokens from row q_start[r] on and has ctx_len[r] rows with them; those with more than
-// `max_queries` are left alone, and none may have more than `longest` rows (one that has sets the error flag).
+// `max_queries` are left alone, and none may have more than `longest` rows (one that has sets the error flag).  new_lists: the kernel launched just
+// before may be the one that writes the lists or the table, which are else read beside its end: this one then starts behind it.
 CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
     const AttnInt4Call& c = *call;
     if (c.n_req <= 0 || c.max_queries <= 0) return 0;
@@ -1068,7 +1069,7 @@ CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
     const Shape shape(device, c.n_req, c.max_queries, c.longest, c.hq, c.hkv, c.window, c.keep_first);
     if (shape.splits > 65535 || (long long)c.n_req * shape.tiles >= 1ll << 31) return -2;
     const int group = c.hq / c.hkv;
-    const bool mass = c.mass != nullptr;
+    const bool mass = c.mass != nullptr, early = g_pdl && !c.new_lists;
     Args a{};
     a.q = (const T*)c.q; a.out = (T*)c.out; a.k_cache = (const unsigned char*)c.k_cache; a.v_cache = (const unsigned char*)c.v_cache;
     a.req_slot = c.req_slot; a.table = c.block_table; a.width = c.width; a.q_start = c.q_start; a.q_len = c.q_len; a.ctx_len = c.ctx_len;
@@ -1081,8 +1082,8 @@ CISR_EXPORT int cisr_attn_int4(const AttnInt4Call* call) {
     a.longest = c.longest; a.hq = c.hq; a.hkv = c.hkv; a.page_size = c.page_size; a.window = c.window; a.keep_first = c.keep_first;
     a.scale = (float)c.scale; a.sink_all = (float)c.sink; a.sink_heads = c.sink_heads; a.error = g_error;
 #if STORAGE_BF16
-    if (shape.rows == 24) return launch<3, 4>(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
+    if (shape.rows == 24) return launch<3, 4>(device, a, shape, c.n_req, c.mass, early, (cudaStream_t)c.stream);
 #endif
     const auto run = shape.rows == 16 ? launch<2, 4> : shape.warps == MOST_WARPS ? launch<1, MOST_WARPS> : launch<1, 4>;
-    return run(device, a, shape, c.n_req, c.mass, (cudaStream_t)c.stream);
+    return run(device, a, shape, c.n_req, c.mass, early, (cudaStream_t)c.stream);
 }

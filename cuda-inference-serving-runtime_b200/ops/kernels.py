@@ -618,7 +618,7 @@ def _int4_lists(what: str, device: int, table: torch.Tensor, count: int, names: 
 _ROW_LISTS, _REQUEST_LISTS = ("req_slot", "token_req", "positions"), ("req_slot", "q_start", "q_len", "ctx_len")
 # The calls' arguments in the order of csrc/int4_rows.cu and csrc/attention_int4.cu.
 _STORE_CALL, _READ_CALL, _EVICT_CALL = struct.Struct("@10P4q6i").pack, struct.Struct("@11P3q7i").pack, struct.Struct("@9P10i").pack
-_ATTN_INT4_CALL = struct.Struct("@13P2d9i").pack
+_ATTN_INT4_CALL = struct.Struct("@13P2d10i").pack
 _NO_SINK = (float("-inf"), 0)
 
 
@@ -702,7 +702,7 @@ def int4_expand(k_cache: torch.Tensor, v_cache: torch.Tensor, k_out: torch.Tenso
 
 def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor,
                      q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, max_queries: int, longest: int, page_size: int, scale: float,
-                     window: Optional[int] = None, sink=None, keep_first: int = 0, mass: Optional[torch.Tensor] = None) -> None:
+                     window: Optional[int] = None, sink=None, keep_first: int = 0, mass: Optional[torch.Tensor] = None, new_lists: bool = False) -> None:
     """Attention of new tokens, few per request (one in a decode step), over a 4-bit cache: q, out [tokens, heads, head_dim].
     Request r brings q_len[r] tokens from row q_start[r] of q on and has ctx_len[r] rows in the cache, theirs included; requests that
     bring none, or more than `max_queries`, are left alone; tokens before a request's first row (it brings more than it has) see nothing and
@@ -711,7 +711,10 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
 
     `mass` float [pages, kv_heads, page_size]: every key's number grows by the weights that the query heads of its key head, and all of
     the request's new tokens, have given it (a sink takes its part of them).  The same call gives the same numbers, unless requests of
-    it share a page: that grows by the weights of each, in no certain order."""
+    it share a page: that grows by the weights of each, in no certain order.
+
+    `new_lists`: in captured steps with dependent launch the lists and the table are read beside the end of the kernel launched
+    just before, which must then not be the one that writes them; where it may be, say so, and this call starts behind it."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     tokens, hq, dim = q.shape
     hkv, device = _int4_cache("attn_decode_int4", k_cache, v_cache, page_size, None, dim)
@@ -736,7 +739,7 @@ def attn_decode_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     try:
         packed = _ATTN_INT4_CALL(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), q_start.data_ptr(),
                                  q_len.data_ptr(), ctx_len.data_ptr(), 0 if scratch is None else scratch.data_ptr(), 0 if mass is None else mass.data_ptr(), per_head, _stream(),
-                                 scale, number, block_table.size(1), n, max_queries, longest, hq, hkv, page_size, window or 0, keep_first)
+                                 scale, number, block_table.size(1), n, max_queries, longest, hq, hkv, page_size, window or 0, keep_first, bool(new_lists))
     except struct.error as err:
         raise KernelError(f"attn_decode_int4: {err}") from err
     _check(call[0](packed), "attn_decode_int4", own=call[2])
@@ -774,7 +777,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     if span == PREFILL_TILE:
         lists = (req_slot, q_start, q_len, ctx_len) if requests is None else [t[requests.long()] for t in (req_slot, q_start, q_len, ctx_len)]
         _untimed["attn_decode_int4"](q, out, k_cache, v_cache, lists[0], block_table, *lists[1:], max(1, min(max_queries or q.shape[0], q.shape[0])), longest, page_size, scale, window, sink,
-                         keep_first)
+                         keep_first, new_lists=requests is not None)
         return
     if q.dtype != torch.bfloat16 or dim not in TCGEN05_HEAD_DIMS:
         raise KernelError(f"attn_prefill_int4: tiles of {span} queries are for bfloat16 and head sizes {TCGEN05_HEAD_DIMS}")

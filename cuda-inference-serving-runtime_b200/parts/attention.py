@@ -208,9 +208,9 @@ def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, win
     lens, ends = ctx.host.q_len, ctx.host.ctx_len
     most, weighed = max(lens), kernels.INT4_WEIGHED
 
-    def over_pages(q_start, q_len, queries, longest, mass):
+    def over_pages(q_start, q_len, queries, longest, mass, new_lists=False):
         kernels.attn_decode_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, q_start, q_len, ctx.ctx_len, queries, max(longest, ctx.host.ctx_bound or 0),
-                                 cache.page_size, scale, window, mass=mass)
+                                 cache.page_size, scale, window, mass=mass, new_lists=new_lists)
 
     by_portions = most > kernels.INT4_FEW and q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS
     if by_portions:
@@ -235,7 +235,7 @@ def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, win
     if latest is None:
         n = ctx.q_len.clamp(max=weighed)
         latest = ctx.shared["int4_latest"] = (ctx.q_start + ctx.q_len - n, n)
-    over_pages(*latest, weighed, max(ends), cache.mass)
+    over_pages(*latest, weighed, max(ends), cache.mass, new_lists=True)
     return out
 
 

@@ -130,3 +130,43 @@ def test_tokens_that_see_nothing_give_no_weight(dtype, hq, hkv, sink):
         # weights as far off as `bound` says of scores, and float sums beside 0.25
         assert ((sums - want).abs() <= 2 * 70 * 8 * 2.0 ** -23 * want + 2.0 ** -22).all(), (r, sums, want)
         at += n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lists_made_just_before_the_attention(monkeypatch, dtype):
+    """With dependent launch: the call that gathers the listed requests' lists itself says so to the kernel (which must not read them before it
+    waits), a call with lists from before does not, and replays follow the lists that the step makes."""
+    hq, hkv, dim, page = 8, 2, 96, 16
+    cache = Cache([300, 180, 90], hkv, dim, page)
+    q = queries(60, hq, dim, dtype)
+    q_len, q_start, which = i32([20, 30, 10]), i32([0, 20, 50]), i32([2, 0])
+    tiles, places, out = i32([0]), i32([1, -9, 0]), torch.zeros_like(q)
+    said = []
+    pack = kernels._ATTN_INT4_CALL
+    monkeypatch.setattr(kernels, "_ATTN_INT4_CALL", lambda *args: (said.append(args[-1]), pack(*args))[1])
+    first = i32([0, 20, 50])
+
+    def turn():
+        q_start.copy_(first + 0)
+        kernels.attn_prefill_int4(q, out, cache.k_cache, cache.v_cache, cache.slots, cache.table, tiles, tiles, q_start, q_len, cache.ctx, 300, page, dim ** -0.5, span=64,
+                                  portions=(which, places))
+
+    turn()
+    kernels.attn_decode_int4(q, out, cache.k_cache, cache.v_cache, cache.slots, cache.table, q_start, q_len, cache.ctx, 30, 300, page, dim ** -0.5)
+    assert said == [True, False]
+    graph = torch.cuda.CUDAGraph()
+    kernels.set_pdl(True)
+    try:
+        with torch.cuda.graph(graph):
+            turn()
+    finally:
+        kernels.set_pdl(False)
+    for listed in ([2, 0], [1, 2], [0, 0]):
+        which.copy_(i32(listed))
+        out.fill_(7.0)
+        graph.replay()
+        want = torch.full_like(q, 7.0)
+        for r in set(listed):
+            only = i32([n if i == r else 0 for i, n in enumerate((20, 30, 10))])
+            kernels.attn_decode_int4(q, want, cache.k_cache, cache.v_cache, cache.slots, cache.table, first, only, cache.ctx, 60, 300, page, dim ** -0.5)
+        assert torch.equal(out == 7, want == 7) and torch.allclose(out.float(), want.float(), rtol=2 ** -6, atol=2 ** -8)
