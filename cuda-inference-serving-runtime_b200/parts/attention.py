@@ -132,7 +132,7 @@ class GQAAttention(Mixer):
             if cache.write:
                 kernels.int4_store(to.k[0].transpose(0, 1), to.v[0].transpose(0, 1), cache.k, cache.v, ctx.token_req, token_rows(ctx, cache), ctx.req_slot,
                                    cache.block_table, cache.page_size, mass=cache.mass)
-            out = int4_attention(ctx.plan_for(self), q, cache, ctx, hq, self.scale, self.window)
+            out = int4_attention(q, cache, ctx, hq, self.scale, self.window)
             return linear_to_stream(out.view(tokens, hq * dim), self.o, h0)
         out = torch.empty((tokens, hq, dim), dtype=self.dtype, device=device)
         plan = ctx.plan_for(self)
@@ -200,37 +200,73 @@ def token_rows(ctx, cache) -> torch.Tensor:
     return rows
 
 
-def int4_attention(plan, q: torch.Tensor, cache, ctx, hq: int, scale: float, window) -> torch.Tensor:
+def portion_groups(q_len, ctx_len, few: int) -> list:
+    """The requests with portions of more than `few` tokens, longest first, in groups for one call each: a call writes all its requests' rows out
+    at the length of its longest, and a group ends where that would be more than half as much again as they have."""
+    groups, rows = [], 0
+    for r in sorted((r for r, n in enumerate(q_len) if n > few), key=lambda r: -ctx_len[r]):
+        if groups and 2 * (len(groups[-1]) + 1) * ctx_len[groups[-1][0]] <= 3 * (rows + ctx_len[r]):
+            groups[-1].append(r)
+            rows += ctx_len[r]
+        else:
+            groups.append([r])
+            rows = ctx_len[r]
+    return groups
+
+
+def int4_portions(ctx, heads: int, window) -> list:
+    """The calls for a step's portions of more than a few tokens: (tiles, span, (requests, places), rows of the longest) each, once per step and
+    kind of layer."""
+    calls = ctx.shared.get(("int4_portions", heads, window))
+    if calls is not None:
+        return calls
+    lens, ends = ctx.host.q_len, ctx.host.ctx_len
+    groups = portion_groups(lens, ends, kernels.INT4_FEW)
+    sms, spans, flat = kernels.sm_count(ctx.device), [], []
+    for which in groups:
+        of = [lens[r] for r in which]
+        span = kernels.WIDE_TILE
+        if sum(-(-n // span) for n in of) * heads > sms:
+            span = wide_span(of, [ends[r] for r in which], heads, window, 0, sms)
+        # a portion's last tile first (it has the longest key loop), but those of 128 queries or fewer in tiles of 256 last (they take half the time)
+        tiles = [(r, a) for r, n in zip(which, of) for a in range((n - 1) // span * span, -1, -span)]
+        if span == kernels.WIDE_PAIR:
+            tiles.sort(key=lambda t: lens[t[0]] - t[1] <= kernels.WIDE_TILE)
+        spans.append(span)
+        place = {r: i for i, r in enumerate(which)}
+        flat += [[r for r, _ in tiles], [a for _, a in tiles], which, [place.get(r, 0) for r in range(len(lens))]]
+    lists = torch.tensor([x for part in flat for x in part], dtype=torch.int32, device=ctx.device).split([len(part) for part in flat])
+    calls = [(lists[4 * i:4 * i + 2], span, lists[4 * i + 2:4 * i + 4], ends[which[0]]) for i, (which, span) in enumerate(zip(groups, spans))]
+    ctx.shared["int4_portions", heads, window] = calls
+    return calls
+
+
+def int4_attention(q: torch.Tensor, cache, ctx, hq: int, scale: float, window) -> torch.Tensor:
     """Attention of a step's queries over pages held in 4 bits: portions of more than a few tokens by the prompt kernel over the rows written
     out as values, where the queries' type and head size have one, all others straight over the pages.  Where keys are weighed,
     what counts are the latest tokens of every portion: those run over the pages, too."""
     out = torch.empty_like(q)
     lens, ends = ctx.host.q_len, ctx.host.ctx_len
-    most, weighed = max(lens), kernels.INT4_WEIGHED
+    most, weighed, few = max(lens), kernels.INT4_WEIGHED, kernels.INT4_FEW
 
     def over_pages(q_start, q_len, queries, longest, mass, new_lists=False):
         kernels.attn_decode_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, q_start, q_len, ctx.ctx_len, queries, max(longest, ctx.host.ctx_bound or 0),
                                  cache.page_size, scale, window, mass=mass, new_lists=new_lists)
 
-    by_portions = most > kernels.INT4_FEW and q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS
-    if by_portions:
-        step = ctx.shared.get("int4_portions")
-        if step is None:                     # once per step: which requests bring portions, and the place of each among them
-            which = [r for r, n in enumerate(lens) if n > 1]
-            places = [which.index(r) if n > 1 else 0 for r, n in enumerate(lens)]
-            lists = torch.tensor(which + places, dtype=torch.int32, device=ctx.device)
-            step = ctx.shared["int4_portions"] = (lists[:len(which)], lists[len(which):], max(ends[r] for r in which))
-        (tile_req, tile_q0), span = wide_tiles(plan, ctx, hq, window)
-        kernels.attn_prefill_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, tile_req, tile_q0, ctx.q_start, ctx.q_len, ctx.ctx_len, step[2],
-                                  cache.page_size, scale, window, span=span, portions=step[:2])
-    if cache.mass is None or most <= weighed:
-        if not by_portions:
-            over_pages(ctx.q_start, ctx.q_len, most, max(ends), cache.mass)
-        elif plan.info["n_decode"]:
-            over_pages(ctx.q_start, ctx.q_len, 1, max(c for n, c in zip(lens, ends) if n == 1), None)
+    if most > few and q.dtype == torch.bfloat16 and q.shape[2] in kernels.TCGEN05_HEAD_DIMS:
+        for tiles, span, portions, longest in int4_portions(ctx, hq, window):
+            kernels.attn_prefill_int4(q, out, cache.k, cache.v, ctx.req_slot, cache.block_table, *tiles, ctx.q_start, ctx.q_len, ctx.ctx_len, longest, cache.page_size, scale,
+                                      window, span=span, portions=portions)
+        short = [n for n in lens if n <= few]
+        if short and max(short) > (0 if cache.mass is None else weighed):          # (fewer that are weighed are below)
+            over_pages(ctx.q_start, ctx.q_len, max(short), max(c for n, c in zip(lens, ends) if n <= few), None)
+    elif cache.mass is None or most <= weighed:
+        over_pages(ctx.q_start, ctx.q_len, most, max(ends), cache.mass)
         return out
-    if not by_portions:
+    else:
         over_pages(ctx.q_start, ctx.q_len, most, max(ends), None)
+    if cache.mass is None:
+        return out
     latest = ctx.shared.get("int4_latest")
     if latest is None:
         n = ctx.q_len.clamp(max=weighed)

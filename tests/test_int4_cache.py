@@ -211,3 +211,21 @@ def test_a_request_that_never_fits_is_refused():
         engine.submit(Request("r", [1] * 200, max_new_tokens=100))
     engine.submit(Request("s", [1] * 20, max_new_tokens=10))
     assert len(engine.run()[-1].generated) == 10
+
+
+def test_portions_go_in_groups_of_like_lengths():
+    """A call writes every request's rows out at the length of its longest: at most half as much again as they have."""
+    from cisr_b200.parts.attention import portion_groups
+
+    assert portion_groups([1, 1, 2, 32], [5, 900, 40, 40], 32) == [] and portion_groups([], [], 32) == []
+    assert portion_groups([100, 1, 60, 33], [1000, 9000, 900, 1000], 32) == [[0, 3, 2]]
+    assert portion_groups([33] + [40] * 30 + [2] * 30, [100000] + [40] * 30 + [100000] * 30, 32) == [[0], list(range(1, 31))]
+    rng = np.random.default_rng(3)
+    for _ in range(200):
+        n = int(rng.integers(1, 40))
+        lens = rng.integers(0, 80, n).tolist()
+        ends = [k + int(10 ** rng.uniform(0, 5)) for k in lens]
+        groups = portion_groups(lens, ends, 32)
+        assert sorted(r for g in groups for r in g) == [r for r, k in enumerate(lens) if k > 32]
+        for g in groups:
+            assert ends[g[0]] == max(ends[r] for r in g) and 2 * len(g) * ends[g[0]] <= 3 * sum(ends[r] for r in g)

@@ -3,10 +3,108 @@ rows that the cache really holds."""
 import pytest
 import torch
 
+import plain_int4
 from test_int4_cache import Launching
-from test_int4_engine_gpu import model_of, stepper_of, tokens_of
+from test_int4_engine_gpu import RAW, model_of, stepper_of, tokens_of
 
 pytestmark = pytest.mark.gpu
+
+
+def read_out(stepper, key):
+    """Keys and values that the cache holds of a request, of every layer: pairs of [kv_heads, rows, dim] in 64 bits."""
+    from cisr_b200.ops import kernels
+
+    cache, found = stepper.cache, []
+    for entry in range(len(stepper.model.spec.run)):
+        b = cache.binding(entry)
+        n, mixer = cache.length(key), stepper.model.layers[entry].parts()["mixer"]
+        k, v = torch.empty((2, 1, mixer.hkv, n, mixer.dim), device="cuda")
+        one = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")
+        group = cache.page_groups[cache.entry_group[entry][1]]
+        table = torch.from_numpy(group.host_table[cache.slot(key)][None]).cuda()
+        kernels.int4_expand(b.k, b.v, k, v, one(0), table, one(n), cache.page_size)
+        found.append((k[0].double(), v[0].double()))
+    return found
+
+
+def on_held_rows(stepper, key, tokens, check_rows=True):
+    """Logits [tokens, vocab] in 64 bits of the latest `tokens` of a request, whose rows are in the cache: with the keys and values that the cache
+    holds, so that what is left are roundings.  Rounded to the model's type where the engine does.
+
+    The tokens' own rows are checked: a held value is within half a step of what was stored, and that is within 2^-5 of the
+    group's largest of the plain one (in float 2^-14), seven steps."""
+    model, n = stepper.model, len(tokens)
+    rounded = lambda x: x.to(model.dtype).double()
+    norm = lambda x, part: x * torch.rsqrt(x.square().mean(-1, keepdim=True) + RAW["rms_norm_eps"]) * part.weight.double()
+    rows, first = stepper.cache.length(key), stepper.cache.seen(key) - n
+    at = torch.arange(rows - n, rows, device="cuda")[:, None]
+    j = torch.arange(rows, device="cuda")[None]
+    x = model.embedding.table[torch.tensor(tokens, device="cuda")].double()
+    for layer, (keys, values) in zip(model.layers, read_out(stepper, key)):
+        mixer, ff, n1, n2 = (layer.parts()[p] for p in ("mixer", "feed_forward", "mixer_norm", "feed_forward_norm"))
+        hq, hkv, dim = mixer.hq, mixer.hkv, mixer.dim
+        qkv = (rounded(norm(x, n1)) @ mixer.qkv.double().T).view(n, hq + 2 * hkv, dim)
+        inv = RAW["rope_theta"] ** (-torch.arange(0, dim, 2, dtype=torch.float64, device="cuda") / dim)
+        angle = torch.arange(first, first + n, device="cuda", dtype=torch.float64)[:, None, None] * inv
+        a, b = qkv[:, :hq + hkv, :dim // 2], qkv[:, :hq + hkv, dim // 2:]
+        turned = rounded(torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1))
+        for new, held in ((turned[:, hq:], keys), (rounded(qkv[:, hq + hkv:]), values)):
+            top = new.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True).expand(n, hkv, dim // 32, 32).flatten(2)
+            off = (held[:, rows - n:].transpose(0, 1) - new).abs()
+            if check_rows:
+                assert (off <= top / 14 + top * (2.0 ** -5 if model.dtype == torch.bfloat16 else 2.0 ** -14)).all(), float((off / top).max())
+        ok = j <= at
+        if mixer.window:
+            ok &= at - j < mixer.window
+        p = plain_int4.weights(turned[:, :hq], keys, dim ** -0.5, ok)
+        mixed = torch.einsum("hnj,hjd->nhd", p, values.repeat_interleave(hq // hkv, 0))
+        x = x + rounded(mixed.reshape(n, -1)) @ mixer.o.double().T
+        gate, up = (rounded(norm(x, n2)) @ ff.gate_up.double().T).chunk(2, -1)
+        x = x + rounded(torch.nn.functional.silu(gate) * up) @ ff.down.double().T
+    return rounded(norm(x, model.final_norm)) @ model.head.weight.double().T
+
+
+def logits_bound(dtype, layers=2):
+    """Of the logits' spread.  bfloat16: seven places a layer and one behind are rounded, on both sides of numbers that are not quite the same: an
+    independent rounding each, 2^-8 at most and 2^-8 / sqrt 3 in the mean square, which are added as if they all pointed one way.  float: as
+    many places of 2^-16 (products of three bfloat16 parts and their sums), and an attention's scores as `bound` has them, 1.3e-4 a layer."""
+    places = 7 * layers + 1
+    return places * 2.0 ** -8 / 3 ** 0.5 if dtype == torch.bfloat16 else places * 2.0 ** -16 + layers * 1.3e-4
+
+
+def check_step(stepper, got, portions):
+    """A step's logits, all rows of all portions {key: tokens}: every one within the bound."""
+    at = 0
+    for key, tokens in portions.items():
+        want = on_held_rows(stepper, key, tokens)
+        off = (got[at:at + len(tokens)].double() - want).square().mean(-1).sqrt() / want.std()
+        assert (off <= logits_bound(stepper.model.dtype, len(stepper.model.layers))).all(), (key, off.tolist())
+        at += len(tokens)
+    stepper.check_kernels()
+
+
+def run_step(stepper, portions):
+    from cisr_b200 import StepEntry
+
+    return stepper.step([StepEntry(key, tokens, list(range(len(tokens)))) for key, tokens in portions.items()]).clone()
+
+
+SHAPES = [("float32", 4, 2, 128), ("bfloat16", 4, 2, 256), ("bfloat16", 9, 3, 576), ("bfloat16", 4, 2, 384), ("bfloat16", 8, 2, 1024)]
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,hidden", SHAPES)
+def test_portions_of_every_length_in_one_step(dtype, heads, kv_heads, hidden):
+    """A long portion behind many rows, short and single ones beside it: by groups of like lengths, and straight over the pages."""
+    stepper = stepper_of(model_of(dtype, heads, kv_heads, hidden), n_pages=300, max_slots=8)
+    before = dict(zip("abcdefgh", (400, 3, 90, 0, 33, 200, 1, 60)))
+    for seed, (key, n) in enumerate(before.items()):
+        stepper.create(key)
+        if n:
+            run_step(stepper, {key: tokens_of(n, seed)})
+    for seed, lens in enumerate([(60, 40, 33, 70, 20, 1, 2, 32), (35, 1, 1, 1, 9, 33, 1, 150)]):
+        portions = {key: tokens_of(n, 20 + 10 * seed + i) for i, (key, n) in enumerate(zip(before, lens))}
+        check_step(stepper, run_step(stepper, portions), portions)
+    stepper.cache.check()
 
 
 @pytest.mark.parametrize("keep", [None, 64])
