@@ -170,3 +170,53 @@ def test_lists_made_just_before_the_attention(monkeypatch, dtype):
             only = i32([n if i == r else 0 for i, n in enumerate((20, 30, 10))])
             kernels.attn_decode_int4(q, want, cache.k_cache, cache.v_cache, cache.slots, cache.table, first, only, cache.ctx, 60, 300, page, dim ** -0.5)
         assert torch.equal(out == 7, want == 7) and torch.allclose(out.float(), want.float(), rtol=2 ** -6, atol=2 ** -8)
+
+
+def squared_errors(q, k, v, p, scale):
+    """What the portions' float16 operands are off by in the mean square, [n, heads, dim], errors of one place independent of another's: a rounding is 2^-11 of
+    a number at most and 2^-11 / sqrt 3 in the mean square (a bound for all mantissas).  Probabilities and values: as much of p v each.
+    Keys: of every product q k of a score, and a score's error e turns p into p (1 + e - the mean of e): p (v - out) e."""
+    u = 2.0 ** -22 / 3
+    group = q.shape[1] // k.shape[0]
+    k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+    e = torch.einsum("nhd,hjd->hnj", q.double().square(), k.square()) * scale ** 2 * u
+    out = torch.einsum("hnj,hjd->nhd", p, v)
+    spread = torch.einsum("hnj,hjd->nhd", p.square() * e, v.square()) - 2 * out * torch.einsum("hnj,hjd->nhd", p.square() * e, v)
+    spread += out.square() * (p.square() * e).sum(-1).transpose(0, 1)[..., None]
+    return 2 * u * torch.einsum("hnj,hjd->nhd", p.square(), v.square()) + spread
+
+
+@pytest.mark.parametrize("hq,hkv,dim,span", [(8, 2, 64, 128), (8, 2, 128, 128), (32, 8, 128, 256), (9, 3, 64, 256)])
+@pytest.mark.parametrize("std", [0.3, 1.5, 3.0])
+def test_portions_are_as_exact_as_their_operands(hq, hkv, dim, span, std):
+    """In the mean square over each request: the output's own rounding, which is known to the digit, and what float16 operands add.  In a
+    model on the CPU float16 operands are at 0.96 to 0.98 of the two; bfloat16 ones, eight times as coarse, at 1.27 and more (probabilities, queries of 0.3),
+    1.3 (values) and 1.7 (keys, queries of 1.5 and more)."""
+    lens, q_len = [1000, 300, 140], [290, 300, 40]
+    cache = Cache(lens, hkv, dim, 16)
+    q = queries(sum(q_len), hq, dim, torch.bfloat16, std=std)
+    got = portions(cache, q, q_len, span, dim ** -0.5)
+    at = 0
+    for r, n in enumerate(q_len):
+        held = cache.held(r)
+        want, size, p = plain.attention(q[at:at + n], *held, dim ** -0.5, plain.seen(n, lens[r]))
+        own = (want.to(torch.bfloat16).double() - want).square().mean()
+        rest = squared_errors(q[at:at + n], *held, p, dim ** -0.5).mean()
+        off = (got[at:at + n].double() - want).square().mean()
+        assert off <= 1.1 ** 2 * (own + rest), (r, float((off / (own + rest)).sqrt()), float((own / want.square().mean()).sqrt()), float((rest / want.square().mean()).sqrt()))
+        at += n
+
+
+@pytest.mark.parametrize("dim,span", [(64, 128), (128, 256), (96, 64)])
+@pytest.mark.parametrize("large,small", [(2000.0, 1e-3), (4e5, 1.0), (60.0, 1e-2)])
+def test_portions_with_a_large_group_among_small_ones(dim, span, large, small):
+    """Values down to 2^-28 of a key head's largest keep all their digits in float16 (its normal numbers reach from 2^-14 to 2^16)."""
+    hq, hkv, scale = 8, 2, dim ** -0.5
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = torch.randn((2, 700, hkv, dim), generator=g, device="cuda")
+    v = v * small
+    v[100, :, 32:64] = large * torch.randn((hkv, 32), generator=g, device="cuda")
+    v[650, 0, :32] = large
+    cache = Cache([700], hkv, dim, 16, k=[k], v=[v])
+    q = queries(200, hq, dim, torch.bfloat16)
+    check_portions(cache, q, portions(cache, q, [200], span, scale), [200], span, scale)

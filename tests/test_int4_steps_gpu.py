@@ -136,3 +136,109 @@ def test_nothing_is_made_between_the_embedding_and_the_first_product(monkeypatch
     assert between == [], mode.seen
     attend = [i for i, name in enumerate(mode.seen) if name == "attn_decode_int4"]
     assert attend and all(mode.seen[i - 1] == "int4_store" for i in attend), mode.seen       # it waits before it lets the attention start
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,hidden", SHAPES + [("bfloat16", 32, 8, 4096)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_every_step_of_batches_of_changing_size(dtype, heads, kv_heads, hidden, graph):
+    """Single tokens of one to eight requests by turns (captured steps of 1, 2, 4 and 8 rows, of two context sizes, that share their memory), a portion
+    between them: every row of every step."""
+    stepper = stepper_of(model_of(dtype, heads, kv_heads, hidden), n_pages=400, max_slots=8, graph=graph)
+    keys = "abcdefgh"
+    for i, key in enumerate(keys):
+        stepper.create(key)
+        portions = {key: tokens_of(5 + 35 * i, i)}
+        check_step(stepper, run_step(stepper, portions), portions)
+    turns = ["a", "abcdefgh", "cb", "abc", "h", "gfedcba", "bd", "a", "ah", "abcdefgh", "efg", "hg", "a"]
+    for turn in range(2):
+        for i, which in enumerate(turns):
+            portions = {key: tokens_of(1, 100 * turn + 10 * i + j) for j, key in enumerate(which)}
+            check_step(stepper, run_step(stepper, portions), portions)
+            stepper.cache.check()
+        portions = {"a": tokens_of(40, turn), "c": tokens_of(1, 7)}
+        check_step(stepper, run_step(stepper, portions), portions)
+    if graph:
+        assert stepper.graphs.hits > 10 and {rows for rows, _ in stepper.graphs.graphs} == {1, 2, 4, 8}
+
+
+@pytest.mark.parametrize("dtype,dim", [("float32", 32), ("bfloat16", 64), ("bfloat16", 128), ("bfloat16", 96)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_every_step_of_a_layer_with_a_window(dtype, dim, graph):
+    """One layer that sees 40 keys, whose pages go back as they are passed, and one that sees all."""
+    from cisr_b200 import Model
+    from test_toy_parts_gpu import W_CONFIG, register_windowed_toy
+
+    register_windowed_toy()
+    stepper = stepper_of(Model.from_config(dict(W_CONFIG, hidden_size=4 * dim, head_dim=dim, vocab_size=256), seed=5, dtype=dtype), n_pages=100, graph=graph)
+    commit, late = stepper.cache.commit, []
+
+    def commit_later(key, n):                                    # the rows of a step are looked at before passed pages go back
+        stepper.cache.requests[key].length += n
+        stepper.cache.requests[key].seen += n
+        late.append((key, n))
+
+    stepper.cache.commit = commit_later
+    stepper.create("a"); stepper.create("b")
+    steps = [{"a": n, "b": n // 3 + 1} for n in (100, 45, 3, 20, 52)] + [dict.fromkeys(("ab", "a", "ba")[i % 3], 1) for i in range(60)]
+    for i, lens in enumerate(steps):
+        portions = {key: tokens_of(n, 10 * i + j) for j, (key, n) in enumerate(lens.items())}
+        check_step(stepper, run_step(stepper, portions), portions)
+        while late:
+            key, n = late.pop()
+            stepper.cache.requests[key].length -= n
+            stepper.cache.requests[key].seen -= n
+            commit(key, n)
+        stepper.cache.check()
+    windowed = next(g for g in stepper.cache.page_groups if g.use.window)
+    assert windowed.pool.n_used <= 2 * (40 // 8 + 1)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("chunk", [5, 48])
+def test_every_step_of_requests_that_are_cut(dtype, graph, chunk):
+    """Two requests that are cut again and again, alone and together: every step's logits are those of the rows that were held in it."""
+    from cisr_b200.engine.step import Keep
+
+    keep = Keep(rows=48, recent=12, first=2, slack=8)
+    stepper = stepper_of(model_of(dtype, 4, 2, 256), keep=keep, graph=graph, n_pages=100)
+    cuts = []
+    cut = stepper._cut
+    stepper._cut = lambda keys: cuts.append(list(keys))          # the rows of a step are looked at before it cuts
+    stepper.create("a"); stepper.create("b")
+    plan = [{"a": chunk, "b": 3}, {"a": chunk}, {"b": chunk, "a": 1}] + [{"a": 1, "b": 1}] * 20 + [{"a": 1}] * 9 + [{"b": chunk}] + [{"a": 1, "b": 1}] * 20
+    sizes = []
+    for i, lens in enumerate(plan):
+        portions = {key: tokens_of(n, 1000 + 10 * i) for key, n in lens.items()}
+        got = run_step(stepper, portions)
+        check_step(stepper, got, portions)
+        sizes.append(stepper.cache.length("a"))
+        cut(cuts.pop())
+        stepper.cache.check()
+        assert all(stepper.cache.length(key) < keep.rows + keep.slack for key in portions)
+    assert max(sizes) >= keep.rows + keep.slack and any(b < a for a, b in zip(sizes, sizes[1:]))
+
+
+@pytest.mark.parametrize("keep", [None, 64])
+@pytest.mark.parametrize("dtype,n", [("float32", 2), ("bfloat16", 1), ("bfloat16", 3)])
+def test_tokens_that_the_device_chose(dtype, n, keep):
+    """Steps that run one behind another without the host: each token is the largest logit of the rows that were held (or as good as it)."""
+    from cisr_b200 import StepEntry
+
+    stepper = stepper_of(model_of(dtype, 4, 2, 256), graph=True, keep=keep, n_pages=100)
+    keys = [f"r{i}" for i in range(n)]
+    for i, key in enumerate(keys):
+        stepper.create(key)
+        stepper.step([StepEntry(key, tokens_of(20 + i, i))])
+    fed = {key: [i + 1] for i, key in enumerate(keys)}
+    stepper.step([StepEntry(key, fed[key], [0]) for key in keys])
+    first = stepper.last_tokens.tolist()
+    chosen = stepper.decode_ahead(12).tolist()
+    assert len(chosen) == 12
+    stepper.check_kernels()
+    for i, key in enumerate(keys):
+        fed[key] += [first[i]] + [row[i] for row in chosen[:-1]]
+        want = on_held_rows(stepper, key, fed[key])
+        picked = want.gather(1, torch.tensor([[first[i]]] + [[row[i]] for row in chosen], device="cuda"))[:, 0]
+        # a logit is off by several times what all are in the mean square
+        assert (want.amax(-1) - picked <= 2 * 4 * logits_bound(stepper.model.dtype) * want.std()).all()
