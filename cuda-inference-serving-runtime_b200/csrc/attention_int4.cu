@@ -56,7 +56,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // a float16, and products down to 2^-23 keep all their digits (smaller ones are off by 2^-34 at most).  A warp whose sums come out not finite
 // does its keys again with bfloat16 operands, which no step can overflow: codes, which they hold exactly, and products of a probability and a
 // step, made in float, as two terms (16 digits; for float queries three, 24).  So it does not matter to a small group that another one is large.
-// (Looking at every step instead took 8 instructions per 16 keys.)
+// (32 requests of 4000 rows, all of whose values are large: 87 us instead of 36; with float16 and weights times 2^-5, which took 61, groups beside a large
+// one came out up to 2e-3 off.  Looking at every step instead took 8 instructions per 16 keys.)
 constexpr float SLACK = 4.f, SHIFT = 9.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
 constexpr int MAX_RANKED = 128;                                    // requests that are put in order of length, a thread each
@@ -101,10 +102,10 @@ template <int EXPONENT> __device__ __forceinline__ uint32_t centred(uint32_t n) 
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&n), __float2half2_rn((float)(1 << EXPONENT)), __float2half2_rn(-8.f / 512.f));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two codes n, one in each half's low four bits, as bfloat16 n - 8: 128 + n is one by its bits, and 136 less is exact.
-__device__ __forceinline__ uint32_t centred_bf16(uint32_t n) {
+// Two codes n, one in each half's low four bits, as bfloat16 (n - 8) 2^-DOWN: 128 + n is one by its bits, and the rest is exact, in one instruction.
+template <int DOWN> __device__ __forceinline__ uint32_t centred_bf16(uint32_t n) {
     const uint32_t x = n | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(136.f));
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(1.f / (1 << DOWN)), __float2bfloat162_rn(-136.f / (1 << DOWN)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -584,8 +585,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t x = k ? r0 >> 8 : r0, y = k ? r1 >> 8 : r1;
                     if constexpr (LARGE) {
-                        const uint32_t a0 = centred_bf16(x & 0x000f000fu), a1 = centred_bf16((x >> 4) & 0x000f000fu), a2 = centred_bf16(y & 0x000f000fu),
-                                       a3 = centred_bf16((y >> 4) & 0x000f000fu);
+                        constexpr int DOWN = OFFSET ? 24 : 9, SECOND_DOWN = OFFSET ? 20 : 9;      // the units of the usual sums
+                        const uint32_t a0 = centred_bf16<DOWN>(x & 0x000f000fu), a1 = centred_bf16<SECOND_DOWN>((x >> 4) & 0x000f000fu), a2 = centred_bf16<DOWN>(y & 0x000f000fu),
+                                       a3 = centred_bf16<SECOND_DOWN>((y >> 4) & 0x000f000fu);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -625,34 +627,30 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
             l_run[nt][0] = l_run[nt][1] = 0.f;
         }
     };
-    clear();
-    int t = warp;
-    for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), std::false_type(), t);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
-    for (; t < n_tiles; t += WARPS) step(std::true_type(), std::false_type(), t);
-    float all = 0.f;                                                // an overflow is in the sums of the constant operand too
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < (OFFSET ? NG : D / 16); ++i) {
-            const float* v = OFFSET ? r_off[OFFSET ? i : 0][nt] : o[i][nt];
-            all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
-        }
-    if (__any_sync(0xffffffffu, all != 0.f)) {
+    for (bool large = false;; large = true) {
         clear();
+        if (large) {
+            for (int t = warp; t < n_tiles; t += WARPS) step(std::true_type(), std::true_type(), t);
+            break;
+        }
+        int t = warp;
+        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), std::false_type(), t);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
+        for (; t < n_tiles; t += WARPS) step(std::true_type(), std::false_type(), t);
+        float all = 0.f;                                            // an overflow is in the sums of the constant operand too
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < (OFFSET ? NG : D / 16); ++i) {
+                const float* v = OFFSET ? r_off[OFFSET ? i : 0][nt] : o[i][nt];
+                all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
+            }
+        if (!__any_sync(0xffffffffu, all != 0.f)) break;
         here = look_up(warp); next = look_up(warp + WARPS);
         begin();
-        for (t = warp; t < n_tiles; t += WARPS) step(std::true_type(), std::true_type(), t);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)                             // in the units of the usual sums
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                o[i][nt][0] *= OFFSET ? 0x1p-24f : 0x1p-9f; o[i][nt][1] *= OFFSET ? 0x1p-24f : 0x1p-9f;
-                o[i][nt][2] *= OFFSET ? 0x1p-20f : 0x1p-9f; o[i][nt][3] *= OFFSET ? 0x1p-20f : 0x1p-9f;
-            }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                                // every warp is done with its tiles: their place becomes the merge area
