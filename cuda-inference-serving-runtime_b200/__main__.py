@@ -45,7 +45,8 @@ def build_parser() -> argparse.ArgumentParser:
     parser.add_argument("--prefill-chunk", type=int, default=8)
     parser.add_argument("--max-active", type=int, default=8)
     parser.add_argument("--cache", choices=["int4"], help="int4: keys and values held in 4 bits (default: in the compute dtype)")
-    parser.add_argument("--keep", type=int, help="with --cache int4: cut a request down to this many rows, those that attention has looked at most")
+    parser.add_argument("--keep", type=int, help="with --cache int4: cut a request down to this many rows, those that attention has looked at most "
+                        "(of a prompt's portions the latest 16 tokens count, so --prefill-chunk has a part in which rows stay)")
     return parser
 
 

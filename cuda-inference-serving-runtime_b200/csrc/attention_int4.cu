@@ -20,9 +20,11 @@
 // the row's largest lose digits); of probabilities 11 bits.  Float queries take two float16 terms (22 bits) for both.
 // Scores, running maxima, sums and outputs are float.
 //
-// What bounds it: with many long requests the instructions around the products (219 per 16 keys and warp at head size 128 and up to 8
-// rows) at 71 % of the rate of memory: 64 requests of 4000 to 8000 rows, 32 heads over 8 of 128, 96 us of 68; float queries, whose
-// products are two, half of that rate; with few or short requests the way from one trip to memory to the next, some 5 us of a block
+// What bounds it: with many long requests no unit alone, but each warp's chain of products, exponentials, transpositions and products, of which
+// 128 registers a thread leave four to a scheduler: 64 requests of 4000 to 8000 rows, 32 heads over 8 of 128, 97 us where memory takes 68 and
+// the instructions (219 per 16 keys and warp at head size 128 and up to 8 rows) 37; counters: DRAM 56 %, issue slots 52 %, tensor pipe 36 %.  Float
+// queries, whose products are two, take twice as long.  Several tokens, in tiles of 24 rows, have 255 registers and two warps to a scheduler (DRAM 11 %,
+// issue 32 %, tensor pipe 16 %).  With few or short requests it is the way from one trip to memory to the next, some 5 us of a block
 // (one request of 700 rows 8 to 10 us, of 8000 12).  Besides (us, 32 heads over 8 of 128): 32 x 4000 rows 38 (memory 22), 48 x 3000 41 (25), 64 x 500 16 (6);
 // five tokens each of 8 requests of 3000 rows 24.
 #include <climits>
@@ -162,6 +164,7 @@ template <int TK> struct Span {
     }
 };
 template <int ROWS, int TK> __device__ __forceinline__ bool find_span(Span<TK>& s, const Args& a, int x) {
+    static_assert(TK - 1 + ROWS - 1 < 2 * TK, "with one query head per key head a tile's rows are as many tokens, whose windows begin in two tiles of keys");
     s.req = a.by_tiles(x);
     const int tile = x - s.req * a.tiles;
     s.n = a.q_len[s.req]; s.ctx = a.ctx_len[s.req]; s.slot = a.req_slot[s.req]; s.tok0 = a.q_start[s.req];      // one trip to memory
@@ -181,7 +184,7 @@ template <int ROWS, int TK> __device__ __forceinline__ bool find_span(Span<TK>& 
         s.window_base = begin & ~(TK - 1);
     }
     s.tiles = s.last_pos < 0 ? 0 : s.kept_tiles + (s.last_pos - s.window_base) / TK + 1;
-    s.lead = a.window > 0 && s.last_pos >= a.window ? min(s.tiles, s.kept_tiles + 2) : 0;      // the rows' windows begin within 16 keys
+    s.lead = a.window > 0 && s.last_pos >= a.window ? min(s.tiles, s.kept_tiles + 2) : 0;      // the rows' windows begin within ROWS keys
     s.plain = min(s.tiles - s.lead, max(0, s.first_pos + 1 < s.window_base ? 0 : (s.first_pos + 1 - s.window_base) / TK + s.kept_tiles - s.lead));
     return true;
 }
@@ -944,6 +947,9 @@ struct Shape {
     // block's start and end FIXED, the launch and a cluster's joining some more.  Blocks beyond those that run at once come in rounds.
     // Fitted to 1 to 128 requests of 150 to 8000 keys in 1 to 8 splits; right within a fifth, and in the order of what it compares: us of
     // 8 and 4 warps, 8 key heads of 128: 48 x 3000 keys 49 and 41, 64 x 500 22.6 and 16.1, 32 x 4000 38 and 41, in two splits 49 and 41.
+    // The units are those of head size 128; at the smaller ones, where a tile is less work, the same constants choose as well: of 77 launches (single
+    // tokens, 1 to 128 requests of 150 to 4000 keys, head sizes 32 to 128, float at 64) 70 take at most 7 % longer than the best of all forms, 75 at most
+    // 12 %, and two of few blocks at head size 64 16 and 21 % (3 key heads, 32 x 4000 keys: 15.9 us, in four splits 13.1; float 18.7 and 16.1).
     double estimate(long long blocks, int room, int sms, int w, double tiles_of_warp, int parts) const {
         const double FIXED = rows == 8 ? (TERMS == 1 ? 29 : 18) : rows == 24 ? 50 : (TERMS == 1 ? 63 : 51), LATENCY = rows == 8 ? (TERMS == 1 ? 8 : 5) : 5;
         const auto round = [&](long long n) {                       // of n blocks

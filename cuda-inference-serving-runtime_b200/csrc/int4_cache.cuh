@@ -20,8 +20,7 @@
 namespace {
 constexpr int INT4_GROUP = 32, INT4_BLOCK = 8;
 
-__host__ __device__ constexpr int int4_row_bytes(int dim) { return dim / 2; }
-__host__ __device__ constexpr int int4_block_bytes(int dim) { return 9 * dim / 2; }
+__host__ __device__ constexpr int int4_block_bytes(int dim) { return INT4_BLOCK * (dim / 2 + 2 * dim / INT4_GROUP); }
 
 __device__ __forceinline__ int int4_value_slot(int r) { return (r >> 1) + 4 * (r & 1); }          // where a block keeps row r of the values
 template <int D> __device__ __forceinline__ int int4_value_turn(int slot) { return D == 128 ? ((slot >> 1) & 1) << 2 : 0; }

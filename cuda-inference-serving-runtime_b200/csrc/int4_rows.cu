@@ -1,7 +1,8 @@
 // Rows of a cache held in 4 bits (int4_cache.cuh): new keys and values brought in, rows handed back as values, and the rows
 // that attention has looked at least taken out.
 //
-// All of these move memory: a row of keys and values is 4 D bytes as bfloat16 and 9 D / 8 as held.  Head sizes 32, 64, 96 and 128.
+// All of these move memory, a row of keys and values of 4 D bytes as bfloat16 and 9 D / 8 as held, and all but the writing out of whole requests
+// take longer than that, for what each says.  Head sizes 32, 64, 96 and 128.
 #include <type_traits>
 
 #include "int4_cache.cuh"
@@ -196,8 +197,10 @@ __device__ __forceinline__ void store_rows(const T* __restrict__ x, long long to
     }
 }
 
-// The first half of the thread blocks for the keys, the second for the values.  Bound by memory: 8192 tokens of 8 heads of 128 12.4 us in
-// bfloat16 and 20.6 in float (6.6 and 11.7 at its rate); a few tokens by the launch.
+// The first half of the thread blocks for the keys, the second for the values.  8192 tokens of 8 heads of 128: 12.4 us in bfloat16 and 20.6 in
+// float, at memory's rate 6.6 and 11.7.  Neither memory nor issue slots are full then (bfloat16, counters: DRAM 25 %, issue 52 %, 63 % of the warps): it is
+// 1.7 rounds of thread blocks, each of which waits for its rows and their pages, converts and stores, and 2.5 us are the launch's start and
+// end.  A few tokens are the launch alone.
 template <int D, typename T>
 __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_token, long long k_head, long long v_token,
                                                              long long v_head, unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache, float* __restrict__ mass,
@@ -212,8 +215,11 @@ __global__ void __launch_bounds__(THREADS) int4_store_kernel(const T* __restrict
 
 // Rows as values.  `out` is [tokens][heads] with strides of their own; places without a page, and with `ends` those behind a
 // request's end, give zeros.  float16 (three binary digits times eleven, rounded to eleven): divided by the key head's factor (int4_top_kernel).
-// Bound by memory: 8192 rows of 8 heads of 128 as bfloat16 10.4 us of 6.6, as float 20.6 of 11.7; 24 x 2048 rows 43 of 39 and 101 of 70.
+// Whole requests as bfloat16 are bound by memory: 24 x 2048 rows of 8 heads of 128 43 us of 39 (counters: issue 78 % as well).  As float 101
+// of 70: nine tenths of the bytes are those written, by a warp to eight rows at a time.  8192 rows as bfloat16 10.4 us of 6.6, as float 20.6 of 11.7, where issue
+// slots (58 %) and the launch's start and end count more than memory (DRAM 9 %: the rows lie in L2).
 constexpr int READ_ROWS = 1;         // of a thread, and eight thread blocks to an SM: with four rows on their way together, and so fewer threads, 47 and 130
+                                     // (the same lines without the arrays spilled registers: 24 x 2048 rows 46 us)
 template <int D, typename T, bool VALUES>
 __device__ __forceinline__ void read_rows(const unsigned char* __restrict__ cache, T* __restrict__ out, long long req_stride, long long token_stride, long long head_stride,
                                           const Place& at, Divider by_tokens, const int* __restrict__ ends, const int* __restrict__ which, const float* __restrict__ factors,

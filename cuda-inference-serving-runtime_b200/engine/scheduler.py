@@ -107,7 +107,8 @@ class Engine:
     def for_model(cls, model, pages: int = 128, page_size: int = 16, max_active: int = 8, token_budget: int = 32,
                   prefill_chunk: int = 8, policy: str = "chunked", reserve: str = "full", graph: bool = False, cache: Optional[str] = None,
                   keep=None) -> "Engine":
-        """`cache` "int4": keys and values in 4 bits; `keep`, with it: a number of rows (or a `Keep`) that requests are cut down to."""
+        """`cache` "int4": keys and values in 4 bits; `keep`, with it: a number of rows (or a `Keep`) that requests are cut down to, those that
+        attention has looked at most.  Of a portion of a prompt the latest 16 tokens count, so which rows stay depends on `prefill_chunk`."""
         from ..sampling import DeviceSampler
         from .step import Stepper
 

@@ -121,7 +121,10 @@ class StagedTokens:
 @dataclass(frozen=True)
 class Keep:
     """How far a request's cache may grow, and what stays when it is cut: as soon as it has `rows` + `slack` rows, the first `first`,
-    the latest `recent`, and of those between the ones that attention has given most weight so far, `rows` in all, per key head."""
+    the latest `recent`, and of those between the ones that attention has given most weight so far, `rows` in all, per key head.
+
+    The weight is that of every token that was chosen one at a time, and of the latest 16 tokens of every portion of a prompt
+    (`ops.kernels.INT4_WEIGHED`): the same prompt in portions of another size keeps other rows."""
     rows: int
     recent: int
     first: int

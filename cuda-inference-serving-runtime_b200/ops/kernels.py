@@ -535,7 +535,8 @@ INT4_MAX_BYTES = 1 << 36         # of a plane: places in it are counted in 16 by
 # tokens, 32 requests of 2500 rows, 64 heads over 8 of 128: 464 against 490, 902 against 503; 32 over 8: 239 against 297, 463 against 304;
 # 9 over 3 of 64: 51 against 80, 96 against 81; one request of 6000 rows, 32 over 8 of 128: 29 against 70, 47 against 70.
 INT4_FEW = 32
-INT4_WEIGHED = 16                # the latest tokens of a portion by whose weights keys are judged (a score per query and key is kept meanwhile)
+INT4_WEIGHED = 16                # the latest tokens of a portion by whose weights keys are judged (a score per query and key is kept meanwhile); so the
+                                 # weights, and what a cut keeps, depend on how a prompt is cut into portions
 _int4_rows_state = {}
 _attention_int4_libs = {}
 _attention_int4_calls = {}       # by the sizes of a call: the function, the floats of scratch it takes, the kernels it launches
@@ -574,7 +575,7 @@ def int4_page_bytes(page_size: int, head_dim: int) -> int:
         raise KernelError(f"a page of a 4-bit cache holds a multiple of {INT4_BLOCK} rows, not {page_size}")
     if head_dim not in INT4_HEAD_DIMS:
         raise KernelError(f"a 4-bit cache takes head sizes {', '.join(map(str, INT4_HEAD_DIMS))}, not {head_dim}")
-    return page_size * 9 * head_dim // 16
+    return page_size * (head_dim // 2 + 2 * head_dim // INT4_GROUP)
 
 
 def _int4_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, hkv: Optional[int], dim: int) -> tuple:
@@ -758,7 +759,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     written out, and for every request of the step its place in that list (any number for the others); None: all, in order.
 
     `span` 64 is for the other types and head sizes: `attn_decode_int4` of the requests that are listed (the tiles are not looked at), no
-    portion longer than `max_queries` (None: than q).  The rows written out in float for a kernel of its own took two to five
+    portion longer than `max_queries` (None: than q).  scale, window, sink, keep_first: as for `attn_decode_int4`.  The rows written out in float for a kernel of its own took two to five
     times as long (us, 4 requests of 1000 queries: 440 against 966, float with 32 heads over 8 of 128; 144 against 463, bfloat16 with 16 over 8 of 96)."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     hq, dim = q.shape[1], q.shape[2]

@@ -92,10 +92,12 @@ def run_step(stepper, portions):
 SHAPES = [("float32", 4, 2, 128), ("bfloat16", 4, 2, 256), ("bfloat16", 9, 3, 576), ("bfloat16", 4, 2, 384), ("bfloat16", 8, 2, 1024)]
 
 
+@pytest.mark.parametrize("keep", [None, 600])
 @pytest.mark.parametrize("dtype,heads,kv_heads,hidden", SHAPES)
-def test_portions_of_every_length_in_one_step(dtype, heads, kv_heads, hidden):
-    """A long portion behind many rows, short and single ones beside it: by groups of like lengths, and straight over the pages."""
-    stepper = stepper_of(model_of(dtype, heads, kv_heads, hidden), n_pages=300, max_slots=8)
+def test_portions_of_every_length_in_one_step(dtype, heads, kv_heads, hidden, keep):
+    """A long portion behind many rows, short and single ones beside it: by groups of like lengths, and straight over the pages, without and
+    with keys that are weighed."""
+    stepper = stepper_of(model_of(dtype, heads, kv_heads, hidden), n_pages=300, max_slots=8, keep=keep)
     before = dict(zip("abcdefgh", (400, 3, 90, 0, 33, 200, 1, 60)))
     for seed, (key, n) in enumerate(before.items()):
         stepper.create(key)
