@@ -58,7 +58,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // a float16, and products down to 2^-23 keep all their digits (smaller ones are off by 2^-34 at most).  A warp whose sums come out not finite
 // does its keys again with bfloat16 operands, which no step can overflow: codes, which they hold exactly, and products of a probability and a
 // step, made in float, as two terms (16 digits; for float queries three, 24).  So it does not matter to a small group that another one is large.
-// (32 requests of 4000 rows, all of whose values are large: 87 us instead of 36; with float16 and weights times 2^-5, which took 61, groups beside a large
+// (32 requests of 4000 rows, all of whose values are large: 90 us instead of 36; with float16 and weights times 2^-5, which took 61, groups beside a large
 // one came out up to 2e-3 off.  Looking at every step instead took 8 instructions per 16 keys.)
 constexpr float SLACK = 4.f, SHIFT = 9.f;
 constexpr int MAX_CLUSTER = 8;                                     // thread blocks of a portable cluster
@@ -417,18 +417,24 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     };
 
     float* scores = a.scores ? a.scores + ((size_t)unit_of * a.hkv + kvh) * a.longest * a.row_stride : nullptr;
-    // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.  LARGE: products with steps as bfloat16.
-    const auto step = [&](auto is_edge, auto is_large, int t) {
+    // A tile: scores, running maxima, sums.  EDGE: some row does not see some of its keys.  LARGE: 16 keys of one that is there (the `part`th),
+    // with products with steps as bfloat16.  (A whole tile of them was so much code that a captured step of 30 layers took 18 us more, although it
+    // never ran.)
+    const auto step = [&](auto is_edge, auto is_large, int t, int part) {
         constexpr bool EDGE = decltype(is_edge)::value, LARGE = decltype(is_large)::value;
         constexpr int PARTS = LARGE ? TERMS + 1 : TERMS;
         constexpr bool HALVES_PRODUCT = TERMS == 1 && !LARGE;       // of probability and step, in float16
-        const int k0 = span.key(t0 + t);
-        float s[HALVES][NT][4];
-        asm volatile("cp.async.wait_group 1;" ::: "memory");        // the keys
-        __syncwarp();
+        constexpr int COUNT = LARGE ? 1 : HALVES;
+        const int k0 = span.key(t0 + t) + 16 * part;
+        const unsigned char *keys = ks + 2 * part * BLOCK_BYTES, *values = vs + 2 * part * BLOCK_BYTES;
+        float s[COUNT][NT][4];
+        if constexpr (!LARGE) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");    // the keys
+            __syncwarp();
+        }
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {                          // 16 keys: blocks 2 h and 2 h + 1
-            const unsigned char* b0 = ks + 2 * h * BLOCK_BYTES;
+        for (int h = 0; h < COUNT; ++h) {                           // 16 keys: blocks 2 h and 2 h + 1
+            const unsigned char* b0 = keys + 2 * h * BLOCK_BYTES;
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             const Share<4 * NG> w0 = load_share<4 * NG>(b0 + g * (D / 2) + c * 4 * NG), w1 = load_share<4 * NG>(b1 + g * (D / 2) + c * 4 * NG);
             const Share<2 * NG> s0 = load_share<2 * NG>(b0 + 4 * D + g * 2 * NG), s1 = load_share<2 * NG>(b1 + 4 * D + g * 2 * NG);
@@ -466,14 +472,16 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     for (int e = 0; e < 4; ++e) s[h][nt][e] = OFFSET || j ? fmaf(e < 2 ? f0 : f1, acc[nt][e], s[h][nt][e]) : (e < 2 ? f0 : f1) * acc[nt][e];
             }
         }
-        __syncwarp();                                               // every lane has read the keys
         const bool again = t + WARPS < n_tiles;
-        fetch(a.k_cache, landing, next, again);
+        if constexpr (!LARGE) {
+            __syncwarp();                                           // every lane has read the keys
+            fetch(a.k_cache, landing, next, again);
+        }
         bool more = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
+            for (int h = 0; h < COUNT; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (EDGE) {
@@ -483,9 +491,9 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     }
                     more |= s[h][nt][e] > limit[nt][e & 1];
                 }
-        if (scores) {
+        if (!LARGE && scores) {
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
+            for (int h = 0; h < COUNT; ++h)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                 for (int e = 0; e < 2; ++e) {
                     float mx = s[0][nt][e];
 #pragma unroll
-                    for (int h = 0; h < HALVES; ++h) mx = fmaxf(mx, fmaxf(s[h][nt][e], s[h][nt][e + 2]));
+                    for (int h = 0; h < COUNT; ++h) mx = fmaxf(mx, fmaxf(s[h][nt][e], s[h][nt][e + 2]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -521,7 +529,7 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
             for (int e = 0; e < 2; ++e) {
                 const float top = SHIFT - (m_run[nt][e] == -INFINITY ? 0.f : m_run[nt][e] * unit[nt][e]);
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) {
+                for (int h = 0; h < COUNT; ++h) {
                     float p0 = exp2_fast(fmaf(s[h][nt][e], unit[nt][e], top)), p1 = exp2_fast(fmaf(s[h][nt][e + 2], unit[nt][e], top));
                     l_run[nt][e] += p0 + p1;
                     if constexpr (EDGE) {                                     // a key out of sight gets -0, by which it is told from one of no weight
@@ -531,10 +539,12 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     s[h][nt][e] = p0; s[h][nt][e + 2] = p1;
                 }
             }
-        asm volatile("cp.async.wait_group 1;" ::: "memory");        // the values
-        __syncwarp();
+        if constexpr (!LARGE) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");    // the values
+            __syncwarp();
+        }
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
+        for (int h = 0; h < COUNT; ++h) {
             // probabilities as B: rows of the product above are keys, here columns: two 8 x 8 transpositions per 16 keys
             uint32_t pt[NT][2];
             if constexpr (HALVES_PRODUCT) {
@@ -544,11 +554,11 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                     pt[nt][1] = transposed(pack_f16(s[h][nt][2], s[h][nt][3]));
                 }
             }
-            const unsigned char* b0 = vs + 2 * h * BLOCK_BYTES;
+            const unsigned char* b0 = values + 2 * h * BLOCK_BYTES;
             const unsigned char* b1 = b0 + BLOCK_BYTES;
             Share<4 * NG> sv[2];                                    // the steps of two neighbouring keys side by side
 #pragma unroll
-            for (int b = 0; b < 2; ++b) sv[b] = load_share<4 * NG>(vs + (2 * h + b) * BLOCK_BYTES + 4 * D + c * 4 * NG);
+            for (int b = 0; b < 2; ++b) sv[b] = load_share<4 * NG>(values + (2 * h + b) * BLOCK_BYTES + 4 * D + c * 4 * NG);
             const int turned = (g ^ int4_value_turn<D>(c)) * 2 * NG;
             const Share<2 * NG> u0 = load_share<2 * NG>(b0 + c * (D / 2) + turned), u1 = load_share<2 * NG>(b0 + (4 + c) * (D / 2) + turned);
             const Share<2 * NG> u2 = load_share<2 * NG>(b1 + c * (D / 2) + turned), u3 = load_share<2 * NG>(b1 + (4 + c) * (D / 2) + turned);
@@ -613,10 +623,12 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                 }
             }
         }
-        __syncwarp();                                               // every lane has read the values
-        here = next;
-        fetch(a.v_cache, landing + PLANE_BYTES, here, again);
-        next = look_up(t + 2 * WARPS);
+        if constexpr (!LARGE) {
+            __syncwarp();                                           // every lane has read the values
+            here = next;
+            fetch(a.v_cache, landing + PLANE_BYTES, here, again);
+            next = look_up(t + 2 * WARPS);
+        }
     };
 
     const auto clear = [&] {
@@ -633,16 +645,26 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
     for (bool large = false;; large = true) {
         clear();
         if (large) {
-            for (int t = warp; t < n_tiles; t += WARPS) step(std::true_type(), std::true_type(), t);
+            here = look_up(warp);
+            for (int t = warp; t < n_tiles; t += WARPS) {
+                next = look_up(t + WARPS);
+                begin();
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll 1
+                for (int part = 0; part < HALVES; ++part) step(std::true_type(), std::true_type(), t, part);
+                __syncwarp();
+                here = next;
+            }
             break;
         }
         int t = warp;
-        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), std::false_type(), t);
+        for (const int plain = min(n_tiles, span.plain - t0); t < plain; t += WARPS) step(std::false_type(), std::false_type(), t, 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) own_pos[nt][h] = span.ctx - span.n + a.by_group(span.row0 + min(nt * 8 + 2 * c + h, span.rows - 1));
-        for (; t < n_tiles; t += WARPS) step(std::true_type(), std::false_type(), t);
+        for (; t < n_tiles; t += WARPS) step(std::true_type(), std::false_type(), t, 0);
         float all = 0.f;                                            // an overflow is in the sums of the constant operand too
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -652,8 +674,6 @@ __global__ void __launch_bounds__(32 * WARPS, blocks_of<NT, WARPS>()) attn_int4_
                 all += (v[0] + v[1] + (OFFSET ? 0.f : v[2] + v[3])) * 0.f;
             }
         if (!__any_sync(0xffffffffu, all != 0.f)) break;
-        here = look_up(warp); next = look_up(warp + WARPS);
-        begin();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                                // every warp is done with its tiles: their place becomes the merge area
