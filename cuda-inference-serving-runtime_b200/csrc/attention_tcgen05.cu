@@ -170,6 +170,13 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     pdl_trigger();
     const int tile = blockIdx.x / hq, head = blockIdx.x % hq;   // neighbours share a tile's length: the long ones start first
     const int req = tile_req[tile], q0 = tile_q0[tile];
+    if (HALF_OPERANDS) {                                        // a tile of a request whose rows were not written out for this call
+        const int place = req_slot[req];
+        if (place < 0 || (long long)place * hkv * page_size >= cache_rows) {
+            if (threadIdx.x == 0) atomicExch(error, 7);
+            return pdl_wait();
+        }
+    }
     const int rows = min(span, q_len[req] - q0);
     const int tok0 = q_start[req] + q0;
     const int ctx = ctx_len[req];

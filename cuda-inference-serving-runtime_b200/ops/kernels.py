@@ -756,7 +756,8 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     operands, whose eleven binary digits are those of a held value; a held value that is NaN reaches the queries before it, too, as
     it does there.  `longest`: no request that is written out has more rows (a bound will do; one that has sets the
     flag that `raise_if_kernel_gave_up` reads).  `portions` (requests, places): the requests that are
-    written out, and for every request of the step its place in that list (any number for the others); None: all, in order.
+    written out, and for every request of the step its place in that list (a negative number for the others, whose tiles would set that
+    flag); None: all, in order.  A request has at least as many rows as it brings tokens.
 
     `span` 64 is for the other types and head sizes: `attn_decode_int4` of the requests that are listed (the tiles are not looked at), no
     portion longer than `max_queries` (None: than q).  scale, window, sink, keep_first: as for `attn_decode_int4`.  The rows written out in float for a kernel of its own took two to five
@@ -2605,7 +2606,8 @@ _GAVE_UP = {1: "a tcgen05 matrix product gave up waiting on a barrier",
             3: "an attention kernel gave up waiting on a tensor-map copy",
             4: "a weight-streaming product gave up waiting on a tensor-map copy",
             5: "the tcgen05 attention gave up waiting on a barrier",
-            6: "an attention over a 4-bit cache met a request longer than the bound it was given"}
+            6: "an attention over a 4-bit cache met a request longer than the bound it was given",
+            7: "an attention over a 4-bit cache met a tile of a request that is not among the portions it was given"}
 
 
 def error_flag_tensor() -> Optional[torch.Tensor]:

@@ -234,7 +234,7 @@ def int4_portions(ctx, heads: int, window) -> list:
             tiles.sort(key=lambda t: lens[t[0]] - t[1] <= kernels.WIDE_TILE)
         spans.append(span)
         place = {r: i for i, r in enumerate(which)}
-        flat += [[r for r, _ in tiles], [a for _, a in tiles], which, [place.get(r, 0) for r in range(len(lens))]]
+        flat += [[r for r, _ in tiles], [a for _, a in tiles], which, [place.get(r, -1) for r in range(len(lens))]]
     lists = torch.tensor([x for part in flat for x in part], dtype=torch.int32, device=ctx.device).split([len(part) for part in flat])
     calls = [(lists[4 * i:4 * i + 2], span, lists[4 * i + 2:4 * i + 4], ends[which[0]]) for i, (which, span) in enumerate(zip(groups, spans))]
     ctx.shared["int4_portions", heads, window] = calls

@@ -220,3 +220,24 @@ def test_portions_with_a_large_group_among_small_ones(dim, span, large, small):
     cache = Cache([700], hkv, dim, 16, k=[k], v=[v])
     q = queries(200, hq, dim, torch.bfloat16)
     check_portions(cache, q, portions(cache, q, [200], span, scale), [200], span, scale)
+
+
+@pytest.mark.parametrize("dim,span", [(64, 128), (128, 256)])
+def test_tiles_of_requests_that_are_not_listed_are_reported(dim, span):
+    """They are left alone, and the listed ones come out as they do alone."""
+    hq, hkv = 4, 2
+    cache = Cache([300, 200, 90], hkv, dim, 16)
+    q = queries(120, hq, dim, torch.bfloat16)
+    lists = (i32([0, 50, 90]), i32([50, 40, 30]), cache.ctx, 300, 16, dim ** -0.5)
+    outs = []
+    for tiles, places in (([0, 1, 2], [-1, 0, 5]), ([1], [-1, 0, -1])):
+        out = torch.full_like(q, 7.0)
+        kernels.attn_prefill_int4(q, out, cache.k_cache, cache.v_cache, cache.slots, cache.table, i32(tiles), i32([0] * len(tiles)), *lists, span=span,
+                                  portions=(i32([1]), i32(places)))
+        if len(tiles) == 3:
+            with pytest.raises(KernelError, match="not among the portions"):
+                kernels.raise_if_kernel_gave_up()
+        kernels.raise_if_kernel_gave_up()
+        assert (out[:50] == 7).all() and (out[90:] == 7).all()
+        outs.append(out)
+    assert torch.equal(*outs)
