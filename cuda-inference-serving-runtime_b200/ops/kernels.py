@@ -761,7 +761,7 @@ def attn_prefill_int4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
 
     `span` 64 is for the other types and head sizes: `attn_decode_int4` of the requests that are listed (the tiles are not looked at), no
     portion longer than `max_queries` (None: than q).  scale, window, sink, keep_first: as for `attn_decode_int4`.  The rows written out in float for a kernel of its own took two to five
-    times as long (us, 4 requests of 1000 queries: 440 against 966, float with 32 heads over 8 of 128; 144 against 463, bfloat16 with 16 over 8 of 96)."""
+    times as long (us, 4 requests of 1000 queries: 440 against 966, float with 32 heads over 8 of 128; 144 (now 128) against 463, bfloat16 with 16 over 8 of 96)."""
     _need(q, None, "q", 3); _need(out, q.dtype, "out", 3)
     hq, dim = q.shape[1], q.shape[2]
     hkv, device = _int4_cache("attn_prefill_int4", k_cache, v_cache, page_size, None, dim)
